@@ -195,6 +195,27 @@ int pcb_qdense_fwd(const pcb_dense_desc* desc, const void* x, const void* w, con
 int pcb_qdense_bwd(const pcb_dense_desc* desc, const void* x, const void* w, const void* dy, void* dw, void* dx,
                    void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- The dense layer in 8-bit floating point (no counterpart in the reference) --------------------------------------
+ * A block of values is held as e4m3 numbers times 2^e, e the smallest whole number with max|x| <= 448 * 2^e (0 for a block of
+ * zeros, -126 at least). Infinities and NaN become NaN and do not enter the maximum.
+ *   Filter: `values` holds [D][rows][pitch] bytes, rows x columns as the filter layout says (I x O, or O x I with filter_oi),
+ *   pitch = columns rounded up to 16 (the rest of a row is not read); `scales` holds the byte e + 127 of each 128 x 128 block,
+ *   [D][blocks of rows][blocks of columns]. Both are the caller's (the sizes below); values 16-byte aligned.
+ *   x and dy come in desc->dtype and are quantised inside the call, in the workspace, with one scale for each 128 values along the axis that
+ *   the product sums over: features for y and dx, samples for dw.
+ * Products are exact, sums are held in fp32, results are rounded once to desc->dtype. Every algebra; engine AUTO or TENSOR; `variant` has no
+ * meaning here. The workspace must be 16-byte aligned. dw is written in [D, I, O] orientation whatever filter_oi says. In backward w8 may be
+ * null when require_input_grad is 0. pcb_quantize_filter8 does not read desc->batch. */
+size_t pcb_filter8_values_size(const pcb_dense_desc* desc);
+size_t pcb_filter8_scales_size(const pcb_dense_desc* desc);
+int pcb_quantize_filter8(const pcb_dense_desc* desc, const void* w, void* values, void* scales, void* stream);
+size_t pcb_qdense8_fwd_workspace_size(const pcb_dense_desc* desc);
+size_t pcb_qdense8_bwd_workspace_size(const pcb_dense_desc* desc);
+int pcb_qdense8_fwd(const pcb_dense_desc* desc, const void* x, const void* w8, const void* w8_scales, const void* bias, void* y,
+                    void* workspace, size_t workspace_bytes, void* stream);
+int pcb_qdense8_bwd(const pcb_dense_desc* desc, const void* x, const void* w8, const void* w8_scales, const void* dy, void* dw, void* dx,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
 /* Which kernel family a forward / backward call with this descriptor will run: 1 = CUDA-core fp32,
  * 2 = tcgen05 tensor-core. pass: 0 forward, 1 backward-data, 2 backward-filter. Negative = status.
  * (Plays the role of QuatKernelPointwiseConvManager::canRun, src/backend/cudnn/quat_pointwise_conv2d.cc:33-77,

@@ -59,6 +59,13 @@ SYMBOLS = {
     "pcb_qconv2d_bwd_filter_noalloc": (_i, [_cd, _vp, _vp, _vp, _vp]),
     "pcb_qdense_fwd": (_i, [_dd, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "pcb_qdense_bwd": (_i, [_dd, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "pcb_filter8_values_size": (_sz, [_dd]),
+    "pcb_filter8_scales_size": (_sz, [_dd]),
+    "pcb_quantize_filter8": (_i, [_dd, _vp, _vp, _vp, _vp]),
+    "pcb_qdense8_fwd_workspace_size": (_sz, [_dd]),
+    "pcb_qdense8_bwd_workspace_size": (_sz, [_dd]),
+    "pcb_qdense8_fwd": (_i, [_dd, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "pcb_qdense8_bwd": (_i, [_dd, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "pcb_qconv2d_engine_for": (_i, [_cd, _i]),
     "pcb_qdense_engine_for": (_i, [_dd, _i]),
     "pcb_check_device_status": (_i, [_vp, _sz, _vp]),

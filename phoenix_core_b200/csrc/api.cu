@@ -7,6 +7,7 @@
 #include <unordered_map>
 
 #include "common.cuh"
+#include "dense8.cuh"
 #include "tc_common.cuh"
 #include "tensor_path.cuh"
 #include "umma.cuh"
@@ -390,6 +391,68 @@ int conv_bwd_both(const pcb_conv2d_desc* desc, const void* x, const void* w, con
     return rc;
 }
 
+// ---- dense layer in 8-bit floating point: where its copies of the operands lie in the workspace
+struct Dense8Space {
+    size_t x_rows, x_words, dy_rows, dy_row_words, dy_cols, dy_col_words, x_cols, x_col_words, total;
+};
+size_t align256(size_t v) { return (v + 255) / 256 * 256; }
+size_t q8_value_bytes(int comps, int rows, int cols) { return (size_t)comps * rows * q8_pitch(cols); }
+size_t q8_word_bytes(int comps, int extent, int summed) { return (size_t)comps * q8_groups(summed) * extent * 4; }
+Dense8Space dense8_space(const Geom& g, bool backward, bool need_dx) {
+    Dense8Space s = {};
+    size_t at = WS_HEADER;
+    auto take = [&](size_t bytes) { const size_t here = at; at = align256(at + bytes); return here; };
+    if (!backward) {
+        s.x_rows = take(q8_value_bytes(g.nc, g.Nb, g.Ci));
+        s.x_words = take(q8_word_bytes(g.nc, g.Nb, g.Ci));
+    } else {
+        if (need_dx) {
+            s.dy_rows = take(q8_value_bytes(g.nc, g.Nb, g.Co));
+            s.dy_row_words = take(q8_word_bytes(g.nc, g.Nb, g.Co));
+        }
+        s.dy_cols = take(q8_value_bytes(g.nc, g.Nb, g.Co));
+        s.dy_col_words = take(q8_word_bytes(g.nc, g.Co, g.Nb));
+        s.x_cols = take(q8_value_bytes(g.nc, g.Nb, g.Ci));
+        s.x_col_words = take(q8_word_bytes(g.nc, g.Ci, g.Nb));
+    }
+    s.total = at;
+    return s;
+}
+int dense8_geom(const pcb_dense_desc* d, Geom& g) {
+    const int rc = dense_geom(d, g);
+    if (rc != PCB_OK) return rc;
+    if (d->engine != PCB_ENGINE_AUTO && d->engine != PCB_ENGINE_TENSOR) {
+        set_error("8-bit dense layers run on the tensor cores only");
+        return PCB_ERR_UNSUPPORTED;
+    }
+    // (the 8-bit copies have rows of whole 16 bytes)
+    if ((long long)g.nc * g.Nb * q8_pitch(g.Ci) > MAX_NUMEL || (long long)g.nc * g.Nb * q8_pitch(g.Co) > MAX_NUMEL ||
+        (long long)g.nc * g.Ci * q8_pitch(g.Co) > MAX_NUMEL || (long long)g.nc * q8_pitch(g.Ci) * g.Co > MAX_NUMEL) {
+        set_error("tensor too large for 32-bit element offsets");
+        return PCB_ERR_TOO_LARGE;
+    }
+    return PCB_OK;
+}
+int dense8_workspace(const void* workspace, size_t have, size_t need) {
+    if (!workspace || have < need) { set_error("workspace of %zu bytes, %zu needed", workspace ? have : (size_t)0, need); return PCB_ERR_WORKSPACE; }
+    if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) { set_error("the workspace of an 8-bit dense layer must be 16-byte aligned"); return PCB_ERR_INVALID_ARGUMENT; }
+    return PCB_OK;
+}
+// The filter as an operand whose own axis is `out_features` (forward) or in_features (backward-data).
+Q8Operand dense8_filter(const Geom& g, const void* values, const void* scales, bool forward) {
+    const int cols = g.w_io ? g.Co : g.Ci;
+    Q8Operand o = {static_cast<const uint8_t*>(values), scales, q8_pitch(cols), 1, 0, 0, 0};
+    o.mn_major = forward ? g.w_io : !g.w_io;                            // rows of the filter run along the operand's own axis
+    const int row_stride = q8_blocks(cols);
+    o.bytes_k = o.mn_major ? row_stride : 1;
+    o.bytes_mn = o.mn_major ? 1 : row_stride;
+    return o;
+}
+int dense8_check_filter(const void* values) {
+    if (reinterpret_cast<uintptr_t>(values) % 16 != 0) { set_error("8-bit filter values must be 16-byte aligned"); return PCB_ERR_INVALID_ARGUMENT; }
+    return PCB_OK;
+}
+
 }  // namespace
 }  // namespace pcb
 
@@ -614,6 +677,86 @@ int pcb_check_device_status(const void* workspace, size_t workspace_bytes_, void
         return PCB_ERR_DEVICE_TIMEOUT;
     }
     return PCB_OK;
+}
+
+size_t pcb_filter8_values_size(const pcb_dense_desc* desc) {
+    Geom g;
+    if (dense8_geom(desc, g) != PCB_OK) return 0;
+    return q8_value_bytes(g.nc, g.w_io ? g.Ci : g.Co, g.w_io ? g.Co : g.Ci);
+}
+size_t pcb_filter8_scales_size(const pcb_dense_desc* desc) {
+    Geom g;
+    if (dense8_geom(desc, g) != PCB_OK) return 0;
+    return (size_t)g.nc * q8_blocks(g.Ci) * q8_blocks(g.Co);
+}
+int pcb_quantize_filter8(const pcb_dense_desc* desc, const void* w, void* values, void* scales, void* stream) {
+    Geom g;
+    int rc = dense8_geom(desc, g);
+    if (rc != PCB_OK) return rc;
+    if (!w || !values || !scales) { set_error("null tensor pointer"); return PCB_ERR_INVALID_ARGUMENT; }
+    if ((rc = dense8_check_filter(values)) != PCB_OK) return rc;
+    return q8_quantize_blocks(desc->dtype, g.nc, g.w_io ? g.Ci : g.Co, g.w_io ? g.Co : g.Ci, w, static_cast<uint8_t*>(values), static_cast<uint8_t*>(scales),
+                              (cudaStream_t)stream);
+}
+size_t pcb_qdense8_fwd_workspace_size(const pcb_dense_desc* desc) {
+    Geom g;
+    return dense8_geom(desc, g) == PCB_OK ? dense8_space(g, false, false).total : 0;
+}
+size_t pcb_qdense8_bwd_workspace_size(const pcb_dense_desc* desc) {
+    Geom g;
+    return dense8_geom(desc, g) == PCB_OK ? dense8_space(g, true, desc->require_input_grad != 0).total : 0;
+}
+int pcb_qdense8_fwd(const pcb_dense_desc* desc, const void* x, const void* w8, const void* w8_scales, const void* bias, void* y, void* workspace,
+                    size_t workspace_bytes_, void* stream) {
+    Geom g;
+    int rc = dense8_geom(desc, g);
+    if (rc != PCB_OK) return rc;
+    if (g.Nb == 0) return PCB_OK;
+    if (!x || !w8 || !w8_scales || !y || (g.has_bias && !bias)) { set_error("null tensor pointer"); return PCB_ERR_INVALID_ARGUMENT; }
+    const Dense8Space at = dense8_space(g, false, false);
+    if ((rc = dense8_workspace(workspace, workspace_bytes_, at.total)) != PCB_OK || (rc = dense8_check_filter(w8)) != PCB_OK) return rc;
+    forget_kept(workspace);
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    int* status = reinterpret_cast<int*>(ws);
+    const Q8Target rows = {ws + at.x_rows, reinterpret_cast<uint32_t*>(ws + at.x_words)};
+    rc = q8_quantize(desc->dtype, g.nc, g.Nb, g.Ci, x, rows, Q8Target{}, status, (cudaStream_t)stream);
+    if (rc != PCB_OK) return rc;
+    const Q8Operand tokens = {rows.values, rows.words, q8_pitch(g.Ci), 0, 0, 0, 0}, filter = dense8_filter(g, w8, w8_scales, true);
+    Q8Product q = {PASS_FWD, q8_swapped(g.Nb) ? 1 : 0, g.Nb, g.Co, g.Ci, tokens, filter, y, desc->dtype, g.has_bias ? bias : nullptr, status};
+    if (q.swapped) { q.m = g.Co; q.n = g.Nb; q.a = filter; q.b = tokens; }
+    return q8_product(g, q, (cudaStream_t)stream);
+}
+int pcb_qdense8_bwd(const pcb_dense_desc* desc, const void* x, const void* w8, const void* w8_scales, const void* dy, void* dw, void* dx, void* workspace,
+                    size_t workspace_bytes_, void* stream) {
+    Geom g;
+    int rc = dense8_geom(desc, g);
+    if (rc != PCB_OK) return rc;
+    if (!dw) { set_error("null tensor pointer"); return PCB_ERR_INVALID_ARGUMENT; }
+    if (g.Nb == 0) {
+        PCB_CUDA_TRY(cudaMemsetAsync(dw, 0, (size_t)g.nc * g.Co * g.Ci * dtype_size(desc->dtype), (cudaStream_t)stream));
+        return PCB_OK;
+    }
+    const bool need_dx = desc->require_input_grad != 0;
+    if (!x || !dy || (need_dx && (!dx || !w8 || !w8_scales))) { set_error("null tensor pointer"); return PCB_ERR_INVALID_ARGUMENT; }
+    const Dense8Space at = dense8_space(g, true, need_dx);
+    if ((rc = dense8_workspace(workspace, workspace_bytes_, at.total)) != PCB_OK || (need_dx && (rc = dense8_check_filter(w8)) != PCB_OK)) return rc;
+    forget_kept(workspace);
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    int* status = reinterpret_cast<int*>(ws);
+    const cudaStream_t st = (cudaStream_t)stream;
+    const Q8Target dy_rows = {need_dx ? ws + at.dy_rows : nullptr, reinterpret_cast<uint32_t*>(ws + at.dy_row_words)};
+    const Q8Target dy_cols = {ws + at.dy_cols, reinterpret_cast<uint32_t*>(ws + at.dy_col_words)};
+    const Q8Target x_cols = {ws + at.x_cols, reinterpret_cast<uint32_t*>(ws + at.x_col_words)};
+    rc = q8_quantize(desc->dtype, g.nc, g.Nb, g.Co, dy, dy_rows, dy_cols, status, st);
+    if (rc == PCB_OK) rc = q8_quantize(desc->dtype, g.nc, g.Nb, g.Ci, x, Q8Target{}, x_cols, nullptr, st);
+    if (rc != PCB_OK) return rc;
+    const Q8Operand a = {x_cols.values, x_cols.words, q8_pitch(g.Ci), 0, 0, 0, 1}, b = {dy_cols.values, dy_cols.words, q8_pitch(g.Co), 0, 0, 0, 1};
+    rc = q8_product(g, Q8Product{PASS_BWD_FILTER, 0, g.Ci, g.Co, g.Nb, a, b, dw, desc->dtype, nullptr, status}, st);
+    if (rc != PCB_OK || !need_dx) return rc;
+    const Q8Operand tokens = {dy_rows.values, dy_rows.words, q8_pitch(g.Co), 0, 0, 0, 0}, filter = dense8_filter(g, w8, w8_scales, false);
+    Q8Product q = {PASS_BWD_DATA, q8_swapped(g.Nb) ? 1 : 0, g.Nb, g.Ci, g.Co, tokens, filter, dx, desc->dtype, nullptr, status};
+    if (q.swapped) { q.m = g.Ci; q.n = g.Nb; q.a = filter; q.b = tokens; }
+    return q8_product(g, q, st);
 }
 
 }  // extern "C"

@@ -1,0 +1,498 @@
+// Products of 8-bit operands with block scales on the tensor cores: forward, backward-data and filter gradient of the dense layer (dense8.cuh).
+//
+//   out[c][m][n] = sum over (component j of the reduction, k) of sign(c, j) * 2^(ea + eb) * qa[m][k] * qb[n][k]      (+ bias)
+//
+// The algebra's block is a choice of operand components and a sign per (c, j); the sign is the negation bit of the instruction, so a quaternion
+// layer is sixteen products of the same tiles and no operand is changed. The scales are powers of two, which tcgen05.mma.kind::mxf8f6f4
+// multiplies in itself: one e8m0 byte per operand row and 32 values, here the same byte four times over (the blocks have 128). Products are
+// exact and sums are held in fp32 in tensor memory over the whole reduction.
+//
+// Roles: warp 0 copies the operand tiles (TMA; both majornesses are read where they lie), warp 1 issues, warp 2 lays the scales out (a word per
+// row holds the bytes of four blocks; 32 x 4 words are 512 bytes in the order that tcgen05.cp takes to tensor memory), warps 4-11 drain the accumulators.
+// Tiles are 128 x BN; a tile's reduction is cut over the CTAs of a cluster where there are fewer tiles than SMs, whose partial sums
+// are added in a fixed order through distributed shared memory.
+#include "dense8.cuh"
+#include "tc_common.cuh"
+
+namespace pcb {
+namespace {
+
+using namespace umma;
+using namespace tc;
+
+constexpr int D8_BM = 128, D8_BK = 128;
+constexpr int D8_THREADS = 384, D8_EPI_WARPS = 8;
+constexpr uint32_t D8_A_BYTES = D8_BM * D8_BK;
+constexpr int D8_SF_STAGES = 4;
+constexpr uint32_t D8_SF_BYTES = 512 * 3;                       // one set of 128 rows for A, up to two for B
+constexpr int ST_D8_PRODUCER = 0x100, ST_D8_MMA = 0x200, ST_D8_SCALES = 0x400, ST_D8_EPILOGUE = 0x800;
+
+template <int BN> struct D8Config {
+    static constexpr int B_ROWS = BN < 32 ? 32 : BN;             // (tiles start on 1024 bytes: 8 rows)
+    static constexpr uint32_t B_BYTES = B_ROWS * D8_BK;
+    static constexpr uint32_t STAGE = D8_A_BYTES + B_BYTES;
+    static constexpr int STAGES = BN >= 256 ? 4 : (BN >= 128 ? 6 : (BN >= 64 ? 8 : 10));
+    static constexpr int ACC = BN >= 256 ? 1 : 2;                // accumulators in tensor memory
+    static constexpr uint32_t ACC_COLS = BN < 32 ? 32 : BN;
+    static constexpr uint32_t SF_COL = 496;                      // scales: 4 columns for A, 8 for B
+    static constexpr uint32_t STAGED = EPI_ROWS_BYTES * D8_EPI_WARPS;
+    static constexpr uint32_t BARS = 256;
+    static constexpr size_t SMEM = 1024 + STAGES * STAGE + D8_SF_STAGES * D8_SF_BYTES + (BN >= 128 ? STAGED : 0) + BARS;
+};
+
+struct D8Params {
+    int pass, ga, comps;
+    unsigned long long neg;
+    int m, n, k;
+    int chunks, groups;                 // blocks of 128 and groups of four of them per component of the reduction
+    int m_tiles, n_tiles, tiles;        // tiles: over all output components
+    int splits;                         // CTAs of the cluster that share a tile
+    int a_mn, b_mn;                     // operands run along their own axis
+    int a_blocks, b_blocks;             // scales are bytes per 128 x 128 block, else words
+    const uint8_t *a_scales, *b_scales;
+    int a_bk, a_bm, a_bc, b_bk, b_bm, b_bc;   // strides of the bytes: blocks of the reduction, blocks of the own axis, components
+    int dtype;
+    long long out_comp; int out_ld;     // element (c, slow, fast) of the output at c * out_comp + slow * out_ld + fast
+    void* out;
+    const void* bias;                   // [comps][fast extent], or null
+};
+
+// Operand components and sign of term j of output component c.
+__device__ __forceinline__ void d8_term(const D8Params& p, int c, int j, int& x_comp, int& other, bool& neg) {
+    if (p.pass == PASS_FWD)           { x_comp = j; other = alg_pair(p.ga, j, c); neg = alg_negative(p.neg, j, c); }                       // x_l, w_r
+    else if (p.pass == PASS_BWD_DATA) { x_comp = j; other = alg_pair(p.ga, c, j); neg = alg_negative(p.neg, c, j); }                       // dy_d, w_r
+    else                              { x_comp = j; other = alg_pair(p.ga, j, c); neg = alg_negative(p.neg, j, other); }                   // x_l, dy_d
+}
+
+// kind::mxf8f6f4, e4m3 operands, e8m0 scales, fp32 sums
+__device__ __forceinline__ uint32_t d8_idesc(int M, int N, bool a_mn, bool b_mn, bool a_neg) {
+    return ((uint32_t)a_neg << 13) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(N >> 3) << 17) | (1u << 23) | ((uint32_t)(M >> 4) << 24);
+}
+__device__ __forceinline__ void mma_mxf8(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                         uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+        "mov.b64 da, {%1, %2};\n\t"
+        "mov.b64 db, {%3, %4};\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], da, db, %5, [%7], [%8], p;\n\t}"
+        ::"r"(d_tmem), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb) : "memory");
+}
+// 32 rows of 16 bytes to four columns of tensor memory, in each of the four groups of 32 lanes
+__device__ __forceinline__ void copy_scales(uint32_t tmem, uint32_t smem_addr) {
+    const uint64_t desc = (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | ((uint64_t)(128 >> 4) << 16) | ((uint64_t)(128 >> 4) << 32) | DESC_VERSION_SM100;
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+
+__device__ __forceinline__ float ld_typed(const void* p, int dtype, size_t i) {
+    if (dtype == PCB_F32) return ld_chained(static_cast<const float*>(p) + i);
+    const uint16_t h = ld_chained(static_cast<const uint16_t*>(p) + i);
+    return dtype == PCB_F16 ? __half2float(__ushort_as_half(h)) : __uint_as_float((uint32_t)h << 16);
+}
+__device__ __forceinline__ uint16_t to_16(float v, int dtype) {
+    return dtype == PCB_F16 ? __half_as_ushort(__float2half_rn(v)) : __bfloat16_as_ushort(__float2bfloat16_rn(v));
+}
+__device__ __forceinline__ void st_typed(void* p, int dtype, size_t i, float v) {
+    if (dtype == PCB_F32) static_cast<float*>(p)[i] = v;
+    else static_cast<uint16_t*>(p)[i] = to_16(v, dtype);
+}
+__device__ __forceinline__ uint32_t pack_16(float a, float b, int dtype) {
+    if (dtype == PCB_F16) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// A warp's 32 rows (one per lane) x 32 columns of floats whose rows start anywhere: through shared memory, sixteen columns at a time, so that the
+// lanes of an instruction write neighbours. rows, cols: how many exist.
+__device__ __forceinline__ void store_floats(uint32_t buf, const uint32_t (&v)[32], float* out, int rows, int cols, int ld, int lane) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) asm volatile("st.shared.u32 [%0], %1;" ::"r"(buf + (uint32_t)(lane * EPI_ROWS_PITCH + e) * 4u), "r"(v[16 * h + e]) : "memory");
+        __syncwarp();
+        const int col = lane & 15;
+#pragma unroll 4
+        for (int r = lane >> 4; r < 32; r += 2) {
+            float x;
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(buf + (uint32_t)(r * EPI_ROWS_PITCH + col) * 4u) : "memory");
+            if (r < rows && 16 * h + col < cols) out[(long long)r * ld + 16 * h + col] = x;
+        }
+    }
+}
+
+// Tile order: the tiles of eight rows of tiles together, so that the CTAs at work share both operands' tiles in L2.
+__device__ __forceinline__ void d8_tile(const D8Params& p, int tile, int& c, int& mt, int& nt) {
+    const int per = p.m_tiles * p.n_tiles;
+    c = tile / per;
+    const int r = tile - c * per, band = 8 * p.n_tiles, b = r / band, in = r - b * band;
+    const int height = min(8, p.m_tiles - b * 8);
+    mt = b * 8 + in % height;
+    nt = in / height;
+}
+
+// SWAP: operand A is the filter, so that tile rows run along the output's fast axis.
+template <int BN, bool SWAP>
+__global__ void __launch_bounds__(D8_THREADS, 1)
+dense8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const D8Params p, int* status) {
+    using C = D8Config<BN>;
+    extern __shared__ uint8_t smem_raw[];
+    const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+    uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* sf = base + C::STAGES * C::STAGE;
+    uint8_t* staged = sf + D8_SF_STAGES * D8_SF_BYTES;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(staged + (BN >= 128 ? C::STAGED : 0));
+    const uint32_t base_addr = smem_u32(base), sf_addr = smem_u32(sf);
+    const uint32_t full = smem_u32(bars), empty = full + 8 * C::STAGES, sf_full = empty + 8 * C::STAGES, sf_empty = sf_full + 8 * D8_SF_STAGES;
+    const uint32_t acc_full = sf_empty + 8 * D8_SF_STAGES, acc_empty = acc_full + 8 * C::ACC, slot = acc_empty + 8 * C::ACC;
+
+    if (t == 0) {
+        for (int s = 0; s < C::STAGES; ++s) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 1); }
+        for (int s = 0; s < D8_SF_STAGES; ++s) { mbar_init(sf_full + 8 * s, 1); mbar_init(sf_empty + 8 * s, 1); }
+        for (int s = 0; s < C::ACC; ++s) { mbar_init(acc_full + 8 * s, 1); mbar_init(acc_empty + 8 * s, D8_EPI_WARPS); }
+        fence_barrier_init();
+    }
+    if (warp == 1) tmem_alloc(slot, 512);
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    uint32_t tmem;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(slot));
+    chain_wait();
+    chain_next();
+
+    const int split = p.splits > 1 ? (int)cluster_ctarank() : 0;
+    const int first = blockIdx.x / p.splits, stride = gridDim.x / p.splits;
+    // this CTA's groups of the reduction (numbered over all its components)
+    const int all_groups = p.comps * p.groups;
+    const int g_begin = (int)((long long)all_groups * split / p.splits), g_end = (int)((long long)all_groups * (split + 1) / p.splits);
+
+    if (warp == 0) {
+        int s = 0;
+        uint32_t par = 1;
+        bool ok = true;
+        for (int tile = first; tile < p.tiles && ok; tile += stride) {
+            int c, mt, nt;
+            d8_tile(p, tile, c, mt, nt);
+            for (int g = g_begin; g < g_end && ok; ++g) {
+                const int j = g / p.groups, k0 = (g - j * p.groups) * 4, k1 = min(k0 + 4, p.chunks);
+                int first_comp, second_comp;
+                bool neg;
+                d8_term(p, c, j, first_comp, second_comp, neg);
+                const int ca = SWAP ? second_comp : first_comp, cb = SWAP ? first_comp : second_comp;
+                for (int k = k0; k < k1; ++k) {
+                    ok = warp_wait_bounded(empty + 8 * s, par, status, ST_D8_PRODUCER);
+                    if (!ok) break;
+                    if (elect_one()) {
+                        const uint32_t a = base_addr + s * C::STAGE, b = a + D8_A_BYTES, bar = full + 8 * s;
+                        mbar_arrive_expect_tx(bar, D8_A_BYTES + BN * D8_BK);
+                        if (p.a_mn) tma_load_3d(a, &map_a, mt * D8_BM, k * D8_BK, ca, bar);
+                        else tma_load_3d(a, &map_a, k * D8_BK, mt * D8_BM, ca, bar);
+                        if (BN >= 128 && p.b_mn) {
+#pragma unroll
+                            for (int h = 0; h < BN / 128; ++h) tma_load_3d(b + h * 128 * D8_BK, &map_b, nt * BN + h * 128, k * D8_BK, cb, bar);
+                        } else tma_load_3d(b, &map_b, k * D8_BK, nt * BN, cb, bar);
+                    }
+                    __syncwarp();
+                    if (++s == C::STAGES) { s = 0; par ^= 1u; }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        const bool elected = elect_one();              // one lane issues and commits throughout
+        int s = 0, q = 0, acc = 0;
+        uint32_t par = 0, sf_par = 0, acc_par = 1;
+        bool ok = true;
+        const bool a_mn = p.a_mn, b_mn = BN >= 128 && p.b_mn;
+        const uint32_t a_step = a_mn ? 32 * 128 / 16 : 32 / 16, b_step = b_mn ? 32 * 128 / 16 : 32 / 16;
+        const uint32_t sfa = tmem + C::SF_COL, sfb = sfa + 4;
+        for (int tile = first; tile < p.tiles && ok; tile += stride) {
+            int c, mt, nt;
+            d8_tile(p, tile, c, mt, nt);
+            ok = warp_wait_bounded(acc_empty + 8 * acc, acc_par, status, ST_D8_MMA);
+            if (!ok) break;
+            tc_fence_after_sync();
+            const uint32_t d = tmem + acc * C::ACC_COLS;
+            uint32_t accumulate = 0;
+            for (int g = g_begin; g < g_end && ok; ++g) {
+                const int j = g / p.groups, k0 = (g - j * p.groups) * 4, k1 = min(k0 + 4, p.chunks);
+                int first_comp, second_comp;
+                bool neg;
+                d8_term(p, c, j, first_comp, second_comp, neg);
+                const uint32_t idesc = d8_idesc(D8_BM, BN, a_mn, b_mn, neg);
+                ok = warp_wait_bounded(sf_full + 8 * q, sf_par, status, ST_D8_MMA);
+                if (!ok) break;
+                tc_fence_after_sync();
+                if (elected) {
+                    const uint32_t src = sf_addr + q * D8_SF_BYTES;
+                    copy_scales(sfa, src);
+                    copy_scales(sfb, src + 512);
+                    if (BN > 128) copy_scales(sfb + 4, src + 1024);
+                }
+                __syncwarp();
+                for (int k = k0; k < k1; ++k) {
+                    ok = warp_wait_bounded(full + 8 * s, par, status, ST_D8_MMA);
+                    if (!ok) break;
+                    tc_fence_after_sync();
+                    if (elected) {
+                        const uint32_t a = base_addr + s * C::STAGE, b = a + D8_A_BYTES;
+                        const uint64_t da = make_desc_kmajor(a), db = b_mn ? make_desc_mnmajor(b, 128 * D8_BK) : make_desc_kmajor(b);
+                        const uint32_t id = idesc | ((uint32_t)(k & 3) << 4) | ((uint32_t)(k & 3) << 29);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            mma_mxf8(d, (uint32_t)da + i * a_step, (uint32_t)(da >> 32), (uint32_t)db + i * b_step, (uint32_t)(db >> 32), id, sfa, sfb, accumulate);
+                            accumulate = 1;
+                        }
+                        mma_commit(empty + 8 * s);
+                    }
+                    accumulate = 1;
+                    __syncwarp();
+                    if (++s == C::STAGES) { s = 0; par ^= 1u; }
+                }
+                if (!ok) break;
+                if (elected) mma_commit(sf_empty + 8 * q);
+                __syncwarp();
+                if (++q == D8_SF_STAGES) { q = 0; sf_par ^= 1u; }
+            }
+            if (!ok) break;
+            if (elected) mma_commit(acc_full + 8 * acc);
+            __syncwarp();
+            if (++acc == C::ACC) { acc = 0; acc_par ^= 1u; }
+        }
+    } else if (warp == 2) {
+        int q = 0;
+        uint32_t par = 1;
+        bool ok = true;
+        // the words of rows row0 + lane + 32 i: what lane puts at byte 16 * lane of a set of 128 rows
+        auto gather = [&](bool blocks, const uint8_t* scales, int bk, int bm, int bc, int comp, int group, int row0, int extent) {
+            uint32_t w[4];
+            if (blocks) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    // (blocks of 128 rows: a set of 128 rows that starts on a multiple of 128 lies in one)
+                    uint32_t word = 0;
+                    if (i == 0) {
+                        const uint8_t* src = scales + (size_t)comp * bc + (size_t)(row0 / 128) * bm;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            word |= (uint32_t)(row0 < extent && group * 4 + e < p.chunks ? *reinterpret_cast<const volatile uint8_t*>(src + (size_t)(group * 4 + e) * bk) : 127) << (8 * e);
+                        w[0] = word;
+                    } else w[i] = w[0];
+                }
+            } else {
+                const uint32_t* src = reinterpret_cast<const uint32_t*>(scales) + ((size_t)comp * p.groups + group) * extent + row0 + lane;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = row0 + lane + 32 * i < extent ? ld_chained(src + 32 * i) : 0x7f7f7f7fu;
+            }
+            return make_uint4(w[0], w[1], w[2], w[3]);
+        };
+        for (int tile = first; tile < p.tiles && ok; tile += stride) {
+            int c, mt, nt;
+            d8_tile(p, tile, c, mt, nt);
+            for (int g = g_begin; g < g_end && ok; ++g) {
+                const int j = g / p.groups, group = g - j * p.groups;
+                int first_comp, second_comp;
+                bool neg;
+                d8_term(p, c, j, first_comp, second_comp, neg);
+                const int ca = SWAP ? second_comp : first_comp, cb = SWAP ? first_comp : second_comp;
+                const uint4 wa = gather(p.a_blocks, p.a_scales, p.a_bk, p.a_bm, p.a_bc, ca, group, mt * D8_BM, p.m);
+                uint4 wb[2];
+                wb[0] = gather(p.b_blocks, p.b_scales, p.b_bk, p.b_bm, p.b_bc, cb, group, nt * BN, p.n);
+                if (BN > 128) wb[1] = gather(p.b_blocks, p.b_scales, p.b_bk, p.b_bm, p.b_bc, cb, group, nt * BN + 128, p.n);
+                ok = warp_wait_bounded(sf_empty + 8 * q, par, status, ST_D8_SCALES);
+                if (!ok) break;
+                const uint32_t dst = sf_addr + q * D8_SF_BYTES + lane * 16;
+                st_shared_v4(dst, wa.x, wa.y, wa.z, wa.w);
+                st_shared_v4(dst + 512, wb[0].x, wb[0].y, wb[0].z, wb[0].w);
+                if (BN > 128) st_shared_v4(dst + 1024, wb[1].x, wb[1].y, wb[1].z, wb[1].w);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (elect_one()) mbar_arrive(sf_full + 8 * q);
+                __syncwarp();
+                if (++q == D8_SF_STAGES) { q = 0; par ^= 1u; }
+            }
+        }
+    } else if (warp >= 4) {
+        const int quarter = warp & 3, half = (warp - 4) >> 2;
+        constexpr int COLS = BN < 64 ? 32 : BN / 2;               // columns per warp; with a narrow tile the second four warps have none
+        constexpr int BLOCKS = COLS / 32;
+        const bool idle = BN < 64 && half > 0;
+        const int col0 = half * COLS;
+        const uint32_t buf = smem_u32(staged) + (warp - 4) * EPI_ROWS_BYTES;
+        const int fast = SWAP ? p.m : p.n;
+        int acc = 0;
+        uint32_t par = 0;
+        bool ok = true;
+        for (int tile = first; tile < p.tiles && ok; tile += stride) {
+            int c, mt, nt;
+            d8_tile(p, tile, c, mt, nt);
+            const int before = read_status(status);
+            ok = warp_may_store(warp_wait_bounded(acc_full + 8 * acc, par, status, ST_D8_EPILOGUE), before);
+            if (!ok) break;
+            tc_fence_after_sync();
+            const uint32_t src = tmem + ((uint32_t)(quarter * 32) << 16) + acc * C::ACC_COLS + col0;
+            uint32_t v[BLOCKS][32];
+            if (!idle) {
+#pragma unroll
+                for (int b = 0; b < BLOCKS; ++b) tmem_ld_32x32b_x32(src + 32 * b, v[b]);
+                tmem_ld_wait();
+#pragma unroll
+                for (int b = 0; b < BLOCKS; ++b) tmem_regs_ready(v[b]);
+            }
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acc_empty + 8 * acc);
+            if (++acc == C::ACC) { acc = 0; par ^= 1u; }
+            if (idle) continue;
+            const int row = quarter * 32 + lane, m = mt * D8_BM + row, n0 = nt * BN + col0;
+            if (p.splits > 1) {
+                // partial sums to shared memory (the ring: every MMA has read it), the fast axis of the output contiguous
+                float* part = reinterpret_cast<float*>(base);
+#pragma unroll
+                for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        const int n = col0 + 32 * b + e;
+                        if (n < BN) part[SWAP ? n * D8_BM + row : row * (BN + 1) + n] = __uint_as_float(v[b][e]);
+                    }
+                continue;
+            }
+            const long long comp0 = (long long)c * p.out_comp;
+            if (SWAP) {
+                const float add = p.bias && m < p.m ? ld_typed(p.bias, p.dtype, (size_t)c * fast + m) : 0.f;
+#pragma unroll
+                for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        const int n = n0 + 32 * b + e;
+                        if (m < p.m && n < p.n && 32 * b + e < BN - col0) st_typed(p.out, p.dtype, comp0 + (long long)n * p.out_ld + m, __uint_as_float(v[b][e]) + add);
+                    }
+            } else {
+#pragma unroll
+                for (int b = 0; b < BLOCKS; ++b) {
+                    const int n = n0 + 32 * b;
+                    if (n >= p.n) break;
+                    if (p.bias) {
+                        const float add = n + lane < p.n ? ld_typed(p.bias, p.dtype, (size_t)c * fast + n + lane) : 0.f;
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) v[b][e] = __float_as_uint(__uint_as_float(v[b][e]) + __shfl_sync(0xffffffffu, add, e));
+                    }
+                    // vectors of 16 bytes where every row's piece of the tile starts on them
+                    const bool whole = n + 32 <= p.n;
+                    if (p.dtype == PCB_F32) {
+                        float* out = static_cast<float*>(p.out) + comp0 + (long long)m * p.out_ld + n;
+                        if (whole && p.out_ld % 4 == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.out_comp % 4 == 0) {
+                            if (m < p.m)
+#pragma unroll
+                                for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(out + e) = make_uint4(v[b][e], v[b][e + 1], v[b][e + 2], v[b][e + 3]);
+                        } else store_floats(buf, v[b], static_cast<float*>(p.out) + comp0 + (long long)(mt * D8_BM + quarter * 32) * p.out_ld + n, p.m - (mt * D8_BM + quarter * 32),
+                                            p.n - n, p.out_ld, lane);
+                    } else {
+                        uint32_t packed[16];
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) packed[e] = pack_16(__uint_as_float(v[b][2 * e]), __uint_as_float(v[b][2 * e + 1]), p.dtype);
+                        uint16_t* out = static_cast<uint16_t*>(p.out) + comp0 + (long long)m * p.out_ld + n;
+                        if (whole && p.out_ld % 8 == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.out_comp % 8 == 0) {
+                            if (m < p.m)
+#pragma unroll
+                                for (int e = 0; e < 16; e += 4) *reinterpret_cast<uint4*>(out + 2 * e) = make_uint4(packed[e], packed[e + 1], packed[e + 2], packed[e + 3]);
+                        } else store_rows<1>(buf, packed, static_cast<uint16_t*>(p.out) + comp0 + (long long)(mt * D8_BM + quarter * 32) * p.out_ld, m < p.m ? lane * p.out_ld : -1,
+                                             n + lane < p.n ? n + lane : -1, lane);
+                    }
+                }
+            }
+        }
+    }
+    if (p.splits > 1) {
+        // one tile per cluster: every CTA adds its share of the tile's elements, in the order of the ranks
+        __syncthreads();
+        cluster_sync_all();
+        int c, mt, nt;
+        d8_tile(p, first, c, mt, nt);
+        const int ms = min(D8_BM, p.m - mt * D8_BM), ns = min(BN, p.n - nt * BN);
+        const int fast_n = SWAP ? ms : ns, slow_n = SWAP ? ns : ms, fast0 = SWAP ? mt * D8_BM : nt * BN, slow0 = SWAP ? nt * BN : mt * D8_BM;
+        const int pitch = SWAP ? D8_BM : BN + 1;
+        if (read_status(status) == 0) {
+            for (int e = split * D8_THREADS + t; e < slow_n * fast_n; e += p.splits * D8_THREADS) {
+                const int slow = e / fast_n, fast = e - slow * fast_n;
+                const uint32_t local = base_addr + (uint32_t)(slow * pitch + fast) * 4u;
+                float sum = 0.f;
+                for (int r = 0; r < p.splits; ++r) {
+                    float x;
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(map_to_cta(local, r)) : "memory");
+                    sum += x;
+                }
+                if (p.bias) sum += ld_typed(p.bias, p.dtype, (size_t)c * (SWAP ? p.m : p.n) + fast0 + fast);
+                st_typed(p.out, p.dtype, (long long)c * p.out_comp + (long long)(slow0 + slow) * p.out_ld + fast0 + fast, sum);
+            }
+        }
+        cluster_sync_all();                 // nobody leaves while its partial sums are read
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after_sync();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+int operand_map(CUtensorMap* map, const Q8Operand& o, int extent, int k, int comps, int box_rows, const char* what) {
+    const int inner = o.mn_major ? extent : k, outer = o.mn_major ? k : extent;
+    const cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)outer, (cuuint64_t)comps};
+    const cuuint64_t strides[2] = {(cuuint64_t)o.pitch, (cuuint64_t)o.pitch * outer};
+    const cuuint32_t box[3] = {128, (cuuint32_t)(o.mn_major ? 128 : box_rows), 1};
+    return make_tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, o.values, 3, dims, strides, box, nullptr, CU_TENSOR_MAP_SWIZZLE_128B, what);
+}
+
+template <int BN, bool SWAP>
+int launch(const Geom& g, const Q8Product& q, int splits, cudaStream_t stream) {
+    using C = D8Config<BN>;
+    D8Params p = {};
+    p.pass = q.pass; p.ga = g.ga; p.comps = g.nc; p.neg = g.neg;
+    p.m = q.m; p.n = q.n; p.k = q.k;
+    p.chunks = q8_blocks(q.k); p.groups = q8_groups(q.k);
+    p.m_tiles = q8_blocks(q.m); p.n_tiles = (q.n + BN - 1) / BN; p.tiles = p.m_tiles * p.n_tiles * g.nc;
+    p.splits = splits;
+    p.a_mn = q.a.mn_major; p.b_mn = q.b.mn_major;
+    p.a_blocks = q.a.block_scales; p.b_blocks = q.b.block_scales;
+    p.a_scales = static_cast<const uint8_t*>(q.a.scales); p.b_scales = static_cast<const uint8_t*>(q.b.scales);
+    p.a_bk = q.a.bytes_k; p.a_bm = q.a.bytes_mn; p.b_bk = q.b.bytes_k; p.b_bm = q.b.bytes_mn;
+    p.a_bc = q8_blocks(q.m) * q8_blocks(q.k); p.b_bc = q8_blocks(q.n) * q8_blocks(q.k);
+    p.dtype = q.dtype; p.out = q.out; p.bias = q.bias;
+    p.out_ld = SWAP ? q.m : q.n;
+    p.out_comp = (long long)q.m * q.n;
+    CUtensorMap ma, mb;
+    int rc = operand_map(&ma, q.a, q.m, q.k, g.nc, D8_BM, "8-bit operand A");
+    if (rc == PCB_OK) rc = operand_map(&mb, q.b, q.n, q.k, g.nc, BN, "8-bit operand B");
+    if (rc != PCB_OK) return rc;
+    const size_t smem = C::SMEM > ONE_CTA_SMEM ? C::SMEM : ONE_CTA_SMEM;
+    PCB_CUDA_TRY(cudaFuncSetAttribute(dense8_kernel<BN, SWAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    const int grid = splits > 1 ? p.tiles * splits : (p.tiles < sm_count() ? p.tiles : sm_count());
+    PCB_CUDA_TRY(launch_clusters(splits, true, dense8_kernel<BN, SWAP>, grid, D8_THREADS, smem, stream, ma, mb, p, q.status));
+    return PCB_OK;
+}
+
+}  // namespace
+
+bool q8_swapped(int tokens) { return tokens <= 128; }
+
+int q8_product(const Geom& g, const Q8Product& q, cudaStream_t stream) {
+    const int m_tiles = q8_blocks(q.m), groups = g.nc * q8_groups(q.k);
+    // CTAs that share a tile: as many as the SMs and the groups of the reduction allow, up to a portable cluster
+    auto splits_for = [&](int bn) {
+        const long long tiles = (long long)m_tiles * ((q.n + bn - 1) / bn) * g.nc;
+        int s = 1;
+        while (s < 8 && tiles * s * 2 <= sm_count() && s * 2 <= groups) s *= 2;
+        return s;
+    };
+    if (q.swapped) {
+        if (q.n <= 16) return launch<16, true>(g, q, splits_for(16), stream);
+        if (q.n <= 64) return launch<64, true>(g, q, splits_for(64), stream);
+        return launch<128, true>(g, q, splits_for(128), stream);
+    }
+    const long long wide = (long long)m_tiles * ((q.n + 255) / 256) * g.nc;
+    if (wide >= 2LL * sm_count()) return launch<256, false>(g, q, 1, stream);
+    return launch<128, false>(g, q, splits_for(128), stream);
+}
+
+}  // namespace pcb
