@@ -241,6 +241,53 @@ int pcb_check_device_status(const void* workspace, size_t workspace_bytes, void*
 int pcb_selftest_wait_expiry(const pcb_conv2d_desc* desc, const void* x, const void* w, void* y, void* workspace,
                              size_t workspace_bytes, long long limit_clocks, void* stream);
 
+/* ---- The norms before and after a residual block, with its gate and residual scale (no counterpart in the reference) -----------
+ * A sample is all its components' features (D * features values, the components stacked on the leading axis as everywhere):
+ *   n(v) = v / sqrt(mean(v^2) + epsilon)
+ *   y = x + residual_scale * gate * (n(branch) * post)          h = n(y) * pre
+ * x, branch, y, h and their gradients are [D * batch, features], the gate [D * gate_rows, features] with gate_rows dividing batch: row i of a
+ * component applies to samples i * batch / gate_rows and on (gate_rows 0: no gate, 1: one for all samples, batch: one for each value). post and pre
+ * are fp32 [features], shared by the components; null means ones. Without branch (null, with gate and post) only h is computed, of x, and y may be
+ * null; without h (null, with pre) only y. `stats` is fp32 [2][batch], 1 / sqrt(...) of branch and of y, and may be null where no backward call
+ * follows. y and h are rounded once; h is computed from y before its rounding.
+ * Backward: dy is the gradient of y from elsewhere (null: none), dh the gradient of h (null: no norm behind the block; one of them is given).
+ * dx, the gradient of x, is written always, dbranch where there is a branch, dgate, dpost and dpre where not null. Tensors of fewer than 2^31
+ * elements; results must not share memory with operands. Sums over samples are fp32, in an order that depends on the sizes alone. */
+typedef struct pcb_norm_desc {
+    int32_t dtype;            /* pcb_dtype of x, branch, gate, y, h and their gradients */
+    int32_t algebra;          /* pcb_algebra */
+    int32_t batch, features;
+    int32_t gate_rows;
+    float residual_scale, epsilon;
+} pcb_norm_desc;
+int pcb_residual_norm_fwd(const pcb_norm_desc* desc, const void* x, const void* branch, const void* gate, const float* post, const float* pre,
+                          void* y, void* h, float* stats, void* stream);
+size_t pcb_residual_norm_bwd_workspace_size(const pcb_norm_desc* desc);
+int pcb_residual_norm_bwd(const pcb_norm_desc* desc, const void* y, const void* branch, const void* gate, const float* post, const float* pre,
+                          const float* stats, const void* dy, const void* dh, void* dx, void* dbranch, void* dgate, float* dpost, float* dpre,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- Distillation from a teacher's largest logits, mixed with the labels' cross-entropy (no counterpart in the reference) -----------
+ * `logits` is what a dense layer of `units` output features writes, [D * batch, units]: a sample has D * units classes, class = component * units + unit.
+ *   p = softmax(teacher / T) over the named classes,  q = softmax(logits / T) over all
+ *   loss = (1 - alpha) * cross_entropy(logits, label) + alpha * T^2 * sum_i p_i (log p_i - log q_i)
+ * `teacher` and `index` are [batch, entries]: logits (of the type of `logits`) and their classes, in any order; an entry whose class is outside
+ * [0, D * units) is left out, a class named twice counts twice. `labels` is [batch]; one outside the classes leaves the first term out. A sample without an entry
+ * has no second term, one whose logits are all -infinity counts for nothing. labels may be null, and so may teacher and index with entries 0; their term is then
+ * left out. `loss` is fp32 [batch]. `stats` (fp32 [3][batch], may be null) is kept for the backward call: maximum, sum of
+ * exp(z - max), sum of exp((z - max) / T), infinity in place of a sum that the gradient has no term of.
+ * Backward: dlogits = grad_loss[sample] * d loss / d logits; must not share memory with the logits. Up to 4096 entries, D * units < 2^31. */
+typedef struct pcb_distill_desc {
+    int32_t dtype;            /* pcb_dtype of logits, teacher, dlogits */
+    int32_t algebra;          /* pcb_algebra: components of the layer that made the logits */
+    int32_t batch, units, entries;
+    float alpha, temperature;
+} pcb_distill_desc;
+int pcb_distill_fwd(const pcb_distill_desc* desc, const void* logits, const long long* labels, const void* teacher, const long long* index,
+                    float* loss, float* stats, void* stream);
+int pcb_distill_bwd(const pcb_distill_desc* desc, const void* logits, const long long* labels, const void* teacher, const long long* index,
+                    const float* stats, const float* grad_loss, void* dlogits, void* stream);
+
 /* ---- Auxiliary kernels of the QResNet-18 training harness (not part of the drop-in path) ---------------------
  * The reference has no normalisation layer (its TensorFlow plugin leaves batch-norm to TensorFlow), so these two
  * have no counterpart there. Batch-norm with one mean / variance per channel over a stacked tensor

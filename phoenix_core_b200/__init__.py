@@ -9,6 +9,8 @@ from .descriptors import (Algebra, Conv2DBwdDescriptor, Conv2DFwdDescriptor, Dat
                           DenseFwdDescriptor, FilterLayout, Padding, compute_windowed_output_size_and_padding)
 from .context import Context, ConvFp16ComputePolicy
 from .dense8 import Filter8, dense8Bwd, dense8Fwd, quantizeFilter8
+from .distill import DistillDescriptor, distillBwd, distillFwd
+from .residual_norm import ResidualNormDescriptor, residualNormBwd, residualNormFwd
 from .ops import KeptInput, conv2DBwd, conv2DFwd, denseBwd, denseFwd, getSmMargin, setSmMargin
 
 __all__ = [
@@ -16,4 +18,6 @@ __all__ = [
     "DenseFwdDescriptor", "DenseBwdDescriptor", "compute_windowed_output_size_and_padding", "Context",
     "ConvFp16ComputePolicy", "conv2DFwd", "conv2DBwd", "denseFwd", "denseBwd", "setSmMargin", "getSmMargin", "KeptInput",
     "Filter8", "quantizeFilter8", "dense8Fwd", "dense8Bwd",
+    "ResidualNormDescriptor", "residualNormFwd", "residualNormBwd",
+    "DistillDescriptor", "distillFwd", "distillBwd",
 ]

@@ -38,9 +38,21 @@ class DenseDesc(ctypes.Structure):
         "engine", "algebra")]
 
 
+class NormDesc(ctypes.Structure):
+    """pcb_norm_desc"""
+    _fields_ = [(k, ctypes.c_int32) for k in ("dtype", "algebra", "batch", "features", "gate_rows")] + [
+        (k, ctypes.c_float) for k in ("residual_scale", "epsilon")]
+
+
+class DistillDesc(ctypes.Structure):
+    """pcb_distill_desc"""
+    _fields_ = [(k, ctypes.c_int32) for k in ("dtype", "algebra", "batch", "units", "entries")] + [
+        (k, ctypes.c_float) for k in ("alpha", "temperature")]
+
+
 # name -> (restype, argtypes); this is every symbol include/phoenix_core_b200.h declares
 _vp, _sz, _i = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int
-_cd, _dd = ctypes.POINTER(ConvDesc), ctypes.POINTER(DenseDesc)
+_cd, _dd, _nd, _td = (ctypes.POINTER(t) for t in (ConvDesc, DenseDesc, NormDesc, DistillDesc))
 SYMBOLS = {
     "pcb_version": (ctypes.c_char_p, []),
     "pcb_status_string": (ctypes.c_char_p, [_i]),
@@ -66,6 +78,11 @@ SYMBOLS = {
     "pcb_qdense8_bwd_workspace_size": (_sz, [_dd]),
     "pcb_qdense8_fwd": (_i, [_dd, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "pcb_qdense8_bwd": (_i, [_dd, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "pcb_residual_norm_fwd": (_i, [_nd] + [_vp] * 9),
+    "pcb_residual_norm_bwd_workspace_size": (_sz, [_nd]),
+    "pcb_residual_norm_bwd": (_i, [_nd] + [_vp] * 14 + [_sz, _vp]),
+    "pcb_distill_fwd": (_i, [_td] + [_vp] * 7),
+    "pcb_distill_bwd": (_i, [_td] + [_vp] * 8),
     "pcb_qconv2d_engine_for": (_i, [_cd, _i]),
     "pcb_qdense_engine_for": (_i, [_dd, _i]),
     "pcb_check_device_status": (_i, [_vp, _sz, _vp]),

@@ -1,0 +1,449 @@
+// Distillation from a teacher's largest logits, mixed with the cross-entropy of the labels.
+//
+// A sample has V = D * U logits z (U units of each of D components, class = component * U + unit), a label c, and for k classes i the teacher's logits t_i.
+//   p = softmax(t / T) over the k classes, q = softmax(z / T) over all of them
+//   loss = (1 - a) * (log sum_j exp z_j - z_c) + a * T^2 * sum_i p_i (log p_i - log q_i)
+//   dz_j = g * ((1 - a) * (softmax(z)_j - [j = c]) + a * T * (q_j - p_j))
+// Both sums over the vocabulary are taken in one pass with a running maximum; the gradient reads the logits once more and writes
+// them once. With T = 2 the exponentials of T = 1 are the squares of the others: one exponential per logit, which keeps the pass bound by memory
+// (16 exponentials per clock and SM are two thirds of what a pass over 16-bit logits takes at full bandwidth).
+// Few rows are cut over the CTAs of a cluster, whose maxima and sums are joined through distributed shared memory.
+#include "common.cuh"
+#include "tc_common.cuh"
+
+namespace pcb {
+namespace {
+
+using namespace tc;
+
+constexpr int DI_MAX_ENTRIES = 4096;
+constexpr float LOG2E = 1.4426950408889634f;
+
+enum { DI_HARD = 0, DI_SOFT = 1, DI_SAME = 2, DI_SQUARE = 3, DI_BOTH = 4 };   // exponentials: at 1, at T, T == 1, T == 2, both
+
+struct DIParams {
+    int comps, n, units, entries, splits;
+    float alpha, temp, inv_temp;
+    const void *logits, *teacher;
+    const long long *labels, *index;
+    float *loss, *stats;                 // stats [3][n]: maximum, sum at 1, sum at T (infinity: no entry of the teacher's)
+    const float* grad;
+    void* dlogits;
+};
+
+template <typename T> struct Bits;       // one value, and 16 bytes of them
+template <> struct Bits<float> {
+    static constexpr int VEC = 4;
+    static __device__ __forceinline__ float one(const float* p) { return ld_chained(p); }
+    static __device__ __forceinline__ void unpack(const uint4& r, float* v) { v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y); v[2] = __uint_as_float(r.z); v[3] = __uint_as_float(r.w); }
+    static __device__ __forceinline__ uint4 pack(const float* v) { return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])); }
+    static __device__ __forceinline__ void put(float* p, float v) { *p = v; }
+};
+template <> struct Bits<__half> {
+    static constexpr int VEC = 8;
+    static __device__ __forceinline__ float one(const __half* p) { return __half2float(__ushort_as_half(ld_chained(reinterpret_cast<const uint16_t*>(p)))); }
+    static __device__ __forceinline__ void unpack(const uint4& r, float* v) {
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i])); v[2 * i] = f.x; v[2 * i + 1] = f.y; }
+    }
+    static __device__ __forceinline__ uint4 pack(const float* v) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]); w[i] = *reinterpret_cast<const uint32_t*>(&h); }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    static __device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
+};
+template <> struct Bits<__nv_bfloat16> {
+    static constexpr int VEC = 8;
+    static __device__ __forceinline__ float one(const __nv_bfloat16* p) { return __uint_as_float((uint32_t)ld_chained(reinterpret_cast<const uint16_t*>(p)) << 16); }
+    static __device__ __forceinline__ void unpack(const uint4& r, float* v) {
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+    }
+    static __device__ __forceinline__ uint4 pack(const float* v) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]); w[i] = *reinterpret_cast<const uint32_t*>(&h); }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    static __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+};
+
+__device__ __forceinline__ float ex2(float x) { return exp2f(x); }
+// exponentials of d = z - max <= 0 at temperature 1 and T
+template <int KIND>
+__device__ __forceinline__ void exps(float d, float c_temp, float& e1, float& et) {
+    if (KIND == DI_HARD) { e1 = ex2(d * LOG2E); et = 0.f; }
+    else if (KIND == DI_SOFT) { et = ex2(d * c_temp); e1 = 0.f; }
+    else if (KIND == DI_SAME) { e1 = et = ex2(d * LOG2E); }
+    else if (KIND == DI_SQUARE) { et = ex2(d * c_temp); e1 = et * et; }
+    else { e1 = ex2(d * LOG2E); et = ex2(d * c_temp); }
+}
+
+struct Sums { float m, s1, st; };
+template <int KIND>
+__device__ __forceinline__ void raise(Sums& a, float m, float c_temp) {          // the sums relative to a larger maximum
+    float f1, ft;
+    exps<KIND>(a.m - m, c_temp, f1, ft);
+    a.s1 *= f1;
+    a.st *= ft;
+    a.m = m;
+}
+template <int KIND>
+__device__ __forceinline__ void join(Sums& a, Sums b, float c_temp) {
+    if (b.m > a.m) { const Sums s = a; a = b; b = s; }
+    if (b.m == -INFINITY) { a.s1 += b.s1; a.st += b.st; return; }                 // nothing there (or not a number)
+    raise<KIND>(b, a.m, c_temp);
+    a.s1 += b.s1;
+    a.st += b.st;
+}
+template <int KIND, int N>
+__device__ __forceinline__ void add(Sums& a, const float (&v)[N], float c_temp) {
+    float top = v[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) top = fmaxf(top, v[i]);
+    if (top > a.m) raise<KIND>(a, top, c_temp);
+    const float m = a.m == -INFINITY ? 0.f : a.m;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        float e1, et;
+        exps<KIND>(v[i] - m, c_temp, e1, et);
+        a.s1 += e1;
+        a.st += et;
+    }
+}
+
+// Calls vec(pointer to 16 aligned bytes of the row, first class) and one(pointer, class) over classes [lo, hi) of a sample, `threads` threads together.
+template <typename T, bool VECTORS, int UNROLL, typename VecFn, typename OneFn>
+__device__ __forceinline__ void over_classes(const T* logits, const DIParams& p, int row, int lo, int hi, int tid, int threads, VecFn vec, OneFn one) {
+    constexpr int VEC = Bits<T>::VEC;
+    for (int c = lo / p.units; c * p.units < hi; ++c) {
+        const int a = max(lo, c * p.units), b = min(hi, (c + 1) * p.units);
+        const T* first = logits + ((size_t)c * p.n + row) * p.units + (a - c * p.units);
+        if (!VECTORS) {
+            for (int i = a + tid; i < b; i += threads) one(first + (i - a), i);
+            continue;
+        }
+        const int head = min(b - a, (int)((16 - (reinterpret_cast<uintptr_t>(first) & 15)) & 15) / (int)sizeof(T)), body = (b - a - head) / VEC;
+        for (int i = tid; i < head; i += threads) one(first + i, a + i);
+        const T* start = first + head;
+        int v = tid;
+        for (; v + (UNROLL - 1) * threads < body; v += UNROLL * threads) {
+            uint4 raw[UNROLL];
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) raw[u] = ld_chained(reinterpret_cast<const uint4*>(start) + v + u * threads);
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) vec(raw[u], a + head + (v + u * threads) * VEC, start + (size_t)(v + u * threads) * VEC);
+        }
+        for (; v < body; v += threads) vec(ld_chained(reinterpret_cast<const uint4*>(start) + v), a + head + v * VEC, start + (size_t)v * VEC);
+        for (int i = a + head + body * VEC + tid; i < b; i += threads) one(first + (i - a), i);
+    }
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ float logit(const DIParams& p, int row, int cls) {
+    const int c = cls / p.units;
+    return Bits<T>::one(static_cast<const T*>(p.logits) + ((size_t)c * p.n + row) * p.units + (cls - c * p.units));
+}
+// The class of the teacher's entry i of a row, or -1 where it names none, and its logit over T.
+template <typename T>
+__device__ __forceinline__ int entry(const DIParams& p, int row, int i, float& t) {
+    const long long at = (long long)row * p.entries + i;
+    const uint2 w = ld_chained(reinterpret_cast<const uint2*>(p.index + at));
+    const long long cls = (long long)(((unsigned long long)w.y << 32) | w.x);
+    if (cls < 0 || cls >= (long long)p.comps * p.units) { t = -INFINITY; return -1; }
+    t = Bits<T>::one(static_cast<const T*>(p.teacher) + at) * p.inv_temp;
+    return (int)cls;
+}
+__device__ __forceinline__ int label_of(const DIParams& p, int row) {
+    if (!p.labels) return -1;
+    const uint2 w = ld_chained(reinterpret_cast<const uint2*>(p.labels + row));
+    const long long cls = (long long)(((unsigned long long)w.y << 32) | w.x);
+    return cls < 0 || cls >= (long long)p.comps * p.units ? -1 : (int)cls;
+}
+
+template <typename T, bool VECTORS, int KIND, int THREADS>
+__global__ void __launch_bounds__(THREADS) distill_fwd_kernel(const DIParams p) {
+    constexpr int WARPS = THREADS / 32;
+    __shared__ Sums words[WARPS];
+    __shared__ Sums whole;
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const int row = blockIdx.x / p.splits, split = blockIdx.x - row * p.splits;
+    const int classes = p.comps * p.units;
+    const int lo = (int)((long long)classes * split / p.splits), hi = (int)((long long)classes * (split + 1) / p.splits);
+    const float c_temp = LOG2E * p.inv_temp;
+    chain_wait();
+    chain_next();
+    Sums a = {-INFINITY, 0.f, 0.f};
+    over_classes<T, VECTORS, 4>(static_cast<const T*>(p.logits), p, row, lo, hi, t, THREADS,
+        [&](const uint4& raw, int, const T*) {
+            float v[Bits<T>::VEC];
+            Bits<T>::unpack(raw, v);
+            add<KIND>(a, v, c_temp);
+        },
+        [&](const T* at, int) {
+            const float v[1] = {Bits<T>::one(at)};
+            add<KIND>(a, v, c_temp);
+        });
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        Sums b;
+        b.m = __shfl_xor_sync(0xffffffffu, a.m, o); b.s1 = __shfl_xor_sync(0xffffffffu, a.s1, o); b.st = __shfl_xor_sync(0xffffffffu, a.st, o);
+        join<KIND>(a, b, c_temp);
+    }
+    if (lane == 0) words[warp] = a;
+    __syncthreads();
+    if (warp == 0) {
+        a = lane < WARPS ? words[lane] : Sums{-INFINITY, 0.f, 0.f};
+#pragma unroll
+        for (int o = WARPS / 2; o; o >>= 1) {
+            Sums b;
+            b.m = __shfl_xor_sync(0xffffffffu, a.m, o); b.s1 = __shfl_xor_sync(0xffffffffu, a.s1, o); b.st = __shfl_xor_sync(0xffffffffu, a.st, o);
+            join<KIND>(a, b, c_temp);
+        }
+        if (lane == 0) whole = a;
+    }
+    if (p.splits > 1) {
+        __syncthreads();
+        cluster_sync_all();
+        if (split == 0 && warp == 0) {
+            a = {-INFINITY, 0.f, 0.f};
+            if (lane < p.splits) {
+                const uint32_t src = map_to_cta((uint32_t)__cvta_generic_to_shared(&whole), lane);
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(a.m) : "r"(src) : "memory");
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(a.s1) : "r"(src + 4) : "memory");
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(a.st) : "r"(src + 8) : "memory");
+            }
+#pragma unroll
+            for (int o = 4; o; o >>= 1) {
+                Sums b;
+                b.m = __shfl_xor_sync(0xffffffffu, a.m, o); b.s1 = __shfl_xor_sync(0xffffffffu, a.s1, o); b.st = __shfl_xor_sync(0xffffffffu, a.st, o);
+                join<KIND>(a, b, c_temp);
+            }
+        }
+        cluster_sync_all();                       // nobody leaves while its sums are read
+    }
+    if (split != 0 || warp != 0) return;
+    a.m = __shfl_sync(0xffffffffu, a.m, 0); a.s1 = __shfl_sync(0xffffffffu, a.s1, 0); a.st = __shfl_sync(0xffffffffu, a.st, 0);
+    const bool none = a.m == -INFINITY && a.s1 == 0.f && a.st == 0.f;    // no class left: the row counts for nothing
+    float loss = 0.f;
+    if (KIND != DI_SOFT && !none) {
+        const int cls = label_of(p, row);
+        if (cls >= 0) loss = (1.f - p.alpha) * (logf(a.s1) - (logit<T>(p, row, cls) - a.m));
+    }
+    bool any = false;
+    if (KIND != DI_HARD && !none) {
+        float peak = -INFINITY;
+        for (int i = lane; i < p.entries; i += 32) { float x; if (entry<T>(p, row, i, x) >= 0) { any = true; peak = fmaxf(peak, x); } }
+        peak = warp_max(peak);
+        any = __any_sync(0xffffffffu, any) && peak != -INFINITY;
+        float total = 0.f;
+        for (int i = lane; i < p.entries; i += 32) { float x; if (entry<T>(p, row, i, x) >= 0 && any) total += ex2((x - peak) * LOG2E); }
+        total = warp_sum(total);
+        const float log_total = logf(total), log_st = logf(a.st);
+        float sum = 0.f;
+        for (int i = lane; i < p.entries; i += 32) {
+            float x;
+            const int cls = entry<T>(p, row, i, x);
+            if (cls < 0 || !any) continue;
+            const float pi = ex2((x - peak) * LOG2E) / total;
+            if (pi > 0.f || pi != pi) sum += pi * ((x - peak - log_total) - ((logit<T>(p, row, cls) - a.m) * p.inv_temp - log_st));
+        }
+        loss += p.alpha * p.temp * p.temp * warp_sum(sum);
+    }
+    if (lane == 0) {
+        p.loss[row] = loss;
+        if (p.stats) {
+            p.stats[row] = none || a.m > -INFINITY ? a.m : NAN;            // (minus infinity: nothing there; NaN: nothing but that)
+            p.stats[p.n + row] = KIND == DI_SOFT ? INFINITY : a.s1;
+            p.stats[2 * p.n + row] = KIND == DI_HARD || !any ? INFINITY : a.st;
+        }
+    }
+}
+
+template <typename T, bool VECTORS, int KIND, int THREADS>
+__global__ void __launch_bounds__(THREADS) distill_bwd_kernel(const DIParams p) {
+    extern __shared__ float shared[];                          // [entries] classes of the teacher's entries, [entries] probabilities
+    int* classes_of = reinterpret_cast<int*>(shared);
+    float* probs = shared + p.entries;
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const int row = blockIdx.x / p.splits, split = blockIdx.x - row * p.splits;
+    const int classes = p.comps * p.units;
+    const int lo = (int)((long long)classes * split / p.splits), hi = (int)((long long)classes * (split + 1) / p.splits);
+    const float c_temp = LOG2E * p.inv_temp;
+    chain_wait();
+    chain_next();
+    const float g = ld_chained(p.grad + row), m = ld_chained(p.stats + row), s1 = ld_chained(p.stats + p.n + row), st = ld_chained(p.stats + 2 * p.n + row);
+    const int label = KIND == DI_SOFT ? -1 : label_of(p, row);
+    const bool none = m == -INFINITY, soft = KIND != DI_HARD && st != INFINITY;
+    const float c1 = label >= 0 && !none ? g * (1.f - p.alpha) / s1 : 0.f, ct = soft && !none ? g * p.alpha * p.temp / st : 0.f;
+    const float base = none ? 0.f : m;
+    auto value = [&](float z) {
+        float e1, et;
+        exps<KIND>(z - base, c_temp, e1, et);
+        if (none) return 0.f;
+        if (KIND == DI_HARD) return c1 * e1;
+        if (KIND == DI_SOFT) return ct * et;
+        if (KIND == DI_SAME) return (c1 + ct) * e1;
+        return fmaf(c1, e1, ct * et);
+    };
+    T* out = static_cast<T*>(p.dlogits);
+    const T* in = static_cast<const T*>(p.logits);
+    over_classes<T, VECTORS, 4>(in, p, row, lo, hi, t, THREADS,
+        [&](const uint4& raw, int, const T* at) {
+            float v[Bits<T>::VEC];
+            Bits<T>::unpack(raw, v);
+#pragma unroll
+            for (int i = 0; i < Bits<T>::VEC; ++i) v[i] = value(v[i]);
+            *reinterpret_cast<uint4*>(out + (at - in)) = Bits<T>::pack(v);
+        },
+        [&](const T* at, int) { Bits<T>::put(out + (at - in), value(Bits<T>::one(at))); });
+    // the classes of the label and of the teacher's entries once more, with their own terms
+    if (soft && !none && warp == 0) {
+        float peak = -INFINITY;
+        for (int i = lane; i < p.entries; i += 32) {
+            float x;
+            classes_of[i] = entry<T>(p, row, i, x);
+            probs[i] = x;
+            peak = fmaxf(peak, x);
+        }
+        peak = warp_max(peak);
+        float total = 0.f;
+        for (int i = lane; i < p.entries; i += 32) { const float e = classes_of[i] >= 0 ? ex2((probs[i] - peak) * LOG2E) : 0.f; probs[i] = e; total += e; }
+        total = warp_sum(total);
+        for (int i = lane; i < p.entries; i += 32) probs[i] /= total;
+    }
+    __syncthreads();
+    if (none) return;
+    const int entries = soft ? p.entries : 0;
+    for (int i = t; i <= entries; i += THREADS) {
+        const int cls = i < entries ? classes_of[i] : label;
+        if (cls < lo || cls >= hi) continue;
+        float prob = 0.f;
+        for (int j = 0; j < entries; ++j) prob += classes_of[j] == cls ? probs[j] : 0.f;      // (a class may be named twice; all who write it write the same)
+        float v = value(logit<T>(p, row, cls)) - g * p.alpha * p.temp * prob;
+        if (cls == label) v -= g * (1.f - p.alpha);
+        const int c = cls / p.units;
+        Bits<T>::put(out + ((size_t)c * p.n + row) * p.units + (cls - c * p.units), v);
+    }
+}
+
+int check_distill(const pcb_distill_desc* d, int& comps) {
+    if (!d) { set_error("null descriptor"); return PCB_ERR_INVALID_ARGUMENT; }
+    if (d->dtype < PCB_F32 || d->dtype > PCB_BF16) { set_error("unknown dtype %d", d->dtype); return PCB_ERR_INVALID_ARGUMENT; }
+    Geom g = {};
+    if (!algebra_setup(d->algebra, g)) { set_error("unknown algebra %d", d->algebra); return PCB_ERR_INVALID_ARGUMENT; }
+    comps = g.nc;
+    if (d->batch < 0 || d->units <= 0 || d->entries < 0) { set_error("invalid distillation geometry"); return PCB_ERR_INVALID_ARGUMENT; }
+    if (!(d->alpha >= 0.f && d->alpha <= 1.f) || !(d->temperature > 0.f) || d->temperature == INFINITY) {
+        set_error("alpha in [0, 1] and a positive temperature expected");
+        return PCB_ERR_INVALID_ARGUMENT;
+    }
+    if (d->entries > DI_MAX_ENTRIES) { set_error("%d entries of the teacher's, %d at most", d->entries, DI_MAX_ENTRIES); return PCB_ERR_UNSUPPORTED; }
+    if ((long long)comps * d->units > 2147483647LL || (long long)comps * d->units * d->batch > (1LL << 40) || (long long)d->batch * 8 > 2147483647LL) {
+        set_error("too many classes or rows");
+        return PCB_ERR_TOO_LARGE;
+    }
+    return PCB_OK;
+}
+DIParams distill_params(const pcb_distill_desc* d, int comps) {
+    DIParams p = {};
+    p.comps = comps; p.n = d->batch; p.units = d->units; p.entries = d->entries;
+    p.alpha = d->alpha; p.temp = d->temperature; p.inv_temp = 1.f / d->temperature;
+    return p;
+}
+int kind_of(const DIParams& p, bool hard, bool soft) {
+    if (!soft || p.alpha == 0.f) return DI_HARD;
+    if (!hard || p.alpha == 1.f) return DI_SOFT;
+    return p.temp == 1.f ? DI_SAME : (p.temp == 2.f ? DI_SQUARE : DI_BOTH);
+}
+// CTAs that share a row: enough for four CTAs on every SM, with 4096 classes each
+int row_splits(const DIParams& p) {
+    const long long classes = (long long)p.comps * p.units;
+    int s = 1;
+    while (s < 8 && (long long)p.n * s * 2 <= 4LL * sm_count() && classes >= 4096LL * s * 2) s *= 2;
+    return s;
+}
+template <typename T, bool VECTORS, int KIND>
+cudaError_t launch_kind(bool forward, const DIParams& p, cudaStream_t s) {
+    const long long per = (long long)p.comps * p.units / p.splits;
+    const unsigned grid = (unsigned)p.n * (unsigned)p.splits;
+    if (forward) {
+        if (per <= 4096) return launch_clusters(p.splits, true, distill_fwd_kernel<T, VECTORS, KIND, 128>, grid, 128, 0, s, p);
+        return launch_clusters(p.splits, true, distill_fwd_kernel<T, VECTORS, KIND, 512>, grid, 512, 0, s, p);
+    }
+    const size_t smem = (size_t)p.entries * 8;
+    if (per <= 4096) return launch_chained(distill_bwd_kernel<T, VECTORS, KIND, 128>, grid, 128, smem, s, p);
+    return launch_chained(distill_bwd_kernel<T, VECTORS, KIND, 512>, grid, 512, smem, s, p);
+}
+template <typename T, bool VECTORS>
+cudaError_t launch_any(bool forward, int kind, const DIParams& p, cudaStream_t s) {
+    switch (kind) {
+        case DI_HARD: return launch_kind<T, VECTORS, DI_HARD>(forward, p, s);
+        case DI_SOFT: return launch_kind<T, VECTORS, DI_SOFT>(forward, p, s);
+        case DI_SAME: return launch_kind<T, VECTORS, DI_SAME>(forward, p, s);
+        case DI_SQUARE: return launch_kind<T, VECTORS, DI_SQUARE>(forward, p, s);
+        default: return launch_kind<T, VECTORS, DI_BOTH>(forward, p, s);
+    }
+}
+template <typename T>
+int launch_typed(bool forward, const DIParams& p, cudaStream_t s) {
+    const int kind = kind_of(p, p.labels != nullptr, p.entries > 0);
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p.logits), b = reinterpret_cast<uintptr_t>(p.dlogits);
+    const bool vec = forward || a % 16 == b % 16;              // rows may start anywhere, but a row and its gradient at the same place in 16 bytes
+    if (vec) PCB_CUDA_TRY((launch_any<T, true>(forward, kind, p, s)));
+    else PCB_CUDA_TRY((launch_any<T, false>(forward, kind, p, s)));
+    return PCB_OK;
+}
+int launch_distill(bool forward, int dtype, const DIParams& p, cudaStream_t s) {
+    if (dtype == PCB_F32) return launch_typed<float>(forward, p, s);
+    return dtype == PCB_F16 ? launch_typed<__half>(forward, p, s) : launch_typed<__nv_bfloat16>(forward, p, s);
+}
+
+}  // namespace
+}  // namespace pcb
+
+using namespace pcb;
+
+extern "C" {
+
+int pcb_distill_fwd(const pcb_distill_desc* d, const void* logits, const long long* labels, const void* teacher, const long long* index, float* loss,
+                    float* stats, void* stream) {
+    int comps;
+    const int rc = check_distill(d, comps);
+    if (rc != PCB_OK || d->batch == 0) return rc;
+    if (!logits || !loss || (d->entries > 0 && (!teacher || !index))) { set_error("null tensor pointer"); return PCB_ERR_INVALID_ARGUMENT; }
+    DIParams p = distill_params(d, comps);
+    p.logits = logits; p.labels = labels; p.teacher = teacher; p.index = index; p.loss = loss; p.stats = stats;
+    p.splits = row_splits(p);
+    return launch_distill(true, d->dtype, p, (cudaStream_t)stream);
+}
+
+int pcb_distill_bwd(const pcb_distill_desc* d, const void* logits, const long long* labels, const void* teacher, const long long* index, const float* stats,
+                    const float* grad_loss, void* dlogits, void* stream) {
+    int comps;
+    const int rc = check_distill(d, comps);
+    if (rc != PCB_OK || d->batch == 0) return rc;
+    if (!logits || !stats || !grad_loss || !dlogits || (d->entries > 0 && (!teacher || !index))) { set_error("null tensor pointer"); return PCB_ERR_INVALID_ARGUMENT; }
+    const size_t bytes = (size_t)comps * d->batch * d->units * dtype_size(d->dtype);
+    if (overlaps(logits, bytes, dlogits, bytes)) { set_error("the gradient must not share memory with the logits"); return PCB_ERR_INVALID_ARGUMENT; }
+    DIParams p = distill_params(d, comps);
+    p.logits = logits; p.labels = labels; p.teacher = teacher; p.index = index; p.stats = const_cast<float*>(stats); p.grad = grad_loss; p.dlogits = dlogits;
+    p.splits = row_splits(p);
+    return launch_distill(false, d->dtype, p, (cudaStream_t)stream);
+}
+
+}  // extern "C"
