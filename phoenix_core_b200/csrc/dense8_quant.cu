@@ -6,10 +6,9 @@
 // exact, so the result is one rounding of x and the same whatever computes it. Infinities and NaN become the type's NaN and do not
 // enter the maximum.
 //
-// A CTA takes a tile of 128 x 128 values in registers, 8 x 8 per thread: the blocks of 1 x 128, of 128 x 1 and of 128 x 128 all lie within it, so the
-// backward pass reads dy once for both of its products.
-#include <cuda_fp8.h>
-
+// A CTA takes a tile of 128 x 128 values in registers, 4 x 8 per thread: the blocks of 1 x 128, of 128 x 1 and of 128 x 128 all lie within it, so the
+// backward pass reads dy once for both of its products. The tile stays as it was loaded (as fp32 it took 176 registers, and one CTA per SM moved 2.2 TB/s);
+// maxima are taken over the bits of the magnitudes, two 16-bit values at a time.
 #include "dense8.cuh"
 #include "tc_common.cuh"
 
@@ -18,7 +17,7 @@ namespace {
 
 using namespace tc;
 
-constexpr int QT_THREADS = 256;
+constexpr int QT_THREADS = 512, QT_WARPS = QT_THREADS / 32, QT_PER = 4, QT_STEP = QT_THREADS / 16;   // rows per thread, and between them
 
 __device__ __forceinline__ int scale_byte(uint32_t amax_bits) {            // e + 127 of a block with that fp32 maximum (finite)
     if (amax_bits == 0) return 127;
@@ -30,11 +29,6 @@ __device__ __forceinline__ int scale_byte(uint32_t amax_bits) {            // e 
 }
 __device__ __forceinline__ float inverse_scale(int byte) { return __uint_as_float((uint32_t)(254 - byte) << 23); }   // 2^-e, byte in [1, 247]
 
-// |v| as bits, or zero for what is no finite number
-__device__ __forceinline__ uint32_t finite_abs(float v) {
-    const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
-    return b < 0x7f800000u ? b : 0u;
-}
 __device__ __forceinline__ uint32_t to_e4m3x4(float a, float b, float c, float d) {
     uint16_t lo, hi;
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
@@ -45,39 +39,66 @@ __device__ __forceinline__ float finite_or_nan(float v) {                  // (t
     return (__float_as_uint(v) & 0x7fffffffu) == 0x7f800000u ? __uint_as_float(0x7fffffffu) : v;
 }
 
-template <typename T> __device__ __forceinline__ void unpack8(const uint4& raw, float (&v)[8]);
-template <> __device__ __forceinline__ void unpack8<__half>(const uint4& raw, float (&v)[8]) {
-    const __half2* h = reinterpret_cast<const __half2*>(&raw);
+// Eight neighbours as loaded. A key is a value's magnitude as bits (monotonic); a 32-bit word holds the keys of two 16-bit values or of one fp32 value.
+template <typename T> struct Eight;
+template <> struct Eight<float> {
+    static constexpr int WORDS = 8;
+    static constexpr uint32_t INF_KEY = 0x7f800000u;
+    uint32_t w[8];
+    static __device__ __forceinline__ uint32_t keys(uint32_t w) { return w & 0x7fffffffu; }
+    static __device__ __forceinline__ uint32_t finite_keys(uint32_t w) { const uint32_t k = keys(w); return k < INF_KEY ? k : 0u; }
+    static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return max(a, b); }
+    static __device__ __forceinline__ uint32_t whole(uint32_t keys) { return keys; }                       // the largest key of a word
+    static __device__ __forceinline__ uint32_t bits(uint32_t key) { return key; }                           // as fp32
+    __device__ __forceinline__ float value(int i) const { return __uint_as_float(w[i]); }
+    __device__ __forceinline__ void zero() {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { const float2 f = __half22float2(h[i]); v[2 * i] = f.x; v[2 * i + 1] = f.y; }
-}
-template <> __device__ __forceinline__ void unpack8<__nv_bfloat16>(const uint4& raw, float (&v)[8]) {
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
-}
-__device__ __forceinline__ float load1(const float* p) { return ld_chained(p); }
-__device__ __forceinline__ float load1(const __half* p) { return __half2float(__ushort_as_half(ld_chained(reinterpret_cast<const uint16_t*>(p)))); }
-__device__ __forceinline__ float load1(const __nv_bfloat16* p) { return __uint_as_float((uint32_t)ld_chained(reinterpret_cast<const uint16_t*>(p)) << 16); }
-
-// Eight neighbours of a row; `valid` of them exist. VEC: the row starts on 16 bytes and valid is 0 or 8.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* p, int valid, float (&v)[8]) {
-    if (VEC) {
-        if (valid <= 0) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = 0.f;
-        } else if (sizeof(T) == 4) {
-            const float4 a = ld_chained(reinterpret_cast<const float4*>(p)), b = ld_chained(reinterpret_cast<const float4*>(p) + 1);
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-        } else {
-            if constexpr (sizeof(T) == 2) unpack8<T>(ld_chained(reinterpret_cast<const uint4*>(p)), v);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < valid ? load1(p + i) : 0.f;
+        for (int i = 0; i < 8; ++i) w[i] = 0;
     }
-}
+    __device__ __forceinline__ void load(const float* p) {
+        const uint4 a = ld_chained(reinterpret_cast<const uint4*>(p)), b = ld_chained(reinterpret_cast<const uint4*>(p) + 1);
+        w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w; w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+    }
+    __device__ __forceinline__ void load(const float* p, int valid) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = ld_chained(reinterpret_cast<const uint32_t*>(p) + i, i < valid);
+    }
+};
+template <typename T> struct Eight16 {
+    static constexpr int WORDS = 4;
+    uint32_t w[4];
+    static __device__ __forceinline__ uint32_t keys(uint32_t w) { return w & 0x7fff7fffu; }
+    static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return __vmaxu2(a, b); }
+    static __device__ __forceinline__ uint32_t whole(uint32_t keys) { return max(keys & 0xffffu, keys >> 16); }
+    __device__ __forceinline__ void zero() { w[0] = w[1] = w[2] = w[3] = 0; }
+    __device__ __forceinline__ void load(const T* p) {
+        const uint4 a = ld_chained(reinterpret_cast<const uint4*>(p));
+        w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+    }
+    __device__ __forceinline__ void load(const T* p, int valid) {
+        const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = (uint32_t)ld_chained(h + 2 * i, 2 * i < valid) | ((uint32_t)ld_chained(h + 2 * i + 1, 2 * i + 1 < valid) << 16);
+    }
+};
+template <> struct Eight<__half> : Eight16<__half> {
+    static constexpr uint32_t INF_KEY = 0x7c00u;
+    static __device__ __forceinline__ uint32_t finite_keys(uint32_t w) {
+        const uint32_t k = keys(w), lo = k & 0xffffu, hi = k >> 16;
+        return (lo < INF_KEY ? lo : 0u) | ((hi < INF_KEY ? hi : 0u) << 16);
+    }
+    static __device__ __forceinline__ uint32_t bits(uint32_t key) { return __float_as_uint(__half2float(__ushort_as_half((uint16_t)key))); }
+    __device__ __forceinline__ float value(int i) const { return __half2float(__ushort_as_half((uint16_t)(i & 1 ? w[i >> 1] >> 16 : w[i >> 1]))); }
+};
+template <> struct Eight<__nv_bfloat16> : Eight16<__nv_bfloat16> {
+    static constexpr uint32_t INF_KEY = 0x7f80u;
+    static __device__ __forceinline__ uint32_t finite_keys(uint32_t w) {
+        const uint32_t k = keys(w), lo = k & 0xffffu, hi = k >> 16;
+        return (lo < INF_KEY ? lo : 0u) | ((hi < INF_KEY ? hi : 0u) << 16);
+    }
+    static __device__ __forceinline__ uint32_t bits(uint32_t key) { return key << 16; }
+    __device__ __forceinline__ float value(int i) const { return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16); }
+};
 
 enum { QT_ROWS = 1, QT_COLS = 2, QT_BLOCKS = 4 };
 
@@ -89,89 +110,117 @@ struct QTParams {
     int* status;                                 // cleared by the first CTA, or null
 };
 
-// Thread t holds columns 8 * (t % 16) .. + 7 of rows (t / 16) + 16 * i: the lanes of half a warp hold one row.
+// Thread t holds columns 8 * (t % 16) .. + 7 of rows (t / 16) + 32 * i: the lanes of half a warp hold one row.
+// VEC: rows start on 16 bytes and are whole vectors.
 template <typename T, int MODE, bool VEC>
-__global__ void __launch_bounds__(QT_THREADS) quantize_tile_kernel(const T* x, QTParams p) {
-    __shared__ uint32_t col_max[8][Q8_BLOCK];
-    __shared__ uint32_t warp_max[8];
+__global__ void __launch_bounds__(QT_THREADS, sizeof(T) == 4 ? 1 : 2) quantize_tile_kernel(const T* x, QTParams p) {
+    typedef Eight<T> E;
+    __shared__ uint32_t col_max[QT_WARPS][16 * E::WORDS];
+    __shared__ uint32_t warp_max[QT_WARPS];
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31, c8 = (t & 15) * 8, r0 = t >> 4;
     const int comp = blockIdx.z, row_block = blockIdx.y, col_block = blockIdx.x;
-    const int col = col_block * Q8_BLOCK + c8;
+    const int col = col_block * Q8_BLOCK + c8, first_row = row_block * Q8_BLOCK + r0;
     chain_wait();
     chain_next();
     if (p.status && t == 0 && comp == 0 && row_block == 0 && col_block == 0) *p.status = 0;
     const int valid = min(8, p.cols - col);
-    float v[8][8];
+    E v[QT_PER];
+    {
+        const T* src = x + ((size_t)comp * p.rows + first_row) * p.cols + col;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int row = row_block * Q8_BLOCK + r0 + 16 * i;
-        load8<T, VEC>(x + ((size_t)comp * p.rows + row) * p.cols + col, row < p.rows ? valid : 0, v[i]);
+        for (int i = 0; i < QT_PER; ++i) {
+            const bool live = first_row + QT_STEP * i < p.rows && valid > 0;
+            if (VEC) {
+                if (live) v[i].load(src + (size_t)QT_STEP * i * p.cols);
+                else v[i].zero();
+            } else v[i].load(src + (size_t)QT_STEP * i * p.cols, live ? valid : 0);
+        }
+    }
+    uint32_t row_keys[QT_PER], most = 0;
+#pragma unroll
+    for (int i = 0; i < QT_PER; ++i) {
+        row_keys[i] = 0;
+#pragma unroll
+        for (int j = 0; j < E::WORDS; ++j) row_keys[i] = E::larger(row_keys[i], E::keys(v[i].w[j]));
+        row_keys[i] = E::whole(row_keys[i]);
+        most = max(most, row_keys[i]);
+    }
+    // whether the tile holds infinities or NaN, which are kept out of the maxima and become NaN (the conversion would saturate an infinity)
+    const bool odd = __syncthreads_or(most >= E::INF_KEY);
+    if (odd) {
+        most = 0;
+#pragma unroll
+        for (int i = 0; i < QT_PER; ++i) {
+            row_keys[i] = 0;
+#pragma unroll
+            for (int j = 0; j < E::WORDS; ++j) row_keys[i] = E::larger(row_keys[i], E::finite_keys(v[i].w[j]));
+            row_keys[i] = E::whole(row_keys[i]);
+            most = max(most, row_keys[i]);
+        }
     }
     auto store = [&](uint8_t* values, int i, const float (&s)[8]) {
-        const int row = row_block * Q8_BLOCK + r0 + 16 * i;
+        const int row = first_row + QT_STEP * i;
         if (row >= p.rows || col >= p.pitch) return;
-        uint2 w;
-        w.x = to_e4m3x4(finite_or_nan(v[i][0]) * s[0], finite_or_nan(v[i][1]) * s[1], finite_or_nan(v[i][2]) * s[2], finite_or_nan(v[i][3]) * s[3]);
-        w.y = to_e4m3x4(finite_or_nan(v[i][4]) * s[4], finite_or_nan(v[i][5]) * s[5], finite_or_nan(v[i][6]) * s[6], finite_or_nan(v[i][7]) * s[7]);
-        *reinterpret_cast<uint2*>(values + ((size_t)comp * p.rows + row) * p.pitch + col) = w;
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = (odd ? finite_or_nan(v[i].value(j)) : v[i].value(j)) * s[j];
+        *reinterpret_cast<uint2*>(values + ((size_t)comp * p.rows + row) * p.pitch + col) = make_uint2(to_e4m3x4(f[0], f[1], f[2], f[3]), to_e4m3x4(f[4], f[5], f[6], f[7]));
     };
-    if (MODE & (QT_ROWS | QT_BLOCKS)) {
-        uint32_t tile = 0;
+    if constexpr ((MODE & QT_ROWS) != 0) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            uint32_t m = 0;
+        for (int i = 0; i < QT_PER; ++i) {
+            uint32_t m = row_keys[i];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) m = max(m, finite_abs(v[i][j]));
-            if constexpr ((MODE & QT_BLOCKS) != 0) {
-                tile = max(tile, m);
-            } else {
-#pragma unroll
-                for (int o = 8; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-                const int byte = scale_byte(m), row = row_block * Q8_BLOCK + r0 + 16 * i;
-                const float f = inverse_scale(byte);
-                const float s[8] = {f, f, f, f, f, f, f, f};
-                store(p.row_values, i, s);
-                if ((t & 15) == 0 && row < p.rows)
-                    reinterpret_cast<uint8_t*>(p.row_words + ((size_t)comp * p.row_groups + (col_block >> 2)) * p.rows + row)[col_block & 3] = (uint8_t)byte;
-            }
-        }
-        if constexpr ((MODE & QT_BLOCKS) != 0) {
-            tile = __reduce_max_sync(0xffffffffu, tile);
-            if (lane == 0) warp_max[warp] = tile;
-            __syncthreads();
-#pragma unroll
-            for (int w = 0; w < 8; ++w) tile = max(tile, warp_max[w]);
-            const int byte = scale_byte(tile);
+            for (int o = 8; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+            const int byte = scale_byte(E::bits(m)), row = first_row + QT_STEP * i;
             const float f = inverse_scale(byte);
             const float s[8] = {f, f, f, f, f, f, f, f};
-#pragma unroll
-            for (int i = 0; i < 8; ++i) store(p.row_values, i, s);
-            if (t == 0) reinterpret_cast<uint8_t*>(p.row_words)[((size_t)comp * gridDim.y + row_block) * gridDim.x + col_block] = (uint8_t)byte;
+            store(p.row_values, i, s);
+            if ((t & 15) == 0 && row < p.rows)
+                reinterpret_cast<uint8_t*>(p.row_words + ((size_t)comp * p.row_groups + (col_block >> 2)) * p.rows + row)[col_block & 3] = (uint8_t)byte;
         }
     }
-    if (MODE & QT_COLS) {
+    if constexpr ((MODE & QT_BLOCKS) != 0) {
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (lane == 0) warp_max[warp] = most;
+        __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            uint32_t m = 0;
+        for (int w = 0; w < QT_WARPS; ++w) most = max(most, warp_max[w]);
+        const int byte = scale_byte(E::bits(most));
+        const float f = inverse_scale(byte);
+        const float s[8] = {f, f, f, f, f, f, f, f};
 #pragma unroll
-            for (int i = 0; i < 8; ++i) m = max(m, finite_abs(v[i][j]));
-            m = max(m, __shfl_xor_sync(0xffffffffu, m, 16));                // the warp's other half holds other rows of these columns
-            if (lane < 16) col_max[warp][c8 + j] = m;
+        for (int i = 0; i < QT_PER; ++i) store(p.row_values, i, s);
+        if (t == 0) reinterpret_cast<uint8_t*>(p.row_words)[((size_t)comp * gridDim.y + row_block) * gridDim.x + col_block] = (uint8_t)byte;
+    }
+    if constexpr ((MODE & QT_COLS) != 0) {
+        uint32_t m[E::WORDS];
+#pragma unroll
+        for (int j = 0; j < E::WORDS; ++j) {
+            m[j] = 0;
+#pragma unroll
+            for (int i = 0; i < QT_PER; ++i) m[j] = E::larger(m[j], odd ? E::finite_keys(v[i].w[j]) : E::keys(v[i].w[j]));
+            m[j] = E::larger(m[j], __shfl_xor_sync(0xffffffffu, m[j], 16));       // the warp's other half holds other rows of these columns
+            if (lane < 16) col_max[warp][lane * E::WORDS + j] = m[j];
         }
         __syncthreads();
         float s[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            uint32_t m = 0;
+        for (int j = 0; j < E::WORDS; ++j) {
+            uint32_t k = 0;
 #pragma unroll
-            for (int w = 0; w < 8; ++w) m = max(m, col_max[w][c8 + j]);
-            const int byte = scale_byte(m);
-            s[j] = inverse_scale(byte);
-            if (t < 16 && col + j < p.cols)
-                reinterpret_cast<uint8_t*>(p.col_words + ((size_t)comp * p.col_groups + (row_block >> 2)) * p.cols + col + j)[row_block & 3] = (uint8_t)byte;
+            for (int w = 0; w < QT_WARPS; ++w) k = E::larger(k, col_max[w][(t & 15) * E::WORDS + j]);
+            constexpr int PER = 8 / E::WORDS;                                      // columns per word
+#pragma unroll
+            for (int h = 0; h < PER; ++h) {
+                const int byte = scale_byte(E::bits(PER == 1 ? k : (h ? k >> 16 : k & 0xffffu))), e = j * PER + h;
+                s[e] = inverse_scale(byte);
+                if (t < 16 && col + e < p.cols)
+                    reinterpret_cast<uint8_t*>(p.col_words + ((size_t)comp * p.col_groups + (row_block >> 2)) * p.cols + col + e)[row_block & 3] = (uint8_t)byte;
+            }
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) store(p.col_values, i, s);
+        for (int i = 0; i < QT_PER; ++i) store(p.col_values, i, s);
     }
 }
 

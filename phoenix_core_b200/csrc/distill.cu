@@ -38,6 +38,12 @@ template <> struct Bits<float> {
     static __device__ __forceinline__ void unpack(const uint4& r, float* v) { v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y); v[2] = __uint_as_float(r.z); v[3] = __uint_as_float(r.w); }
     static __device__ __forceinline__ uint4 pack(const float* v) { return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])); }
     static __device__ __forceinline__ void put(float* p, float v) { *p = v; }
+    template <int N> static __device__ __forceinline__ float largest(const uint4 (&raw)[N]) {      // (of what is a number)
+        float m = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < N; ++u) m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(raw[u].x), __uint_as_float(raw[u].y)), fmaxf(__uint_as_float(raw[u].z), __uint_as_float(raw[u].w))));
+        return m;
+    }
 };
 template <> struct Bits<__half> {
     static constexpr int VEC = 8;
@@ -54,6 +60,17 @@ template <> struct Bits<__half> {
         return make_uint4(w[0], w[1], w[2], w[3]);
     }
     static __device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
+    template <int N> static __device__ __forceinline__ float largest(const uint4 (&raw)[N]) {
+        __half2 m = *reinterpret_cast<const __half2*>(&raw[0].x);
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m = __hmax2(m, *reinterpret_cast<const __half2*>(&w[i]));
+        }
+        const float2 f = __half22float2(m);
+        return fmaxf(f.x, f.y);
+    }
 };
 template <> struct Bits<__nv_bfloat16> {
     static constexpr int VEC = 8;
@@ -70,17 +87,54 @@ template <> struct Bits<__nv_bfloat16> {
         return make_uint4(w[0], w[1], w[2], w[3]);
     }
     static __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+    template <int N> static __device__ __forceinline__ float largest(const uint4 (&raw)[N]) {
+        __nv_bfloat162 m = *reinterpret_cast<const __nv_bfloat162*>(&raw[0].x);
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m = __hmax2(m, *reinterpret_cast<const __nv_bfloat162*>(&w[i]));
+        }
+        const float2 f = __bfloat1622float2(m);
+        return fmaxf(f.x, f.y);
+    }
 };
 
-__device__ __forceinline__ float ex2(float x) { return exp2f(x); }
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Two fp32 values per instruction: a pass over 16-bit logits at full bandwidth is 11.5 logits per clock and SM, and one value per instruction (nine for a logit)
+// left it bound by issue slots, 4.6 TB/s.
+struct Pair { unsigned long long v; };
+__device__ __forceinline__ Pair pair(float a, float b) { Pair r; asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ void halves(Pair p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p.v)); }
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) { Pair r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) { Pair r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) { Pair r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v)); return r; }
+__device__ __forceinline__ Pair ex2(Pair x) {
+    float a, b;
+    halves(x, a, b);
+    return pair(ex2(a), ex2(b));
+}
 // exponentials of d = z - max <= 0 at temperature 1 and T
 template <int KIND>
+__device__ __forceinline__ void exps(Pair d, float c_temp, Pair& e1, Pair& et) {
+    const Pair one = pair(LOG2E, LOG2E), ct = pair(c_temp, c_temp);
+    if (KIND == DI_HARD) { e1 = ex2(d * one); et = pair(0.f, 0.f); }
+    else if (KIND == DI_SOFT) { et = ex2(d * ct); e1 = pair(0.f, 0.f); }
+    else if (KIND == DI_SAME) { e1 = et = ex2(d * one); }
+    else if (KIND == DI_SQUARE) { et = ex2(d * ct); e1 = et * et; }
+    else { e1 = ex2(d * one); et = ex2(d * ct); }
+}
+template <int KIND>
 __device__ __forceinline__ void exps(float d, float c_temp, float& e1, float& et) {
-    if (KIND == DI_HARD) { e1 = ex2(d * LOG2E); et = 0.f; }
-    else if (KIND == DI_SOFT) { et = ex2(d * c_temp); e1 = 0.f; }
-    else if (KIND == DI_SAME) { e1 = et = ex2(d * LOG2E); }
-    else if (KIND == DI_SQUARE) { et = ex2(d * c_temp); e1 = et * et; }
-    else { e1 = ex2(d * LOG2E); et = ex2(d * c_temp); }
+    Pair a, b;
+    float unused;
+    exps<KIND>(pair(d, 0.f), c_temp, a, b);
+    halves(a, e1, unused);
+    halves(b, et, unused);
 }
 
 struct Sums { float m, s1, st; };
@@ -100,46 +154,86 @@ __device__ __forceinline__ void join(Sums& a, Sums b, float c_temp) {
     a.s1 += b.s1;
     a.st += b.st;
 }
-template <int KIND, int N>
-__device__ __forceinline__ void add(Sums& a, const float (&v)[N], float c_temp) {
-    float top = v[0];
-#pragma unroll
-    for (int i = 1; i < N; ++i) top = fmaxf(top, v[i]);
-    if (top > a.m) raise<KIND>(a, top, c_temp);
+// The running sums of a thread: two of each, added up at the end.
+struct Running { float m; Pair s1, st; };
+template <int KIND, typename T, int UNROLL>
+__device__ __forceinline__ void add(Running& a, const uint4 (&raw)[UNROLL], float c_temp) {
+    const float top = Bits<T>::largest(raw);
+    if (top > a.m) {
+        float f1, ft;
+        exps<KIND>(a.m - top, c_temp, f1, ft);
+        a.s1 = a.s1 * pair(f1, f1);
+        a.st = a.st * pair(ft, ft);
+        a.m = top;
+    }
     const float m = a.m == -INFINITY ? 0.f : a.m;
+    const Pair minus = pair(-m, -m);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        float e1, et;
-        exps<KIND>(v[i] - m, c_temp, e1, et);
-        a.s1 += e1;
-        a.st += et;
+    for (int u = 0; u < UNROLL; ++u) {
+        float v[Bits<T>::VEC];
+        Bits<T>::unpack(raw[u], v);
+#pragma unroll
+        for (int i = 0; i < Bits<T>::VEC; i += 2) {
+            Pair e1, et;
+            exps<KIND>(pair(v[i], v[i + 1]) + minus, c_temp, e1, et);
+            if (KIND != DI_SOFT) a.s1 = a.s1 + e1;
+            if (KIND != DI_HARD && KIND != DI_SAME) a.st = a.st + et;
+        }
     }
 }
+template <int KIND>
+__device__ __forceinline__ void add(Running& a, float v, float c_temp) {
+    if (v > a.m) {
+        float f1, ft;
+        exps<KIND>(a.m - v, c_temp, f1, ft);
+        a.s1 = a.s1 * pair(f1, f1);
+        a.st = a.st * pair(ft, ft);
+        a.m = v;
+    }
+    float e1, et;
+    exps<KIND>(v - (a.m == -INFINITY ? 0.f : a.m), c_temp, e1, et);
+    a.s1 = a.s1 + pair(e1, 0.f);
+    if (KIND != DI_SAME) a.st = a.st + pair(et, 0.f);
+}
+template <int KIND>
+__device__ __forceinline__ Sums sums_of(const Running& a) {
+    float x, y;
+    Sums r;
+    r.m = a.m;
+    halves(a.s1, x, y);
+    r.s1 = x + y;
+    halves(a.st, x, y);
+    r.st = KIND == DI_SAME ? r.s1 : x + y;
+    return r;
+}
 
-// Calls vec(pointer to 16 aligned bytes of the row, first class) and one(pointer, class) over classes [lo, hi) of a sample, `threads` threads together.
-template <typename T, bool VECTORS, int UNROLL, typename VecFn, typename OneFn>
-__device__ __forceinline__ void over_classes(const T* logits, const DIParams& p, int row, int lo, int hi, int tid, int threads, VecFn vec, OneFn one) {
+// Over classes [lo, hi) of a sample, `threads` threads together: vec(UNROLL times 16 bytes, UNROLL, where the first of them lies, bytes between them),
+// vec1 for single ones behind those, one(pointer) for what is not whole 16 bytes of the row.
+template <typename T, bool VECTORS, int UNROLL, typename VecFn, typename Vec1Fn, typename OneFn>
+__device__ __forceinline__ void over_classes(const T* logits, const DIParams& p, int row, int lo, int hi, int tid, int threads, VecFn vec, Vec1Fn vec1, OneFn one) {
     constexpr int VEC = Bits<T>::VEC;
     for (int c = lo / p.units; c * p.units < hi; ++c) {
         const int a = max(lo, c * p.units), b = min(hi, (c + 1) * p.units);
         const T* first = logits + ((size_t)c * p.n + row) * p.units + (a - c * p.units);
         if (!VECTORS) {
-            for (int i = a + tid; i < b; i += threads) one(first + (i - a), i);
+            for (int i = tid; i < b - a; i += threads) one(first + i);
             continue;
         }
         const int head = min(b - a, (int)((16 - (reinterpret_cast<uintptr_t>(first) & 15)) & 15) / (int)sizeof(T)), body = (b - a - head) / VEC;
-        for (int i = tid; i < head; i += threads) one(first + i, a + i);
+        if (tid < head) one(first + tid);
         const T* start = first + head;
         int v = tid;
         for (; v + (UNROLL - 1) * threads < body; v += UNROLL * threads) {
             uint4 raw[UNROLL];
 #pragma unroll
             for (int u = 0; u < UNROLL; ++u) raw[u] = ld_chained(reinterpret_cast<const uint4*>(start) + v + u * threads);
-#pragma unroll
-            for (int u = 0; u < UNROLL; ++u) vec(raw[u], a + head + (v + u * threads) * VEC, start + (size_t)(v + u * threads) * VEC);
+            vec(raw, start + (size_t)v * VEC);
         }
-        for (; v < body; v += threads) vec(ld_chained(reinterpret_cast<const uint4*>(start) + v), a + head + v * VEC, start + (size_t)v * VEC);
-        for (int i = a + head + body * VEC + tid; i < b; i += threads) one(first + (i - a), i);
+        for (; v < body; v += threads) {
+            const uint4 raw[1] = {ld_chained(reinterpret_cast<const uint4*>(start) + v)};
+            vec1(raw, start + (size_t)v * VEC);
+        }
+        for (int i = head + body * VEC + tid; i < b - a; i += threads) one(first + i);
     }
 }
 
@@ -187,17 +281,12 @@ __global__ void __launch_bounds__(THREADS) distill_fwd_kernel(const DIParams p) 
     const float c_temp = LOG2E * p.inv_temp;
     chain_wait();
     chain_next();
-    Sums a = {-INFINITY, 0.f, 0.f};
+    Running run = {-INFINITY, pair(0.f, 0.f), pair(0.f, 0.f)};
     over_classes<T, VECTORS, 4>(static_cast<const T*>(p.logits), p, row, lo, hi, t, THREADS,
-        [&](const uint4& raw, int, const T*) {
-            float v[Bits<T>::VEC];
-            Bits<T>::unpack(raw, v);
-            add<KIND>(a, v, c_temp);
-        },
-        [&](const T* at, int) {
-            const float v[1] = {Bits<T>::one(at)};
-            add<KIND>(a, v, c_temp);
-        });
+        [&](const uint4 (&raw)[4], const T*) { add<KIND, T, 4>(run, raw, c_temp); },
+        [&](const uint4 (&raw)[1], const T*) { add<KIND, T, 1>(run, raw, c_temp); },
+        [&](const T* at) { add<KIND>(run, Bits<T>::one(at), c_temp); });
+    Sums a = sums_of<KIND>(run);
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
         Sums b;
@@ -280,7 +369,8 @@ __global__ void __launch_bounds__(THREADS) distill_bwd_kernel(const DIParams p) 
     int* classes_of = reinterpret_cast<int*>(shared);
     float* probs = shared + p.entries;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    const int row = blockIdx.x / p.splits, split = blockIdx.x - row * p.splits;
+    // from the last row on: the forward pass has left the last rows in L2
+    const int back = blockIdx.x / p.splits, row = p.n - 1 - back, split = blockIdx.x - back * p.splits;
     const int classes = p.comps * p.units;
     const int lo = (int)((long long)classes * split / p.splits), hi = (int)((long long)classes * (split + 1) / p.splits);
     const float c_temp = LOG2E * p.inv_temp;
@@ -302,15 +392,33 @@ __global__ void __launch_bounds__(THREADS) distill_bwd_kernel(const DIParams p) 
     };
     T* out = static_cast<T*>(p.dlogits);
     const T* in = static_cast<const T*>(p.logits);
-    over_classes<T, VECTORS, 4>(in, p, row, lo, hi, t, THREADS,
-        [&](const uint4& raw, int, const T* at) {
-            float v[Bits<T>::VEC];
-            Bits<T>::unpack(raw, v);
+    const Pair minus = pair(-base, -base), p1 = pair(c1, c1), pt = pair(ct, ct);
+    auto values = [&](const uint4& raw, T* at) {
+        float v[Bits<T>::VEC];
+        Bits<T>::unpack(raw, v);
 #pragma unroll
-            for (int i = 0; i < Bits<T>::VEC; ++i) v[i] = value(v[i]);
-            *reinterpret_cast<uint4*>(out + (at - in)) = Bits<T>::pack(v);
+        for (int i = 0; i < Bits<T>::VEC; i += 2) {
+            Pair e1, et, d;
+            exps<KIND>(pair(v[i], v[i + 1]) + minus, c_temp, e1, et);
+            if (KIND == DI_HARD) d = p1 * e1;
+            else if (KIND == DI_SOFT) d = pt * et;
+            else if (KIND == DI_SAME) d = (p1 + pt) * e1;
+            else d = fma2(p1, e1, pt * et);
+            halves(d, v[i], v[i + 1]);
+        }
+        if (none) {
+#pragma unroll
+            for (int i = 0; i < Bits<T>::VEC; ++i) v[i] = 0.f;
+        }
+        *reinterpret_cast<uint4*>(at) = Bits<T>::pack(v);
+    };
+    over_classes<T, VECTORS, 4>(in, p, row, lo, hi, t, THREADS,
+        [&](const uint4 (&raw)[4], const T* at) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) values(raw[u], out + (at - in) + (size_t)u * THREADS * Bits<T>::VEC);
         },
-        [&](const T* at, int) { Bits<T>::put(out + (at - in), value(Bits<T>::one(at))); });
+        [&](const uint4 (&raw)[1], const T* at) { values(raw[0], out + (at - in)); },
+        [&](const T* at) { Bits<T>::put(out + (at - in), value(Bits<T>::one(at))); });
     // the classes of the label and of the teacher's entries once more, with their own terms
     if (soft && !none && warp == 0) {
         float peak = -INFINITY;
