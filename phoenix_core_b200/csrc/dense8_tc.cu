@@ -7,10 +7,15 @@
 // multiplies in itself: one e8m0 byte per operand row and 32 values, here the same byte four times over (the blocks have 128). Products are
 // exact and sums are held in fp32 in tensor memory over the whole reduction.
 //
-// Roles: warp 0 copies the operand tiles (TMA; both majornesses are read where they lie), warp 1 issues, warp 2 lays the scales out (a word per
+// Roles: warp 0 copies the operand tiles (TMA; both majornesses are read where they lie), warp 1 issues, warps 2 and 3 lay the scales out (a word per
 // row holds the bytes of four blocks; 32 x 4 words are 512 bytes in the order that tcgen05.cp takes to tensor memory), warps 4-11 drain the accumulators.
-// Tiles are 128 x BN; a tile's reduction is cut over the CTAs of a cluster where there are fewer tiles than SMs, whose partial sums
-// are added in a fixed order through distributed shared memory.
+// Three forms:
+//   PAIR      256 x 256 tiles on pairs of SMs, half of either operand in each one's shared memory. An 8-bit MMA of 128 x 256 x 32 takes 128 clocks and reads 12 KB of
+//             shared memory, into which TMA writes as much again: more than the 128 bytes a clock that shared memory moves. On one SM a block of 128 took
+//             0.53 us where the MMAs alone take 0.27; a pair moves a third less.
+//   single    128 x 128 tiles; a tile's reduction is cut over the CTAs of a cluster where there are fewer tiles than SMs, whose partial sums are added in a
+//             fixed order through distributed shared memory.
+//   SWAP      few tokens: the filter is operand A, a tile is 128 features x 16, 64 or 128 tokens; bound by the filter's bytes.
 #include "dense8.cuh"
 #include "tc_common.cuh"
 
@@ -27,17 +32,19 @@ constexpr int D8_SF_STAGES = 4;
 constexpr uint32_t D8_SF_BYTES = 512 * 3;                       // one set of 128 rows for A, up to two for B
 constexpr int ST_D8_PRODUCER = 0x100, ST_D8_MMA = 0x200, ST_D8_SCALES = 0x400, ST_D8_EPILOGUE = 0x800;
 
-template <int BN> struct D8Config {
-    static constexpr int B_ROWS = BN < 32 ? 32 : BN;             // (tiles start on 1024 bytes: 8 rows)
+template <int BN, bool SWAP, bool PAIR> struct D8Config {
+    static constexpr int B_ROWS = PAIR ? BN / 2 : (BN < 32 ? 32 : BN);   // rows of B in a CTA's shared memory (tiles start on 1024 bytes: 8 rows)
     static constexpr uint32_t B_BYTES = B_ROWS * D8_BK;
     static constexpr uint32_t STAGE = D8_A_BYTES + B_BYTES;
-    static constexpr int STAGES = BN >= 256 ? 4 : (BN >= 128 ? 6 : (BN >= 64 ? 8 : 10));
+    static constexpr int STAGES = BN >= 128 ? (SWAP ? 6 : 5) : (BN >= 64 ? 8 : 10);
     static constexpr int ACC = BN >= 256 ? 1 : 2;                // accumulators in tensor memory
     static constexpr uint32_t ACC_COLS = BN < 32 ? 32 : BN;
     static constexpr uint32_t SF_COL = 496;                      // scales: 4 columns for A, 8 for B
-    static constexpr uint32_t STAGED = EPI_ROWS_BYTES * D8_EPI_WARPS;
+    static constexpr int CTAS = PAIR ? 2 : 1;
+    static constexpr int M = D8_BM * CTAS;                       // rows of a tile
+    static constexpr uint32_t OUT_BYTES = SWAP ? 0 : 4096;       // per epilogue warp: 32 rows of 128 bytes on their way out
     static constexpr uint32_t BARS = 256;
-    static constexpr size_t SMEM = 1024 + STAGES * STAGE + D8_SF_STAGES * D8_SF_BYTES + (BN >= 128 ? STAGED : 0) + BARS;
+    static constexpr size_t SMEM = 1024 + STAGES * STAGE + D8_EPI_WARPS * OUT_BYTES + D8_SF_STAGES * D8_SF_BYTES + BARS;
 };
 
 struct D8Params {
@@ -46,6 +53,7 @@ struct D8Params {
     int m, n, k;
     int chunks, groups;                 // blocks of 128 and groups of four of them per component of the reduction
     int m_tiles, n_tiles, tiles;        // tiles: over all output components
+    int out_map;                        // the output is written through its tensor map
     int splits;                         // CTAs of the cluster that share a tile
     int a_mn, b_mn;                     // operands run along their own axis
     int a_blocks, b_blocks;             // scales are bytes per 128 x 128 block, else words
@@ -68,21 +76,49 @@ __device__ __forceinline__ void d8_term(const D8Params& p, int c, int j, int& x_
 __device__ __forceinline__ uint32_t d8_idesc(int M, int N, bool a_mn, bool b_mn, bool a_neg) {
     return ((uint32_t)a_neg << 13) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(N >> 3) << 17) | (1u << 23) | ((uint32_t)(M >> 4) << 24);
 }
+template <bool PAIR>
 __device__ __forceinline__ void mma_mxf8(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t sfa, uint32_t sfb,
                                          uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
-        "mov.b64 da, {%1, %2};\n\t"
-        "mov.b64 db, {%3, %4};\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], da, db, %5, [%7], [%8], p;\n\t}"
-        ::"r"(d_tmem), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb) : "memory");
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+            "mov.b64 da, {%1, %2};\n\t"
+            "mov.b64 db, {%3, %4};\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], da, db, %5, [%7], [%8], p;\n\t}"
+            ::"r"(d_tmem), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb) : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+            "mov.b64 da, {%1, %2};\n\t"
+            "mov.b64 db, {%3, %4};\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], da, db, %5, [%7], [%8], p;\n\t}"
+            ::"r"(d_tmem), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb) : "memory");
 }
-// 32 rows of 16 bytes to four columns of tensor memory, in each of the four groups of 32 lanes
+// 32 rows of 16 bytes to four columns of tensor memory, in each of the four groups of 32 lanes (PAIR: in both CTAs, each from its own shared memory)
+template <bool PAIR>
 __device__ __forceinline__ void copy_scales(uint32_t tmem, uint32_t smem_addr) {
     const uint64_t desc = (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | ((uint64_t)(128 >> 4) << 16) | ((uint64_t)(128 >> 4) << 32) | DESC_VERSION_SM100;
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+    if constexpr (PAIR) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+    else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
 }
+// The scales of the odd CTA are written by its own threads: the arrival that announces them in the even CTA releases at cluster scope, the wait acquires there.
+__device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+__device__ __forceinline__ bool warp_wait_acquire_cluster(uint32_t bar, uint32_t parity, int* status, int code) {
+    const bool ok = warp_wait_bounded(bar, parity, status, code);
+    if (ok) {
+        [[maybe_unused]] uint32_t done;                          // (complete already: this one orders)
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    }
+    return ok;
+}
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(src), "r"(c0), "r"(c1), "r"(c2) : "memory");
+}
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 __device__ __forceinline__ float ld_typed(const void* p, int dtype, size_t i) {
     if (dtype == PCB_F32) return ld_chained(static_cast<const float*>(p) + i);
@@ -121,6 +157,27 @@ __device__ __forceinline__ void store_floats(uint32_t buf, const uint32_t (&v)[3
     }
 }
 
+// Where a warp is in its CTA's part of a reduction: group `group` of component j, with the operands' components and the sign. Stepped, not computed anew: the
+// divisions of one step took a warp about as long as the MMAs of a block.
+struct D8Walk {
+    int left, j, group, first, second;       // groups left, component of the reduction, its group; components of x (or dy) and of the other operand
+    bool neg;
+    __device__ __forceinline__ void start(const D8Params& p, int c, int g_begin, int g_end, int j_begin) {
+        left = g_end - g_begin;
+        j = j_begin;
+        group = g_begin - j_begin * p.groups;
+        term(p, c);
+    }
+    __device__ __forceinline__ void term(const D8Params& p, int c) {
+        if (j < p.comps) d8_term(p, c, j, first, second, neg);
+    }
+    __device__ __forceinline__ void step(const D8Params& p, int c) {
+        --left;
+        if (++group == p.groups) { group = 0; ++j; term(p, c); }
+    }
+    __device__ __forceinline__ int blocks(const D8Params& p) const { return min(4, p.chunks - 4 * group); }
+};
+
 // Tile order: the tiles of eight rows of tiles together, so that the CTAs at work share both operands' tiles in L2.
 __device__ __forceinline__ void d8_tile(const D8Params& p, int tile, int& c, int& mt, int& nt) {
     const int per = p.m_tiles * p.n_tiles;
@@ -131,30 +188,35 @@ __device__ __forceinline__ void d8_tile(const D8Params& p, int tile, int& c, int
     nt = in / height;
 }
 
-// SWAP: operand A is the filter, so that tile rows run along the output's fast axis.
-template <int BN, bool SWAP>
+// SWAP: operand A is the filter, so that tile rows run along the output's fast axis. PAIR: clusters of two; the even CTA issues for both.
+template <int BN, bool SWAP, bool PAIR>
 __global__ void __launch_bounds__(D8_THREADS, 1)
-dense8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const D8Params p, int* status) {
-    using C = D8Config<BN>;
+dense8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_out, const D8Params p, int* status) {
+    using C = D8Config<BN, SWAP, PAIR>;
     extern __shared__ uint8_t smem_raw[];
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* sf = base + C::STAGES * C::STAGE;
-    uint8_t* staged = sf + D8_SF_STAGES * D8_SF_BYTES;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(staged + (BN >= 128 ? C::STAGED : 0));
+    uint8_t* staged = base + C::STAGES * C::STAGE;               // (on 1024 bytes, as the swizzle of the output's boxes needs)
+    uint8_t* sf = staged + D8_EPI_WARPS * C::OUT_BYTES;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sf + D8_SF_STAGES * D8_SF_BYTES);
+    const uint32_t rank = PAIR ? cluster_ctarank() : 0;
     const uint32_t base_addr = smem_u32(base), sf_addr = smem_u32(sf);
     const uint32_t full = smem_u32(bars), empty = full + 8 * C::STAGES, sf_full = empty + 8 * C::STAGES, sf_empty = sf_full + 8 * D8_SF_STAGES;
     const uint32_t acc_full = sf_empty + 8 * D8_SF_STAGES, acc_empty = acc_full + 8 * C::ACC, slot = acc_empty + 8 * C::ACC;
 
     if (t == 0) {
         for (int s = 0; s < C::STAGES; ++s) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 1); }
-        for (int s = 0; s < D8_SF_STAGES; ++s) { mbar_init(sf_full + 8 * s, 1); mbar_init(sf_empty + 8 * s, 1); }
-        for (int s = 0; s < C::ACC; ++s) { mbar_init(acc_full + 8 * s, 1); mbar_init(acc_empty + 8 * s, D8_EPI_WARPS); }
+        for (int s = 0; s < D8_SF_STAGES; ++s) { mbar_init(sf_full + 8 * s, 2 * C::CTAS); mbar_init(sf_empty + 8 * s, 1); }
+        for (int s = 0; s < C::ACC; ++s) { mbar_init(acc_full + 8 * s, 1); mbar_init(acc_empty + 8 * s, D8_EPI_WARPS * C::CTAS); }
         fence_barrier_init();
     }
-    if (warp == 1) tmem_alloc(slot, 512);
+    if (warp == 1) {
+        if (PAIR) tmem_alloc_pair(slot, 512);
+        else tmem_alloc(slot, 512);
+    }
     tc_fence_before_sync();
     __syncthreads();
+    if (PAIR) cluster_sync_all();                                // both CTAs' barriers exist before anything signals them
     tc_fence_after_sync();
     uint32_t tmem;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(slot));
@@ -162,10 +224,11 @@ dense8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     chain_next();
 
     const int split = p.splits > 1 ? (int)cluster_ctarank() : 0;
-    const int first = blockIdx.x / p.splits, stride = gridDim.x / p.splits;
+    const int share = PAIR ? 2 : p.splits, first = blockIdx.x / share, stride = gridDim.x / share;
     // this CTA's groups of the reduction (numbered over all its components)
     const int all_groups = p.comps * p.groups;
-    const int g_begin = (int)((long long)all_groups * split / p.splits), g_end = (int)((long long)all_groups * (split + 1) / p.splits);
+    const int g_begin = (int)((long long)all_groups * split / p.splits), g_end = (int)((long long)all_groups * (split + 1) / p.splits), j_begin = g_begin / p.groups;
+    D8Walk w;
 
     if (warp == 0) {
         int s = 0;
@@ -174,36 +237,43 @@ dense8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         for (int tile = first; tile < p.tiles && ok; tile += stride) {
             int c, mt, nt;
             d8_tile(p, tile, c, mt, nt);
-            for (int g = g_begin; g < g_end && ok; ++g) {
-                const int j = g / p.groups, k0 = (g - j * p.groups) * 4, k1 = min(k0 + 4, p.chunks);
-                int first_comp, second_comp;
-                bool neg;
-                d8_term(p, c, j, first_comp, second_comp, neg);
-                const int ca = SWAP ? second_comp : first_comp, cb = SWAP ? first_comp : second_comp;
+            for (w.start(p, c, g_begin, g_end, j_begin); w.left > 0 && ok; w.step(p, c)) {
+                const int k0 = w.group * 4, k1 = k0 + w.blocks(p), ca = SWAP ? w.second : w.first, cb = SWAP ? w.first : w.second;
                 for (int k = k0; k < k1; ++k) {
                     ok = warp_wait_bounded(empty + 8 * s, par, status, ST_D8_PRODUCER);
                     if (!ok) break;
                     if (elect_one()) {
                         const uint32_t a = base_addr + s * C::STAGE, b = a + D8_A_BYTES, bar = full + 8 * s;
-                        mbar_arrive_expect_tx(bar, D8_A_BYTES + BN * D8_BK);
-                        if (p.a_mn) tma_load_3d(a, &map_a, mt * D8_BM, k * D8_BK, ca, bar);
-                        else tma_load_3d(a, &map_a, k * D8_BK, mt * D8_BM, ca, bar);
-                        if (BN >= 128 && p.b_mn) {
-#pragma unroll
-                            for (int h = 0; h < BN / 128; ++h) tma_load_3d(b + h * 128 * D8_BK, &map_b, nt * BN + h * 128, k * D8_BK, cb, bar);
-                        } else tma_load_3d(b, &map_b, k * D8_BK, nt * BN, cb, bar);
+                        const int m0 = mt * C::M + (int)rank * D8_BM, n0 = nt * BN + (PAIR ? (int)rank * C::B_ROWS : 0);
+                        if constexpr (PAIR) {
+                            // one box of either operand per CTA; the even CTA's barrier counts the bytes of both
+                            const uint32_t lead = map_to_cta(bar, 0);
+                            if (rank == 0) mbar_arrive_expect_tx(bar, 2 * C::STAGE);
+                            tma_load_3d_pair(a, &map_a, p.a_mn ? m0 : k * D8_BK, p.a_mn ? k * D8_BK : m0, ca, lead);
+                            tma_load_3d_pair(b, &map_b, p.b_mn ? n0 : k * D8_BK, p.b_mn ? k * D8_BK : n0, cb, lead);
+                        } else {
+                            mbar_arrive_expect_tx(bar, D8_A_BYTES + BN * D8_BK);
+                            tma_load_3d(a, &map_a, p.a_mn ? m0 : k * D8_BK, p.a_mn ? k * D8_BK : m0, ca, bar);
+                            tma_load_3d(b, &map_b, p.b_mn ? n0 : k * D8_BK, p.b_mn ? k * D8_BK : n0, cb, bar);
+                        }
                     }
                     __syncwarp();
                     if (++s == C::STAGES) { s = 0; par ^= 1u; }
                 }
             }
         }
+    } else if (warp == 1 && rank != 0) {
     } else if (warp == 1) {
         const bool elected = elect_one();              // one lane issues and commits throughout
         int s = 0, q = 0, acc = 0;
         uint32_t par = 0, sf_par = 0, acc_par = 1;
         bool ok = true;
         const bool a_mn = p.a_mn, b_mn = BN >= 128 && p.b_mn;
+        // a barrier of both CTAs, by its address in the even one
+        auto commit_both = [&](uint32_t bar) {
+            if constexpr (PAIR) { mma_commit_pair(map_to_cta(bar, 0)); mma_commit_pair(map_to_cta(bar, 1)); }
+            else mma_commit(bar);
+        };
         const uint32_t a_step = a_mn ? 32 * 128 / 16 : 32 / 16, b_step = b_mn ? 32 * 128 / 16 : 32 / 16;
         const uint32_t sfa = tmem + C::SF_COL, sfb = sfa + 4;
         for (int tile = first; tile < p.tiles && ok; tile += stride) {
@@ -214,111 +284,136 @@ dense8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             tc_fence_after_sync();
             const uint32_t d = tmem + acc * C::ACC_COLS;
             uint32_t accumulate = 0;
-            for (int g = g_begin; g < g_end && ok; ++g) {
-                const int j = g / p.groups, k0 = (g - j * p.groups) * 4, k1 = min(k0 + 4, p.chunks);
-                int first_comp, second_comp;
-                bool neg;
-                d8_term(p, c, j, first_comp, second_comp, neg);
-                const uint32_t idesc = d8_idesc(D8_BM, BN, a_mn, b_mn, neg);
-                ok = warp_wait_bounded(sf_full + 8 * q, sf_par, status, ST_D8_MMA);
+            for (w.start(p, c, g_begin, g_end, j_begin); w.left > 0 && ok; w.step(p, c)) {
+                const int blocks = w.blocks(p);
+                const uint32_t idesc = d8_idesc(C::M, BN, a_mn, b_mn, w.neg);
+                ok = PAIR ? warp_wait_acquire_cluster(sf_full + 8 * q, sf_par, status, ST_D8_MMA) : warp_wait_bounded(sf_full + 8 * q, sf_par, status, ST_D8_MMA);
                 if (!ok) break;
                 tc_fence_after_sync();
                 if (elected) {
                     const uint32_t src = sf_addr + q * D8_SF_BYTES;
-                    copy_scales(sfa, src);
-                    copy_scales(sfb, src + 512);
-                    if (BN > 128) copy_scales(sfb + 4, src + 1024);
+                    copy_scales<PAIR>(sfa, src);
+                    copy_scales<PAIR>(sfb, src + 512);
+                    if (BN > 128) copy_scales<PAIR>(sfb + 4, src + 1024);
                 }
                 __syncwarp();
-                for (int k = k0; k < k1; ++k) {
+                for (int k = 0; k < blocks; ++k) {
                     ok = warp_wait_bounded(full + 8 * s, par, status, ST_D8_MMA);
                     if (!ok) break;
                     tc_fence_after_sync();
                     if (elected) {
                         const uint32_t a = base_addr + s * C::STAGE, b = a + D8_A_BYTES;
-                        const uint64_t da = make_desc_kmajor(a), db = b_mn ? make_desc_mnmajor(b, 128 * D8_BK) : make_desc_kmajor(b);
-                        const uint32_t id = idesc | ((uint32_t)(k & 3) << 4) | ((uint32_t)(k & 3) << 29);
+                        const uint64_t da = make_desc_kmajor(a), db = make_desc_kmajor(b);      // (tiles of 128 rows: one block of 128 bytes in either majorness)
+                        const uint32_t id = idesc | ((uint32_t)k << 4) | ((uint32_t)k << 29);      // byte k of the scales' words
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            mma_mxf8(d, (uint32_t)da + i * a_step, (uint32_t)(da >> 32), (uint32_t)db + i * b_step, (uint32_t)(db >> 32), id, sfa, sfb, accumulate);
+                            mma_mxf8<PAIR>(d, (uint32_t)da + i * a_step, (uint32_t)(da >> 32), (uint32_t)db + i * b_step, (uint32_t)(db >> 32), id, sfa, sfb, accumulate);
                             accumulate = 1;
                         }
-                        mma_commit(empty + 8 * s);
+                        commit_both(empty + 8 * s);
                     }
                     accumulate = 1;
                     __syncwarp();
                     if (++s == C::STAGES) { s = 0; par ^= 1u; }
                 }
                 if (!ok) break;
-                if (elected) mma_commit(sf_empty + 8 * q);
+                if (elected) commit_both(sf_empty + 8 * q);
                 __syncwarp();
                 if (++q == D8_SF_STAGES) { q = 0; sf_par ^= 1u; }
             }
             if (!ok) break;
-            if (elected) mma_commit(acc_full + 8 * acc);
+            if (elected) commit_both(acc_full + 8 * acc);
             __syncwarp();
             if (++acc == C::ACC) { acc = 0; acc_par ^= 1u; }
         }
-    } else if (warp == 2) {
+    } else if (warp < 4) {
+        // Warp 2 the scales of A, warp 3 those of B, a group of the reduction at a time. The words of the next group are loaded before those of this one are waited for: one
+        // warp that loaded them when they were due took 2600 clocks a group, where the MMAs of a group take 2048.
+        const bool b_side = warp == 3;
+        const bool blocks = b_side ? p.b_blocks : p.a_blocks;
+        const uint8_t* scales = b_side ? p.b_scales : p.a_scales;
+        const int bk = b_side ? p.b_bk : p.a_bk, bm = b_side ? p.b_bm : p.a_bm, bc = b_side ? p.b_bc : p.a_bc, extent = b_side ? p.n : p.m;
+        constexpr int SETS = BN > 128 ? 2 : 1;                   // sets of 128 rows of B
+        struct Words { uint32_t w[SETS][4]; };
+        int tile = first, c = 0, row0[SETS];
+        const uint8_t* at[SETS];                                 // where this lane's words (blocks: byte) of the walk's group lie
+        auto aim = [&]() {
+            const int comp = SWAP == b_side ? w.first : w.second;
+#pragma unroll
+            for (int h = 0; h < SETS; ++h)
+                at[h] = blocks ? scales + (size_t)comp * bc + (size_t)(row0[h] / 128) * bm + (size_t)(w.group * 4 + (lane & 3)) * bk
+                               : scales + (((size_t)comp * p.groups + w.group) * extent + row0[h] + lane) * 4;
+        };
+        auto begin = [&]() {
+            if (tile >= p.tiles) return;
+            int mt, nt;
+            d8_tile(p, tile, c, mt, nt);
+#pragma unroll
+            for (int h = 0; h < SETS; ++h) row0[h] = b_side ? nt * BN + h * 128 : mt * C::M + (int)rank * D8_BM;
+            w.start(p, c, g_begin, g_end, j_begin);
+            aim();
+        };
+        begin();
+        // the words of rows row0 + lane + 32 i: what lane puts at byte 16 * lane of a set of 128 rows
+        auto load = [&](Words& out) {
+            if (tile >= p.tiles) return;
+#pragma unroll
+            for (int h = 0; h < SETS; ++h) {
+                if (h > 0 && !b_side) break;
+                if (blocks) {
+                    // (a set of 128 rows that starts on a multiple of 128 lies in one block: lane e loads the byte of block e of the reduction)
+                    out.w[h][0] = row0[h] < extent && w.group * 4 + (lane & 3) < p.chunks ? *reinterpret_cast<const volatile uint8_t*>(at[h]) : 127u;
+                    at[h] += 4 * (size_t)bk;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) out.w[h][i] = ld_chained(reinterpret_cast<const uint32_t*>(at[h]) + 32 * i, row0[h] + lane + 32 * i < extent);
+                    at[h] += 4 * (size_t)extent;
+                }
+            }
+            const int j = w.j;
+            w.step(p, c);
+            if (w.left == 0) { tile += stride; begin(); }
+            else if (w.j != j) aim();
+        };
         int q = 0;
         uint32_t par = 1;
         bool ok = true;
-        // the words of rows row0 + lane + 32 i: what lane puts at byte 16 * lane of a set of 128 rows
-        auto gather = [&](bool blocks, const uint8_t* scales, int bk, int bm, int bc, int comp, int group, int row0, int extent) {
-            uint32_t w[4];
-            if (blocks) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    // (blocks of 128 rows: a set of 128 rows that starts on a multiple of 128 lies in one)
-                    uint32_t word = 0;
-                    if (i == 0) {
-                        const uint8_t* src = scales + (size_t)comp * bc + (size_t)(row0 / 128) * bm;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            word |= (uint32_t)(row0 < extent && group * 4 + e < p.chunks ? *reinterpret_cast<const volatile uint8_t*>(src + (size_t)(group * 4 + e) * bk) : 127) << (8 * e);
-                        w[0] = word;
-                    } else w[i] = w[0];
-                }
-            } else {
-                const uint32_t* src = reinterpret_cast<const uint32_t*>(scales) + ((size_t)comp * p.groups + group) * extent + row0 + lane;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = row0 + lane + 32 * i < extent ? ld_chained(src + 32 * i) : 0x7f7f7f7fu;
-            }
-            return make_uint4(w[0], w[1], w[2], w[3]);
-        };
-        for (int tile = first; tile < p.tiles && ok; tile += stride) {
-            int c, mt, nt;
-            d8_tile(p, tile, c, mt, nt);
-            for (int g = g_begin; g < g_end && ok; ++g) {
-                const int j = g / p.groups, group = g - j * p.groups;
-                int first_comp, second_comp;
-                bool neg;
-                d8_term(p, c, j, first_comp, second_comp, neg);
-                const int ca = SWAP ? second_comp : first_comp, cb = SWAP ? first_comp : second_comp;
-                const uint4 wa = gather(p.a_blocks, p.a_scales, p.a_bk, p.a_bm, p.a_bc, ca, group, mt * D8_BM, p.m);
-                uint4 wb[2];
-                wb[0] = gather(p.b_blocks, p.b_scales, p.b_bk, p.b_bm, p.b_bc, cb, group, nt * BN, p.n);
-                if (BN > 128) wb[1] = gather(p.b_blocks, p.b_scales, p.b_bk, p.b_bm, p.b_bc, cb, group, nt * BN + 128, p.n);
+        Words next, now;
+        load(next);
+        for (int t_ = first; t_ < p.tiles && ok; t_ += stride)
+            for (int i = g_begin; i < g_end && ok; ++i) {
+                now = next;
+                load(next);
                 ok = warp_wait_bounded(sf_empty + 8 * q, par, status, ST_D8_SCALES);
                 if (!ok) break;
-                const uint32_t dst = sf_addr + q * D8_SF_BYTES + lane * 16;
-                st_shared_v4(dst, wa.x, wa.y, wa.z, wa.w);
-                st_shared_v4(dst + 512, wb[0].x, wb[0].y, wb[0].z, wb[0].w);
-                if (BN > 128) st_shared_v4(dst + 1024, wb[1].x, wb[1].y, wb[1].z, wb[1].w);
+                const uint32_t dst = sf_addr + q * D8_SF_BYTES + (b_side ? 512 : 0) + lane * 16;
+#pragma unroll
+                for (int h = 0; h < SETS; ++h) {
+                    if (h > 0 && !b_side) break;
+                    uint32_t* v = now.w[h];
+                    if (blocks) {
+                        const uint32_t word = __shfl_sync(0xffffffffu, v[0], 0) | (__shfl_sync(0xffffffffu, v[0], 1) << 8) | (__shfl_sync(0xffffffffu, v[0], 2) << 16) |
+                                              (__shfl_sync(0xffffffffu, v[0], 3) << 24);
+                        v[0] = v[1] = v[2] = v[3] = word;
+                    }
+                    st_shared_v4(dst + h * 512, v[0], v[1], v[2], v[3]);
+                }
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (elect_one()) mbar_arrive(sf_full + 8 * q);
+                if (elect_one()) {
+                    if constexpr (PAIR) mbar_arrive_release_cluster(map_to_cta(sf_full + 8 * q, 0));
+                    else mbar_arrive(sf_full + 8 * q);
+                }
                 __syncwarp();
                 if (++q == D8_SF_STAGES) { q = 0; par ^= 1u; }
             }
-        }
     } else if (warp >= 4) {
         const int quarter = warp & 3, half = (warp - 4) >> 2;
         constexpr int COLS = BN < 64 ? 32 : BN / 2;               // columns per warp; with a narrow tile the second four warps have none
         constexpr int BLOCKS = COLS / 32;
         const bool idle = BN < 64 && half > 0;
         const int col0 = half * COLS;
-        const uint32_t buf = smem_u32(staged) + (warp - 4) * EPI_ROWS_BYTES;
+        const uint32_t buf = smem_u32(staged) + (warp - 4) * C::OUT_BYTES;
         const int fast = SWAP ? p.m : p.n;
         int acc = 0;
         uint32_t par = 0;
@@ -341,10 +436,13 @@ dense8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             }
             tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive(acc_empty + 8 * acc);
+            if (lane == 0) {
+                if constexpr (PAIR) mbar_arrive_cluster(map_to_cta(acc_empty + 8 * acc, 0));
+                else mbar_arrive(acc_empty + 8 * acc);
+            }
             if (++acc == C::ACC) { acc = 0; par ^= 1u; }
             if (idle) continue;
-            const int row = quarter * 32 + lane, m = mt * D8_BM + row, n0 = nt * BN + col0;
+            const int row = quarter * 32 + lane, row0 = mt * C::M + (int)rank * D8_BM + quarter * 32, m = row0 + lane, n0 = nt * BN + col0;
             if (p.splits > 1) {
                 // partial sums to shared memory (the ring: every MMA has read it), the fast axis of the output contiguous
                 float* part = reinterpret_cast<float*>(base);
@@ -377,31 +475,43 @@ dense8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
 #pragma unroll
                         for (int e = 0; e < 32; ++e) v[b][e] = __float_as_uint(__uint_as_float(v[b][e]) + __shfl_sync(0xffffffffu, add, e));
                     }
-                    // vectors of 16 bytes where every row's piece of the tile starts on them
-                    const bool whole = n + 32 <= p.n;
-                    if (p.dtype == PCB_F32) {
-                        float* out = static_cast<float*>(p.out) + comp0 + (long long)m * p.out_ld + n;
-                        if (whole && p.out_ld % 4 == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.out_comp % 4 == 0) {
-                            if (m < p.m)
-#pragma unroll
-                                for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(out + e) = make_uint4(v[b][e], v[b][e + 1], v[b][e + 2], v[b][e + 3]);
-                        } else store_floats(buf, v[b], static_cast<float*>(p.out) + comp0 + (long long)(mt * D8_BM + quarter * 32) * p.out_ld + n, p.m - (mt * D8_BM + quarter * 32),
-                                            p.n - n, p.out_ld, lane);
-                    } else {
-                        uint32_t packed[16];
+                    uint32_t packed[16];
+                    if (p.dtype != PCB_F32) {
 #pragma unroll
                         for (int e = 0; e < 16; ++e) packed[e] = pack_16(__uint_as_float(v[b][2 * e]), __uint_as_float(v[b][2 * e + 1]), p.dtype);
-                        uint16_t* out = static_cast<uint16_t*>(p.out) + comp0 + (long long)m * p.out_ld + n;
-                        if (whole && p.out_ld % 8 == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.out_comp % 8 == 0) {
-                            if (m < p.m)
+                    }
+                    if (p.out_map) {
+                        // rows of 128 bytes (64 or 32 columns), swizzled as the output's boxes are; the copy leaves out what lies beyond the output
+                        const bool f32 = p.dtype == PCB_F32;
+                        if (f32 || (b & 1) == 0) {
+                            if (lane == 0) bulk_wait_read_all();
+                            __syncwarp();
+                        }
+                        const uint32_t line = buf + lane * 128;
+                        if (f32) {
 #pragma unroll
-                                for (int e = 0; e < 16; e += 4) *reinterpret_cast<uint4*>(out + 2 * e) = make_uint4(packed[e], packed[e + 1], packed[e + 2], packed[e + 3]);
-                        } else store_rows<1>(buf, packed, static_cast<uint16_t*>(p.out) + comp0 + (long long)(mt * D8_BM + quarter * 32) * p.out_ld, m < p.m ? lane * p.out_ld : -1,
-                                             n + lane < p.n ? n + lane : -1, lane);
+                            for (int e = 0; e < 8; ++e) st_shared_v4(line + ((e ^ (lane & 7)) << 4), v[b][4 * e], v[b][4 * e + 1], v[b][4 * e + 2], v[b][4 * e + 3]);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) st_shared_v4(line + (((e + 4 * (b & 1)) ^ (lane & 7)) << 4), packed[4 * e], packed[4 * e + 1], packed[4 * e + 2], packed[4 * e + 3]);
+                        }
+                        if (f32 || (b & 1) || n + 32 >= p.n) {
+                            fence_proxy_async_smem();
+                            __syncwarp();
+                            if (lane == 0 && row0 < p.m) {
+                                tma_store_3d(&map_out, buf, f32 ? n : n - 32 * (b & 1), row0, c);
+                                bulk_commit_group();
+                            }
+                        }
+                    } else if (p.dtype == PCB_F32) {
+                        store_floats(buf, v[b], static_cast<float*>(p.out) + comp0 + (long long)row0 * p.out_ld + n, p.m - row0, p.n - n, p.out_ld, lane);
+                    } else {
+                        store_rows<1>(buf, packed, static_cast<uint16_t*>(p.out) + comp0 + (long long)row0 * p.out_ld, m < p.m ? lane * p.out_ld : -1, n + lane < p.n ? n + lane : -1, lane);
                     }
                 }
             }
         }
+        if (!SWAP && lane == 0) bulk_wait_all();
     }
     if (p.splits > 1) {
         // one tile per cluster: every CTA adds its share of the tile's elements, in the order of the ranks
@@ -430,9 +540,11 @@ dense8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     }
     tc_fence_before_sync();
     __syncthreads();
+    if (PAIR) cluster_sync_all();
     if (warp == 1) {
         tc_fence_after_sync();
-        tmem_dealloc(tmem, 512);
+        if (PAIR) tmem_dealloc_pair(tmem, 512);
+        else tmem_dealloc(tmem, 512);
     }
 }
 
@@ -444,14 +556,14 @@ int operand_map(CUtensorMap* map, const Q8Operand& o, int extent, int k, int com
     return make_tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, o.values, 3, dims, strides, box, nullptr, CU_TENSOR_MAP_SWIZZLE_128B, what);
 }
 
-template <int BN, bool SWAP>
+template <int BN, bool SWAP, bool PAIR>
 int launch(const Geom& g, const Q8Product& q, int splits, cudaStream_t stream) {
-    using C = D8Config<BN>;
+    using C = D8Config<BN, SWAP, PAIR>;
     D8Params p = {};
     p.pass = q.pass; p.ga = g.ga; p.comps = g.nc; p.neg = g.neg;
     p.m = q.m; p.n = q.n; p.k = q.k;
     p.chunks = q8_blocks(q.k); p.groups = q8_groups(q.k);
-    p.m_tiles = q8_blocks(q.m); p.n_tiles = (q.n + BN - 1) / BN; p.tiles = p.m_tiles * p.n_tiles * g.nc;
+    p.m_tiles = (q.m + C::M - 1) / C::M; p.n_tiles = (q.n + BN - 1) / BN; p.tiles = p.m_tiles * p.n_tiles * g.nc;
     p.splits = splits;
     p.a_mn = q.a.mn_major; p.b_mn = q.b.mn_major;
     p.a_blocks = q.a.block_scales; p.b_blocks = q.b.block_scales;
@@ -461,14 +573,23 @@ int launch(const Geom& g, const Q8Product& q, int splits, cudaStream_t stream) {
     p.dtype = q.dtype; p.out = q.out; p.bias = q.bias;
     p.out_ld = SWAP ? q.m : q.n;
     p.out_comp = (long long)q.m * q.n;
-    CUtensorMap ma, mb;
+    CUtensorMap ma, mb, mo = {};
     int rc = operand_map(&ma, q.a, q.m, q.k, g.nc, D8_BM, "8-bit operand A");
-    if (rc == PCB_OK) rc = operand_map(&mb, q.b, q.n, q.k, g.nc, BN, "8-bit operand B");
+    if (rc == PCB_OK) rc = operand_map(&mb, q.b, q.n, q.k, g.nc, PAIR ? C::B_ROWS : BN, "8-bit operand B");
+    const size_t size = dtype_size(q.dtype);
+    p.out_map = !SWAP && splits == 1 && q.n * size % 16 == 0 && reinterpret_cast<uintptr_t>(q.out) % 16 == 0;
+    if (rc == PCB_OK && p.out_map) {
+        const cuuint64_t dims[3] = {(cuuint64_t)q.n, (cuuint64_t)q.m, (cuuint64_t)g.nc}, strides[2] = {q.n * size, (cuuint64_t)q.n * q.m * size};
+        const cuuint32_t box[3] = {(cuuint32_t)(128 / size), 32, 1};
+        const CUtensorMapDataType type = q.dtype == PCB_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : (q.dtype == PCB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16);
+        rc = make_tensor_map(&mo, type, q.out, 3, dims, strides, box, nullptr, CU_TENSOR_MAP_SWIZZLE_128B, "8-bit product's output");
+    }
     if (rc != PCB_OK) return rc;
     const size_t smem = C::SMEM > ONE_CTA_SMEM ? C::SMEM : ONE_CTA_SMEM;
-    PCB_CUDA_TRY(cudaFuncSetAttribute(dense8_kernel<BN, SWAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    const int grid = splits > 1 ? p.tiles * splits : (p.tiles < sm_count() ? p.tiles : sm_count());
-    PCB_CUDA_TRY(launch_clusters(splits, true, dense8_kernel<BN, SWAP>, grid, D8_THREADS, smem, stream, ma, mb, p, q.status));
+    static_assert(C::SMEM <= MAX_CTA_SMEM, "shared memory of a CTA");
+    PCB_CUDA_TRY(cudaFuncSetAttribute(dense8_kernel<BN, SWAP, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    const int grid = PAIR ? 2 * (p.tiles < sm_pairs() ? p.tiles : sm_pairs()) : (splits > 1 ? p.tiles * splits : (p.tiles < sm_count() ? p.tiles : sm_count()));
+    PCB_CUDA_TRY(launch_clusters(PAIR ? 2 : splits, true, dense8_kernel<BN, SWAP, PAIR>, grid, D8_THREADS, smem, stream, ma, mb, mo, p, q.status));
     return PCB_OK;
 }
 
@@ -486,13 +607,13 @@ int q8_product(const Geom& g, const Q8Product& q, cudaStream_t stream) {
         return s;
     };
     if (q.swapped) {
-        if (q.n <= 16) return launch<16, true>(g, q, splits_for(16), stream);
-        if (q.n <= 64) return launch<64, true>(g, q, splits_for(64), stream);
-        return launch<128, true>(g, q, splits_for(128), stream);
+        if (q.n <= 16) return launch<16, true, false>(g, q, splits_for(16), stream);
+        if (q.n <= 64) return launch<64, true, false>(g, q, splits_for(64), stream);
+        return launch<128, true, false>(g, q, splits_for(128), stream);
     }
-    const long long wide = (long long)m_tiles * ((q.n + 255) / 256) * g.nc;
-    if (wide >= 2LL * sm_count()) return launch<256, false>(g, q, 1, stream);
-    return launch<128, false>(g, q, splits_for(128), stream);
+    const long long wide = (long long)((q.m + 255) / 256) * ((q.n + 255) / 256) * g.nc;
+    if (wide >= sm_pairs()) return launch<256, false, true>(g, q, 1, stream);
+    return launch<128, false, false>(g, q, splits_for(128), stream);
 }
 
 }  // namespace pcb
