@@ -29,14 +29,16 @@ __device__ __forceinline__ int scale_byte(uint32_t amax_bits) {            // e 
 }
 __device__ __forceinline__ float inverse_scale(int byte) { return __uint_as_float((uint32_t)(254 - byte) << 23); }   // 2^-e, byte in [1, 247]
 
-__device__ __forceinline__ uint32_t to_e4m3x4(float a, float b, float c, float d) {
-    uint16_t lo, hi;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
-    return (uint32_t)lo | ((uint32_t)hi << 16);
-}
-__device__ __forceinline__ float finite_or_nan(float v) {                  // (the conversion would saturate an infinity)
-    return (__float_as_uint(v) & 0x7fffffffu) == 0x7f800000u ? __uint_as_float(0x7fffffffu) : v;
+// two values times their scales, rounded
+__device__ __forceinline__ uint32_t to_e4m3x2(float a, float b, float2 s) {
+    unsigned long long v, f;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    asm("mov.b64 %0, {%1, %2};" : "=l"(f) : "f"(s.x), "f"(s.y));
+    asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(v) : "l"(f));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+    uint16_t q;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(q) : "f"(b), "f"(a));
+    return q;
 }
 
 // Eight neighbours as loaded. A key is a value's magnitude as bits (monotonic); a 32-bit word holds the keys of two 16-bit values or of one fp32 value.
@@ -50,7 +52,8 @@ template <> struct Eight<float> {
     static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return max(a, b); }
     static __device__ __forceinline__ uint32_t whole(uint32_t keys) { return keys; }                       // the largest key of a word
     static __device__ __forceinline__ uint32_t bits(uint32_t key) { return key; }                           // as fp32
-    __device__ __forceinline__ float value(int i) const { return __uint_as_float(w[i]); }
+    __device__ __forceinline__ void two(int j, float& a, float& b) const { a = __uint_as_float(w[2 * j]); b = __uint_as_float(w[2 * j + 1]); }
+    __device__ __forceinline__ void numbers(int j) { if (keys(w[j]) == INF_KEY) w[j] = 0x7fffffffu; }             // infinities to NaN: the conversion would saturate them
     __device__ __forceinline__ void zero() {
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[i] = 0;
@@ -88,7 +91,8 @@ template <> struct Eight<__half> : Eight16<__half> {
         return (lo < INF_KEY ? lo : 0u) | ((hi < INF_KEY ? hi : 0u) << 16);
     }
     static __device__ __forceinline__ uint32_t bits(uint32_t key) { return __float_as_uint(__half2float(__ushort_as_half((uint16_t)key))); }
-    __device__ __forceinline__ float value(int i) const { return __half2float(__ushort_as_half((uint16_t)(i & 1 ? w[i >> 1] >> 16 : w[i >> 1]))); }
+    __device__ __forceinline__ void two(int j, float& a, float& b) const { const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j])); a = f.x; b = f.y; }
+    __device__ __forceinline__ void numbers(int j) { w[j] |= ((keys(w[j]) & 0xffffu) == INF_KEY ? 0x7fffu : 0u) | (keys(w[j]) >> 16 == INF_KEY ? 0x7fff0000u : 0u); }
 };
 template <> struct Eight<__nv_bfloat16> : Eight16<__nv_bfloat16> {
     static constexpr uint32_t INF_KEY = 0x7f80u;
@@ -97,7 +101,8 @@ template <> struct Eight<__nv_bfloat16> : Eight16<__nv_bfloat16> {
         return (lo < INF_KEY ? lo : 0u) | ((hi < INF_KEY ? hi : 0u) << 16);
     }
     static __device__ __forceinline__ uint32_t bits(uint32_t key) { return key << 16; }
-    __device__ __forceinline__ float value(int i) const { return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16); }
+    __device__ __forceinline__ void two(int j, float& a, float& b) const { a = __uint_as_float(w[j] << 16); b = __uint_as_float(w[j] & 0xffff0000u); }
+    __device__ __forceinline__ void numbers(int j) { w[j] |= ((keys(w[j]) & 0xffffu) == INF_KEY ? 0x7fffu : 0u) | (keys(w[j]) >> 16 == INF_KEY ? 0x7fff0000u : 0u); }
 };
 
 enum { QT_ROWS = 1, QT_COLS = 2, QT_BLOCKS = 4 };
@@ -117,6 +122,7 @@ __global__ void __launch_bounds__(QT_THREADS, sizeof(T) == 4 ? 1 : 2) quantize_t
     typedef Eight<T> E;
     __shared__ uint32_t col_max[QT_WARPS][16 * E::WORDS];
     __shared__ uint32_t warp_max[QT_WARPS];
+    __shared__ __align__(16) float col_scale[Q8_BLOCK];
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31, c8 = (t & 15) * 8, r0 = t >> 4;
     const int comp = blockIdx.z, row_block = blockIdx.y, col_block = blockIdx.x;
     const int col = col_block * Q8_BLOCK + c8, first_row = row_block * Q8_BLOCK + r0;
@@ -158,27 +164,46 @@ __global__ void __launch_bounds__(QT_THREADS, sizeof(T) == 4 ? 1 : 2) quantize_t
             most = max(most, row_keys[i]);
         }
     }
-    auto store = [&](uint8_t* values, int i, const float (&s)[8]) {
-        const int row = first_row + QT_STEP * i;
-        if (row >= p.rows || col >= p.pitch) return;
-        float f[8];
+    // Rounds and stores the tile with a scale for each row (ROW) or each column.
+    auto store = [&](uint8_t* values, auto scale_of) {
+        if (col >= p.pitch) return;
+        uint8_t* dst = values + ((size_t)comp * p.rows + first_row) * p.pitch + col;
+        if (odd) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = (odd ? finite_or_nan(v[i].value(j)) : v[i].value(j)) * s[j];
-        *reinterpret_cast<uint2*>(values + ((size_t)comp * p.rows + row) * p.pitch + col) = make_uint2(to_e4m3x4(f[0], f[1], f[2], f[3]), to_e4m3x4(f[4], f[5], f[6], f[7]));
+            for (int i = 0; i < QT_PER; ++i) {
+#pragma unroll
+                for (int j = 0; j < E::WORDS; ++j) v[i].numbers(j);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < QT_PER; ++i) {
+            if (first_row + QT_STEP * i >= p.rows) break;
+            uint32_t lo = 0, hi = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float a, b;
+                v[i].two(j, a, b);
+                const float2 s = scale_of(i, j);
+                const uint32_t q = to_e4m3x2(a, b, s);
+                if (j < 2) lo |= q << (16 * j);
+                else hi |= q << (16 * (j - 2));
+            }
+            *reinterpret_cast<uint2*>(dst + (size_t)QT_STEP * i * p.pitch) = make_uint2(lo, hi);
+        }
     };
     if constexpr ((MODE & QT_ROWS) != 0) {
+        float f[QT_PER];
 #pragma unroll
         for (int i = 0; i < QT_PER; ++i) {
             uint32_t m = row_keys[i];
 #pragma unroll
             for (int o = 8; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
             const int byte = scale_byte(E::bits(m)), row = first_row + QT_STEP * i;
-            const float f = inverse_scale(byte);
-            const float s[8] = {f, f, f, f, f, f, f, f};
-            store(p.row_values, i, s);
+            f[i] = inverse_scale(byte);
             if ((t & 15) == 0 && row < p.rows)
                 reinterpret_cast<uint8_t*>(p.row_words + ((size_t)comp * p.row_groups + (col_block >> 2)) * p.rows + row)[col_block & 3] = (uint8_t)byte;
         }
+        store(p.row_values, [&](int i, int) { return make_float2(f[i], f[i]); });
     }
     if constexpr ((MODE & QT_BLOCKS) != 0) {
         most = __reduce_max_sync(0xffffffffu, most);
@@ -188,9 +213,7 @@ __global__ void __launch_bounds__(QT_THREADS, sizeof(T) == 4 ? 1 : 2) quantize_t
         for (int w = 0; w < QT_WARPS; ++w) most = max(most, warp_max[w]);
         const int byte = scale_byte(E::bits(most));
         const float f = inverse_scale(byte);
-        const float s[8] = {f, f, f, f, f, f, f, f};
-#pragma unroll
-        for (int i = 0; i < QT_PER; ++i) store(p.row_values, i, s);
+        store(p.row_values, [&](int, int) { return make_float2(f, f); });
         if (t == 0) reinterpret_cast<uint8_t*>(p.row_words)[((size_t)comp * gridDim.y + row_block) * gridDim.x + col_block] = (uint8_t)byte;
     }
     if constexpr ((MODE & QT_COLS) != 0) {
@@ -198,29 +221,35 @@ __global__ void __launch_bounds__(QT_THREADS, sizeof(T) == 4 ? 1 : 2) quantize_t
 #pragma unroll
         for (int j = 0; j < E::WORDS; ++j) {
             m[j] = 0;
+            if (odd) {
 #pragma unroll
-            for (int i = 0; i < QT_PER; ++i) m[j] = E::larger(m[j], odd ? E::finite_keys(v[i].w[j]) : E::keys(v[i].w[j]));
+                for (int i = 0; i < QT_PER; ++i) m[j] = E::larger(m[j], E::finite_keys(v[i].w[j]));
+            } else {
+#pragma unroll
+                for (int i = 0; i < QT_PER; ++i) m[j] = E::larger(m[j], E::keys(v[i].w[j]));
+            }
             m[j] = E::larger(m[j], __shfl_xor_sync(0xffffffffu, m[j], 16));       // the warp's other half holds other rows of these columns
             if (lane < 16) col_max[warp][lane * E::WORDS + j] = m[j];
         }
         __syncthreads();
-        float s[8];
-#pragma unroll
-        for (int j = 0; j < E::WORDS; ++j) {
+        // the first eight warps' threads each join a word of the sixteen warps' and leave the inverse scales of its columns
+        constexpr int PER = 8 / E::WORDS;                                          // columns per word
+        if (t < 16 * E::WORDS) {
             uint32_t k = 0;
 #pragma unroll
-            for (int w = 0; w < QT_WARPS; ++w) k = E::larger(k, col_max[w][(t & 15) * E::WORDS + j]);
-            constexpr int PER = 8 / E::WORDS;                                      // columns per word
+            for (int w = 0; w < QT_WARPS; ++w) k = E::larger(k, col_max[w][t]);
 #pragma unroll
             for (int h = 0; h < PER; ++h) {
-                const int byte = scale_byte(E::bits(PER == 1 ? k : (h ? k >> 16 : k & 0xffffu))), e = j * PER + h;
-                s[e] = inverse_scale(byte);
-                if (t < 16 && col + e < p.cols)
-                    reinterpret_cast<uint8_t*>(p.col_words + ((size_t)comp * p.col_groups + (row_block >> 2)) * p.cols + col + e)[row_block & 3] = (uint8_t)byte;
+                const int byte = scale_byte(E::bits(PER == 1 ? k : (h ? k >> 16 : k & 0xffffu))), e = t * PER + h, at = col_block * Q8_BLOCK + e;
+                col_scale[e] = inverse_scale(byte);
+                if (at < p.cols) reinterpret_cast<uint8_t*>(p.col_words + ((size_t)comp * p.col_groups + (row_block >> 2)) * p.cols + at)[row_block & 3] = (uint8_t)byte;
             }
         }
-#pragma unroll
-        for (int i = 0; i < QT_PER; ++i) store(p.col_values, i, s);
+        __syncthreads();
+        const float4 sa = *reinterpret_cast<const float4*>(&col_scale[c8]), sb = *reinterpret_cast<const float4*>(&col_scale[c8 + 4]);
+        store(p.col_values, [&](int, int j) {
+            return j == 0 ? make_float2(sa.x, sa.y) : (j == 1 ? make_float2(sa.z, sa.w) : (j == 2 ? make_float2(sb.x, sb.y) : make_float2(sb.z, sb.w)));
+        });
     }
 }
 

@@ -9,6 +9,7 @@
 // (16 exponentials per clock and SM are two thirds of what a pass over 16-bit logits takes at full bandwidth).
 // Few rows are cut over the CTAs of a cluster, whose maxima and sums are joined through distributed shared memory.
 #include "common.cuh"
+#include "packed.cuh"
 #include "tc_common.cuh"
 
 namespace pcb {
@@ -105,14 +106,8 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// Two fp32 values per instruction: a pass over 16-bit logits at full bandwidth is 11.5 logits per clock and SM, and one value per instruction (nine for a logit)
-// left it bound by issue slots, 4.6 TB/s.
-struct Pair { unsigned long long v; };
-__device__ __forceinline__ Pair pair(float a, float b) { Pair r; asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b)); return r; }
-__device__ __forceinline__ void halves(Pair p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p.v)); }
-__device__ __forceinline__ Pair operator+(Pair a, Pair b) { Pair r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
-__device__ __forceinline__ Pair operator*(Pair a, Pair b) { Pair r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
-__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) { Pair r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v)); return r; }
+// (Packed pairs: a pass over 16-bit logits at full bandwidth is 11.5 logits per clock and SM, and one value per instruction, nine instructions a logit, left it bound by
+// issue slots at 4.6 TB/s.)
 __device__ __forceinline__ Pair ex2(Pair x) {
     float a, b;
     halves(x, a, b);

@@ -13,6 +13,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "packed.cuh"
 #include "residual_norm.h"
 #include "tc_common.cuh"
 
@@ -54,23 +55,6 @@ template <typename T> struct Vec<T, 1> {
     static __device__ __forceinline__ raw pack(const float* v) { return (uint16_t)pack16<T>(v[0], 0.f); }
 };
 
-// VEC weights (fp32, ones where there are none). Plain loads: nothing marks these pointers as read-only, and the compiler may place them.
-template <int VEC>
-__device__ __forceinline__ void load_weights(const float* w, int f, bool ok, float* v) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = 1.f;
-    if (!w || !ok) return;
-    if (VEC == 1) {
-        v[0] = w[f];
-    } else {
-#pragma unroll
-        for (int i = 0; i < VEC; i += 4) {
-            const float4 a = *reinterpret_cast<const float4*>(w + f + i);
-            v[i] = a.x; v[i + 1] = a.y; v[i + 2] = a.z; v[i + 3] = a.w;
-        }
-    }
-}
-
 // Sum over the threads of a row: a warp, or the whole CTA of WPR warps. `turn` alternates between two sets of words.
 template <int WPR>
 __device__ __forceinline__ float row_sum(float v, float (*words)[32], int& turn) {
@@ -80,11 +64,16 @@ __device__ __forceinline__ float row_sum(float v, float (*words)[32], int& turn)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (lane == 0) words[turn][warp] = v;
     __syncthreads();
-    v = lane < WPR ? words[turn][lane] : 0.f;
+    v = words[turn][lane & (WPR - 1)];
 #pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    for (int o = WPR / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     turn ^= 1;
     return v;
+}
+template <int WPR>
+__device__ __forceinline__ void row_sync() {
+    if (WPR == 1) __syncwarp();
+    else __syncthreads();
 }
 
 // Where value e of a sample lies: component e / F, feature e % F.
@@ -93,223 +82,319 @@ __device__ __forceinline__ int comp_of(const RNParams& p, int e) { return p.comp
 // Threads of a CTA: four rows of one warp each, or one row.
 __host__ __device__ constexpr int rn_threads(int wpr) { return wpr == 1 ? 128 : 32 * wpr; }
 
-// ---- rows on their way in: a ring of row buffers in shared memory, filled by cp.async some rows ahead, so that the loads in flight cost no registers.
-// With VEC > 1 a thread copies exactly the 16 bytes that it reads later and nobody else's (its slots lie 16 * threads bytes apart), so that no barrier is needed. With
-// VEC == 1 (rows that start anywhere) the threads of a row copy the aligned 16-byte units that cover each component's values; units are cut where the tensor ends.
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// bytes of one component's values of a row in the ring, VEC == 1
-__host__ __device__ inline int segment_bytes(int features, int size) { return (features * size + 14 + 15) / 16 * 16; }
+// A thread's values of a row, EPT of them in pairs, and the ring of row buffers in shared memory that cp.async fills some rows ahead, so that loads in flight cost
+// no registers. Everything that does not change from row to row is worked out once: with 8 values per thread and that arithmetic in the loop a row
+// took 44 instructions a value, and the pass was bound by issue slots at 4.1 TB/s.
+//   VEC > 1    a thread owns vectors of 16 bytes, tid + TPR * i; it copies exactly what it reads later, and no barrier is needed for that
+//   VEC == 1   rows start anywhere: a thread owns values tid + TPR * i; the threads of a row copy the aligned 16-byte units that cover each component's values
+//              (cut where the tensor ends) and wait for each other
+constexpr int RN_RING_BYTES = 218 * 1024;      // of all CTAs of an SM
+template <typename T, int VEC, int EPT, int WPR, int TENSORS, int MAX_STAGES, int PER_SM>
+struct Row {
+    static constexpr int TPR = 32 * WPR, THREADS = rn_threads(WPR), ROWS = THREADS / TPR, NV = EPT / VEC, PAIRS = EPT / 2, SIZE = sizeof(T);
+    static constexpr int TENSOR = VEC > 1 ? NV * TPR * 16 : TPR * EPT * SIZE + 8 * 32;        // bytes of a tensor's row (eight components, each with up to 29 bytes around it)
+    static constexpr int STAGE = TENSORS * TENSOR, FIT = RN_RING_BYTES / PER_SM / (ROWS * STAGE), STAGES = FIT < 1 ? 1 : (FIT < MAX_STAGES ? FIT : MAX_STAGES);
+    static constexpr size_t SMEM = (size_t)ROWS * STAGES * STAGE;
+    static constexpr int UNITS = VEC > 1 ? NV : (TENSOR / 16 + TPR - 1) / TPR;               // 16-byte units that a thread copies
+    static constexpr int RAW = SIZE == 4 ? EPT : PAIRS;                                       // registers of a tensor's values as loaded
+    uint32_t base;
+    int tid, width;
+    uint32_t off[NV];                       // element of vector (value) i relative to its row: component * (rows - 1) * F + e
+    uint32_t feature[NV];
+    uint32_t live;                          // bit i: vector (value) i exists
+    // VEC == 1
+    uint32_t at[VEC > 1 ? 1 : NV];          // shared-memory offset of value i without its component's shift
+    uint32_t phase[VEC > 1 ? 1 : NV];       // bytes modulo 16 at which its component starts
+    uint32_t unit_in[VEC > 1 ? 1 : UNITS], unit_dst[VEC > 1 ? 1 : UNITS];
+    int unit_comp[VEC > 1 ? 1 : UNITS];     // -1: none
 
-constexpr int RN_RING_BYTES = 220 * 1024;      // of all CTAs of an SM
-template <typename T, int VEC, int NV, int WPR, int MAX_TENSORS, int MAX_STAGES, int PER_SM>
-struct Ring {
-    static constexpr int TPR = 32 * WPR, THREADS = rn_threads(WPR);
-    static constexpr int MOST = MAX_TENSORS * (VEC > 1 ? NV * THREADS * 16 : (THREADS / TPR) * (TPR * NV * (int)sizeof(T) + 8 * 32));   // bytes of a stage at most
-    static constexpr int FIT = RN_RING_BYTES / PER_SM / MOST, STAGES = FIT < 1 ? 1 : (FIT < MAX_STAGES ? FIT : MAX_STAGES);
-    uint32_t base;          // this row's part of the ring
-    int stage_bytes, tensor_bytes, seg;
-    __device__ __forceinline__ Ring(uint32_t smem, const RNParams& p, int tensors) {
-        if (VEC > 1) {
-            tensor_bytes = NV * THREADS * 16;
-            stage_bytes = tensors * tensor_bytes;
-            base = smem + threadIdx.x * 16;
-            seg = 0;
-        } else {
-            seg = segment_bytes(p.features, sizeof(T));
-            tensor_bytes = p.comps * seg;
-            stage_bytes = tensors * tensor_bytes;
-            base = smem + (threadIdx.x / TPR) * STAGES * stage_bytes;
+    __device__ __forceinline__ Row(uint32_t smem, const RNParams& p) {
+        tid = threadIdx.x % TPR;
+        width = p.comps * p.features;
+        base = smem + (threadIdx.x / TPR) * STAGES * STAGE;
+        live = 0;
+        const int seg = (p.features * SIZE + 14 + 15) / 16 * 16;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int e = (i * TPR + tid) * VEC, c = comp_of(p, e);
+            if (e < width) live |= 1u << i;
+            off[i] = (uint32_t)c * (uint32_t)(p.n - 1) * (uint32_t)p.features + e;
+            feature[i] = e - c * p.features;
+            if constexpr (VEC == 1) {
+                at[i] = c * seg + feature[i] * SIZE;
+                phase[i] = (uint32_t)c * (uint32_t)p.n * (uint32_t)p.features * SIZE & 15u;
+            }
+        }
+        if constexpr (VEC == 1) {
+            const int units = seg / 16;
+#pragma unroll
+            for (int i = 0; i < UNITS; ++i) {
+                const int u = i * TPR + tid, c = u / units;
+                unit_comp[i] = c < p.comps ? c : -1;
+                unit_in[i] = (u - c * units) * 16;
+                unit_dst[i] = u * 16;
+            }
         }
     }
-    static size_t bytes(const RNParams& p, int tensors) {
-        return VEC > 1 ? (size_t)STAGES * tensors * NV * THREADS * 16 : (size_t)(THREADS / TPR) * STAGES * tensors * p.comps * segment_bytes(p.features, sizeof(T));
-    }
-    // starts the copy of a row of tensor k ([comps][rows of the tensor][features]) into a stage
-    __device__ __forceinline__ void fetch(const RNParams& p, int stage, int k, const void* tensor, int row, int rows) const {
-        const int tid = threadIdx.x % TPR, width = p.comps * p.features;
-        const uint32_t dst = base + stage * stage_bytes + k * tensor_bytes;
-        if (VEC > 1) {
+    // starts the copies of a row of each tensor (null: none)
+    __device__ __forceinline__ void fetch(const RNParams& p, int stage, int row, const void* const (&tensors)[TENSORS]) const {
+        const uint32_t dst = base + stage * STAGE;
+        if constexpr (VEC > 1) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const int e = (i * TPR + tid) * VEC, c = comp_of(p, e);
-                if (e < width) copy16(dst + i * THREADS * 16, static_cast<const T*>(tensor) + (size_t)row * p.features + (size_t)c * (rows - 1) * p.features + e, 16);
+                if (!(live >> i & 1)) continue;
+                const size_t byte = ((size_t)row * p.features + off[i]) * SIZE;
+#pragma unroll
+                for (int k = 0; k < TENSORS; ++k)
+                    if (tensors[k]) copy16(dst + k * TENSOR + (i * TPR + tid) * 16, static_cast<const uint8_t*>(tensors[k]) + byte, 16);
             }
         } else {
-            const size_t end = (size_t)p.comps * rows * p.features * sizeof(T);
-            const int units = seg / 16;
-            for (int u = tid; u < p.comps * units; u += TPR) {
-                const int c = p.comps == 1 ? 0 : u / units, in = u - c * units;
-                const size_t first = ((size_t)c * rows + row) * p.features * sizeof(T), at = (first & ~size_t(15)) + (size_t)in * 16;
-                if (at < first + (size_t)p.features * sizeof(T)) copy16(dst + c * seg + in * 16, static_cast<const uint8_t*>(tensor) + at, (uint32_t)(end - at < 16 ? end - at : 16));
+            const size_t line = (size_t)p.features * SIZE, end = (size_t)p.comps * p.n * line;
+#pragma unroll
+            for (int i = 0; i < UNITS; ++i) {
+                if (unit_comp[i] < 0) continue;
+                const size_t first = ((size_t)unit_comp[i] * p.n + row) * line, from = (first & ~size_t(15)) + unit_in[i];
+                if (from >= first + line) continue;
+                const uint32_t bytes = end - from < 16 ? (uint32_t)(end - from) : 16u;
+#pragma unroll
+                for (int k = 0; k < TENSORS; ++k)
+                    if (tensors[k]) copy16(dst + k * TENSOR + unit_dst[i], static_cast<const uint8_t*>(tensors[k]) + from, bytes);
             }
         }
     }
-    // value (VEC > 1: vector) i of this thread, of a row fetched before
-    __device__ __forceinline__ typename Vec<T, VEC>::raw get(const RNParams& p, int stage, int k, int i, int row, int rows) const {
-        typedef typename Vec<T, VEC>::raw raw;
-        const int tid = threadIdx.x % TPR;
-        uint32_t at = base + stage * stage_bytes + k * tensor_bytes;
-        raw r = raw();
+    // this thread's values of tensor k of a row that has arrived, as loaded (zeros where there are none)
+    __device__ __forceinline__ void get(const RNParams& p, int stage, int row, int k, uint32_t (&raw)[RAW]) const {
+        const uint32_t src = base + stage * STAGE + k * TENSOR;
         if constexpr (VEC > 1) {
-            at += i * THREADS * 16;
-            if ((i * TPR + tid) * VEC < p.comps * p.features) r = ld_shared_v4(at);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                if (live >> i & 1) v = ld_shared_v4(src + (i * TPR + tid) * 16);
+                raw[4 * i] = v.x; raw[4 * i + 1] = v.y; raw[4 * i + 2] = v.z; raw[4 * i + 3] = v.w;
+            }
         } else {
-            const int e = i * TPR + tid, c = comp_of(p, e);
-            if (e < p.comps * p.features) {
-                const uint32_t shift = ((uint32_t)c * (uint32_t)rows + (uint32_t)row) * (uint32_t)p.features * (uint32_t)sizeof(T) & 15u;
-                at += c * seg + shift + (e - c * p.features) * sizeof(T);
-                if constexpr (sizeof(T) == 4) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r) : "r"(at) : "memory");
-                else asm volatile("ld.shared.u16 %0, [%1];" : "=h"(r) : "r"(at) : "memory");
+            const uint32_t shift = (uint32_t)row * (uint32_t)p.features * SIZE;
+            uint32_t v[NV];
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const uint32_t a = src + at[i] + ((phase[i] + shift) & 15u);
+                v[i] = 0;
+                if (live >> i & 1) {
+                    if constexpr (SIZE == 4) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[i]) : "r"(a) : "memory");
+                    else {
+                        uint16_t h;
+                        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(a) : "memory");
+                        v[i] = h;
+                    }
+                }
+            }
+            if constexpr (SIZE == 4) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i) raw[i] = v[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < PAIRS; ++i) raw[i] = v[2 * i] | (v[2 * i + 1] << 16);
             }
         }
-        return r;
+    }
+    __device__ __forceinline__ static Pair value(const uint32_t (&raw)[RAW], int q) {
+        if constexpr (SIZE == 4) return pair(__uint_as_float(raw[2 * q]), __uint_as_float(raw[2 * q + 1]));
+        else return pair(from16<T>(raw[q] & 0xffffu), from16<T>(raw[q] >> 16));
+    }
+    // values of a tensor in global memory: `row` of a tensor of `rows` rows per component
+    __device__ __forceinline__ void load(const RNParams& p, const void* tensor, int row, int rows, uint32_t (&raw)[RAW]) const {
+        typedef typename Vec<T, VEC>::raw R;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = comp_of(p, (i * TPR + tid) * VEC);
+            const R* src = reinterpret_cast<const R*>(static_cast<const T*>(tensor) + ((size_t)c * rows + row) * p.features + feature[i]);
+            const R v = ld_chained(src, live >> i & 1);
+            if constexpr (VEC > 1) { raw[4 * i] = v.x; raw[4 * i + 1] = v.y; raw[4 * i + 2] = v.z; raw[4 * i + 3] = v.w; }
+            else if constexpr (SIZE == 4) raw[i] = v;
+            else raw[i / 2] = i & 1 ? raw[i / 2] | ((uint32_t)v << 16) : (uint32_t)v;
+        }
+    }
+    __device__ __forceinline__ void store(void* tensor, size_t row_element, const Pair (&v)[PAIRS]) const {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if (!(live >> i & 1)) continue;
+            T* dst = static_cast<T*>(tensor) + row_element + off[i];
+            if constexpr (VEC > 1) {
+                float f[VEC];
+#pragma unroll
+                for (int j = 0; j < VEC / 2; ++j) halves(v[i * (VEC / 2) + j], f[2 * j], f[2 * j + 1]);
+                *reinterpret_cast<uint4*>(dst) = Vec<T, VEC>::pack(f);
+            } else {
+                float a, b;
+                halves(v[i / 2], a, b);
+                const float f[1] = {i & 1 ? b : a};
+                *reinterpret_cast<typename Vec<T, 1>::raw*>(dst) = Vec<T, 1>::pack(f);
+            }
+        }
+    }
+    __device__ __forceinline__ void store_gate(const RNParams& p, void* tensor, int group, const Pair (&v)[PAIRS]) const {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if (!(live >> i & 1)) continue;
+            const int c = comp_of(p, (i * TPR + tid) * VEC);
+            T* dst = static_cast<T*>(tensor) + ((size_t)c * p.groups + group) * p.features + feature[i];
+            float f[VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                float a, b;
+                halves(v[(i * VEC + j) / 2], a, b);
+                f[j] = (i * VEC + j) & 1 ? b : a;
+            }
+            *reinterpret_cast<typename Vec<T, VEC>::raw*>(dst) = Vec<T, VEC>::pack(f);
+        }
+    }
+    // weights of this thread's features (plain loads: nothing marks these pointers as read-only, and the compiler may place them); ones where there are none
+    __device__ __forceinline__ void weights(const float* w, Pair (&v)[PAIRS]) const {
+#pragma unroll
+        for (int q = 0; q < PAIRS; ++q) v[q] = pair(1.f);
+        if (!w) return;
+        if constexpr (VEC > 1) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                if (!(live >> i & 1)) continue;
+#pragma unroll
+                for (int j = 0; j < VEC; j += 4) {
+                    const float4 a = *reinterpret_cast<const float4*>(w + feature[i] + j);
+                    v[(i * VEC + j) / 2] = pair(a.x, a.y);
+                    v[(i * VEC + j) / 2 + 1] = pair(a.z, a.w);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int q = 0; q < PAIRS; ++q) v[q] = pair(live >> (2 * q) & 1 ? w[feature[2 * q]] : 1.f, live >> (2 * q + 1) & 1 ? w[feature[2 * q + 1]] : 1.f);
+        }
+    }
+    // adds up in fp32: out[e] of this thread's values
+    __device__ __forceinline__ void store_sums(float* out, const Pair (&v)[PAIRS]) const {
+#pragma unroll
+        for (int q = 0; q < PAIRS; ++q) {
+            float a, b;
+            halves(v[q], a, b);
+            if constexpr (VEC > 1) {
+                const int i = 2 * q / VEC;
+                if (live >> i & 1) *reinterpret_cast<float2*>(out + (i * TPR + tid) * VEC + 2 * q % VEC) = make_float2(a, b);
+            } else {
+                if (live >> (2 * q) & 1) out[2 * q * TPR + tid] = a;
+                if (live >> (2 * q + 1) & 1) out[(2 * q + 1) * TPR + tid] = b;
+            }
+        }
     }
 };
 
 // Rows of a group of threads: piece `slot` of `slots` nearly equal runs of consecutive rows.
 __device__ __forceinline__ int run_start(int rows, int slot, int slots) { return (int)((long long)rows * slot / slots); }
 
-template <int WPR>
-__device__ __forceinline__ void row_sync() {
-    if (WPR == 1) __syncwarp();
-    else __syncthreads();
-}
-
 constexpr int RN_FWD_STAGES = 4, RN_BWD_STAGES = 3;
-template <typename T, int VEC, int NV, int WPR, int PER_SM> using FwdRing = Ring<T, VEC, NV, WPR, 3, RN_FWD_STAGES, PER_SM>;   // x, branch, a gate for each value
-template <typename T, int VEC, int NV, int WPR, int PER_SM> using BwdRing = Ring<T, VEC, NV, WPR, 5, RN_BWD_STAGES, PER_SM>;   // y, dh, dy, branch, a gate for each value
+template <typename T, int VEC, int EPT, int WPR, int PER_SM> using FwdRow = Row<T, VEC, EPT, WPR, 3, RN_FWD_STAGES, PER_SM>;              // x, branch, a gate for each value
+template <typename T, int VEC, int EPT, int WPR, int GATE, int PER_SM> using BwdRow = Row<T, VEC, EPT, WPR, GATE == 1 ? 5 : 4, RN_BWD_STAGES, PER_SM>;   // y, dh, dy, branch, gate
 
-template <typename T, int VEC, int NV, int WPR, int PER_SM>
+template <typename T, int VEC, int EPT, int WPR, int PER_SM>
 __global__ void __launch_bounds__(rn_threads(WPR), PER_SM) residual_norm_fwd_kernel(const RNParams p) {
-    typedef Vec<T, VEC> V;
-    typedef typename V::raw raw;
-    typedef FwdRing<T, VEC, NV, WPR, PER_SM> R;
-    constexpr int TPR = 32 * WPR, ROWS = rn_threads(WPR) / TPR, STAGES = R::STAGES;
+    typedef FwdRow<T, VEC, EPT, WPR, PER_SM> R;
+    constexpr int STAGES = R::STAGES, PAIRS = R::PAIRS;
     extern __shared__ __align__(16) uint8_t ring_smem[];
     __shared__ float words[2][32];
-    const int tid = threadIdx.x % TPR, sub = threadIdx.x / TPR, width = p.comps * p.features;
-    const bool own_gates = p.gate && p.groups == p.n;            // a gate for each value
-    const R ring(smem_u32(ring_smem), p, own_gates ? 3 : 2);
+    const R r(smem_u32(ring_smem), p);
     int turn = 0;
     chain_wait();
     chain_next();
-    const float inv_width = 1.f / (float)width;
-    const int slots = gridDim.x * ROWS, slot = blockIdx.x * ROWS + sub;
+    const bool own_gates = p.gate && p.groups == p.n;            // a gate for each value
+    const float inv_width = 1.f / (float)r.width;
+    const int slots = gridDim.x * R::ROWS, slot = blockIdx.x * R::ROWS + threadIdx.x / R::TPR;
     const int begin = run_start(p.n, slot, slots), end = run_start(p.n, slot + 1, slots);
-    auto fetch = [&](int row) {
-        if (row < end) {
-            const int stage = (row - begin) % STAGES;
-            ring.fetch(p, stage, 0, p.x, row, p.n);
-            if (p.branch) ring.fetch(p, stage, 1, p.branch, row, p.n);
-            if (own_gates) ring.fetch(p, stage, 2, p.gate, row, p.n);
-        }
+    const void* const tensors[3] = {p.x, p.branch, own_gates ? p.gate : nullptr};
+    auto fetch = [&](int row, int stage) {
+        if (row < end) r.fetch(p, stage, row, tensors);
         copies_commit();
     };
-    for (int i = 0; i < STAGES; ++i) fetch(begin + i);
-    raw gr[NV];
-    int group = -1;
+    for (int i = 0; i < STAGES; ++i) fetch(begin + i, i);
+    uint32_t graw[R::RAW];
+    int group_end = 0, stage = 0;                                // (shared gates: the row behind the present group)
     // (with a CTA per row the runs of all its threads are one; with a warp per row there are no barriers)
     for (int row = begin; row < end; ++row) {
-        const int stage = (row - begin) % STAGES;
         copies_wait<STAGES - 1>();
         if (VEC == 1) row_sync<WPR>();
-        if (p.gate && !own_gates && row / p.per_group != group) {
-            group = row / p.per_group;
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int e = (i * TPR + tid) * VEC, c = comp_of(p, e);
-                gr[i] = ld_chained(reinterpret_cast<const raw*>(static_cast<const T*>(p.gate) + (size_t)group * p.features + (size_t)c * (p.groups - 1) * p.features + e), e < width);
-            }
+        if (p.gate && !own_gates && row >= group_end) {
+            const int group = row / p.per_group;
+            group_end = (group + 1) * p.per_group;
+            r.load(p, p.gate, group, p.groups, graw);
         }
-        const size_t row_at = (size_t)row * p.features;
-        float y[NV][VEC];
-        raw br[NV];
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            V::unpack(ring.get(p, stage, 0, i, row, p.n), y[i]);
-            if (p.branch) br[i] = ring.get(p, stage, 1, i, row, p.n);
-            if (own_gates) gr[i] = ring.get(p, stage, 2, i, row, p.n);
-        }
+        Pair y[PAIRS];
         float rb = 0.f;
-        if (!p.branch) row_sync<WPR>();
-        if (p.branch) {
-            float sum = 0.f;
+        {
+            uint32_t xraw[R::RAW], braw[R::RAW];
+            r.get(p, stage, row, 0, xraw);
+            if (p.branch) r.get(p, stage, row, 1, braw);
+            if (own_gates) r.get(p, stage, row, 2, graw);
+            if (p.branch) {
+                Pair s = pair(0.f);
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                float v[VEC];
-                V::unpack(br[i], v);
+                for (int q = 0; q < PAIRS; ++q) { const Pair b = R::value(braw, q); s = fma2(b, b, s); }
+                rb = rsqrtf(row_sum<WPR>(sum(s), words, turn) * inv_width + p.eps);
+            } else row_sync<WPR>();
+            fetch(row + STAGES, stage);                          // into the stage that every thread of the row has read by now
+            if (p.branch) {
+                const Pair f = pair(p.scale * rb);
+                Pair w[PAIRS];
+                r.weights(p.post, w);
+                if (p.gate) {
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) sum = fmaf(v[j], v[j], sum);
+                    for (int q = 0; q < PAIRS; ++q) w[q] = w[q] * R::value(graw, q);
+                }
+#pragma unroll
+                for (int q = 0; q < PAIRS; ++q) y[q] = fma2(R::value(braw, q) * f, w[q], R::value(xraw, q));
+            } else {
+#pragma unroll
+                for (int q = 0; q < PAIRS; ++q) y[q] = R::value(xraw, q);
             }
-            rb = rsqrtf(row_sum<WPR>(sum, words, turn) * inv_width + p.eps);
         }
-        fetch(row + STAGES);                    // into the stage that every thread of the row has read by now
-        if (p.branch) {
-            const float f = p.scale * rb;
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int e = (i * TPR + tid) * VEC, c = comp_of(p, e);
-                float v[VEC], w[VEC], gv[VEC];
-                V::unpack(br[i], v);
-                load_weights<VEC>(p.post, e - c * p.features, e < width, w);
-                if (p.gate) V::unpack(gr[i], gv);
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) y[i][j] = fmaf(v[j] * f, p.gate ? w[j] * gv[j] : w[j], y[i][j]);
-            }
-        }
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int e = (i * TPR + tid) * VEC, c = comp_of(p, e);
-            if (p.y && e < width) *reinterpret_cast<raw*>(static_cast<T*>(p.y) + row_at + (size_t)c * (p.n - 1) * p.features + e) = V::pack(y[i]);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) sum = fmaf(y[i][j], y[i][j], sum);
-        }
+        const size_t at = (size_t)row * p.features;
+        if (p.y) r.store(p.y, at, y);
         float ry = 0.f;
         if (p.h) {
-            ry = rsqrtf(row_sum<WPR>(sum, words, turn) * inv_width + p.eps);
+            Pair s = pair(0.f), w[PAIRS];
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int e = (i * TPR + tid) * VEC, c = comp_of(p, e);
-                float w[VEC];
-                load_weights<VEC>(p.pre, e - c * p.features, e < width, w);
+            for (int q = 0; q < PAIRS; ++q) s = fma2(y[q], y[q], s);
+            r.weights(p.pre, w);
+            ry = rsqrtf(row_sum<WPR>(sum(s), words, turn) * inv_width + p.eps);
+            const Pair f = pair(ry);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) w[j] *= y[i][j] * ry;
-                if (e < width) *reinterpret_cast<raw*>(static_cast<T*>(p.h) + row_at + (size_t)c * (p.n - 1) * p.features + e) = V::pack(w);
-            }
+            for (int q = 0; q < PAIRS; ++q) y[q] = y[q] * f * w[q];
+            r.store(p.h, at, y);
         }
-        if (p.stats && tid == 0) { p.stats[row] = rb; p.stats[p.n + row] = ry; }
+        if (p.stats && r.tid == 0) { p.stats[row] = rb; p.stats[p.n + row] = ry; }
+        if (++stage == STAGES) stage = 0;
     }
     copies_wait<0>();
 }
 
-// SHARED: gates shared by the samples of a group, whose gradients are sums
-template <typename T, int VEC, int NV, int WPR, bool SHARED, int PER_SM>
+// GATE: 0 none, 1 a gate for each value, 2 gates shared by the samples of a group, whose gradients are sums
+template <typename T, int VEC, int EPT, int WPR, int GATE, int PER_SM>
 __global__ void __launch_bounds__(rn_threads(WPR), PER_SM) residual_norm_bwd_kernel(const RNParams p) {
-    typedef Vec<T, VEC> V;
-    typedef typename V::raw raw;
-    typedef BwdRing<T, VEC, NV, WPR, PER_SM> R;
-    constexpr int TPR = 32 * WPR, ROWS = rn_threads(WPR) / TPR, STAGES = R::STAGES;
+    typedef BwdRow<T, VEC, EPT, WPR, GATE, PER_SM> R;
+    constexpr int STAGES = R::STAGES, PAIRS = R::PAIRS;
     extern __shared__ __align__(16) uint8_t ring_smem[];
     __shared__ float words[2][32];
-    const int tid = threadIdx.x % TPR, sub = threadIdx.x / TPR, width = p.comps * p.features;
-    const bool own_gates = !SHARED && p.gate;                    // a gate for each value
-    const R ring(smem_u32(ring_smem), p, own_gates ? 5 : 4);
+    const R r(smem_u32(ring_smem), p);
     int turn = 0;
     chain_wait();
     chain_next();
-    const float inv_width = 1.f / (float)width;
-    float dpre[NV][VEC], dpost[NV][VEC], dgate[SHARED ? NV : 1][VEC];
+    const float inv_width = 1.f / (float)r.width;
+    Pair dpre[PAIRS], dpost[PAIRS], dgate[GATE == 2 ? PAIRS : 1];
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) dpre[i][j] = dpost[i][j] = 0.f;
-    const int slots = gridDim.x * ROWS, slot = blockIdx.x * ROWS + sub;
+    for (int q = 0; q < PAIRS; ++q) dpre[q] = dpost[q] = pair(0.f);
+    const int slots = gridDim.x * R::ROWS, slot = blockIdx.x * R::ROWS + threadIdx.x / R::TPR;
     // an item is a piece of a group of samples; the threads of a row take a run of items, whose rows follow each other
     const int item_begin = run_start(p.items, slot, slots), item_end = run_start(p.items, slot + 1, slots);
     auto item_row = [&](int item) {
@@ -317,133 +402,116 @@ __global__ void __launch_bounds__(rn_threads(WPR), PER_SM) residual_norm_bwd_ker
         return group * p.per_group + (int)((long long)p.per_group * part / p.parts);
     };
     const int begin = item_row(item_begin), end = item_begin < item_end ? item_row(item_end) : begin;
-    auto fetch = [&](int row) {
-        if (row < end) {
-            const int stage = (row - begin) % STAGES;
-            if (p.dh) { ring.fetch(p, stage, 0, p.y, row, p.n); ring.fetch(p, stage, 1, p.dh, row, p.n); }
-            if (p.dy) ring.fetch(p, stage, 2, p.dy, row, p.n);
-            if (p.branch) ring.fetch(p, stage, 3, p.branch, row, p.n);
-            if (own_gates) ring.fetch(p, stage, 4, p.gate, row, p.n);
-        }
+    const void* tensors[GATE == 1 ? 5 : 4];
+    tensors[0] = p.dh ? p.y : nullptr; tensors[1] = p.dh; tensors[2] = p.dy; tensors[3] = p.branch;
+    if constexpr (GATE == 1) tensors[4] = p.gate;
+    auto fetch = [&](int row, int stage) {
+        if (row < end) r.fetch(p, stage, row, *reinterpret_cast<const void* const(*)[GATE == 1 ? 5 : 4]>(&tensors));
         copies_commit();
     };
-    for (int i = 0; i < STAGES; ++i) fetch(begin + i);
-    raw gr[NV];
-    for (int item = item_begin; item < item_end; ++item) {
-        const int group = item / p.parts, last = item_row(item + 1);
-        if (SHARED) {
+    for (int i = 0; i < STAGES; ++i) fetch(begin + i, i);
+    uint32_t graw[GATE ? R::RAW : 1];
+    int item = item_begin, last = begin, stage = 0;              // last: the row behind the present item
+    if (GATE != 2) last = end;                                   // (nothing happens between the items of other gates)
+    --item;
+    for (int row = begin; row < end; ++row) {
+        if (GATE == 2 && row == last) {
+            ++item;
+            last = item_row(item + 1);
+            r.load(p, p.gate, item / p.parts, p.groups, *reinterpret_cast<uint32_t(*)[R::RAW]>(&graw));
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int e = (i * TPR + tid) * VEC, c = comp_of(p, e);
-                gr[i] = ld_chained(reinterpret_cast<const raw*>(static_cast<const T*>(p.gate) + (size_t)group * p.features + (size_t)c * (p.groups - 1) * p.features + e), e < width);
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) dgate[i][j] = 0.f;
-            }
+            for (int q = 0; q < PAIRS; ++q) dgate[q] = pair(0.f);
         }
-        for (int row = item_row(item); row < last; ++row) {
-            const int stage = (row - begin) % STAGES;
-            const size_t row_at = (size_t)row * p.features;
-            const float rb = p.branch ? ld_chained(p.stats + row) : 0.f, ry = p.dh ? ld_chained(p.stats + p.n + row) : 0.f;
-            copies_wait<STAGES - 1>();
-            if (VEC == 1) row_sync<WPR>();
-            raw br[NV];
-            float dx[NV][VEC], y[NV][VEC];
-            float sum = 0.f;
+        const float rb = p.branch ? ld_chained(p.stats + row) : 0.f, ry = p.dh ? ld_chained(p.stats + p.n + row) : 0.f;
+        copies_wait<STAGES - 1>();
+        if (VEC == 1) row_sync<WPR>();
+        uint32_t braw[R::RAW], yraw[R::RAW];
+        Pair dx[PAIRS];
+        if (p.dy) {
+            uint32_t raw[R::RAW];
+            r.get(p, stage, row, 2, raw);
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int e = (i * TPR + tid) * VEC, c = comp_of(p, e);
-                if (p.dy) V::unpack(ring.get(p, stage, 2, i, row, p.n), dx[i]);
-                else
+            for (int q = 0; q < PAIRS; ++q) dx[q] = R::value(raw, q);
+        } else {
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) dx[i][j] = 0.f;
-                if (p.branch) br[i] = ring.get(p, stage, 3, i, row, p.n);
-                if (own_gates) gr[i] = ring.get(p, stage, 4, i, row, p.n);
-                if (p.dh) {
-                    float t[VEC], w[VEC];
-                    V::unpack(ring.get(p, stage, 0, i, row, p.n), y[i]);
-                    V::unpack(ring.get(p, stage, 1, i, row, p.n), t);
-                    load_weights<VEC>(p.pre, e - c * p.features, e < width, w);
+            for (int q = 0; q < PAIRS; ++q) dx[q] = pair(0.f);
+        }
+        if (p.branch) r.get(p, stage, row, 3, braw);
+        if constexpr (GATE == 1) r.get(p, stage, row, 4, graw);
+        if (p.dh) {
+            uint32_t raw[R::RAW];
+            Pair w[PAIRS], s = pair(0.f);
+            r.get(p, stage, row, 0, yraw);
+            r.get(p, stage, row, 1, raw);
+            r.weights(p.pre, w);
+            const Pair f = pair(ry);
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) {
-                        const float yn = y[i][j] * ry;
-                        dpre[i][j] = fmaf(t[j], yn, dpre[i][j]);
-                        t[j] *= w[j];
-                        sum = fmaf(t[j], yn, sum);
-                        dx[i][j] = fmaf(t[j], ry, dx[i][j]);
+            for (int q = 0; q < PAIRS; ++q) {
+                const Pair yn = R::value(yraw, q) * f, dh = R::value(raw, q), t = dh * w[q];
+                dpre[q] = fma2(dh, yn, dpre[q]);
+                s = fma2(t, yn, s);
+                dx[q] = fma2(t, f, dx[q]);
+            }
+            const Pair m = pair(-(row_sum<WPR>(sum(s), words, turn) * inv_width * ry * ry));
+            fetch(row + STAGES, stage);                          // into the stage that every thread of the row has read by now
+#pragma unroll
+            for (int q = 0; q < PAIRS; ++q) dx[q] = fma2(m, R::value(yraw, q), dx[q]);
+        } else {
+            row_sync<WPR>();
+            fetch(row + STAGES, stage);
+        }
+        const size_t at = (size_t)row * p.features;
+        r.store(p.dx, at, dx);
+        if (p.branch) {
+            Pair w[PAIRS], s = pair(0.f);
+            r.weights(p.post, w);
+            const Pair f = pair(rb), scale = pair(p.scale);
+            if constexpr (GATE == 1) {
+                Pair dg[PAIRS];
+#pragma unroll
+                for (int q = 0; q < PAIRS; ++q) {
+                    const Pair u = R::value(braw, q) * f, sdx = scale * dx[q], dn = sdx * R::value(graw, q);
+                    dg[q] = sdx * u * w[q];
+                    dpost[q] = fma2(dn, u, dpost[q]);
+                    dx[q] = dn * w[q];
+                    s = fma2(dx[q], u, s);
+                }
+                if (p.dgate) r.store(p.dgate, at, dg);
+            } else {
+#pragma unroll
+                for (int q = 0; q < PAIRS; ++q) {
+                    const Pair u = R::value(braw, q) * f, sdx = scale * dx[q];
+                    Pair dn = sdx;
+                    if constexpr (GATE == 2) {
+                        dn = sdx * R::value(*reinterpret_cast<uint32_t(*)[R::RAW]>(&graw), q);
+                        dgate[q] = fma2(sdx * u, w[q], dgate[q]);
                     }
+                    dpost[q] = fma2(dn, u, dpost[q]);
+                    dx[q] = dn * w[q];
+                    s = fma2(dx[q], u, s);
                 }
             }
-            float f = 0.f;
-            if (p.dh) f = row_sum<WPR>(sum, words, turn) * inv_width * ry * ry;
-            else row_sync<WPR>();
-            fetch(row + STAGES);                // into the stage that every thread of the row has read by now
-            if (p.dh) {
+            const Pair m = pair(-(row_sum<WPR>(sum(s), words, turn) * inv_width * rb));
 #pragma unroll
-                for (int i = 0; i < NV; ++i)
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) dx[i][j] = fmaf(-f, y[i][j], dx[i][j]);
-            }
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int e = (i * TPR + tid) * VEC, c = comp_of(p, e);
-                if (e < width) *reinterpret_cast<raw*>(static_cast<T*>(p.dx) + row_at + (size_t)c * (p.n - 1) * p.features + e) = V::pack(dx[i]);
-            }
-            if (p.branch) {
-                sum = 0.f;
-#pragma unroll
-                for (int i = 0; i < NV; ++i) {
-                    const int e = (i * TPR + tid) * VEC, c = comp_of(p, e);
-                    float b[VEC], w[VEC], g[VEC], dg[VEC];
-                    V::unpack(br[i], b);
-                    load_weights<VEC>(p.post, e - c * p.features, e < width, w);
-                    if (SHARED || own_gates) V::unpack(gr[i], g);
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) {
-                        const float u = b[j] * rb, sdx = p.scale * dx[i][j], dn = SHARED || own_gates ? sdx * g[j] : sdx;
-                        dpost[i][j] = fmaf(dn, u, dpost[i][j]);
-                        dg[j] = sdx * u * w[j];
-                        if (SHARED) dgate[i][j] += dg[j];
-                        dx[i][j] = dn * w[j];
-                        sum = fmaf(dx[i][j], u, sum);
-                    }
-                    if (own_gates && p.dgate && e < width) *reinterpret_cast<raw*>(static_cast<T*>(p.dgate) + row_at + (size_t)c * (p.n - 1) * p.features + e) = V::pack(dg);
-                }
-                const float f = row_sum<WPR>(sum, words, turn) * inv_width * rb;
-#pragma unroll
-                for (int i = 0; i < NV; ++i) {
-                    const int e = (i * TPR + tid) * VEC, c = comp_of(p, e);
-                    float b[VEC];
-                    V::unpack(br[i], b);
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) b[j] = rb * fmaf(-f, b[j], dx[i][j]);
-                    if (e < width) *reinterpret_cast<raw*>(static_cast<T*>(p.dbranch) + row_at + (size_t)c * (p.n - 1) * p.features + e) = V::pack(b);
-                }
-            }
+            for (int q = 0; q < PAIRS; ++q) dx[q] = f * fma2(m, R::value(braw, q), dx[q]);
+            r.store(p.dbranch, at, dx);
         }
-        if (SHARED && p.dgate) {
+        if (GATE == 2 && row + 1 == last && p.dgate) {
+            const int group = item / p.parts;
+            if (p.parts == 1) {
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int e = (i * TPR + tid) * VEC, c = comp_of(p, e);
-                if (e >= width) continue;
-                if (p.parts == 1) {
-                    *reinterpret_cast<raw*>(static_cast<T*>(p.dgate) + (size_t)group * p.features + (size_t)c * (p.groups - 1) * p.features + e) = V::pack(dgate[i]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) p.part_gate[(size_t)item * width + e + j] = dgate[i][j];
-                }
-            }
+                for (int q = 0; q < PAIRS; ++q) dx[q] = dgate[q];
+                // (a row of the gate's gradient: component c at (c * groups + group) * F)
+                r.store_gate(p, p.dgate, group, dx);
+            } else r.store_sums(p.part_gate + (size_t)item * r.width, *reinterpret_cast<Pair(*)[PAIRS]>(&dgate));
         }
+        if (++stage == STAGES) stage = 0;
     }
     copies_wait<0>();
     if (p.part_w) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int e = (i * TPR + tid) * VEC;
-            if (e >= width) continue;
-            float* out = p.part_w + (size_t)slot * 2 * width + e;
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) { out[j] = dpre[i][j]; out[width + j] = dpost[i][j]; }
-        }
+        float* out = p.part_w + (size_t)slot * 2 * r.width;
+        r.store_sums(out, dpre);
+        r.store_sums(out + r.width, dpost);
     }
 }
 
@@ -620,34 +688,33 @@ cudaError_t norm_launch(K kernel, int grid, int threads, size_t smem, cudaStream
 }
 template <typename T, int VEC, int EPT, int WPR, int PER_SM>
 cudaError_t fwd_launch(const RNParams& p, cudaStream_t s) {
-    constexpr int NV = EPT / VEC, THREADS = rn_threads(WPR), ROWS = THREADS / (32 * WPR);
-    return norm_launch(residual_norm_fwd_kernel<T, VEC, NV, WPR, PER_SM>, grid_cap(p.n, ROWS, PER_SM), THREADS,
-                       FwdRing<T, VEC, NV, WPR, PER_SM>::bytes(p, p.gate && p.groups == p.n ? 3 : 2), s, p);
+    typedef FwdRow<T, VEC, EPT, WPR, PER_SM> R;
+    return norm_launch(residual_norm_fwd_kernel<T, VEC, EPT, WPR, PER_SM>, grid_cap(p.n, R::ROWS, PER_SM), R::THREADS, R::SMEM, s, p);
 }
 template <typename T, int VEC>
 cudaError_t fwd_any(const RNParams& p, cudaStream_t s) {
-    constexpr int H = VEC == 1 ? 2 : 1;                         // (addresses of single values cost registers: half the CTAs)
     const RNShape k = fwd_shape((long long)p.comps * p.features);
-    if (k.warps == 1) return fwd_launch<T, VEC, 16, 1, 6 / H>(p, s);
-    if (k.warps == 8) return fwd_launch<T, VEC, 8, 8, 4 / H>(p, s);
-    if (k.values == 8) return fwd_launch<T, VEC, 8, 16, 2 / H>(p, s);
-    if (k.values == 16) return fwd_launch<T, VEC, 16, 16, 1>(p, s);
-    return fwd_launch<T, VEC, 32, 16, 1>(p, s);
+    if (k.warps == 1) return k.values == 8 ? fwd_launch<T, VEC, 8, 1, 6>(p, s) : fwd_launch<T, VEC, 32, 1, 3>(p, s);
+    if (k.warps == 4) return k.values == 16 ? fwd_launch<T, VEC, 16, 4, 4>(p, s) : fwd_launch<T, VEC, 32, 4, 3>(p, s);
+    return k.warps == 8 ? fwd_launch<T, VEC, 32, 8, 1>(p, s) : fwd_launch<T, VEC, 32, 16, 1>(p, s);
 }
-template <typename T, int VEC, int NV, int WPR, int PER_SM>
+template <typename T, int VEC, int EPT, int WPR, int GATE, int PER_SM>
+cudaError_t bwd_gate(const RNParams& p, const RNPlan& q, cudaStream_t s) {
+    typedef BwdRow<T, VEC, EPT, WPR, GATE, PER_SM> R;
+    return norm_launch(residual_norm_bwd_kernel<T, VEC, EPT, WPR, GATE, PER_SM>, q.grid, R::THREADS, R::SMEM, s, p);
+}
+template <typename T, int VEC, int EPT, int WPR, int PER_SM>
 cudaError_t bwd_launch(const RNParams& p, const RNPlan& q, cudaStream_t s) {
-    const bool shared = p.gate && p.groups != p.n;
-    const size_t smem = BwdRing<T, VEC, NV, WPR, PER_SM>::bytes(p, p.gate && !shared ? 5 : 4);
-    return shared ? norm_launch(residual_norm_bwd_kernel<T, VEC, NV, WPR, true, PER_SM>, q.grid, rn_threads(WPR), smem, s, p)
-                  : norm_launch(residual_norm_bwd_kernel<T, VEC, NV, WPR, false, PER_SM>, q.grid, rn_threads(WPR), smem, s, p);
+    if (!p.gate) return bwd_gate<T, VEC, EPT, WPR, 0, PER_SM>(p, q, s);
+    return p.groups == p.n ? bwd_gate<T, VEC, EPT, WPR, 1, PER_SM>(p, q, s) : bwd_gate<T, VEC, EPT, WPR, 2, PER_SM>(p, q, s);
 }
 template <typename T, int VEC>
 cudaError_t bwd_any(const RNParams& p, const RNPlan& q, cudaStream_t s) {
     switch (q.shape.warps) {
-        case 1: return bwd_launch<T, VEC, 8 / VEC, 1, 4>(p, q, s);
-        case 4: return bwd_launch<T, VEC, 8 / VEC, 4, 4>(p, q, s);
-        case 8: return bwd_launch<T, VEC, 8 / VEC, 8, 2>(p, q, s);
-        default: return q.shape.values == 8 ? bwd_launch<T, VEC, 8 / VEC, 16, 1>(p, q, s) : bwd_launch<T, VEC, 16 / VEC, 16, 1>(p, q, s);
+        case 1: return q.shape.values == 8 ? bwd_launch<T, VEC, 8, 1, 4>(p, q, s) : bwd_launch<T, VEC, 16, 1, 3>(p, q, s);
+        case 4: return bwd_launch<T, VEC, 16, 4, 3>(p, q, s);
+        case 8: return bwd_launch<T, VEC, 16, 8, 2>(p, q, s);
+        default: return bwd_launch<T, VEC, 16, 16, 1>(p, q, s);
     }
 }
 template <typename T, int VEC>

@@ -26,18 +26,19 @@ struct RNParams {
 // Warps per row and values per thread for a width; warps 0: wider than the registers. CTAs per SM follow from registers and shared memory.
 struct RNShape { int warps, values, per_sm; };
 inline RNShape fwd_shape(long long width) {
-    if (width <= 32 * 16) return {1, 16, 6};
-    if (width <= 256 * 8) return {8, 8, 4};
-    if (width <= 512 * 8) return {16, 8, 2};
-    if (width <= 512 * 16) return {16, 16, 1};
+    if (width <= 32 * 8) return {1, 8, 6};
+    if (width <= 32 * 32) return {1, 32, 3};
+    if (width <= 128 * 16) return {4, 16, 4};
+    if (width <= 128 * 32) return {4, 32, 3};
+    if (width <= 256 * 32) return {8, 32, 1};
     if (width <= 512 * 32) return {16, 32, 1};
     return {0, 0, 4};
 }
 inline RNShape bwd_shape(long long width) {
     if (width <= 32 * 8) return {1, 8, 4};
-    if (width <= 128 * 8) return {4, 8, 4};
-    if (width <= 256 * 8) return {8, 8, 2};
-    if (width <= 512 * 8) return {16, 8, 1};
+    if (width <= 32 * 16) return {1, 16, 3};
+    if (width <= 128 * 16) return {4, 16, 3};
+    if (width <= 256 * 16) return {8, 16, 2};
     if (width <= 512 * 16) return {16, 16, 1};
     return {0, 0, 4};
 }
