@@ -55,32 +55,30 @@ template <typename T> struct Vec<T, 1> {
     static __device__ __forceinline__ raw pack(const float* v) { return (uint16_t)pack16<T>(v[0], 0.f); }
 };
 
-// Sum over the threads of a row: a warp, or the whole CTA of WPR warps. `turn` alternates between two sets of words.
+// The threads of a row (WPR warps; a CTA may hold several rows) wait for each other: barrier 1 + row of the CTA.
 template <int WPR>
-__device__ __forceinline__ float row_sum(float v, float (*words)[32], int& turn) {
+__device__ __forceinline__ void row_sync() {
+    if (WPR == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(1 + (int)threadIdx.x / (32 * WPR)), "n"(32 * WPR) : "memory");
+}
+// Sum over the threads of a row. `words`: two sets of a word per warp, used in turn.
+template <int WPR>
+__device__ __forceinline__ float row_sum(float v, float* words, int& turn) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if (WPR == 1) return v;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (lane == 0) words[turn][warp] = v;
-    __syncthreads();
-    v = words[turn][lane & (WPR - 1)];
+    const int warp = (threadIdx.x >> 5) % WPR, lane = threadIdx.x & 31;
+    if (lane == 0) words[turn * WPR + warp] = v;
+    row_sync<WPR>();
+    v = words[turn * WPR + (lane & (WPR - 1))];
 #pragma unroll
     for (int o = WPR / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     turn ^= 1;
     return v;
 }
-template <int WPR>
-__device__ __forceinline__ void row_sync() {
-    if (WPR == 1) __syncwarp();
-    else __syncthreads();
-}
 
 // Where value e of a sample lies: component e / F, feature e % F.
 __device__ __forceinline__ int comp_of(const RNParams& p, int e) { return p.comps == 1 ? 0 : (p.magic ? (int)__umulhi((uint32_t)e, p.magic) : e); }
-
-// Threads of a CTA: four rows of one warp each, or one row.
-__host__ __device__ constexpr int rn_threads(int wpr) { return wpr == 1 ? 128 : 32 * wpr; }
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -94,16 +92,21 @@ template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("c
 //   VEC > 1    a thread owns vectors of 16 bytes, tid + TPR * i; it copies exactly what it reads later, and no barrier is needed for that
 //   VEC == 1   rows start anywhere: a thread owns values tid + TPR * i; the threads of a row copy the aligned 16-byte units that cover each component's values
 //              (cut where the tensor ends) and wait for each other
-constexpr int RN_RING_BYTES = 218 * 1024;      // of all CTAs of an SM
-template <typename T, int VEC, int EPT, int WPR, int TENSORS, int MAX_STAGES, int PER_SM>
+// One CTA per SM holds ROWS rows at a time, and the weights in shared memory: the ring leaves no L1 to speak of, and weights that came from L2 for every row were as
+// many bytes as the rows (16384 x 4096 bf16: 115 us forward, 190 backward).
+constexpr int RN_SMEM = 218 * 1024;
+template <typename T, int VEC, int EPT, int WPR, int ROWS_, int TENSORS, int MAX_STAGES>
 struct Row {
-    static constexpr int TPR = 32 * WPR, THREADS = rn_threads(WPR), ROWS = THREADS / TPR, NV = EPT / VEC, PAIRS = EPT / 2, SIZE = sizeof(T);
+    static constexpr int ROWS = ROWS_, TPR = 32 * WPR, THREADS = ROWS * TPR, NV = EPT / VEC, PAIRS = EPT / 2, SIZE = sizeof(T);
     static constexpr int TENSOR = VEC > 1 ? NV * TPR * 16 : TPR * EPT * SIZE + 8 * 32;        // bytes of a tensor's row (eight components, each with up to 29 bytes around it)
-    static constexpr int STAGE = TENSORS * TENSOR, FIT = RN_RING_BYTES / PER_SM / (ROWS * STAGE), STAGES = FIT < 1 ? 1 : (FIT < MAX_STAGES ? FIT : MAX_STAGES);
-    static constexpr size_t SMEM = (size_t)ROWS * STAGES * STAGE;
+    static constexpr int STAGE = TENSORS * TENSOR, WEIGHTS = 2 * EPT * TPR * 4;               // bytes of a stage of one row; of both weights
+    static constexpr bool HELD = WEIGHTS + ROWS * STAGE <= RN_SMEM;                           // weights in shared memory
+    static constexpr int FIT = (RN_SMEM - (HELD ? WEIGHTS : 0)) / (ROWS * STAGE), STAGES = FIT < MAX_STAGES ? FIT : MAX_STAGES;
+    static_assert(STAGES >= 1, "a row of every tensor fits");
+    static constexpr size_t SMEM = (size_t)ROWS * STAGES * STAGE + (HELD ? WEIGHTS : 0);
     static constexpr int UNITS = VEC > 1 ? NV : (TENSOR / 16 + TPR - 1) / TPR;               // 16-byte units that a thread copies
     static constexpr int RAW = SIZE == 4 ? EPT : PAIRS;                                       // registers of a tensor's values as loaded
-    uint32_t base;
+    uint32_t base, held;                    // this row's ring; this thread's weights: four at a time (VEC == 1: one), TPR * 16 (4) bytes apart
     int tid, width;
     uint32_t off[NV];                       // element of vector (value) i relative to its row: component * (rows - 1) * F + e
     uint32_t feature[NV];
@@ -117,7 +120,8 @@ struct Row {
     __device__ __forceinline__ Row(uint32_t smem, const RNParams& p) {
         tid = threadIdx.x % TPR;
         width = p.comps * p.features;
-        base = smem + (threadIdx.x / TPR) * STAGES * STAGE;
+        base = smem + (HELD ? WEIGHTS : 0) + (threadIdx.x / TPR) * STAGES * STAGE;
+        held = smem + tid * (VEC > 1 ? 16 : 4);
         live = 0;
         const int seg = (p.features * SIZE + 14 + 15) / 16 * 16;
 #pragma unroll
@@ -254,8 +258,8 @@ struct Row {
             *reinterpret_cast<typename Vec<T, VEC>::raw*>(dst) = Vec<T, VEC>::pack(f);
         }
     }
-    // weights of this thread's features (plain loads: nothing marks these pointers as read-only, and the compiler may place them); ones where there are none
-    __device__ __forceinline__ void weights(const float* w, Pair (&v)[PAIRS]) const {
+    // Weights of this thread's features (`which`: 0 post, 1 pre; ones where there are none), from global memory: plain loads, nothing marks these pointers as read-only.
+    __device__ __forceinline__ void load_weights(const float* w, Pair (&v)[PAIRS]) const {
 #pragma unroll
         for (int q = 0; q < PAIRS; ++q) v[q] = pair(1.f);
         if (!w) return;
@@ -273,6 +277,47 @@ struct Row {
         } else {
 #pragma unroll
             for (int q = 0; q < PAIRS; ++q) v[q] = pair(live >> (2 * q) & 1 ? w[feature[2 * q]] : 1.f, live >> (2 * q + 1) & 1 ? w[feature[2 * q + 1]] : 1.f);
+        }
+    }
+    // the first row's threads put them into shared memory (followed by a barrier of the CTA)
+    __device__ __forceinline__ void hold_weights(const RNParams& p) const {
+        if (!HELD) return;
+        if (threadIdx.x < TPR) {
+#pragma unroll
+            for (int which = 0; which < 2; ++which) {
+                Pair v[PAIRS];
+                load_weights(which ? p.pre : p.post, v);
+                const uint32_t dst = held + which * (WEIGHTS / 2);
+#pragma unroll
+                for (int q = 0; q < PAIRS; ++q) {
+                    if constexpr (VEC > 1) asm volatile("st.shared.b64 [%0], %1;" ::"r"(dst + (q / 2) * TPR * 16 + (q & 1) * 8), "l"(v[q].v) : "memory");
+                    else {
+                        float a, b;
+                        halves(v[q], a, b);
+                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst + 2 * q * TPR * 4), "f"(a) : "memory");
+                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst + (2 * q + 1) * TPR * 4), "f"(b) : "memory");
+                    }
+                }
+            }
+        }
+        __syncthreads();
+    }
+    __device__ __forceinline__ void weights(const RNParams& p, int which, Pair (&v)[PAIRS]) const {
+        if constexpr (!HELD) load_weights(which ? p.pre : p.post, v);
+        else {
+            const uint32_t src = held + which * (WEIGHTS / 2);
+#pragma unroll
+            for (int q = 0; q < PAIRS; ++q) {
+                if constexpr (VEC > 1) {
+                    if (q & 1) continue;
+                    asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(v[q].v), "=l"(v[q + 1].v) : "r"(src + (q / 2) * TPR * 16));
+                } else {
+                    float a, b;
+                    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(a) : "r"(src + 2 * q * TPR * 4));
+                    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(b) : "r"(src + (2 * q + 1) * TPR * 4));
+                    v[q] = pair(a, b);
+                }
+            }
         }
     }
     // adds up in fp32: out[e] of this thread's values
@@ -296,26 +341,30 @@ struct Row {
 __device__ __forceinline__ int run_start(int rows, int slot, int slots) { return (int)((long long)rows * slot / slots); }
 
 constexpr int RN_FWD_STAGES = 4, RN_BWD_STAGES = 3;
-template <typename T, int VEC, int EPT, int WPR, int PER_SM> using FwdRow = Row<T, VEC, EPT, WPR, 3, RN_FWD_STAGES, PER_SM>;              // x, branch, a gate for each value
-template <typename T, int VEC, int EPT, int WPR, int GATE, int PER_SM> using BwdRow = Row<T, VEC, EPT, WPR, GATE == 1 ? 5 : 4, RN_BWD_STAGES, PER_SM>;   // y, dh, dy, branch, gate
+// OWN: a gate for each value
+template <typename T, int VEC, int EPT, int WPR, int ROWS, bool OWN> using FwdRow = Row<T, VEC, EPT, WPR, ROWS, OWN ? 3 : 2, RN_FWD_STAGES>;            // x, branch, gate
+template <typename T, int VEC, int EPT, int WPR, int ROWS, int GATE> using BwdRow = Row<T, VEC, EPT, WPR, ROWS, GATE == 1 ? 5 : 4, RN_BWD_STAGES>;      // y, dh, dy, branch, gate
 
-template <typename T, int VEC, int EPT, int WPR, int PER_SM>
-__global__ void __launch_bounds__(rn_threads(WPR), PER_SM) residual_norm_fwd_kernel(const RNParams p) {
-    typedef FwdRow<T, VEC, EPT, WPR, PER_SM> R;
+template <typename T, int VEC, int EPT, int WPR, int ROWS, bool OWN>
+__global__ void __launch_bounds__(32 * WPR * ROWS, 1) residual_norm_fwd_kernel(const RNParams p) {
+    typedef FwdRow<T, VEC, EPT, WPR, ROWS, OWN> R;
     constexpr int STAGES = R::STAGES, PAIRS = R::PAIRS;
     extern __shared__ __align__(16) uint8_t ring_smem[];
-    __shared__ float words[2][32];
+    __shared__ float all_words[R::ROWS][2 * WPR];
+    float* words = all_words[threadIdx.x / R::TPR];
     const R r(smem_u32(ring_smem), p);
     int turn = 0;
     chain_wait();
     chain_next();
-    const bool own_gates = p.gate && p.groups == p.n;            // a gate for each value
+    r.hold_weights(p);
     const float inv_width = 1.f / (float)r.width;
     const int slots = gridDim.x * R::ROWS, slot = blockIdx.x * R::ROWS + threadIdx.x / R::TPR;
     const int begin = run_start(p.n, slot, slots), end = run_start(p.n, slot + 1, slots);
-    const void* const tensors[3] = {p.x, p.branch, own_gates ? p.gate : nullptr};
+    const void* tensors[OWN ? 3 : 2];
+    tensors[0] = p.x; tensors[1] = p.branch;
+    if constexpr (OWN) tensors[2] = p.gate;
     auto fetch = [&](int row, int stage) {
-        if (row < end) r.fetch(p, stage, row, tensors);
+        if (row < end) r.fetch(p, stage, row, *reinterpret_cast<const void* const(*)[OWN ? 3 : 2]>(&tensors));
         copies_commit();
     };
     for (int i = 0; i < STAGES; ++i) fetch(begin + i, i);
@@ -325,7 +374,7 @@ __global__ void __launch_bounds__(rn_threads(WPR), PER_SM) residual_norm_fwd_ker
     for (int row = begin; row < end; ++row) {
         copies_wait<STAGES - 1>();
         if (VEC == 1) row_sync<WPR>();
-        if (p.gate && !own_gates && row >= group_end) {
+        if (!OWN && p.gate && row >= group_end) {
             const int group = row / p.per_group;
             group_end = (group + 1) * p.per_group;
             r.load(p, p.gate, group, p.groups, graw);
@@ -336,7 +385,7 @@ __global__ void __launch_bounds__(rn_threads(WPR), PER_SM) residual_norm_fwd_ker
             uint32_t xraw[R::RAW], braw[R::RAW];
             r.get(p, stage, row, 0, xraw);
             if (p.branch) r.get(p, stage, row, 1, braw);
-            if (own_gates) r.get(p, stage, row, 2, graw);
+            if constexpr (OWN) r.get(p, stage, row, 2, graw);
             if (p.branch) {
                 Pair s = pair(0.f);
 #pragma unroll
@@ -347,7 +396,7 @@ __global__ void __launch_bounds__(rn_threads(WPR), PER_SM) residual_norm_fwd_ker
             if (p.branch) {
                 const Pair f = pair(p.scale * rb);
                 Pair w[PAIRS];
-                r.weights(p.post, w);
+                r.weights(p, 0, w);
                 if (p.gate) {
 #pragma unroll
                     for (int q = 0; q < PAIRS; ++q) w[q] = w[q] * R::value(graw, q);
@@ -366,7 +415,7 @@ __global__ void __launch_bounds__(rn_threads(WPR), PER_SM) residual_norm_fwd_ker
             Pair s = pair(0.f), w[PAIRS];
 #pragma unroll
             for (int q = 0; q < PAIRS; ++q) s = fma2(y[q], y[q], s);
-            r.weights(p.pre, w);
+            r.weights(p, 1, w);
             ry = rsqrtf(row_sum<WPR>(sum(s), words, turn) * inv_width + p.eps);
             const Pair f = pair(ry);
 #pragma unroll
@@ -380,16 +429,18 @@ __global__ void __launch_bounds__(rn_threads(WPR), PER_SM) residual_norm_fwd_ker
 }
 
 // GATE: 0 none, 1 a gate for each value, 2 gates shared by the samples of a group, whose gradients are sums
-template <typename T, int VEC, int EPT, int WPR, int GATE, int PER_SM>
-__global__ void __launch_bounds__(rn_threads(WPR), PER_SM) residual_norm_bwd_kernel(const RNParams p) {
-    typedef BwdRow<T, VEC, EPT, WPR, GATE, PER_SM> R;
+template <typename T, int VEC, int EPT, int WPR, int ROWS, int GATE>
+__global__ void __launch_bounds__(32 * WPR * ROWS, 1) residual_norm_bwd_kernel(const RNParams p) {
+    typedef BwdRow<T, VEC, EPT, WPR, ROWS, GATE> R;
     constexpr int STAGES = R::STAGES, PAIRS = R::PAIRS;
     extern __shared__ __align__(16) uint8_t ring_smem[];
-    __shared__ float words[2][32];
+    __shared__ float all_words[R::ROWS][2 * WPR];
+    float* words = all_words[threadIdx.x / R::TPR];
     const R r(smem_u32(ring_smem), p);
     int turn = 0;
     chain_wait();
     chain_next();
+    r.hold_weights(p);
     const float inv_width = 1.f / (float)r.width;
     Pair dpre[PAIRS], dpost[PAIRS], dgate[GATE == 2 ? PAIRS : 1];
 #pragma unroll
@@ -443,7 +494,7 @@ __global__ void __launch_bounds__(rn_threads(WPR), PER_SM) residual_norm_bwd_ker
             Pair w[PAIRS], s = pair(0.f);
             r.get(p, stage, row, 0, yraw);
             r.get(p, stage, row, 1, raw);
-            r.weights(p.pre, w);
+            r.weights(p, 1, w);
             const Pair f = pair(ry);
 #pragma unroll
             for (int q = 0; q < PAIRS; ++q) {
@@ -464,7 +515,7 @@ __global__ void __launch_bounds__(rn_threads(WPR), PER_SM) residual_norm_bwd_ker
         r.store(p.dx, at, dx);
         if (p.branch) {
             Pair w[PAIRS], s = pair(0.f);
-            r.weights(p.post, w);
+            r.weights(p, 0, w);
             const Pair f = pair(rb), scale = pair(p.scale);
             if constexpr (GATE == 1) {
                 Pair dg[PAIRS];
@@ -509,9 +560,25 @@ __global__ void __launch_bounds__(rn_threads(WPR), PER_SM) residual_norm_bwd_ker
     }
     copies_wait<0>();
     if (p.part_w) {
-        float* out = p.part_w + (size_t)slot * 2 * r.width;
-        r.store_sums(out, dpre);
-        r.store_sums(out + r.width, dpost);
+        // the rows of the CTA together, in shared memory (nothing reads the ring any more)
+        float* out = p.part_w + (size_t)blockIdx.x * 2 * r.width;
+        if constexpr (R::ROWS > 1) {
+            static_assert((size_t)R::ROWS * 2 * EPT * R::TPR * 4 <= R::SMEM, "sums of the rows");
+            float* sums = reinterpret_cast<float*>(ring_smem);
+            __syncthreads();
+            float* mine = sums + (size_t)(threadIdx.x / R::TPR) * 2 * r.width;
+            r.store_sums(mine, dpre);
+            r.store_sums(mine + r.width, dpost);
+            __syncthreads();
+            for (int e = threadIdx.x; e < 2 * r.width; e += R::THREADS) {
+                float v = sums[e];
+                for (int k = 1; k < R::ROWS; ++k) v += sums[(size_t)k * 2 * r.width + e];
+                out[e] = v;
+            }
+        } else {
+            r.store_sums(out, dpre);
+            r.store_sums(out + r.width, dpost);
+        }
     }
 }
 
@@ -527,7 +594,7 @@ template <typename T> __device__ __forceinline__ void put(void* p, size_t i, flo
 template <typename T>
 __global__ void __launch_bounds__(RN_WIDE_THREADS) residual_norm_fwd_wide_kernel(const RNParams p) {
     constexpr int WPR = RN_WIDE_THREADS / 32;
-    __shared__ float words[2][32];
+    __shared__ float words[2 * WPR];
     int turn = 0;
     chain_wait();
     chain_next();
@@ -568,7 +635,7 @@ __global__ void __launch_bounds__(RN_WIDE_THREADS) residual_norm_fwd_wide_kernel
 template <typename T>
 __global__ void __launch_bounds__(RN_WIDE_THREADS) residual_norm_bwd_wide_kernel(const RNParams p) {
     constexpr int WPR = RN_WIDE_THREADS / 32;
-    __shared__ float words[2][32];
+    __shared__ float words[2 * WPR];
     int turn = 0;
     chain_wait();
     chain_next();
@@ -631,7 +698,7 @@ __global__ void __launch_bounds__(RN_WIDE_THREADS) residual_norm_bwd_wide_kernel
 }
 
 // Adds the pieces. Weights: eight columns (a sector) per CTA, the slots and components over 32 threads of each column. Gates: a thread per value.
-constexpr int RN_SUM_THREADS = 256;
+constexpr int RN_SUM_THREADS = 512;
 template <typename T>
 __global__ void __launch_bounds__(RN_SUM_THREADS) residual_norm_sum_kernel(const RNParams p, int slots, int weight_blocks) {
     const int width = p.comps * p.features;
@@ -642,7 +709,7 @@ __global__ void __launch_bounds__(RN_SUM_THREADS) residual_norm_sum_kernel(const
         const int col = threadIdx.x & 7, slice = threadIdx.x >> 3, f = blockIdx.x * 8 + col;
         float a = 0.f, b = 0.f;
         if (f < p.features) {
-#pragma unroll 4
+#pragma unroll 8
             for (int r = slice; r < slots * p.comps; r += RN_SUM_THREADS / 8) {
                 const int s = r / p.comps, c = r - s * p.comps;
                 const float* src = p.part_w + (size_t)s * 2 * width + (size_t)c * p.features + f;
@@ -686,32 +753,36 @@ cudaError_t norm_launch(K kernel, int grid, int threads, size_t smem, cudaStream
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_CTA_SMEM - 1024);     // (a limit, not what the launch asks for)
     return e != cudaSuccess ? e : launch_chained(kernel, grid, threads, smem, s, p);
 }
-template <typename T, int VEC, int EPT, int WPR, int PER_SM>
+template <typename T, int VEC, int EPT, int WPR, int ROWS, bool OWN>
+cudaError_t fwd_own(const RNParams& p, cudaStream_t s) {
+    typedef FwdRow<T, VEC, EPT, WPR, ROWS, OWN> R;
+    return norm_launch(residual_norm_fwd_kernel<T, VEC, EPT, WPR, ROWS, OWN>, grid_cap(p.n, ROWS, 1), R::THREADS, R::SMEM, s, p);
+}
+template <typename T, int VEC, int EPT, int WPR, int ROWS>
 cudaError_t fwd_launch(const RNParams& p, cudaStream_t s) {
-    typedef FwdRow<T, VEC, EPT, WPR, PER_SM> R;
-    return norm_launch(residual_norm_fwd_kernel<T, VEC, EPT, WPR, PER_SM>, grid_cap(p.n, R::ROWS, PER_SM), R::THREADS, R::SMEM, s, p);
+    return p.gate && p.groups == p.n ? fwd_own<T, VEC, EPT, WPR, ROWS, true>(p, s) : fwd_own<T, VEC, EPT, WPR, ROWS, false>(p, s);
 }
 template <typename T, int VEC>
 cudaError_t fwd_any(const RNParams& p, cudaStream_t s) {
     const RNShape k = fwd_shape((long long)p.comps * p.features);
-    if (k.warps == 1) return k.values == 8 ? fwd_launch<T, VEC, 8, 1, 6>(p, s) : fwd_launch<T, VEC, 32, 1, 3>(p, s);
+    if (k.warps == 1) return k.values == 8 ? fwd_launch<T, VEC, 8, 1, 16>(p, s) : fwd_launch<T, VEC, 32, 1, 12>(p, s);
     if (k.warps == 4) return k.values == 16 ? fwd_launch<T, VEC, 16, 4, 4>(p, s) : fwd_launch<T, VEC, 32, 4, 3>(p, s);
     return k.warps == 8 ? fwd_launch<T, VEC, 32, 8, 1>(p, s) : fwd_launch<T, VEC, 32, 16, 1>(p, s);
 }
-template <typename T, int VEC, int EPT, int WPR, int GATE, int PER_SM>
+template <typename T, int VEC, int EPT, int WPR, int ROWS, int GATE>
 cudaError_t bwd_gate(const RNParams& p, const RNPlan& q, cudaStream_t s) {
-    typedef BwdRow<T, VEC, EPT, WPR, GATE, PER_SM> R;
-    return norm_launch(residual_norm_bwd_kernel<T, VEC, EPT, WPR, GATE, PER_SM>, q.grid, R::THREADS, R::SMEM, s, p);
+    typedef BwdRow<T, VEC, EPT, WPR, ROWS, GATE> R;
+    return norm_launch(residual_norm_bwd_kernel<T, VEC, EPT, WPR, ROWS, GATE>, q.grid, R::THREADS, R::SMEM, s, p);
 }
-template <typename T, int VEC, int EPT, int WPR, int PER_SM>
+template <typename T, int VEC, int EPT, int WPR, int ROWS>
 cudaError_t bwd_launch(const RNParams& p, const RNPlan& q, cudaStream_t s) {
-    if (!p.gate) return bwd_gate<T, VEC, EPT, WPR, 0, PER_SM>(p, q, s);
-    return p.groups == p.n ? bwd_gate<T, VEC, EPT, WPR, 1, PER_SM>(p, q, s) : bwd_gate<T, VEC, EPT, WPR, 2, PER_SM>(p, q, s);
+    if (!p.gate) return bwd_gate<T, VEC, EPT, WPR, ROWS, 0>(p, q, s);
+    return p.groups == p.n ? bwd_gate<T, VEC, EPT, WPR, ROWS, 1>(p, q, s) : bwd_gate<T, VEC, EPT, WPR, ROWS, 2>(p, q, s);
 }
 template <typename T, int VEC>
 cudaError_t bwd_any(const RNParams& p, const RNPlan& q, cudaStream_t s) {
     switch (q.shape.warps) {
-        case 1: return q.shape.values == 8 ? bwd_launch<T, VEC, 8, 1, 4>(p, q, s) : bwd_launch<T, VEC, 16, 1, 3>(p, q, s);
+        case 1: return q.shape.values == 8 ? bwd_launch<T, VEC, 8, 1, 16>(p, q, s) : bwd_launch<T, VEC, 16, 1, 12>(p, q, s);
         case 4: return bwd_launch<T, VEC, 16, 4, 3>(p, q, s);
         case 8: return bwd_launch<T, VEC, 16, 8, 2>(p, q, s);
         default: return bwd_launch<T, VEC, 16, 16, 1>(p, q, s);
@@ -737,7 +808,7 @@ int bwd_typed(const RNParams& p, const RNPlan& q, cudaStream_t s) {
     const long long weight_blocks = p.part_w ? (p.features + 7) / 8 : 0;
     const long long gate_blocks = p.part_gate ? ((long long)p.groups * p.comps * p.features + RN_SUM_THREADS - 1) / RN_SUM_THREADS : 0;
     if (weight_blocks + gate_blocks > 0)
-        PCB_CUDA_TRY(launch_chained(residual_norm_sum_kernel<T>, (unsigned)(weight_blocks + gate_blocks), RN_SUM_THREADS, 0, s, p, q.slots, (int)weight_blocks));
+        PCB_CUDA_TRY(launch_chained(residual_norm_sum_kernel<T>, (unsigned)(weight_blocks + gate_blocks), RN_SUM_THREADS, 0, s, p, q.grid, (int)weight_blocks));
     return PCB_OK;
 }
 

@@ -23,24 +23,24 @@ struct RNParams {
     int parts, items;                              // pieces per group
 };
 
-// Warps per row and values per thread for a width; warps 0: wider than the registers. CTAs per SM follow from registers and shared memory.
-struct RNShape { int warps, values, per_sm; };
+// Warps per row, values per thread and rows of a CTA (one per SM) for a width; warps 0: wider than the registers.
+struct RNShape { int warps, values, rows; };
 inline RNShape fwd_shape(long long width) {
-    if (width <= 32 * 8) return {1, 8, 6};
-    if (width <= 32 * 32) return {1, 32, 3};
+    if (width <= 32 * 8) return {1, 8, 16};
+    if (width <= 32 * 32) return {1, 32, 12};
     if (width <= 128 * 16) return {4, 16, 4};
     if (width <= 128 * 32) return {4, 32, 3};
     if (width <= 256 * 32) return {8, 32, 1};
     if (width <= 512 * 32) return {16, 32, 1};
-    return {0, 0, 4};
+    return {0, 0, 1};
 }
 inline RNShape bwd_shape(long long width) {
-    if (width <= 32 * 8) return {1, 8, 4};
-    if (width <= 32 * 16) return {1, 16, 3};
+    if (width <= 32 * 8) return {1, 8, 16};
+    if (width <= 32 * 16) return {1, 16, 12};
     if (width <= 128 * 16) return {4, 16, 3};
     if (width <= 256 * 16) return {8, 16, 2};
     if (width <= 512 * 16) return {16, 16, 1};
-    return {0, 0, 4};
+    return {0, 0, 1};
 }
 
 struct RNPlan { RNShape shape; int grid, slots, parts, items; size_t part_w, part_gate, total; };
@@ -48,7 +48,7 @@ inline RNPlan bwd_plan(int comps, int n, int features, int groups) {
     RNPlan q = {};
     const long long width = (long long)comps * features;
     q.shape = bwd_shape(width);
-    const int rows_per_cta = q.shape.warps == 1 ? 4 : 1, most = tc::device_sms() * q.shape.per_sm * rows_per_cta;
+    const int rows_per_cta = q.shape.rows, most = tc::device_sms() * (q.shape.warps ? rows_per_cta : 4);      // (wide rows: four CTAs on an SM)
     const bool shared = groups > 0 && groups < n;
     const int g = shared || (groups == n && n > 0) ? groups : 1;
     if (groups == n && groups > 1 && !shared) { q.parts = 1; q.items = n; }          // a gate for each value: every sample is an item
@@ -65,7 +65,7 @@ inline RNPlan bwd_plan(int comps, int n, int features, int groups) {
     }
     const int want = q.items < most ? q.items : most;
     q.grid = (want + rows_per_cta - 1) / rows_per_cta;
-    q.slots = q.shape.warps == 0 ? q.grid : q.grid * rows_per_cta;
+    q.slots = q.grid;                                   // sums of the weights' gradients: one set per CTA
     q.part_w = (size_t)q.slots * 2 * width * 4;
     q.part_gate = shared && (q.parts > 1 || q.shape.warps == 0) ? (size_t)q.items * width * 4 : (groups == n && n > 0 && q.shape.warps == 0 ? (size_t)n * width * 4 : 0);
     q.total = q.part_w + q.part_gate;
