@@ -24,7 +24,6 @@ RNParams norm_params(const pcb_norm_desc* d) {
     RNParams p = {};
     p.comps = norm_comps(d); p.n = d->batch; p.features = d->features;
     p.groups = d->gate_rows; p.per_group = d->gate_rows > 0 ? d->batch / d->gate_rows : d->batch;
-    p.magic = d->features > 1 ? (uint32_t)((0x100000000ull + d->features - 1) / d->features) : 0u;
     p.scale = d->residual_scale; p.eps = d->epsilon;
     return p;
 }
@@ -37,7 +36,7 @@ extern "C" {
 
 size_t pcb_residual_norm_bwd_workspace_size(const pcb_norm_desc* d) {
     if (check_norm(d) != PCB_OK || d->batch == 0) return 0;
-    return bwd_plan(norm_comps(d), d->batch, d->features, d->gate_rows).total;
+    return bwd_plan(norm_comps(d), d->batch, d->features, d->gate_rows, (int)dtype_size(d->dtype)).total;
 }
 
 int pcb_residual_norm_fwd(const pcb_norm_desc* d, const void* x, const void* branch, const void* gate, const float* post, const float* pre, void* y, void* h,
@@ -71,15 +70,13 @@ int pcb_residual_norm_bwd(const pcb_norm_desc* d, const void* y, const void* bra
         set_error("gate, weights or their gradients without what they apply to");
         return PCB_ERR_INVALID_ARGUMENT;
     }
-    RNPlan q = bwd_plan(comps, d->batch, d->features, d->gate_rows);
+    const RNPlan q = bwd_plan(comps, d->batch, d->features, d->gate_rows, (int)dtype_size(d->dtype));
     if (!workspace || workspace_bytes < q.total) { set_error("workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : (size_t)0, q.total); return PCB_ERR_WORKSPACE; }
     if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) { set_error("the workspace must be 16-byte aligned"); return PCB_ERR_INVALID_ARGUMENT; }
     RNParams p = norm_params(d);
     p.branch = branch; p.gate = gate; p.post = post; p.pre = pre; p.y = const_cast<void*>(y); p.stats = const_cast<float*>(stats);
     p.dy = dy; p.dh = dh; p.dx = dx; p.dbranch = dbranch; p.dgate = dgate; p.dpost = dpost; p.dpre = dpre;
-    p.part_w = dpost || dpre ? static_cast<float*>(workspace) : nullptr;
-    p.part_gate = dgate && q.part_gate ? reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + q.part_w) : nullptr;
-    p.parts = q.parts; p.items = q.items;
+    p.workspace = static_cast<uint8_t*>(workspace);
     if (!gate) p.per_group = d->batch;
     if (d->dtype == PCB_F32) return norm_bwd_f32(p, q, s);
     return d->dtype == PCB_F16 ? norm_bwd_f16(p, q, s) : norm_bwd_bf16(p, q, s);

@@ -77,9 +77,6 @@ __device__ __forceinline__ float row_sum(float v, float* words, int& turn) {
     return v;
 }
 
-// Where value e of a sample lies: component e / F, feature e % F.
-__device__ __forceinline__ int comp_of(const RNParams& p, int e) { return p.comps == 1 ? 0 : (p.magic ? (int)__umulhi((uint32_t)e, p.magic) : e); }
-
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
@@ -87,199 +84,146 @@ __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_
 template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // A thread's values of a row, EPT of them in pairs, and the ring of row buffers in shared memory that cp.async fills some rows ahead, so that loads in flight cost
-// no registers. Everything that does not change from row to row is worked out once: with 8 values per thread and that arithmetic in the loop a row
-// took 44 instructions a value, and the pass was bound by issue slots at 4.1 TB/s.
-//   VEC > 1    a thread owns vectors of 16 bytes, tid + TPR * i; it copies exactly what it reads later, and no barrier is needed for that
-//   VEC == 1   rows start anywhere: a thread owns values tid + TPR * i; the threads of a row copy the aligned 16-byte units that cover each component's values
-//              (cut where the tensor ends) and wait for each other
+// no registers. A thread owns aligned vectors of 16 bytes and copies exactly what it reads later, so that no barrier is needed for that. Everything that does not change from
+// row to row is worked out once: with 8 values per thread and that arithmetic in the loop a row took 44 instructions a value, and the pass was bound by issue slots.
+//
+// Rows whose length is no multiple of 16 bytes (!ALIGNED) start at one of `period` places within 16 bytes, and rows `period` apart at the same one. A CTA takes rows of
+// one such class only, so that its threads' vectors hold the same features in every row; vectors that reach into a neighbouring row are masked, and
+// stored value by value. (Value by value throughout, 3001 quaternion rows of 4 x 509 took 61 us backward.)
+//
 // One CTA per SM holds ROWS rows at a time, and the weights in shared memory: the ring leaves no L1 to speak of, and weights that came from L2 for every row were as
 // many bytes as the rows (16384 x 4096 bf16: 115 us forward, 190 backward).
 constexpr int RN_SMEM = 218 * 1024;
-template <typename T, int VEC, int EPT, int WPR, int ROWS_, int TENSORS, int MAX_STAGES>
+template <typename T, int VEC, bool ALIGNED, int EPT, int WPR, int ROWS_, int TENSORS, int MAX_STAGES>
 struct Row {
     static constexpr int ROWS = ROWS_, TPR = 32 * WPR, THREADS = ROWS * TPR, NV = EPT / VEC, PAIRS = EPT / 2, SIZE = sizeof(T);
-    static constexpr int TENSOR = VEC > 1 ? NV * TPR * 16 : TPR * EPT * SIZE + 8 * 32;        // bytes of a tensor's row (eight components, each with up to 29 bytes around it)
-    static constexpr int STAGE = TENSORS * TENSOR, WEIGHTS = 2 * EPT * TPR * 4;               // bytes of a stage of one row; of both weights
+    static constexpr int TENSOR = NV * TPR * 16, STAGE = TENSORS * TENSOR, WEIGHTS = 2 * EPT * TPR * 4;   // bytes of a tensor's row, of a stage of one row, of both weights
     static constexpr bool HELD = WEIGHTS + ROWS * STAGE <= RN_SMEM;                           // weights in shared memory
     static constexpr int FIT = (RN_SMEM - (HELD ? WEIGHTS : 0)) / (ROWS * STAGE), STAGES = FIT < MAX_STAGES ? FIT : MAX_STAGES;
     static_assert(STAGES >= 1, "a row of every tensor fits");
+    static_assert(EPT <= 32, "a bit for every value");
     static constexpr size_t SMEM = (size_t)ROWS * STAGES * STAGE + (HELD ? WEIGHTS : 0);
-    static constexpr int UNITS = VEC > 1 ? NV : (TENSOR / 16 + TPR - 1) / TPR;               // 16-byte units that a thread copies
-    static constexpr int RAW = SIZE == 4 ? EPT : PAIRS;                                       // registers of a tensor's values as loaded
-    uint32_t base, held;                    // this row's ring; this thread's weights: four at a time (VEC == 1: one), TPR * 16 (4) bytes apart
+    static constexpr int RAW = NV * 4;                                                        // registers of a tensor's values as loaded
+    static constexpr uint32_t FULL = (1u << VEC) - 1u;
+    uint32_t base, held;                    // this thread's first vector in its row's ring; its weights: four at a time, TPR * 16 bytes apart
     int tid, width;
-    uint32_t off[NV];                       // element of vector (value) i relative to its row: component * (rows - 1) * F + e
-    uint32_t feature[NV];
-    uint32_t live;                          // bit i: vector (value) i exists
-    // VEC == 1
-    uint32_t at[VEC > 1 ? 1 : NV];          // shared-memory offset of value i without its component's shift
-    uint32_t phase[VEC > 1 ? 1 : NV];       // bytes modulo 16 at which its component starts
-    uint32_t unit_in[VEC > 1 ? 1 : UNITS], unit_dst[VEC > 1 ? 1 : UNITS];
-    int unit_comp[VEC > 1 ? 1 : UNITS];     // -1: none
+    int off[NV], feature[NV], comp[NV];     // first element of vector i relative to row * F; its feature (negative where it reaches back) and component
+    uint32_t mask;                          // bit i * VEC + j: value j of vector i is one of the row's
 
-    __device__ __forceinline__ Row(uint32_t smem, const RNParams& p) {
+    __device__ __forceinline__ Row(uint32_t smem, const RNParams& p, int row) {      // row: any of this CTA's
         tid = threadIdx.x % TPR;
         width = p.comps * p.features;
-        base = smem + (HELD ? WEIGHTS : 0) + (threadIdx.x / TPR) * STAGES * STAGE;
-        held = smem + tid * (VEC > 1 ? 16 : 4);
-        live = 0;
-        const int seg = (p.features * SIZE + 14 + 15) / 16 * 16;
+        base = smem + (HELD ? WEIGHTS : 0) + (threadIdx.x / TPR) * STAGES * STAGE + tid * 16;
+        held = smem + tid * 16;
+        mask = 0;
+        const int per = ALIGNED ? p.features / VEC : (p.features + 2 * VEC - 2) / VEC;        // vectors of a component
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int e = (i * TPR + tid) * VEC, c = comp_of(p, e);
-            if (e < width) live |= 1u << i;
-            off[i] = (uint32_t)c * (uint32_t)(p.n - 1) * (uint32_t)p.features + e;
-            feature[i] = e - c * p.features;
-            if constexpr (VEC == 1) {
-                at[i] = c * seg + feature[i] * SIZE;
-                phase[i] = (uint32_t)c * (uint32_t)p.n * (uint32_t)p.features * SIZE & 15u;
-            }
-        }
-        if constexpr (VEC == 1) {
-            const int units = seg / 16;
+            const int v = i * TPR + tid, c = p.comps == 1 ? 0 : v / per;
+            const long long first = ((long long)c * p.n + row) * p.features;
+            const int shift = ALIGNED ? 0 : (int)(first & (VEC - 1));
+            feature[i] = (v - c * per) * VEC - shift;
+            off[i] = (int)((long long)c * p.n * p.features + feature[i]);
+            comp[i] = c;
+            if (c < p.comps && v - c * per < per) {
 #pragma unroll
-            for (int i = 0; i < UNITS; ++i) {
-                const int u = i * TPR + tid, c = u / units;
-                unit_comp[i] = c < p.comps ? c : -1;
-                unit_in[i] = (u - c * units) * 16;
-                unit_dst[i] = u * 16;
+                for (int j = 0; j < VEC; ++j)
+                    if (ALIGNED || (feature[i] + j >= 0 && feature[i] + j < p.features)) mask |= 1u << (i * VEC + j);
             }
         }
     }
+    __device__ __forceinline__ uint32_t some(int i) const { return mask >> (i * VEC) & FULL; }
     // starts the copies of a row of each tensor (null: none)
     __device__ __forceinline__ void fetch(const RNParams& p, int stage, int row, const void* const (&tensors)[TENSORS]) const {
         const uint32_t dst = base + stage * STAGE;
-        if constexpr (VEC > 1) {
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                if (!(live >> i & 1)) continue;
-                const size_t byte = ((size_t)row * p.features + off[i]) * SIZE;
-#pragma unroll
-                for (int k = 0; k < TENSORS; ++k)
-                    if (tensors[k]) copy16(dst + k * TENSOR + (i * TPR + tid) * 16, static_cast<const uint8_t*>(tensors[k]) + byte, 16);
+        for (int i = 0; i < NV; ++i) {
+            if (!some(i)) continue;
+            const long long element = (long long)row * p.features + off[i];
+            uint32_t bytes = 16;
+            if (!ALIGNED) {                                      // the last vector of a tensor ends where the tensor does
+                const long long left = ((long long)p.n * width - element) * SIZE;
+                bytes = left < 16 ? (uint32_t)left : 16u;
             }
-        } else {
-            const size_t line = (size_t)p.features * SIZE, end = (size_t)p.comps * p.n * line;
 #pragma unroll
-            for (int i = 0; i < UNITS; ++i) {
-                if (unit_comp[i] < 0) continue;
-                const size_t first = ((size_t)unit_comp[i] * p.n + row) * line, from = (first & ~size_t(15)) + unit_in[i];
-                if (from >= first + line) continue;
-                const uint32_t bytes = end - from < 16 ? (uint32_t)(end - from) : 16u;
-#pragma unroll
-                for (int k = 0; k < TENSORS; ++k)
-                    if (tensors[k]) copy16(dst + k * TENSOR + unit_dst[i], static_cast<const uint8_t*>(tensors[k]) + from, bytes);
-            }
+            for (int k = 0; k < TENSORS; ++k)
+                if (tensors[k]) copy16(dst + k * TENSOR + i * TPR * 16, static_cast<const T*>(tensors[k]) + element, bytes);
         }
     }
     // this thread's values of tensor k of a row that has arrived, as loaded (zeros where there are none)
-    __device__ __forceinline__ void get(const RNParams& p, int stage, int row, int k, uint32_t (&raw)[RAW]) const {
+    __device__ __forceinline__ void get(int stage, int k, uint32_t (&raw)[RAW]) const {
         const uint32_t src = base + stage * STAGE + k * TENSOR;
-        if constexpr (VEC > 1) {
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                if (live >> i & 1) v = ld_shared_v4(src + (i * TPR + tid) * 16);
-                raw[4 * i] = v.x; raw[4 * i + 1] = v.y; raw[4 * i + 2] = v.z; raw[4 * i + 3] = v.w;
-            }
-        } else {
-            const uint32_t shift = (uint32_t)row * (uint32_t)p.features * SIZE;
-            uint32_t v[NV];
+        for (int i = 0; i < NV; ++i) {
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if (some(i)) v = ld_shared_v4(src + i * TPR * 16);
+            if (!ALIGNED && some(i) != FULL) {
+                uint32_t* w = &v.x;
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const uint32_t a = src + at[i] + ((phase[i] + shift) & 15u);
-                v[i] = 0;
-                if (live >> i & 1) {
-                    if constexpr (SIZE == 4) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[i]) : "r"(a) : "memory");
-                    else {
-                        uint16_t h;
-                        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(a) : "memory");
-                        v[i] = h;
-                    }
+                for (int j = 0; j < 4; ++j) {
+                    if constexpr (VEC == 8) w[j] &= (mask >> (i * VEC + 2 * j) & 1 ? 0xffffu : 0u) | (mask >> (i * VEC + 2 * j + 1) & 1 ? 0xffff0000u : 0u);
+                    else w[j] = mask >> (i * VEC + j) & 1 ? w[j] : 0u;
                 }
             }
-            if constexpr (SIZE == 4) {
-#pragma unroll
-                for (int i = 0; i < NV; ++i) raw[i] = v[i];
-            } else {
-#pragma unroll
-                for (int i = 0; i < PAIRS; ++i) raw[i] = v[2 * i] | (v[2 * i + 1] << 16);
-            }
+            raw[4 * i] = v.x; raw[4 * i + 1] = v.y; raw[4 * i + 2] = v.z; raw[4 * i + 3] = v.w;
         }
     }
     __device__ __forceinline__ static Pair value(const uint32_t (&raw)[RAW], int q) {
         if constexpr (SIZE == 4) return pair(__uint_as_float(raw[2 * q]), __uint_as_float(raw[2 * q + 1]));
         else return pair(from16<T>(raw[q] & 0xffffu), from16<T>(raw[q] >> 16));
     }
-    // values of a tensor in global memory: `row` of a tensor of `rows` rows per component
-    __device__ __forceinline__ void load(const RNParams& p, const void* tensor, int row, int rows, uint32_t (&raw)[RAW]) const {
-        typedef typename Vec<T, VEC>::raw R;
+    // a row of the gate (once for a group)
+    __device__ __forceinline__ void load_gate(const RNParams& p, int group, Pair (&v)[PAIRS]) const {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = comp_of(p, (i * TPR + tid) * VEC);
-            const R* src = reinterpret_cast<const R*>(static_cast<const T*>(tensor) + ((size_t)c * rows + row) * p.features + feature[i]);
-            const R v = ld_chained(src, live >> i & 1);
-            if constexpr (VEC > 1) { raw[4 * i] = v.x; raw[4 * i + 1] = v.y; raw[4 * i + 2] = v.z; raw[4 * i + 3] = v.w; }
-            else if constexpr (SIZE == 4) raw[i] = v;
-            else raw[i / 2] = i & 1 ? raw[i / 2] | ((uint32_t)v << 16) : (uint32_t)v;
+        for (int q = 0; q < PAIRS; ++q) {
+            const int i = 2 * q / VEC, j = 2 * q % VEC;
+            const typename Vec<T, 1>::raw* src = static_cast<const typename Vec<T, 1>::raw*>(p.gate) + ((size_t)comp[i] * p.groups + group) * p.features + feature[i] + j;
+            float a, b;
+            Vec<T, 1>::unpack(ld_chained(src, mask >> (2 * q) & 1), &a);
+            Vec<T, 1>::unpack(ld_chained(src + 1, mask >> (2 * q + 1) & 1), &b);
+            v[q] = pair(a, b);
         }
     }
-    __device__ __forceinline__ void store(void* tensor, size_t row_element, const Pair (&v)[PAIRS]) const {
+    __device__ __forceinline__ void store_at(T* dst, int i, const Pair (&v)[PAIRS]) const {
+        float f[VEC];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            if (!(live >> i & 1)) continue;
-            T* dst = static_cast<T*>(tensor) + row_element + off[i];
-            if constexpr (VEC > 1) {
-                float f[VEC];
-#pragma unroll
-                for (int j = 0; j < VEC / 2; ++j) halves(v[i * (VEC / 2) + j], f[2 * j], f[2 * j + 1]);
-                *reinterpret_cast<uint4*>(dst) = Vec<T, VEC>::pack(f);
-            } else {
-                float a, b;
-                halves(v[i / 2], a, b);
-                const float f[1] = {i & 1 ? b : a};
-                *reinterpret_cast<typename Vec<T, 1>::raw*>(dst) = Vec<T, 1>::pack(f);
-            }
-        }
-    }
-    __device__ __forceinline__ void store_gate(const RNParams& p, void* tensor, int group, const Pair (&v)[PAIRS]) const {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            if (!(live >> i & 1)) continue;
-            const int c = comp_of(p, (i * TPR + tid) * VEC);
-            T* dst = static_cast<T*>(tensor) + ((size_t)c * p.groups + group) * p.features + feature[i];
-            float f[VEC];
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                float a, b;
-                halves(v[(i * VEC + j) / 2], a, b);
-                f[j] = (i * VEC + j) & 1 ? b : a;
-            }
-            *reinterpret_cast<typename Vec<T, VEC>::raw*>(dst) = Vec<T, VEC>::pack(f);
-        }
-    }
-    // Weights of this thread's features (`which`: 0 post, 1 pre; ones where there are none), from global memory: plain loads, nothing marks these pointers as read-only.
-    __device__ __forceinline__ void load_weights(const float* w, Pair (&v)[PAIRS]) const {
-#pragma unroll
-        for (int q = 0; q < PAIRS; ++q) v[q] = pair(1.f);
-        if (!w) return;
-        if constexpr (VEC > 1) {
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                if (!(live >> i & 1)) continue;
-#pragma unroll
-                for (int j = 0; j < VEC; j += 4) {
-                    const float4 a = *reinterpret_cast<const float4*>(w + feature[i] + j);
-                    v[(i * VEC + j) / 2] = pair(a.x, a.y);
-                    v[(i * VEC + j) / 2 + 1] = pair(a.z, a.w);
-                }
-            }
+        for (int j = 0; j < VEC / 2; ++j) halves(v[i * (VEC / 2) + j], f[2 * j], f[2 * j + 1]);
+        if (ALIGNED || some(i) == FULL) {
+            *reinterpret_cast<uint4*>(dst) = Vec<T, VEC>::pack(f);
         } else {
 #pragma unroll
-            for (int q = 0; q < PAIRS; ++q) v[q] = pair(live >> (2 * q) & 1 ? w[feature[2 * q]] : 1.f, live >> (2 * q + 1) & 1 ? w[feature[2 * q + 1]] : 1.f);
+            for (int j = 0; j < VEC; ++j)
+                if (mask >> (i * VEC + j) & 1) reinterpret_cast<typename Vec<T, 1>::raw*>(dst)[j] = Vec<T, 1>::pack(&f[j]);
         }
     }
-    // the first row's threads put them into shared memory (followed by a barrier of the CTA)
+    __device__ __forceinline__ void store(void* tensor, const RNParams& p, int row, const Pair (&v)[PAIRS]) const {
+        T* line = static_cast<T*>(tensor) + (size_t)row * p.features;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (some(i)) store_at(line + off[i], i, v);
+    }
+    // a row of the gate's gradient (value by value where its rows start elsewhere than the samples')
+    __device__ __forceinline__ void store_gate(const RNParams& p, int group, const Pair (&v)[PAIRS]) const {
+#pragma unroll
+        for (int q = 0; q < PAIRS; ++q) {
+            const int i = 2 * q / VEC, j = 2 * q % VEC;
+            typename Vec<T, 1>::raw* dst = static_cast<typename Vec<T, 1>::raw*>(p.dgate) + ((size_t)comp[i] * p.groups + group) * p.features + feature[i] + j;
+            float a, b;
+            halves(v[q], a, b);
+            if (mask >> (2 * q) & 1) dst[0] = Vec<T, 1>::pack(&a);
+            if (mask >> (2 * q + 1) & 1) dst[1] = Vec<T, 1>::pack(&b);
+        }
+    }
+    // Weights of this thread's features (ones where there are none), from global memory: plain loads, nothing marks these pointers as read-only.
+    __device__ __forceinline__ void load_weights(const float* w, Pair (&v)[PAIRS]) const {
+#pragma unroll
+        for (int q = 0; q < PAIRS; ++q) {
+            v[q] = pair(1.f);
+            const int at = feature[2 * q / VEC] + 2 * q % VEC;
+            if (w) v[q] = pair(mask >> (2 * q) & 1 ? w[at] : 1.f, mask >> (2 * q + 1) & 1 ? w[at + 1] : 1.f);
+        }
+    }
+    // the first row's threads put them into shared memory (followed by a barrier of the CTA); `which`: 0 post, 1 pre
     __device__ __forceinline__ void hold_weights(const RNParams& p) const {
         if (!HELD) return;
         if (threadIdx.x < TPR) {
@@ -289,15 +233,7 @@ struct Row {
                 load_weights(which ? p.pre : p.post, v);
                 const uint32_t dst = held + which * (WEIGHTS / 2);
 #pragma unroll
-                for (int q = 0; q < PAIRS; ++q) {
-                    if constexpr (VEC > 1) asm volatile("st.shared.b64 [%0], %1;" ::"r"(dst + (q / 2) * TPR * 16 + (q & 1) * 8), "l"(v[q].v) : "memory");
-                    else {
-                        float a, b;
-                        halves(v[q], a, b);
-                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst + 2 * q * TPR * 4), "f"(a) : "memory");
-                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst + (2 * q + 1) * TPR * 4), "f"(b) : "memory");
-                    }
-                }
+                for (int q = 0; q < PAIRS; ++q) asm volatile("st.shared.b64 [%0], %1;" ::"r"(dst + (q / 2) * TPR * 16 + (q & 1) * 8), "l"(v[q].v) : "memory");
             }
         }
         __syncthreads();
@@ -307,99 +243,101 @@ struct Row {
         else {
             const uint32_t src = held + which * (WEIGHTS / 2);
 #pragma unroll
-            for (int q = 0; q < PAIRS; ++q) {
-                if constexpr (VEC > 1) {
-                    if (q & 1) continue;
-                    asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(v[q].v), "=l"(v[q + 1].v) : "r"(src + (q / 2) * TPR * 16));
-                } else {
-                    float a, b;
-                    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(a) : "r"(src + 2 * q * TPR * 4));
-                    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(b) : "r"(src + (2 * q + 1) * TPR * 4));
-                    v[q] = pair(a, b);
-                }
-            }
+            for (int q = 0; q < PAIRS; q += 2) asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(v[q].v), "=l"(v[q + 1].v) : "r"(src + (q / 2) * TPR * 16));
         }
     }
-    // adds up in fp32: out[e] of this thread's values
-    __device__ __forceinline__ void store_sums(float* out, const Pair (&v)[PAIRS]) const {
+    // this thread's sums to out[component * F + feature]
+    __device__ __forceinline__ void store_sums(const RNParams& p, float* out, const Pair (&v)[PAIRS]) const {
 #pragma unroll
         for (int q = 0; q < PAIRS; ++q) {
+            const int i = 2 * q / VEC;
+            float* dst = out + (size_t)comp[i] * p.features + feature[i] + 2 * q % VEC;
             float a, b;
             halves(v[q], a, b);
-            if constexpr (VEC > 1) {
-                const int i = 2 * q / VEC;
-                if (live >> i & 1) *reinterpret_cast<float2*>(out + (i * TPR + tid) * VEC + 2 * q % VEC) = make_float2(a, b);
-            } else {
-                if (live >> (2 * q) & 1) out[2 * q * TPR + tid] = a;
-                if (live >> (2 * q + 1) & 1) out[(2 * q + 1) * TPR + tid] = b;
-            }
+            if (mask >> (2 * q) & 1) dst[0] = a;
+            if (mask >> (2 * q + 1) & 1) dst[1] = b;
         }
     }
 };
 
-// Rows of a group of threads: piece `slot` of `slots` nearly equal runs of consecutive rows.
+// Class of a CTA (where its rows start within 16 bytes), its rank within the class, and the class's CTAs.
+__device__ __forceinline__ void class_of(int period, int& cls, int& rank, int& of) {
+    cls = blockIdx.x % period;
+    rank = blockIdx.x / period;
+    of = (gridDim.x - cls + period - 1) / period;
+}
+
+// Where run `slot` of `slots` nearly equal runs of `rows` things starts.
 __device__ __forceinline__ int run_start(int rows, int slot, int slots) { return (int)((long long)rows * slot / slots); }
 
 constexpr int RN_FWD_STAGES = 4, RN_BWD_STAGES = 3;
-// OWN: a gate for each value
-template <typename T, int VEC, int EPT, int WPR, int ROWS, bool OWN> using FwdRow = Row<T, VEC, EPT, WPR, ROWS, OWN ? 3 : 2, RN_FWD_STAGES>;            // x, branch, gate
-template <typename T, int VEC, int EPT, int WPR, int ROWS, int GATE> using BwdRow = Row<T, VEC, EPT, WPR, ROWS, GATE == 1 ? 5 : 4, RN_BWD_STAGES>;      // y, dh, dy, branch, gate
+// OWN, GATE 1: a gate for each value
+template <typename T, int VEC, bool ALIGNED, int EPT, int WPR, int ROWS, bool OWN> using FwdRow = Row<T, VEC, ALIGNED, EPT, WPR, ROWS, OWN ? 3 : 2, RN_FWD_STAGES>;        // x, branch, gate
+template <typename T, int VEC, bool ALIGNED, int EPT, int WPR, int ROWS, int GATE> using BwdRow = Row<T, VEC, ALIGNED, EPT, WPR, ROWS, GATE == 1 ? 5 : 4, RN_BWD_STAGES>;  // y, dh, dy, branch, gate
 
-template <typename T, int VEC, int EPT, int WPR, int ROWS, bool OWN>
+template <typename T, int VEC, bool ALIGNED, int EPT, int WPR, int ROWS, bool OWN>
 __global__ void __launch_bounds__(32 * WPR * ROWS, 1) residual_norm_fwd_kernel(const RNParams p) {
-    typedef FwdRow<T, VEC, EPT, WPR, ROWS, OWN> R;
+    typedef FwdRow<T, VEC, ALIGNED, EPT, WPR, ROWS, OWN> R;
     constexpr int STAGES = R::STAGES, PAIRS = R::PAIRS;
     extern __shared__ __align__(16) uint8_t ring_smem[];
     __shared__ float all_words[R::ROWS][2 * WPR];
     float* words = all_words[threadIdx.x / R::TPR];
-    const R r(smem_u32(ring_smem), p);
-    int turn = 0;
+    const int period = ALIGNED ? 1 : p.period;
+    int cls, rank, of, turn = 0;
+    class_of(period, cls, rank, of);
+    const R r(smem_u32(ring_smem), p, cls);
     chain_wait();
     chain_next();
     r.hold_weights(p);
     const float inv_width = 1.f / (float)r.width;
-    const int slots = gridDim.x * R::ROWS, slot = blockIdx.x * R::ROWS + threadIdx.x / R::TPR;
-    const int begin = run_start(p.n, slot, slots), end = run_start(p.n, slot + 1, slots);
+    const int count = cls < p.n ? (p.n - cls + period - 1) / period : 0;        // rows of the class
+    const int slots = of * R::ROWS, slot = rank * R::ROWS + threadIdx.x / R::TPR;
+    const int begin = run_start(count, slot, slots), end = run_start(count, slot + 1, slots);
     const void* tensors[OWN ? 3 : 2];
     tensors[0] = p.x; tensors[1] = p.branch;
     if constexpr (OWN) tensors[2] = p.gate;
-    auto fetch = [&](int row, int stage) {
-        if (row < end) r.fetch(p, stage, row, *reinterpret_cast<const void* const(*)[OWN ? 3 : 2]>(&tensors));
+    auto fetch = [&](int t, int stage) {
+        if (t < end) r.fetch(p, stage, cls + period * t, *reinterpret_cast<const void* const(*)[OWN ? 3 : 2]>(&tensors));
         copies_commit();
     };
     for (int i = 0; i < STAGES; ++i) fetch(begin + i, i);
-    uint32_t graw[R::RAW];
+    Pair gate[OWN ? 1 : PAIRS];
     int group_end = 0, stage = 0;                                // (shared gates: the row behind the present group)
-    // (with a CTA per row the runs of all its threads are one; with a warp per row there are no barriers)
-    for (int row = begin; row < end; ++row) {
+    // (the threads of a row run through the same rows; different rows of a CTA have no barrier in common)
+    for (int t = begin; t < end; ++t) {
+        const int row = cls + period * t;
         copies_wait<STAGES - 1>();
-        if (VEC == 1) row_sync<WPR>();
-        if (!OWN && p.gate && row >= group_end) {
-            const int group = row / p.per_group;
-            group_end = (group + 1) * p.per_group;
-            r.load(p, p.gate, group, p.groups, graw);
+        if constexpr (!OWN) {
+            if (p.gate && row >= group_end) {
+                const int group = row / p.per_group;
+                group_end = (group + 1) * p.per_group;
+                r.load_gate(p, group, gate);
+            }
         }
         Pair y[PAIRS];
         float rb = 0.f;
         {
-            uint32_t xraw[R::RAW], braw[R::RAW];
-            r.get(p, stage, row, 0, xraw);
-            if (p.branch) r.get(p, stage, row, 1, braw);
-            if constexpr (OWN) r.get(p, stage, row, 2, graw);
+            uint32_t xraw[R::RAW], braw[R::RAW], graw[OWN ? R::RAW : 1];
+            r.get(stage, 0, xraw);
+            if (p.branch) r.get(stage, 1, braw);
+            if constexpr (OWN) r.get(stage, 2, graw);
             if (p.branch) {
                 Pair s = pair(0.f);
 #pragma unroll
                 for (int q = 0; q < PAIRS; ++q) { const Pair b = R::value(braw, q); s = fma2(b, b, s); }
                 rb = rsqrtf(row_sum<WPR>(sum(s), words, turn) * inv_width + p.eps);
             } else row_sync<WPR>();
-            fetch(row + STAGES, stage);                          // into the stage that every thread of the row has read by now
+            fetch(t + STAGES, stage);                            // into the stage that has been read by now
             if (p.branch) {
                 const Pair f = pair(p.scale * rb);
                 Pair w[PAIRS];
                 r.weights(p, 0, w);
-                if (p.gate) {
+                if constexpr (OWN) {
 #pragma unroll
                     for (int q = 0; q < PAIRS; ++q) w[q] = w[q] * R::value(graw, q);
+                } else if (p.gate) {
+#pragma unroll
+                    for (int q = 0; q < PAIRS; ++q) w[q] = w[q] * gate[q];
                 }
 #pragma unroll
                 for (int q = 0; q < PAIRS; ++q) y[q] = fma2(R::value(braw, q) * f, w[q], R::value(xraw, q));
@@ -408,8 +346,7 @@ __global__ void __launch_bounds__(32 * WPR * ROWS, 1) residual_norm_fwd_kernel(c
                 for (int q = 0; q < PAIRS; ++q) y[q] = R::value(xraw, q);
             }
         }
-        const size_t at = (size_t)row * p.features;
-        if (p.y) r.store(p.y, at, y);
+        if (p.y) r.store(p.y, p, row, y);
         float ry = 0.f;
         if (p.h) {
             Pair s = pair(0.f), w[PAIRS];
@@ -420,7 +357,7 @@ __global__ void __launch_bounds__(32 * WPR * ROWS, 1) residual_norm_fwd_kernel(c
             const Pair f = pair(ry);
 #pragma unroll
             for (int q = 0; q < PAIRS; ++q) y[q] = y[q] * f * w[q];
-            r.store(p.h, at, y);
+            r.store(p.h, p, row, y);
         }
         if (p.stats && r.tid == 0) { p.stats[row] = rb; p.stats[p.n + row] = ry; }
         if (++stage == STAGES) stage = 0;
@@ -429,96 +366,109 @@ __global__ void __launch_bounds__(32 * WPR * ROWS, 1) residual_norm_fwd_kernel(c
 }
 
 // GATE: 0 none, 1 a gate for each value, 2 gates shared by the samples of a group, whose gradients are sums
-template <typename T, int VEC, int EPT, int WPR, int ROWS, int GATE>
+template <typename T, int VEC, bool ALIGNED, int EPT, int WPR, int ROWS, int GATE>
 __global__ void __launch_bounds__(32 * WPR * ROWS, 1) residual_norm_bwd_kernel(const RNParams p) {
-    typedef BwdRow<T, VEC, EPT, WPR, ROWS, GATE> R;
+    typedef BwdRow<T, VEC, ALIGNED, EPT, WPR, ROWS, GATE> R;
     constexpr int STAGES = R::STAGES, PAIRS = R::PAIRS;
     extern __shared__ __align__(16) uint8_t ring_smem[];
     __shared__ float all_words[R::ROWS][2 * WPR];
     float* words = all_words[threadIdx.x / R::TPR];
-    const R r(smem_u32(ring_smem), p);
-    int turn = 0;
+    const int period = ALIGNED ? 1 : p.period;
+    int cls, rank, of, turn = 0;
+    class_of(period, cls, rank, of);
+    const R r(smem_u32(ring_smem), p, cls);
     chain_wait();
     chain_next();
     r.hold_weights(p);
     const float inv_width = 1.f / (float)r.width;
-    Pair dpre[PAIRS], dpost[PAIRS], dgate[GATE == 2 ? PAIRS : 1];
-#pragma unroll
-    for (int q = 0; q < PAIRS; ++q) dpre[q] = dpost[q] = pair(0.f);
-    const int slots = gridDim.x * R::ROWS, slot = blockIdx.x * R::ROWS + threadIdx.x / R::TPR;
-    // an item is a piece of a group of samples; the threads of a row take a run of items, whose rows follow each other
-    const int item_begin = run_start(p.items, slot, slots), item_end = run_start(p.items, slot + 1, slots);
-    auto item_row = [&](int item) {
-        const int group = item / p.parts, part = item - group * p.parts;
-        return group * p.per_group + (int)((long long)p.per_group * part / p.parts);
+    const int slots = of * R::ROWS, slot = rank * R::ROWS + threadIdx.x / R::TPR;
+    // Shared gates: an item is a piece of a group's rows of this class; the threads of a row take a run of items, whose rows follow each other. Otherwise a run of rows.
+    const int items = GATE == 2 ? p.groups * p.pieces : (cls < p.n ? (p.n - cls + period - 1) / period : 0);
+    const int item_begin = run_start(items, slot, slots), item_end = run_start(items, slot + 1, slots);
+    auto rows_before = [&](int row) { return row > cls ? (row - cls + period - 1) / period : 0; };           // rows of the class in front of `row`
+    auto item_start = [&](int item) {
+        if (GATE != 2) return item;
+        const int group = item / p.pieces, piece = item - group * p.pieces, a = rows_before(group * p.per_group);
+        return group == p.groups ? rows_before(p.n) : a + run_start(rows_before((group + 1) * p.per_group) - a, piece, p.pieces);
     };
-    const int begin = item_row(item_begin), end = item_begin < item_end ? item_row(item_end) : begin;
+    const int begin = item_start(item_begin), end = item_begin < item_end ? item_start(item_end) : begin;
     const void* tensors[GATE == 1 ? 5 : 4];
     tensors[0] = p.dh ? p.y : nullptr; tensors[1] = p.dh; tensors[2] = p.dy; tensors[3] = p.branch;
     if constexpr (GATE == 1) tensors[4] = p.gate;
-    auto fetch = [&](int row, int stage) {
-        if (row < end) r.fetch(p, stage, row, *reinterpret_cast<const void* const(*)[GATE == 1 ? 5 : 4]>(&tensors));
+    auto fetch = [&](int t, int stage) {
+        if (t < end) r.fetch(p, stage, cls + period * t, *reinterpret_cast<const void* const(*)[GATE == 1 ? 5 : 4]>(&tensors));
         copies_commit();
     };
     for (int i = 0; i < STAGES; ++i) fetch(begin + i, i);
-    uint32_t graw[GATE ? R::RAW : 1];
-    int item = item_begin, last = begin, stage = 0;              // last: the row behind the present item
-    if (GATE != 2) last = end;                                   // (nothing happens between the items of other gates)
-    --item;
-    for (int row = begin; row < end; ++row) {
-        if (GATE == 2 && row == last) {
-            ++item;
-            last = item_row(item + 1);
-            r.load(p, p.gate, item / p.parts, p.groups, *reinterpret_cast<uint32_t(*)[R::RAW]>(&graw));
+    // What a gate that stays the same over rows multiplies can wait for its last row: with a = scale * gate and G = sum of dx * u over the rows,
+    //   dpost += a * G,   dgate = scale * post * G,   v = dx * (a * post)
+    Pair dpre[PAIRS], dpost[PAIRS], g_sum[PAIRS], factor[GATE == 1 ? 1 : PAIRS];
 #pragma unroll
-            for (int q = 0; q < PAIRS; ++q) dgate[q] = pair(0.f);
+    for (int q = 0; q < PAIRS; ++q) dpre[q] = dpost[q] = g_sum[q] = pair(0.f);
+    if constexpr (GATE == 0) {
+        r.weights(p, 0, factor);
+#pragma unroll
+        for (int q = 0; q < PAIRS; ++q) factor[q] = factor[q] * pair(p.scale);
+    }
+    int item = item_begin - 1, last = begin, stage = 0;          // last: behind the rows of the present item
+    for (int t = begin; t < end; ++t) {
+        const int row = cls + period * t;
+        if (GATE == 2 && t == last) {
+            ++item;
+            last = item_start(item + 1);
+            if constexpr (GATE == 2) {
+                Pair w[PAIRS];
+                r.load_gate(p, item / p.pieces, factor);
+                r.weights(p, 0, w);
+#pragma unroll
+                for (int q = 0; q < PAIRS; ++q) { factor[q] = factor[q] * pair(p.scale) * w[q]; g_sum[q] = pair(0.f); }
+            }
         }
         const float rb = p.branch ? ld_chained(p.stats + row) : 0.f, ry = p.dh ? ld_chained(p.stats + p.n + row) : 0.f;
         copies_wait<STAGES - 1>();
-        if (VEC == 1) row_sync<WPR>();
-        uint32_t braw[R::RAW], yraw[R::RAW];
+        uint32_t braw[R::RAW], graw[GATE == 1 ? R::RAW : 1];
         Pair dx[PAIRS];
         if (p.dy) {
             uint32_t raw[R::RAW];
-            r.get(p, stage, row, 2, raw);
+            r.get(stage, 2, raw);
 #pragma unroll
             for (int q = 0; q < PAIRS; ++q) dx[q] = R::value(raw, q);
         } else {
 #pragma unroll
             for (int q = 0; q < PAIRS; ++q) dx[q] = pair(0.f);
         }
-        if (p.branch) r.get(p, stage, row, 3, braw);
-        if constexpr (GATE == 1) r.get(p, stage, row, 4, graw);
+        if (p.branch) r.get(stage, 3, braw);
+        if constexpr (GATE == 1) r.get(stage, 4, graw);
         if (p.dh) {
-            uint32_t raw[R::RAW];
+            uint32_t raw[R::RAW], yraw[R::RAW];
             Pair w[PAIRS], s = pair(0.f);
-            r.get(p, stage, row, 0, yraw);
-            r.get(p, stage, row, 1, raw);
+            r.get(stage, 0, yraw);
+            r.get(stage, 1, raw);
             r.weights(p, 1, w);
             const Pair f = pair(ry);
 #pragma unroll
             for (int q = 0; q < PAIRS; ++q) {
-                const Pair yn = R::value(yraw, q) * f, dh = R::value(raw, q), t = dh * w[q];
-                dpre[q] = fma2(dh, yn, dpre[q]);
-                s = fma2(t, yn, s);
-                dx[q] = fma2(t, f, dx[q]);
+                const Pair y = R::value(yraw, q), z = R::value(raw, q) * f, v = z * w[q];        // dh * r(y), t * r(y)
+                dpre[q] = fma2(z, y, dpre[q]);
+                s = fma2(v, y, s);
+                dx[q] = dx[q] + v;
             }
             const Pair m = pair(-(row_sum<WPR>(sum(s), words, turn) * inv_width * ry * ry));
-            fetch(row + STAGES, stage);                          // into the stage that every thread of the row has read by now
+            fetch(t + STAGES, stage);                            // into the stage that has been read by now
 #pragma unroll
             for (int q = 0; q < PAIRS; ++q) dx[q] = fma2(m, R::value(yraw, q), dx[q]);
         } else {
             row_sync<WPR>();
-            fetch(row + STAGES, stage);
+            fetch(t + STAGES, stage);
         }
-        const size_t at = (size_t)row * p.features;
-        r.store(p.dx, at, dx);
+        r.store(p.dx, p, row, dx);
         if (p.branch) {
-            Pair w[PAIRS], s = pair(0.f);
-            r.weights(p, 0, w);
-            const Pair f = pair(rb), scale = pair(p.scale);
+            Pair s = pair(0.f);
+            const Pair f = pair(rb);
             if constexpr (GATE == 1) {
-                Pair dg[PAIRS];
+                Pair w[PAIRS], dg[PAIRS];
+                const Pair scale = pair(p.scale);
+                r.weights(p, 0, w);
 #pragma unroll
                 for (int q = 0; q < PAIRS; ++q) {
                     const Pair u = R::value(braw, q) * f, sdx = scale * dx[q], dn = sdx * R::value(graw, q);
@@ -527,38 +477,46 @@ __global__ void __launch_bounds__(32 * WPR * ROWS, 1) residual_norm_bwd_kernel(c
                     dx[q] = dn * w[q];
                     s = fma2(dx[q], u, s);
                 }
-                if (p.dgate) r.store(p.dgate, at, dg);
+                if (p.dgate) r.store(p.dgate, p, row, dg);
             } else {
 #pragma unroll
                 for (int q = 0; q < PAIRS; ++q) {
-                    const Pair u = R::value(braw, q) * f, sdx = scale * dx[q];
-                    Pair dn = sdx;
-                    if constexpr (GATE == 2) {
-                        dn = sdx * R::value(*reinterpret_cast<uint32_t(*)[R::RAW]>(&graw), q);
-                        dgate[q] = fma2(sdx * u, w[q], dgate[q]);
-                    }
-                    dpost[q] = fma2(dn, u, dpost[q]);
-                    dx[q] = dn * w[q];
+                    const Pair u = R::value(braw, q) * f;
+                    g_sum[q] = fma2(dx[q], u, g_sum[q]);
+                    dx[q] = dx[q] * factor[q];
                     s = fma2(dx[q], u, s);
                 }
             }
             const Pair m = pair(-(row_sum<WPR>(sum(s), words, turn) * inv_width * rb));
 #pragma unroll
             for (int q = 0; q < PAIRS; ++q) dx[q] = f * fma2(m, R::value(braw, q), dx[q]);
-            r.store(p.dbranch, at, dx);
+            r.store(p.dbranch, p, row, dx);
         }
-        if (GATE == 2 && row + 1 == last && p.dgate) {
-            const int group = item / p.parts;
-            if (p.parts == 1) {
+        if constexpr (GATE == 2) {
+            if (t + 1 == last) {
+                const int group = item / p.pieces, piece = item - group * p.pieces;
+                const Pair scale = pair(p.scale);
+                Pair w[PAIRS], gate[PAIRS];
+                r.load_gate(p, group, gate);
+                r.weights(p, 0, w);
 #pragma unroll
-                for (int q = 0; q < PAIRS; ++q) dx[q] = dgate[q];
-                // (a row of the gate's gradient: component c at (c * groups + group) * F)
-                r.store_gate(p, p.dgate, group, dx);
-            } else r.store_sums(p.part_gate + (size_t)item * r.width, *reinterpret_cast<Pair(*)[PAIRS]>(&dgate));
+                for (int q = 0; q < PAIRS; ++q) {
+                    dpost[q] = fma2(gate[q] * scale, g_sum[q], dpost[q]);
+                    g_sum[q] = g_sum[q] * scale * w[q];
+                }
+                if (p.dgate) {
+                    if (p.part_gate) r.store_sums(p, p.part_gate + ((size_t)group * p.parts + cls * p.pieces + piece) * r.width, g_sum);
+                    else r.store_gate(p, group, g_sum);
+                }
+            }
         }
         if (++stage == STAGES) stage = 0;
     }
     copies_wait<0>();
+    if (GATE == 0) {
+#pragma unroll
+        for (int q = 0; q < PAIRS; ++q) dpost[q] = g_sum[q] * pair(p.scale);
+    }
     if (p.part_w) {
         // the rows of the CTA together, in shared memory (nothing reads the ring any more)
         float* out = p.part_w + (size_t)blockIdx.x * 2 * r.width;
@@ -567,8 +525,8 @@ __global__ void __launch_bounds__(32 * WPR * ROWS, 1) residual_norm_bwd_kernel(c
             float* sums = reinterpret_cast<float*>(ring_smem);
             __syncthreads();
             float* mine = sums + (size_t)(threadIdx.x / R::TPR) * 2 * r.width;
-            r.store_sums(mine, dpre);
-            r.store_sums(mine + r.width, dpost);
+            r.store_sums(p, mine, dpre);
+            r.store_sums(p, mine + r.width, dpost);
             __syncthreads();
             for (int e = threadIdx.x; e < 2 * r.width; e += R::THREADS) {
                 float v = sums[e];
@@ -576,8 +534,8 @@ __global__ void __launch_bounds__(32 * WPR * ROWS, 1) residual_norm_bwd_kernel(c
                 out[e] = v;
             }
         } else {
-            r.store_sums(out, dpre);
-            r.store_sums(out + r.width, dpost);
+            r.store_sums(p, out, dpre);
+            r.store_sums(p, out + r.width, dpost);
         }
     }
 }
@@ -740,12 +698,12 @@ __global__ void __launch_bounds__(RN_SUM_THREADS) residual_norm_sum_kernel(const
     }
 }
 
-// Whether the rows of every tensor are read 16 bytes at a time (vec values), and whether the tensors start on 16 bytes at all.
-inline void alignment(const RNParams& p, int vec, bool& vectors, bool& bases) {
+// Whether every tensor starts on 16 bytes.
+inline bool aligned_bases(const RNParams& p) {
     uintptr_t tensors = 0;
-    for (const void* t : {p.x, p.branch, p.gate, (const void*)p.y, (const void*)p.h, p.dy, p.dh, (const void*)p.dx, (const void*)p.dbranch, (const void*)p.dgate}) tensors |= reinterpret_cast<uintptr_t>(t);
-    bases = tensors % 16 == 0;
-    vectors = bases && p.features % vec == 0 && (reinterpret_cast<uintptr_t>(p.post) | reinterpret_cast<uintptr_t>(p.pre)) % 16 == 0;
+    for (const void* t : {p.x, p.branch, (const void*)p.y, (const void*)p.h, p.dy, p.dh, (const void*)p.dx, (const void*)p.dbranch}) tensors |= reinterpret_cast<uintptr_t>(t);
+    if (p.gate && p.groups == p.n) tensors |= reinterpret_cast<uintptr_t>(p.gate) | reinterpret_cast<uintptr_t>(p.dgate);
+    return tensors % 16 == 0;
 }
 
 template <typename K>
@@ -753,58 +711,61 @@ cudaError_t norm_launch(K kernel, int grid, int threads, size_t smem, cudaStream
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_CTA_SMEM - 1024);     // (a limit, not what the launch asks for)
     return e != cudaSuccess ? e : launch_chained(kernel, grid, threads, smem, s, p);
 }
-template <typename T, int VEC, int EPT, int WPR, int ROWS, bool OWN>
+template <typename T, int VEC, bool ALIGNED, int EPT, int WPR, int ROWS, bool OWN>
 cudaError_t fwd_own(const RNParams& p, cudaStream_t s) {
-    typedef FwdRow<T, VEC, EPT, WPR, ROWS, OWN> R;
-    return norm_launch(residual_norm_fwd_kernel<T, VEC, EPT, WPR, ROWS, OWN>, grid_cap(p.n, ROWS, 1), R::THREADS, R::SMEM, s, p);
+    typedef FwdRow<T, VEC, ALIGNED, EPT, WPR, ROWS, OWN> R;
+    const int least = p.n < p.period ? p.n : p.period, grid = grid_cap(p.n, ROWS, 1);          // a CTA for each place that rows start at
+    return norm_launch(residual_norm_fwd_kernel<T, VEC, ALIGNED, EPT, WPR, ROWS, OWN>, grid < least ? least : grid, R::THREADS, R::SMEM, s, p);
 }
-template <typename T, int VEC, int EPT, int WPR, int ROWS>
+template <typename T, int VEC, bool ALIGNED, int EPT, int WPR, int ROWS>
 cudaError_t fwd_launch(const RNParams& p, cudaStream_t s) {
-    return p.gate && p.groups == p.n ? fwd_own<T, VEC, EPT, WPR, ROWS, true>(p, s) : fwd_own<T, VEC, EPT, WPR, ROWS, false>(p, s);
+    return p.gate && p.groups == p.n ? fwd_own<T, VEC, ALIGNED, EPT, WPR, ROWS, true>(p, s) : fwd_own<T, VEC, ALIGNED, EPT, WPR, ROWS, false>(p, s);
 }
-template <typename T, int VEC>
-cudaError_t fwd_any(const RNParams& p, cudaStream_t s) {
-    const RNShape k = fwd_shape((long long)p.comps * p.features);
-    if (k.warps == 1) return k.values == 8 ? fwd_launch<T, VEC, 8, 1, 16>(p, s) : fwd_launch<T, VEC, 32, 1, 12>(p, s);
-    if (k.warps == 4) return k.values == 16 ? fwd_launch<T, VEC, 16, 4, 4>(p, s) : fwd_launch<T, VEC, 32, 4, 3>(p, s);
-    return k.warps == 8 ? fwd_launch<T, VEC, 32, 8, 1>(p, s) : fwd_launch<T, VEC, 32, 16, 1>(p, s);
+template <typename T, int VEC, bool ALIGNED>
+cudaError_t fwd_any(const RNParams& p, const RNShape& k, cudaStream_t s) {
+    if (k.warps == 1) return k.values == 8 ? fwd_launch<T, VEC, ALIGNED, 8, 1, 16>(p, s) : fwd_launch<T, VEC, ALIGNED, 32, 1, 12>(p, s);
+    if (k.warps == 4) return k.values == 16 ? fwd_launch<T, VEC, ALIGNED, 16, 4, 4>(p, s) : fwd_launch<T, VEC, ALIGNED, 32, 4, 3>(p, s);
+    return k.warps == 8 ? fwd_launch<T, VEC, ALIGNED, 32, 8, 1>(p, s) : fwd_launch<T, VEC, ALIGNED, 32, 16, 1>(p, s);
 }
-template <typename T, int VEC, int EPT, int WPR, int ROWS, int GATE>
+template <typename T, int VEC, bool ALIGNED, int EPT, int WPR, int ROWS, int GATE>
 cudaError_t bwd_gate(const RNParams& p, const RNPlan& q, cudaStream_t s) {
-    typedef BwdRow<T, VEC, EPT, WPR, ROWS, GATE> R;
-    return norm_launch(residual_norm_bwd_kernel<T, VEC, EPT, WPR, ROWS, GATE>, q.grid, R::THREADS, R::SMEM, s, p);
+    typedef BwdRow<T, VEC, ALIGNED, EPT, WPR, ROWS, GATE> R;
+    return norm_launch(residual_norm_bwd_kernel<T, VEC, ALIGNED, EPT, WPR, ROWS, GATE>, q.grid, R::THREADS, R::SMEM, s, p);
 }
-template <typename T, int VEC, int EPT, int WPR, int ROWS>
+template <typename T, int VEC, bool ALIGNED, int EPT, int WPR, int ROWS>
 cudaError_t bwd_launch(const RNParams& p, const RNPlan& q, cudaStream_t s) {
-    if (!p.gate) return bwd_gate<T, VEC, EPT, WPR, ROWS, 0>(p, q, s);
-    return p.groups == p.n ? bwd_gate<T, VEC, EPT, WPR, ROWS, 1>(p, q, s) : bwd_gate<T, VEC, EPT, WPR, ROWS, 2>(p, q, s);
+    if (!p.gate) return bwd_gate<T, VEC, ALIGNED, EPT, WPR, ROWS, 0>(p, q, s);
+    return p.groups == p.n ? bwd_gate<T, VEC, ALIGNED, EPT, WPR, ROWS, 1>(p, q, s) : bwd_gate<T, VEC, ALIGNED, EPT, WPR, ROWS, 2>(p, q, s);
 }
-template <typename T, int VEC>
+template <typename T, int VEC, bool ALIGNED>
 cudaError_t bwd_any(const RNParams& p, const RNPlan& q, cudaStream_t s) {
     switch (q.shape.warps) {
-        case 1: return q.shape.values == 8 ? bwd_launch<T, VEC, 8, 1, 16>(p, q, s) : bwd_launch<T, VEC, 16, 1, 12>(p, q, s);
-        case 4: return bwd_launch<T, VEC, 16, 4, 3>(p, q, s);
-        case 8: return bwd_launch<T, VEC, 16, 8, 2>(p, q, s);
-        default: return bwd_launch<T, VEC, 16, 16, 1>(p, q, s);
+        case 1: return q.shape.values == 8 ? bwd_launch<T, VEC, ALIGNED, 8, 1, 16>(p, q, s) : bwd_launch<T, VEC, ALIGNED, 16, 1, 12>(p, q, s);
+        case 4: return bwd_launch<T, VEC, ALIGNED, 16, 4, 3>(p, q, s);
+        case 8: return bwd_launch<T, VEC, ALIGNED, 16, 8, 2>(p, q, s);
+        default: return bwd_launch<T, VEC, ALIGNED, 16, 16, 1>(p, q, s);
     }
 }
 template <typename T, int VEC>
-int fwd_typed(const RNParams& p, cudaStream_t s) {
-    bool vec, bases;
-    alignment(p, VEC, vec, bases);
-    const RNShape k = fwd_shape((long long)p.comps * p.features);
-    if (k.warps == 0 || !bases) PCB_CUDA_TRY(launch_chained(residual_norm_fwd_wide_kernel<T>, grid_cap(p.n, 1, 4), RN_WIDE_THREADS, 0, s, p));
-    else if (vec) PCB_CUDA_TRY((fwd_any<T, VEC>(p, s)));
-    else PCB_CUDA_TRY((fwd_any<T, 1>(p, s)));
+int fwd_typed(RNParams p, cudaStream_t s) {
+    p.period = row_period(p.features, sizeof(T));
+    const RNShape k = fwd_shape(padded_width(p.comps, p.features, sizeof(T)));
+    if (k.warps == 0 || !aligned_bases(p)) PCB_CUDA_TRY(launch_chained(residual_norm_fwd_wide_kernel<T>, grid_cap(p.n, 1, 4), RN_WIDE_THREADS, 0, s, p));
+    else if (p.period == 1) PCB_CUDA_TRY((fwd_any<T, VEC, true>(p, k, s)));
+    else PCB_CUDA_TRY((fwd_any<T, VEC, false>(p, k, s)));
     return PCB_OK;
 }
 template <typename T, int VEC>
-int bwd_typed(const RNParams& p, const RNPlan& q, cudaStream_t s) {
-    bool vec, bases;
-    alignment(p, VEC, vec, bases);
-    if (q.shape.warps == 0) PCB_CUDA_TRY(launch_chained(residual_norm_bwd_wide_kernel<T>, q.grid, RN_WIDE_THREADS, 0, s, p));
-    else if (vec) PCB_CUDA_TRY((bwd_any<T, VEC>(p, q, s)));
-    else PCB_CUDA_TRY((bwd_any<T, 1>(p, q, s)));
+int bwd_typed(RNParams p, RNPlan q, cudaStream_t s) {
+    p.period = row_period(p.features, sizeof(T));
+    const bool wide = q.shape.warps == 0 || !aligned_bases(p);
+    if (wide) q = q.shape.warps == 0 ? q : wide_plan(p.comps, p.n, p.features, p.gate ? p.groups : 0);
+    p.parts = q.parts; p.pieces = q.pieces; p.items = q.items;
+    p.part_w = p.dpost || p.dpre ? reinterpret_cast<float*>(p.workspace) : nullptr;
+    p.part_gate = p.dgate && q.part_gate ? reinterpret_cast<float*>(p.workspace + q.part_w) : nullptr;
+    if (wide) PCB_CUDA_TRY(launch_chained(residual_norm_bwd_wide_kernel<T>, q.grid, RN_WIDE_THREADS, 0, s, p));
+    else if (p.period == 1) PCB_CUDA_TRY((bwd_any<T, VEC, true>(p, q, s)));
+    else PCB_CUDA_TRY((bwd_any<T, VEC, false>(p, q, s)));
     const long long weight_blocks = p.part_w ? (p.features + 7) / 8 : 0;
     const long long gate_blocks = p.part_gate ? ((long long)p.groups * p.comps * p.features + RN_SUM_THREADS - 1) / RN_SUM_THREADS : 0;
     if (weight_blocks + gate_blocks > 0)

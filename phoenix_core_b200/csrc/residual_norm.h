@@ -8,7 +8,7 @@ namespace pcb {
 
 struct RNParams {
     int comps, n, features, groups, per_group;     // groups: rows of the gate per component (0: no gate); per_group: samples of each
-    uint32_t magic;                                // ceil(2^32 / features): e / features = umulhi(e, magic) for the widths below (0: features == 1)
+    int period;                                    // rows that start at different places within 16 bytes
     float scale, eps;
     const void *x, *branch, *gate;
     const float *post, *pre;
@@ -18,9 +18,10 @@ struct RNParams {
     const void *dy, *dh;
     void *dx, *dbranch, *dgate;
     float *dpost, *dpre;
+    uint8_t* workspace;
     float *part_w;                                 // [CTAs][2][comps * features]: dpre, dpost
     float *part_gate;                              // [groups * parts][comps * features]
-    int parts, items;                              // pieces per group
+    int parts, pieces, items;                      // per group: sums that make its gate's gradient, pieces of each class's rows; pieces in all
 };
 
 // Warps per row, values per thread and rows of a CTA (one per SM) for a width; warps 0: wider than the registers.
@@ -43,32 +44,65 @@ inline RNShape bwd_shape(long long width) {
     return {0, 0, 1};
 }
 
-struct RNPlan { RNShape shape; int grid, slots, parts, items; size_t part_w, part_gate, total; };
-inline RNPlan bwd_plan(int comps, int n, int features, int groups) {
-    RNPlan q = {};
-    const long long width = (long long)comps * features;
-    q.shape = bwd_shape(width);
-    const int rows_per_cta = q.shape.rows, most = tc::device_sms() * (q.shape.warps ? rows_per_cta : 4);      // (wide rows: four CTAs on an SM)
-    const bool shared = groups > 0 && groups < n;
-    const int g = shared || (groups == n && n > 0) ? groups : 1;
-    if (groups == n && groups > 1 && !shared) { q.parts = 1; q.items = n; }          // a gate for each value: every sample is an item
-    else {
-        // pieces per group: as many as fill the machine for one to eight rounds, whichever has the fewest rounds x samples per piece
-        const int per = n / g;
-        long long best = -1;
-        for (long long rounds = 1; rounds <= 8; ++rounds) {
-            const long long fit = rounds * most / g, parts = fit < 1 ? 1 : (fit < per ? fit : per);
-            const long long cost = (g * parts + most - 1) / most * ((per + parts - 1) / parts);
-            if (best < 0 || cost < best) { best = cost; q.parts = (int)parts; }
-        }
-        q.items = g * q.parts;
+// Rows after which a row starts at the same place within 16 bytes again, and values of a row with those that its vectors reach over.
+inline int row_period(int features, int size) {
+    const int bytes = features * size % 16;
+    return bytes == 0 ? 1 : (bytes % 8 == 0 ? 2 : (bytes % 4 == 0 ? 4 : 8));
+}
+inline long long padded_width(int comps, int features, int size) {
+    const int vec = 16 / size;
+    return row_period(features, size) == 1 ? (long long)comps * features : (long long)comps * ((features + 2 * vec - 2) / vec) * vec;
+}
+
+// How a backward call is cut, and the bytes of its sums.
+struct RNPlan { RNShape shape; int grid, parts, pieces, items; size_t part_w, part_gate, total; };
+// Pieces of a group's `per` rows where `groups` of them share `most` workers: as many as fill those for one to eight rounds, whichever has the fewest rounds x rows
+// per piece.
+inline int pieces_of(int groups, int per, long long most) {
+    long long best = -1;
+    int pieces = 1;
+    for (long long rounds = 1; rounds <= 8; ++rounds) {
+        const long long fit = rounds * most / groups, n = fit < 1 ? 1 : (fit < per ? fit : per);
+        const long long cost = (groups * n + most - 1) / most * ((per + n - 1) / n);
+        if (best < 0 || cost < best) { best = cost; pieces = (int)n; }
     }
-    const int want = q.items < most ? q.items : most;
-    q.grid = (want + rows_per_cta - 1) / rows_per_cta;
-    q.slots = q.grid;                                   // sums of the weights' gradients: one set per CTA
-    q.part_w = (size_t)q.slots * 2 * width * 4;
-    q.part_gate = shared && (q.parts > 1 || q.shape.warps == 0) ? (size_t)q.items * width * 4 : (groups == n && n > 0 && q.shape.warps == 0 ? (size_t)n * width * 4 : 0);
+    return pieces;
+}
+inline void sums_of(RNPlan& q, long long width, int gates, int n) {
+    q.part_w = (size_t)q.grid * 2 * width * 4;
+    q.part_gate = gates > 0 && (q.shape.warps == 0 || (gates < n && q.parts > 1)) ? (size_t)gates * q.parts * width * 4 : 0;
     q.total = q.part_w + q.part_gate;
+}
+// Rows wider than the registers, tensors that start anywhere, and groups of fewer rows than there are places for them to start at: four CTAs on an SM, a row each.
+inline RNPlan wide_plan(int comps, int n, int features, int gates) {
+    RNPlan q = {};
+    const int groups = gates > 0 ? gates : 1;
+    const long long most = 4LL * tc::device_sms();
+    q.parts = q.pieces = pieces_of(groups, n / groups, most);
+    q.items = groups * q.parts;
+    q.grid = (int)(q.items < most ? q.items : most);
+    sums_of(q, (long long)comps * features, gates, n);
+    return q;
+}
+inline RNPlan bwd_plan(int comps, int n, int features, int gates, int size) {
+    const int period = row_period(features, size);
+    const bool shared = gates > 0 && gates < n;
+    RNPlan q = {};
+    q.shape = bwd_shape(padded_width(comps, features, size));
+    if (q.shape.warps == 0 || (shared && n / gates < period)) return wide_plan(comps, n, features, gates);
+    const int sms = tc::device_sms(), rows = q.shape.rows;
+    q.pieces = shared ? pieces_of(gates, n / gates / period, (long long)(sms / period > 0 ? sms / period : 1) * rows) : 1;
+    q.parts = shared ? q.pieces * period : 1;
+    // a CTA for each place that rows start at, at least, and no more than have work
+    const long long work = shared ? (long long)gates * q.pieces : (n + period - 1) / period;
+    long long per_class = (work + rows - 1) / rows;
+    if (per_class * period > sms) per_class = sms / period > 0 ? sms / period : 1;
+    q.grid = (int)(per_class * period);
+    if (!shared && q.grid > n) q.grid = n;
+    sums_of(q, (long long)comps * features, gates, n);
+    // (a call whose tensors do not start on 16 bytes takes the other plan: room for either)
+    const RNPlan w = wide_plan(comps, n, features, gates);
+    q.total = q.total > w.total ? q.total : w.total;
     return q;
 }
 
