@@ -587,7 +587,7 @@ int launch(const Geom& g, const Q8Product& q, int splits, cudaStream_t stream) {
     if (rc != PCB_OK) return rc;
     const size_t smem = C::SMEM > ONE_CTA_SMEM ? C::SMEM : ONE_CTA_SMEM;
     static_assert(C::SMEM <= MAX_CTA_SMEM, "shared memory of a CTA");
-    PCB_CUDA_TRY(cudaFuncSetAttribute(dense8_kernel<BN, SWAP, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    PCB_CUDA_TRY((allow_cta_smem<dense8_kernel<BN, SWAP, PAIR>>()));
     const int grid = PAIR ? 2 * (p.tiles < sm_pairs() ? p.tiles : sm_pairs()) : (splits > 1 ? p.tiles * splits : (p.tiles < sm_count() ? p.tiles : sm_count()));
     PCB_CUDA_TRY(launch_clusters(PAIR ? 2 : splits, true, dense8_kernel<BN, SWAP, PAIR>, grid, D8_THREADS, smem, stream, ma, mb, mo, p, q.status));
     return PCB_OK;

@@ -706,16 +706,16 @@ inline bool aligned_bases(const RNParams& p) {
     return tensors % 16 == 0;
 }
 
-template <typename K>
-cudaError_t norm_launch(K kernel, int grid, int threads, size_t smem, cudaStream_t s, const RNParams& p) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_CTA_SMEM - 1024);     // (a limit, not what the launch asks for)
-    return e != cudaSuccess ? e : launch_chained(kernel, grid, threads, smem, s, p);
+template <auto Kernel>
+cudaError_t norm_launch(int grid, int threads, size_t smem, cudaStream_t s, const RNParams& p) {
+    const cudaError_t e = allow_cta_smem<Kernel>(MAX_CTA_SMEM - 1024);             // (the sums' words are static)
+    return e != cudaSuccess ? e : launch_chained(Kernel, grid, threads, smem, s, p);
 }
 template <typename T, int VEC, bool ALIGNED, int EPT, int WPR, int ROWS, bool OWN>
 cudaError_t fwd_own(const RNParams& p, cudaStream_t s) {
     typedef FwdRow<T, VEC, ALIGNED, EPT, WPR, ROWS, OWN> R;
     const int least = p.n < p.period ? p.n : p.period, grid = grid_cap(p.n, ROWS, 1);          // a CTA for each place that rows start at
-    return norm_launch(residual_norm_fwd_kernel<T, VEC, ALIGNED, EPT, WPR, ROWS, OWN>, grid < least ? least : grid, R::THREADS, R::SMEM, s, p);
+    return norm_launch<residual_norm_fwd_kernel<T, VEC, ALIGNED, EPT, WPR, ROWS, OWN>>(grid < least ? least : grid, R::THREADS, R::SMEM, s, p);
 }
 template <typename T, int VEC, bool ALIGNED, int EPT, int WPR, int ROWS>
 cudaError_t fwd_launch(const RNParams& p, cudaStream_t s) {
@@ -730,7 +730,7 @@ cudaError_t fwd_any(const RNParams& p, const RNShape& k, cudaStream_t s) {
 template <typename T, int VEC, bool ALIGNED, int EPT, int WPR, int ROWS, int GATE>
 cudaError_t bwd_gate(const RNParams& p, const RNPlan& q, cudaStream_t s) {
     typedef BwdRow<T, VEC, ALIGNED, EPT, WPR, ROWS, GATE> R;
-    return norm_launch(residual_norm_bwd_kernel<T, VEC, ALIGNED, EPT, WPR, ROWS, GATE>, q.grid, R::THREADS, R::SMEM, s, p);
+    return norm_launch<residual_norm_bwd_kernel<T, VEC, ALIGNED, EPT, WPR, ROWS, GATE>>(q.grid, R::THREADS, R::SMEM, s, p);
 }
 template <typename T, int VEC, bool ALIGNED, int EPT, int WPR, int ROWS>
 cudaError_t bwd_launch(const RNParams& p, const RNPlan& q, cudaStream_t s) {

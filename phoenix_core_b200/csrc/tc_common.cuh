@@ -2,6 +2,7 @@
 // (fetched from the driver at run time, so the library does not link against libcuda), small host utilities.
 #pragma once
 #include "sm_share.h"
+#include <atomic>
 #include <cstdlib>
 
 #include <cuda.h>
@@ -149,6 +150,19 @@ __device__ __forceinline__ float2 ld_chained(const float2* p, bool ok = true) {
 __device__ __forceinline__ float4 ld_chained(const float4* p, bool ok = true) {
     const uint4 v = ld_chained(reinterpret_cast<const uint4*>(p), ok);
     return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+}
+// Gives a kernel the dynamic shared memory that a CTA may have, once per device (the attribute costs a call some 0.4 us). One flag word per kernel.
+template <auto Kernel>
+cudaError_t allow_cta_smem(int bytes = MAX_CTA_SMEM) {
+    static std::atomic<unsigned long long> allowed{0};
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    const unsigned long long bit = device < 64 ? 1ull << device : 0ull;
+    if (bit && (allowed.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+    e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) allowed.fetch_or(bit, std::memory_order_release);
+    return e;
 }
 // `cluster`: CTAs per cluster.
 template <typename... Params, typename... Args>

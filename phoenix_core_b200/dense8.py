@@ -14,8 +14,9 @@ import ctypes
 import torch
 
 from . import _lib
+from .context import Context
 from .descriptors import MULTIVECTOR_DIM, Algebra, FilterLayout
-from .ops import _ALGEBRAS, _DTYPES, Device, _check_tensor, _dense_desc, _OnDevice, _ptr, _stream
+from .ops import _ALGEBRAS, _DTYPES, Device, _build_dense_desc, _launch, _need, _need_input
 
 BLOCK = 128
 
@@ -46,6 +47,8 @@ class Filter8:
             self.values = self.values[0]
         self.scales = torch.full((dim, (rows + BLOCK - 1) // BLOCK, (cols + BLOCK - 1) // BLOCK), 127, dtype=torch.uint8, device=device)
 
+        self._descs = {}
+
     @property
     def device(self):
         return self._storage.device
@@ -58,85 +61,91 @@ class Filter8:
         return (self.values.reshape(dim, rows, cols).float() * scale).reshape(self.shape)
 
 
-def _check_filter8(filter8, descriptor, device):
-    if not isinstance(filter8, Filter8):
-        raise ValueError("filter must be a Filter8 (see quantizeFilter8)")
-    if filter8.shape != tuple(descriptor.getFilterShape()) or filter8.algebra != descriptor.getAlgebra() or filter8.filterLayout != descriptor.getFilterLayout():
-        raise ValueError("filter mismatch: %s vs expected %s" % (filter8.shape, tuple(descriptor.getFilterShape())))
-    if filter8.device != device:
-        raise ValueError("filter is on %s, the input on %s" % (filter8.device, device))
+class _Call:
+    """What a call with a descriptor needs and does not change: the C descriptor, its sizes and shapes."""
 
+    def __init__(self, descriptor, dtype, engine, flag, forward):
+        context = Context({})                                # (the formulation that a context chooses has no meaning here)
+        self.desc = _build_dense_desc(descriptor, dtype, context, engine, has_bias=forward and flag, require_input_grad=not forward and flag)
+        self.ref = ctypes.byref(self.desc)
+        L = _lib.lib()
+        self.workspace = (L.pcb_qdense8_fwd_workspace_size if forward else L.pcb_qdense8_bwd_workspace_size)(self.ref)
+        self.input, self.output, self.bias = descriptor.getInputShape(), descriptor.getOutputShape(), descriptor.getBiasShape()
+        self.filter = tuple(descriptor.getFilterShape())
+        self.filter_grad = self.filter[:-2] + (descriptor.getInputChannels(), descriptor.getOutputChannels())
+        self.algebra, self.layout = descriptor.getAlgebra(), descriptor.getFilterLayout()
 
-def _check_input(t, name, shape):
-    if t.dtype not in _DTYPES:
-        raise ValueError("%s dtype %s: float32, float16 or bfloat16 expected" % (name, t.dtype))
-    _check_tensor(t, name, shape=shape)
+    @staticmethod
+    def of(descriptor, dtype, engine, flag, forward):
+        cache = descriptor.__dict__.setdefault("_pcb_dense8", {})
+        key = (dtype, engine, flag, forward)
+        call = cache.get(key)
+        if call is None:
+            call = cache[key] = _Call(descriptor, dtype, engine, flag, forward)
+        return call
+
+    def check_filter(self, filter8, index):
+        if not isinstance(filter8, Filter8):
+            raise ValueError("filter must be a Filter8 (see quantizeFilter8)")
+        if filter8.shape != self.filter or filter8.algebra != self.algebra or filter8.filterLayout != self.layout:
+            raise ValueError("filter mismatch: %s vs expected %s" % (filter8.shape, self.filter))
+        if filter8._storage.get_device() != index:
+            raise ValueError("filter is on %s, other tensors of the call on cuda:%d" % (filter8.device, index))
 
 
 def quantizeFilter8(filterTensor, filter8):
     """Rounds a filter of 16- or 32-bit numbers into ``filter8``."""
-    _check_input(filterTensor, "filter", filter8.shape)
-    if filter8.device != filterTensor.device:
+    index = _need_input(filterTensor, "filter", filter8.shape)
+    if filter8._storage.get_device() != index:
         raise ValueError("the Filter8 is on %s, the filter on %s" % (filter8.device, filterTensor.device))
-    d = _lib.DenseDesc()
-    oi = filter8.filterLayout == FilterLayout.OI
-    d.dtype, d.algebra, d.filter_oi = _DTYPES[filterTensor.dtype], _ALGEBRAS[filter8.algebra], int(oi)
-    d.in_features, d.out_features = filter8.shape[-1 if oi else -2], filter8.shape[-2 if oi else -1]
-    dev = Device.get(filterTensor.device)
-    with _OnDevice(dev.index):
-        _lib.check(_lib.lib().pcb_quantize_filter8(ctypes.byref(d), _ptr(filterTensor), _ptr(filter8._storage), _ptr(filter8.scales), _stream()))
+    ref = filter8._descs.get(filterTensor.dtype)
+    if ref is None:
+        d = _lib.DenseDesc()
+        oi = filter8.filterLayout == FilterLayout.OI
+        d.dtype, d.algebra, d.filter_oi = _DTYPES[filterTensor.dtype], _ALGEBRAS[filter8.algebra], int(oi)
+        d.in_features, d.out_features = filter8.shape[-1 if oi else -2], filter8.shape[-2 if oi else -1]
+        ref = filter8._descs[filterTensor.dtype] = ctypes.byref(d)
+    _launch(index, _lib.lib().pcb_quantize_filter8, ref, filterTensor.data_ptr(), filter8._storage.data_ptr(), filter8.scales.data_ptr())
 
 
 def dense8Fwd(inputTensor, filter8, biasTensor, outputTensor, descriptor, context=None, engine=_lib.ENGINE_AUTO):
     """``denseFwd`` with a filter held in 8 bits and the input quantised along its features. Input, bias and output share a type."""
-    dev = Device.get(inputTensor.device)
-    context = context or dev.getContext()
-    _check_input(inputTensor, "input", descriptor.getInputShape())
-    _check_filter8(filter8, descriptor, inputTensor.device)
-    _check_tensor(outputTensor, "output", inputTensor.dtype, descriptor.getOutputShape())
-    if biasTensor is not None:
+    dtype, bias = inputTensor.dtype, biasTensor is not None
+    index = _need_input(inputTensor, "input", descriptor.inputShape)
+    call = _Call.of(descriptor, dtype, engine, bias, True)
+    call.check_filter(filter8, index)
+    _need(outputTensor, "output", dtype, call.output, index)
+    if bias:
         if not descriptor.isBiasUsed():
             raise ValueError("Bias application is not configured for this scalar Dense operation")
-        _check_tensor(biasTensor, "bias", inputTensor.dtype, descriptor.getBiasShape())
-    if inputTensor.numel() == 0:
+        _need(biasTensor, "bias", dtype, call.bias, index)
+    if call.input[0] == 0:
         return
-    d = _dense_desc(descriptor, inputTensor.dtype, context, engine, has_bias=biasTensor is not None)
-    L = _lib.lib()
-    with dev.accessControl, _OnDevice(dev.index):
-        need = getattr(d, "_fwd8_need", None)
-        if need is None:
-            need = d._fwd8_need = L.pcb_qdense8_fwd_workspace_size(ctypes.byref(d))
-        ws = dev.requestWorkspace(need)
-        _lib.check(L.pcb_qdense8_fwd(ctypes.byref(d), _ptr(inputTensor), _ptr(filter8._storage), _ptr(filter8.scales), _ptr(biasTensor),
-                                     _ptr(outputTensor), _ptr(ws), ws.numel(), _stream()))
+    dev = Device.at(index)
+    with dev.accessControl:
+        ws = dev.requestWorkspace(call.workspace)
+        _launch(index, _lib.lib().pcb_qdense8_fwd, call.ref, inputTensor.data_ptr(), filter8._storage.data_ptr(), filter8.scales.data_ptr(),
+                biasTensor.data_ptr() if bias else None, outputTensor.data_ptr(), ws.data_ptr(), ws.numel())
         dev._after_op()
 
 
 def dense8Bwd(inputTensor, filter8, gradTensor, filterGradTensor, inputGradTensor, descriptor, context=None, engine=_lib.ENGINE_AUTO):
     """``denseBwd`` in 8 bits: the filter gradient (input-major, ``[D, I, O]``, whatever the filter layout) from the input and the output
     gradient quantised along the samples, the input gradient from the filter and the output gradient quantised along the features."""
-    dev = Device.get(inputTensor.device)
-    context = context or dev.getContext()
-    _check_input(inputTensor, "input", descriptor.getInputShape())
-    _check_filter8(filter8, descriptor, inputTensor.device)
-    _check_tensor(gradTensor, "grad", inputTensor.dtype, descriptor.getOutputShape())
-    _check_tensor(filterGradTensor, "filterGrad", inputTensor.dtype)
-    i, o = descriptor.getInputChannels(), descriptor.getOutputChannels()
-    if tuple(filterGradTensor.shape) != filter8.shape[:-2] + (i, o):
-        raise ValueError("filterGrad shape mismatch: %s vs expected %s" % (tuple(filterGradTensor.shape), filter8.shape[:-2] + (i, o)))
-    need_dx = descriptor.isInputGradientRequired()
+    dtype, need_dx = inputTensor.dtype, descriptor.isInputGradientRequired()
+    index = _need_input(inputTensor, "input", descriptor.inputShape)
+    call = _Call.of(descriptor, dtype, engine, need_dx, False)
+    call.check_filter(filter8, index)
+    _need(gradTensor, "grad", dtype, call.output, index)
+    _need(filterGradTensor, "filterGrad", dtype, call.filter_grad, index)
     if need_dx:
-        _check_tensor(inputGradTensor, "inputGrad", inputTensor.dtype, descriptor.getInputShape())
-    if inputTensor.numel() == 0:
+        _need(inputGradTensor, "inputGrad", dtype, call.input, index)
+    if call.input[0] == 0:
         filterGradTensor.zero_()
         return
-    d = _dense_desc(descriptor, inputTensor.dtype, context, engine, require_input_grad=need_dx)
-    L = _lib.lib()
-    with dev.accessControl, _OnDevice(dev.index):
-        need = getattr(d, "_bwd8_need", None)
-        if need is None:
-            need = d._bwd8_need = L.pcb_qdense8_bwd_workspace_size(ctypes.byref(d))
-        ws = dev.requestWorkspace(need)
-        _lib.check(L.pcb_qdense8_bwd(ctypes.byref(d), _ptr(inputTensor), _ptr(filter8._storage), _ptr(filter8.scales), _ptr(gradTensor),
-                                     _ptr(filterGradTensor), _ptr(inputGradTensor) if need_dx else None, _ptr(ws), ws.numel(), _stream()))
+    dev = Device.at(index)
+    with dev.accessControl:
+        ws = dev.requestWorkspace(call.workspace)
+        _launch(index, _lib.lib().pcb_qdense8_bwd, call.ref, inputTensor.data_ptr(), filter8._storage.data_ptr(), filter8.scales.data_ptr(),
+                gradTensor.data_ptr(), filterGradTensor.data_ptr(), inputGradTensor.data_ptr() if need_dx else None, ws.data_ptr(), ws.numel())
         dev._after_op()

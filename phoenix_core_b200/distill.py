@@ -14,7 +14,7 @@ import torch
 
 from . import _lib
 from .descriptors import MULTIVECTOR_DIM, Algebra
-from .ops import _ALGEBRAS, _DTYPES, Device, _check_tensor, _OnDevice, _ptr, _stream
+from .ops import _ALGEBRAS, _DTYPES, _launch, _need, _need_input
 
 
 class DistillDescriptor:
@@ -31,73 +31,60 @@ class DistillDescriptor:
         if not 0.0 <= self.alpha <= 1.0 or not 0.0 < self.temperature < float("inf"):
             raise ValueError("alpha in [0, 1] and a positive temperature expected")
         self.samples = self.logitsShape[0] // dim
-        self._desc = {}
+        self.teacherShape, self.lossShape, self.statsShape = (self.samples, self.teacherEntries), (self.samples,), (3, self.samples)
+        self._calls = {}
 
     def getLogitsShape(self): return self.logitsShape
     def getClasses(self): return MULTIVECTOR_DIM[self.algebra] * self.logitsShape[1]
-    def getTeacherShape(self): return (self.samples, self.teacherEntries)
-    def getLossShape(self): return (self.samples,)
-    def getStatsShape(self): return (3, self.samples)
+    def getTeacherShape(self): return self.teacherShape
+    def getLossShape(self): return self.lossShape
+    def getStatsShape(self): return self.statsShape
     def getAlgebra(self): return self.algebra
 
-    def _c(self, dtype):
-        d = self._desc.get(dtype)
-        if d is None:
+    def _call(self, dtype):
+        ref = self._calls.get(dtype)
+        if ref is None:
             d = _lib.DistillDesc()
             d.dtype, d.algebra, d.batch, d.units = _DTYPES[dtype], _ALGEBRAS[self.algebra], self.samples, self.logitsShape[1]
             d.entries, d.alpha, d.temperature = self.teacherEntries, self.alpha, self.temperature
-            self._desc[dtype] = d
-        return d
-
-
-def _check(t, name, like, dtype, shape):
-    _check_tensor(t, name, dtype, shape)
-    if t.device != like.device:
-        raise ValueError("%s is on %s, the logits on %s" % (name, t.device, like.device))
+            ref = self._calls[dtype] = ctypes.byref(d)
+        return ref
 
 
 def _check_operands(logits, labels, teacher, index, descriptor):
-    if logits.dtype not in _DTYPES:
-        raise ValueError("logits dtype %s: float32, float16 or bfloat16 expected" % logits.dtype)
-    _check_tensor(logits, "logits", shape=descriptor.getLogitsShape())
+    """The device's index, and the pointers of labels, teacher and index."""
+    device = _need_input(logits, "logits", descriptor.logitsShape)
     if labels is not None:
-        _check(labels, "labels", logits, torch.int64, descriptor.getLossShape())
-    if descriptor.teacherEntries > 0:
-        if teacher is None or index is None:
-            raise ValueError("the descriptor has %d entries of a teacher" % descriptor.teacherEntries)
-        _check(teacher, "teacherLogits", logits, logits.dtype, descriptor.getTeacherShape())
-        _check(index, "teacherIndices", logits, torch.int64, descriptor.getTeacherShape())
+        _need(labels, "labels", torch.int64, descriptor.lossShape, device)
+        labels = labels.data_ptr()
+    if descriptor.teacherEntries == 0:
+        return device, labels, None, None
+    if teacher is None or index is None:
+        raise ValueError("the descriptor has %d entries of a teacher" % descriptor.teacherEntries)
+    _need(teacher, "teacherLogits", logits.dtype, descriptor.teacherShape, device)
+    _need(index, "teacherIndices", torch.int64, descriptor.teacherShape, device)
+    return device, labels, teacher.data_ptr(), index.data_ptr()
 
 
 def distillFwd(logitsTensor, labels, teacherLogits, teacherIndices, lossTensor, statsTensor, descriptor):
     """Losses (fp32, one per sample) of logits against ``labels`` (int64, None: no such term; a value outside the classes leaves a sample's out) and
     the teacher's logits at ``teacherIndices`` (int64; an index outside the classes leaves an entry out). ``statsTensor`` (fp32,
     ``getStatsShape()``) is kept for ``distillBwd`` and may be None."""
-    x = logitsTensor
-    _check_operands(x, labels, teacherLogits, teacherIndices, descriptor)
-    _check(lossTensor, "loss", x, torch.float32, descriptor.getLossShape())
+    device, *operands = _check_operands(logitsTensor, labels, teacherLogits, teacherIndices, descriptor)
+    _need(lossTensor, "loss", torch.float32, descriptor.lossShape, device)
     if statsTensor is not None:
-        _check(statsTensor, "stats", x, torch.float32, descriptor.getStatsShape())
-    if x.numel() == 0:
-        return
-    teacher = descriptor.teacherEntries > 0
-    dev = Device.get(x.device)
-    with _OnDevice(dev.index):
-        _lib.check(_lib.lib().pcb_distill_fwd(ctypes.byref(descriptor._c(x.dtype)), _ptr(x), _ptr(labels), _ptr(teacherLogits) if teacher else None,
-                                              _ptr(teacherIndices) if teacher else None, _ptr(lossTensor), _ptr(statsTensor), _stream()))
+        _need(statsTensor, "stats", torch.float32, descriptor.statsShape, device)
+    if descriptor.samples:
+        _launch(device, _lib.lib().pcb_distill_fwd, descriptor._call(logitsTensor.dtype), logitsTensor.data_ptr(), *operands, lossTensor.data_ptr(),
+                None if statsTensor is None else statsTensor.data_ptr())
 
 
 def distillBwd(logitsTensor, labels, teacherLogits, teacherIndices, statsTensor, gradLoss, gradLogits, descriptor):
     """The gradient of the logits, ``gradLoss`` (fp32) being that of each sample's loss. ``gradLogits`` must not be the logits themselves."""
-    x = logitsTensor
-    _check_operands(x, labels, teacherLogits, teacherIndices, descriptor)
-    _check(statsTensor, "stats", x, torch.float32, descriptor.getStatsShape())
-    _check(gradLoss, "gradLoss", x, torch.float32, descriptor.getLossShape())
-    _check(gradLogits, "gradLogits", x, x.dtype, descriptor.getLogitsShape())
-    if x.numel() == 0:
-        return
-    teacher = descriptor.teacherEntries > 0
-    dev = Device.get(x.device)
-    with _OnDevice(dev.index):
-        _lib.check(_lib.lib().pcb_distill_bwd(ctypes.byref(descriptor._c(x.dtype)), _ptr(x), _ptr(labels), _ptr(teacherLogits) if teacher else None,
-                                              _ptr(teacherIndices) if teacher else None, _ptr(statsTensor), _ptr(gradLoss), _ptr(gradLogits), _stream()))
+    device, *operands = _check_operands(logitsTensor, labels, teacherLogits, teacherIndices, descriptor)
+    _need(statsTensor, "stats", torch.float32, descriptor.statsShape, device)
+    _need(gradLoss, "gradLoss", torch.float32, descriptor.lossShape, device)
+    _need(gradLogits, "gradLogits", logitsTensor.dtype, descriptor.logitsShape, device)
+    if descriptor.samples:
+        _launch(device, _lib.lib().pcb_distill_bwd, descriptor._call(logitsTensor.dtype), logitsTensor.data_ptr(), *operands, statsTensor.data_ptr(),
+                gradLoss.data_ptr(), gradLogits.data_ptr())

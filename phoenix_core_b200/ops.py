@@ -41,6 +41,12 @@ class Device:
         self.check_after_each_op = os.environ.get("PCB_CHECK_DEVICE_STATUS", "0") not in ("", "0")
 
     @classmethod
+    def at(cls, index):
+        """``get`` for a device's index."""
+        dev = cls._devices.get(index)
+        return cls.get(torch.device("cuda", index)) if dev is None else dev
+
+    @classmethod
     def get(cls, torch_device):
         idx = torch_device.index if torch_device.index is not None else torch.cuda.current_device()
         dev = cls._devices.get(idx)                    # entries are made once, under the lock, and never replaced
@@ -153,6 +159,36 @@ class _OnDevice:
             self.guard.__exit__(*exc)
             self.guard = None
         return False
+
+
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _need(t, name, dtype, shape, index):
+    """Raises unless a tensor is what ``_check_tensor`` asks for, on the device `index`: one look for the call that is in order (a microsecond less per
+    tensor than the checks that can say what is wrong, which then follow)."""
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != index or not t.is_contiguous():
+        _check_tensor(t, name, dtype, shape)
+        raise ValueError("%s is on %s, other tensors of the call on cuda:%d" % (name, t.device, index))
+
+
+def _need_input(t, name, shape):
+    """Checks the tensor that settles the type and the device of a call; returns the device's index."""
+    if t.dtype not in _DTYPES:
+        raise ValueError("%s dtype %s: float32, float16 or bfloat16 expected" % (name, t.dtype))
+    index = t.get_device()
+    if index < 0 or t.shape != shape or not t.is_contiguous():
+        _check_tensor(t, name, shape=shape)
+    return index
+
+
+def _launch(index, entry, *args):
+    """Calls an entry point of the library on a device's current stream (its last argument)."""
+    if _current_device() == index:
+        _lib.check(entry(*args, _raw_stream(index)))
+    else:
+        with torch.cuda.device(index):
+            _lib.check(entry(*args, _raw_stream(index)))
 
 
 # upstride::Algebra -> pcb_algebra (the C ABI keeps quaternion at zero)

@@ -17,7 +17,7 @@ import torch
 
 from . import _lib
 from .descriptors import MULTIVECTOR_DIM, Algebra
-from .ops import _ALGEBRAS, _DTYPES, Device, _check_tensor, _OnDevice, _ptr, _stream
+from .ops import _ALGEBRAS, _DTYPES, Device, _launch, _need, _need_input
 
 
 class ResidualNormDescriptor:
@@ -34,70 +34,67 @@ class ResidualNormDescriptor:
             raise ValueError("%d rows of the gate for %d samples" % (self.gateRows, self.samples))
         if not self.epsilon >= 0.0:
             raise ValueError("epsilon must not be negative")
-        self._desc = {}
+        self.gateShape, self.weightShape, self.statsShape = (dim * self.gateRows, self.inputShape[1]), (self.inputShape[1],), (2, self.samples)
+        self._calls = {}
 
     def getInputShape(self): return self.inputShape
-    def getGateShape(self): return (MULTIVECTOR_DIM[self.algebra] * self.gateRows, self.inputShape[1])
-    def getWeightShape(self): return (self.inputShape[1],)
-    def getStatsShape(self): return (2, self.samples)
+    def getGateShape(self): return self.gateShape
+    def getWeightShape(self): return self.weightShape
+    def getStatsShape(self): return self.statsShape
     def getAlgebra(self): return self.algebra
 
-    def _c(self, dtype):
-        d = self._desc.get(dtype)
-        if d is None:
+    def _call(self, dtype):
+        call = self._calls.get(dtype)
+        if call is None:
             d = _lib.NormDesc()
             d.dtype, d.algebra, d.batch, d.features = _DTYPES[dtype], _ALGEBRAS[self.algebra], self.samples, self.inputShape[1]
             d.gate_rows, d.residual_scale, d.epsilon = self.gateRows, self.residualScale, self.epsilon
-            self._desc[dtype] = d
-        return d
+            ref = ctypes.byref(d)
+            call = self._calls[dtype] = (ref, _lib.lib().pcb_residual_norm_bwd_workspace_size(ref))
+        return call
 
 
-def _check_optional(t, name, like, shape, dtype=None):
-    if t is not None:
-        _check_tensor(t, name, like.dtype if dtype is None else dtype, shape)
-        if t.device != like.device:
-            raise ValueError("%s is on %s, the input on %s" % (name, t.device, like.device))
-
-
-def _check_first(t, name, descriptor):
-    if t.dtype not in _DTYPES:
-        raise ValueError("%s dtype %s: float32, float16 or bfloat16 expected" % (name, t.dtype))
-    _check_tensor(t, name, shape=descriptor.getInputShape())
-
-
-def _check_parts(descriptor, like, branch, gate, post, pre):
-    shape, weights = descriptor.getInputShape(), descriptor.getWeightShape()
-    _check_optional(branch, "branch", like, shape)
+def _check_parts(descriptor, dtype, index, branch, gate, post, pre):
+    if branch is not None:
+        _need(branch, "branch", dtype, descriptor.inputShape, index)
+    elif gate is not None or post is not None:
+        raise ValueError("a gate or postWeight without a branch")
     if (gate is None) != (descriptor.gateRows == 0):
         raise ValueError("the descriptor has %d rows of a gate" % descriptor.gateRows)
-    _check_optional(gate, "gate", like, descriptor.getGateShape())
-    _check_optional(post, "postWeight", like, weights, torch.float32)
-    _check_optional(pre, "preWeight", like, weights, torch.float32)
-    if branch is None and (gate is not None or post is not None):
-        raise ValueError("a gate or postWeight without a branch")
+    if gate is not None:
+        _need(gate, "gate", dtype, descriptor.gateShape, index)
+    if post is not None:
+        _need(post, "postWeight", torch.float32, descriptor.weightShape, index)
+    if pre is not None:
+        _need(pre, "preWeight", torch.float32, descriptor.weightShape, index)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def residualNormFwd(residualTensor, branchTensor, gateTensor, postWeight, preWeight, outputTensor, normTensor, statsTensor, descriptor):
     """y into ``outputTensor`` and h into ``normTensor``; ``statsTensor`` (fp32, ``getStatsShape()``) keeps the factors of both norms for the
     backward call and may be None. Without a branch (None, with gate and postWeight) h is the norm of the residual itself and
     ``outputTensor`` may be None; without ``normTensor`` (None, with preWeight) there is no norm behind the block. Weights may be None (ones)."""
-    x = residualTensor
-    _check_first(x, "residual", descriptor)
-    _check_parts(descriptor, x, branchTensor, gateTensor, postWeight, preWeight)
-    if (branchTensor is not None and outputTensor is None) or (outputTensor is None and normTensor is None):
+    x, dtype = residualTensor, residualTensor.dtype
+    shape = descriptor.inputShape
+    index = _need_input(x, "residual", shape)
+    _check_parts(descriptor, dtype, index, branchTensor, gateTensor, postWeight, preWeight)
+    if (branchTensor is not None or normTensor is None) and outputTensor is None:
         raise ValueError("output expected")
-    if normTensor is None and preWeight is not None:
+    if outputTensor is not None:
+        _need(outputTensor, "output", dtype, shape, index)
+    if normTensor is not None:
+        _need(normTensor, "norm", dtype, shape, index)
+    elif preWeight is not None:
         raise ValueError("preWeight without normTensor")
-    _check_optional(outputTensor, "output", x, x.shape)
-    _check_optional(normTensor, "norm", x, x.shape)
-    _check_optional(statsTensor, "stats", x, descriptor.getStatsShape(), torch.float32)
-    if x.numel() == 0:
+    if statsTensor is not None:
+        _need(statsTensor, "stats", torch.float32, descriptor.statsShape, index)
+    if shape[0] == 0:
         return
-    d = descriptor._c(x.dtype)
-    dev = Device.get(x.device)
-    with _OnDevice(dev.index):
-        _lib.check(_lib.lib().pcb_residual_norm_fwd(ctypes.byref(d), _ptr(x), _ptr(branchTensor), _ptr(gateTensor), _ptr(postWeight), _ptr(preWeight),
-                                                    _ptr(outputTensor), _ptr(normTensor), _ptr(statsTensor), _stream()))
+    _launch(index, _lib.lib().pcb_residual_norm_fwd, descriptor._call(dtype)[0], x.data_ptr(), _ptr(branchTensor), _ptr(gateTensor), _ptr(postWeight),
+            _ptr(preWeight), _ptr(outputTensor), _ptr(normTensor), _ptr(statsTensor))
 
 
 def residualNormBwd(outputTensor, branchTensor, gateTensor, postWeight, preWeight, statsTensor, gradOutput, gradNorm, gradResidual, gradBranch,
@@ -105,41 +102,47 @@ def residualNormBwd(outputTensor, branchTensor, gateTensor, postWeight, preWeigh
     """From ``gradOutput`` (of y, from the residual path; None: none) and ``gradNorm`` (of h; None: there was no norm behind the block) the
     gradients of the residual, the branch, the gate and the weights; those of the gate and the weights may be None. ``outputTensor`` is the forward
     call's y (the residual itself where there was no branch), needed where there is a ``gradNorm``."""
-    like = gradResidual
-    _check_first(like, "gradResidual", descriptor)
-    _check_parts(descriptor, like, branchTensor, gateTensor, postWeight, preWeight)
-    shape, weights = descriptor.getInputShape(), descriptor.getWeightShape()
+    dtype, shape, weights = gradResidual.dtype, descriptor.inputShape, descriptor.weightShape
+    index = _need_input(gradResidual, "gradResidual", shape)
+    _check_parts(descriptor, dtype, index, branchTensor, gateTensor, postWeight, preWeight)
     if gradOutput is None and gradNorm is None:
         raise ValueError("gradOutput or gradNorm expected")
-    if gradNorm is not None and outputTensor is None:
-        raise ValueError("output expected: the gradient of its norm needs it")
-    if gradNorm is None and (preWeight is not None or gradPreWeight is not None):
-        raise ValueError("preWeight without gradNorm")
-    if branchTensor is None and gradPostWeight is not None:
+    if gradNorm is None:
+        if preWeight is not None or gradPreWeight is not None:
+            raise ValueError("preWeight without gradNorm")
+    else:
+        if outputTensor is None:
+            raise ValueError("output expected: the gradient of its norm needs it")
+        _need(gradNorm, "gradNorm", dtype, shape, index)
+        _need(outputTensor, "output", dtype, shape, index)
+    if gradOutput is not None:
+        _need(gradOutput, "gradOutput", dtype, shape, index)
+    if branchTensor is not None:
+        if gradBranch is None:
+            raise ValueError("gradBranch expected")
+        _need(gradBranch, "gradBranch", dtype, shape, index)
+    elif gradPostWeight is not None:
         raise ValueError("gradPostWeight without a branch")
-    if (gradGate is not None and gateTensor is None) or (branchTensor is not None and gradBranch is None):
-        raise ValueError("gradGate without a gate, or a branch without gradBranch")
-    for t, name in ((outputTensor, "output"), (gradOutput, "gradOutput"), (gradNorm, "gradNorm"), (gradBranch, "gradBranch")):
-        _check_optional(t, name, like, shape)
-    _check_optional(gradGate, "gradGate", like, descriptor.getGateShape())
-    _check_optional(gradPostWeight, "gradPostWeight", like, weights, torch.float32)
-    _check_optional(gradPreWeight, "gradPreWeight", like, weights, torch.float32)
+    if gradGate is not None:
+        if gateTensor is None:
+            raise ValueError("gradGate without a gate")
+        _need(gradGate, "gradGate", dtype, descriptor.gateShape, index)
+    if gradPostWeight is not None:
+        _need(gradPostWeight, "gradPostWeight", torch.float32, weights, index)
+    if gradPreWeight is not None:
+        _need(gradPreWeight, "gradPreWeight", torch.float32, weights, index)
     if statsTensor is None:
         raise ValueError("stats expected")
-    _check_optional(statsTensor, "stats", like, descriptor.getStatsShape(), torch.float32)
-    if like.numel() == 0:
+    _need(statsTensor, "stats", torch.float32, descriptor.statsShape, index)
+    if shape[0] == 0:
         for t in (gradPostWeight, gradPreWeight, gradGate):
             if t is not None:
                 t.zero_()
         return
-    d = descriptor._c(like.dtype)
-    L, dev = _lib.lib(), Device.get(like.device)
-    with dev.accessControl, _OnDevice(dev.index):
-        need = getattr(d, "_bwd_need", None)
-        if need is None:
-            need = d._bwd_need = L.pcb_residual_norm_bwd_workspace_size(ctypes.byref(d))
+    ref, need = descriptor._call(dtype)
+    dev = Device.at(index)
+    with dev.accessControl:
         ws = dev.requestWorkspace(need + 256)                          # behind the workspace's status block
-        _lib.check(L.pcb_residual_norm_bwd(ctypes.byref(d), _ptr(outputTensor), _ptr(branchTensor), _ptr(gateTensor), _ptr(postWeight),
-                                           _ptr(preWeight), _ptr(statsTensor), _ptr(gradOutput), _ptr(gradNorm), _ptr(gradResidual),
-                                           _ptr(gradBranch), _ptr(gradGate), _ptr(gradPostWeight), _ptr(gradPreWeight),
-                                           _ptr(ws) + 256, ws.numel() - 256, _stream()))
+        _launch(index, _lib.lib().pcb_residual_norm_bwd, ref, _ptr(outputTensor), _ptr(branchTensor), _ptr(gateTensor), _ptr(postWeight), _ptr(preWeight),
+                statsTensor.data_ptr(), _ptr(gradOutput), _ptr(gradNorm), gradResidual.data_ptr(), _ptr(gradBranch), _ptr(gradGate), _ptr(gradPostWeight),
+                _ptr(gradPreWeight), ws.data_ptr() + 256, ws.numel() - 256)
