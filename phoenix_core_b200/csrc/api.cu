@@ -719,11 +719,12 @@ int pcb_qdense8_fwd(const pcb_dense_desc* desc, const void* x, const void* w8, c
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     int* status = reinterpret_cast<int*>(ws);
     const Q8Target rows = {ws + at.x_rows, reinterpret_cast<uint32_t*>(ws + at.x_words)};
-    rc = q8_quantize(desc->dtype, g.nc, g.Nb, g.Ci, x, rows, Q8Target{}, status, (cudaStream_t)stream);
-    if (rc != PCB_OK) return rc;
+    const bool raw = q8_raw_tokens(g.Nb);
+    if (!raw && (rc = q8_quantize(desc->dtype, g.nc, g.Nb, g.Ci, x, rows, Q8Target{}, status, (cudaStream_t)stream)) != PCB_OK) return rc;
     const Q8Operand tokens = {rows.values, rows.words, q8_pitch(g.Ci), 0, 0, 0, 0}, filter = dense8_filter(g, w8, w8_scales, true);
     Q8Product q = {PASS_FWD, q8_swapped(g.Nb) ? 1 : 0, g.Nb, g.Co, g.Ci, tokens, filter, y, desc->dtype, g.has_bias ? bias : nullptr, status};
     if (q.swapped) { q.m = g.Co; q.n = g.Nb; q.a = filter; q.b = tokens; }
+    if (raw) q.tokens = x;
     return q8_product(g, q, (cudaStream_t)stream);
 }
 int pcb_qdense8_bwd(const pcb_dense_desc* desc, const void* x, const void* w8, const void* w8_scales, const void* dy, void* dw, void* dx, void* workspace,

@@ -37,6 +37,7 @@ struct Q8Product {
     int dtype;
     const void* bias;            // [components][features], forward only
     int* status;
+    const void* tokens = nullptr;       // the tokens as the caller has them: quantised by the product itself (then operand b is not read)
 };
 
 // Quantises x ([components][rows][cols], dense): `by_rows` with blocks of 1 x 128, `by_cols` with blocks of 128 x 1 (either may be null values).
@@ -46,5 +47,7 @@ int q8_quantize_blocks(int dtype, int comps, int rows, int cols, const void* x, 
 int q8_product(const Geom& g, const Q8Product& p, cudaStream_t stream);
 // Whether a forward or backward-data product of that many tokens takes the filter as operand A.
 bool q8_swapped(int tokens);
+// Whether the product quantises that many tokens itself.
+bool q8_raw_tokens(int tokens);
 
 }  // namespace pcb

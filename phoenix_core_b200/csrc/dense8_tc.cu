@@ -16,7 +16,10 @@
 //   single    128 x 128 tiles; a tile's reduction is cut over the CTAs of a cluster where there are fewer tiles than SMs, whose partial sums are added in a
 //             fixed order through distributed shared memory.
 //   SWAP      few tokens: the filter is operand A, a tile is 128 features x 16, 64 or 128 tokens; bound by the filter's bytes.
+//   RAW       the same for up to 16 tokens, which are quantised here: four warps each take a block of 128 of the reduction at a time straight from the caller's tensor
+//             into the stage and the scales' words, so that the call is one launch.
 #include "dense8.cuh"
+#include "e4m3.cuh"
 #include "tc_common.cuh"
 
 namespace pcb {
@@ -43,7 +46,7 @@ template <int BN, bool SWAP, bool PAIR> struct D8Config {
     static constexpr int CTAS = PAIR ? 2 : 1;
     static constexpr int M = D8_BM * CTAS;                       // rows of a tile
     static constexpr uint32_t OUT_BYTES = SWAP ? 0 : 4096;       // per epilogue warp: 32 rows of 128 bytes on their way out
-    static constexpr uint32_t BARS = 256;
+    static constexpr uint32_t BARS = 512;
     static constexpr size_t SMEM = 1024 + STAGES * STAGE + D8_EPI_WARPS * OUT_BYTES + D8_SF_STAGES * D8_SF_BYTES + BARS;
 };
 
@@ -63,6 +66,8 @@ struct D8Params {
     long long out_comp; int out_ld;     // element (c, slow, fast) of the output at c * out_comp + slow * out_ld + fast
     void* out;
     const void* bias;                   // [comps][fast extent], or null
+    const void* tokens;                 // RAW: the tokens as the caller has them, [comps][n][k]
+    int* clear;                         // the call's status word, if this launch is to reset it
 };
 
 // Operand components and sign of term j of output component c.
@@ -188,10 +193,92 @@ __device__ __forceinline__ void d8_tile(const D8Params& p, int tile, int& c, int
     nt = in / height;
 }
 
+// RAW: warp 8 + j quantises block j of every group of the reduction for up to BN tokens. It leaves byte j of the tokens' words before it waits for the stage, as the
+// products of the group wait for the words of all four.
+template <int BN, int STAGES, uint32_t STAGE>
+__device__ __forceinline__ void d8_quantize_tokens(const D8Params& p, uint32_t base, uint32_t sf, uint32_t full, uint32_t empty, uint32_t sf_full, uint32_t sf_empty, int first, int stride,
+                                                   int g_begin, int g_end, int j_begin, int* status) {
+    const int lane = threadIdx.x & 31, j = (threadIdx.x >> 5) & 3;
+    const bool quads = p.k % 4 == 0 && reinterpret_cast<uintptr_t>(p.tokens) % 16 == 0;          // four values per load
+    D8Walk w;
+    int q = 0, block0 = 0;                                       // block0: blocks of the groups behind us (their stages follow each other)
+    uint32_t par = 1;
+    for (int tile = first; tile < p.tiles; tile += stride) {
+        int c, mt, nt;
+        d8_tile(p, tile, c, mt, nt);
+        for (w.start(p, c, g_begin, g_end, j_begin); w.left > 0; w.step(p, c)) {
+            const int blocks = w.blocks(p), k = (w.group * 4 + j) * D8_BK + lane * 4;
+            float v[BN][4];
+            if (j < blocks) {
+#pragma unroll
+                for (int r = 0; r < BN; ++r) {
+                    if (r >= p.n) break;
+                    const size_t at = ((size_t)w.first * p.n + r) * p.k + k;
+                    if (quads && p.dtype == PCB_F32) {
+                        const float4 x = ld_chained(static_cast<const float4*>(p.tokens) + at / 4, k < p.k);
+                        v[r][0] = x.x; v[r][1] = x.y; v[r][2] = x.z; v[r][3] = x.w;
+                    } else if (quads) {
+                        const uint2 x = ld_chained(static_cast<const uint2*>(p.tokens) + at / 4, k < p.k);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t h = (e < 2 ? x.x : x.y) >> (16 * (e & 1)) & 0xffffu;
+                            v[r][e] = p.dtype == PCB_F16 ? __half2float(__ushort_as_half((uint16_t)h)) : __uint_as_float(h << 16);
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[r][e] = k + e < p.k ? ld_typed(p.tokens, p.dtype, at + e) : 0.f;
+                    }
+                }
+            }
+            if (!warp_wait_bounded(sf_empty + 8 * q, par, status, ST_D8_SCALES)) return;
+            uint32_t data[BN];
+            if (j < blocks) {
+#pragma unroll
+                for (int r = 0; r < BN; ++r) {
+                    if (r >= p.n) break;
+                    uint32_t top = 0;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t key = __float_as_uint(v[r][e]) & 0x7fffffffu;
+                        if (key < 0x7f800000u) top = max(top, key);
+                        else v[r][e] = __uint_as_float(0x7fffffffu);                // infinities too: the conversion would saturate them
+                    }
+                    const int byte = scale_byte(__reduce_max_sync(0xffffffffu, top));
+                    const float f = inverse_scale(byte);
+                    data[r] = to_e4m3x2(v[r][0], v[r][1], make_float2(f, f)) | to_e4m3x2(v[r][2], v[r][3], make_float2(f, f)) << 16;
+                    if (lane == 0) asm volatile("st.shared.u8 [%0], %1;" ::"r"(sf + q * D8_SF_BYTES + 512u + r * 16u + j), "r"(byte) : "memory");
+                }
+                fence_proxy_async_smem();
+            }
+            __syncwarp();
+            if (elect_one()) mbar_arrive(sf_full + 8 * q);
+            __syncwarp();
+            if (j < blocks) {
+                const int block = block0 + j, s = block % STAGES;
+                if (!warp_wait_bounded(empty + 8 * s, ((uint32_t)(block / STAGES) & 1u) ^ 1u, status, ST_D8_PRODUCER)) return;
+                const uint32_t b = base + s * STAGE + D8_A_BYTES + (uint32_t)(lane & 3) * 4u;
+#pragma unroll
+                for (int r = 0; r < BN; ++r) {
+                    if (r >= p.n) break;
+                    asm volatile("st.shared.u32 [%0], %1;" ::"r"(b + r * 128u + (uint32_t)(((lane >> 2) ^ (r & 7)) << 4)), "r"(data[r]) : "memory");
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (elect_one()) mbar_arrive(full + 8 * s);
+                __syncwarp();
+            }
+            block0 += blocks;
+            if (++q == D8_SF_STAGES) { q = 0; par ^= 1u; }
+        }
+    }
+}
+
 // SWAP: operand A is the filter, so that tile rows run along the output's fast axis. PAIR: clusters of two; the even CTA issues for both.
-template <int BN, bool SWAP, bool PAIR>
+// The waits look at a status word of the CTA's own; the call's gets it at the end.
+template <int BN, bool SWAP, bool PAIR, bool RAW>
 __global__ void __launch_bounds__(D8_THREADS, 1)
-dense8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_out, const D8Params p, int* status) {
+dense8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_out, const D8Params p, int* call_status) {
+    static_assert(!RAW || (SWAP && BN == 16), "raw tokens: up to 16");
     using C = D8Config<BN, SWAP, PAIR>;
     extern __shared__ uint8_t smem_raw[];
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
@@ -203,16 +290,26 @@ dense8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     const uint32_t base_addr = smem_u32(base), sf_addr = smem_u32(sf);
     const uint32_t full = smem_u32(bars), empty = full + 8 * C::STAGES, sf_full = empty + 8 * C::STAGES, sf_empty = sf_full + 8 * D8_SF_STAGES;
     const uint32_t acc_full = sf_empty + 8 * D8_SF_STAGES, acc_empty = acc_full + 8 * C::ACC, slot = acc_empty + 8 * C::ACC;
+    int* status = reinterpret_cast<int*>(bars + 2 * C::STAGES + 2 * D8_SF_STAGES + 2 * C::ACC + 1);
 
     if (t == 0) {
-        for (int s = 0; s < C::STAGES; ++s) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 1); }
-        for (int s = 0; s < D8_SF_STAGES; ++s) { mbar_init(sf_full + 8 * s, 2 * C::CTAS); mbar_init(sf_empty + 8 * s, 1); }
-        for (int s = 0; s < C::ACC; ++s) { mbar_init(acc_full + 8 * s, 1); mbar_init(acc_empty + 8 * s, D8_EPI_WARPS * C::CTAS); }
+        *status = 0;
+        for (int s = 0; s < C::STAGES; ++s) { mbar_init(full + 8 * s, RAW ? 2 : 1); mbar_init(empty + 8 * s, 1); }
+        for (int s = 0; s < D8_SF_STAGES; ++s) { mbar_init(sf_full + 8 * s, RAW ? 5 : 2 * C::CTAS); mbar_init(sf_empty + 8 * s, 1); }
+        for (int s = 0; s < C::ACC; ++s) { mbar_init(acc_full + 8 * s, 1); mbar_init(acc_empty + 8 * s, RAW ? 4 : D8_EPI_WARPS * C::CTAS); }
         fence_barrier_init();
     }
     if (warp == 1) {
         if (PAIR) tmem_alloc_pair(slot, 512);
         else tmem_alloc(slot, 512);
+    }
+    if (RAW) {
+        // rows of tokens that do not exist: zeros with a scale of one
+        for (int i = t; i < C::STAGES * (BN * D8_BK / 16); i += D8_THREADS)
+            st_shared_v4(base_addr + (uint32_t)(i / (BN * D8_BK / 16)) * C::STAGE + D8_A_BYTES + (uint32_t)(i % (BN * D8_BK / 16)) * 16u, 0u, 0u, 0u, 0u);
+        for (int i = t; i < D8_SF_STAGES * 32; i += D8_THREADS)
+            st_shared_v4(sf_addr + (uint32_t)(i / 32) * D8_SF_BYTES + 512u + (uint32_t)(i % 32) * 16u, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu);
+        fence_proxy_async_smem();
     }
     tc_fence_before_sync();
     __syncthreads();
@@ -222,6 +319,7 @@ dense8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(slot));
     chain_wait();
     chain_next();
+    if (p.clear && t == 0 && blockIdx.x == 0) *p.clear = 0;
 
     const int split = p.splits > 1 ? (int)cluster_ctarank() : 0;
     const int share = PAIR ? 2 : p.splits, first = blockIdx.x / share, stride = gridDim.x / share;
@@ -252,9 +350,9 @@ dense8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                             tma_load_3d_pair(a, &map_a, p.a_mn ? m0 : k * D8_BK, p.a_mn ? k * D8_BK : m0, ca, lead);
                             tma_load_3d_pair(b, &map_b, p.b_mn ? n0 : k * D8_BK, p.b_mn ? k * D8_BK : n0, cb, lead);
                         } else {
-                            mbar_arrive_expect_tx(bar, D8_A_BYTES + BN * D8_BK);
+                            mbar_arrive_expect_tx(bar, D8_A_BYTES + (RAW ? 0 : BN * D8_BK));
                             tma_load_3d(a, &map_a, p.a_mn ? m0 : k * D8_BK, p.a_mn ? k * D8_BK : m0, ca, bar);
-                            tma_load_3d(b, &map_b, p.b_mn ? n0 : k * D8_BK, p.b_mn ? k * D8_BK : n0, cb, bar);
+                            if constexpr (!RAW) tma_load_3d(b, &map_b, p.b_mn ? n0 : k * D8_BK, p.b_mn ? k * D8_BK : n0, cb, bar);
                         }
                     }
                     __syncwarp();
@@ -326,6 +424,8 @@ dense8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             __syncwarp();
             if (++acc == C::ACC) { acc = 0; acc_par ^= 1u; }
         }
+    } else if (RAW && (warp == 3 || warp >= 8)) {
+        if (warp >= 8) d8_quantize_tokens<BN, C::STAGES, C::STAGE>(p, base_addr, sf_addr, full, empty, sf_full, sf_empty, first, stride, g_begin, g_end, j_begin, status);
     } else if (warp < 4) {
         // Warp 2 the scales of A, warp 3 those of B, a group of the reduction at a time. The words of the next group are loaded before those of this one are waited for: one
         // warp that loaded them when they were due took 2600 clocks a group, where the MMAs of a group take 2048.
@@ -522,7 +622,13 @@ dense8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         const int ms = min(D8_BM, p.m - mt * D8_BM), ns = min(BN, p.n - nt * BN);
         const int fast_n = SWAP ? ms : ns, slow_n = SWAP ? ns : ms, fast0 = SWAP ? mt * D8_BM : nt * BN, slow0 = SWAP ? nt * BN : mt * D8_BM;
         const int pitch = SWAP ? D8_BM : BN + 1;
-        if (read_status(status) == 0) {
+        bool good = true;                   // no wait ran out in any CTA of the tile
+        for (int r = 0; r < p.splits; ++r) {
+            uint32_t word;
+            asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(word) : "r"(map_to_cta(smem_u32(status), r)) : "memory");
+            good = good && word == 0u;
+        }
+        if (good) {
             for (int e = split * D8_THREADS + t; e < slow_n * fast_n; e += p.splits * D8_THREADS) {
                 const int slow = e / fast_n, fast = e - slow * fast_n;
                 const uint32_t local = base_addr + (uint32_t)(slow * pitch + fast) * 4u;
@@ -540,6 +646,7 @@ dense8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     }
     tc_fence_before_sync();
     __syncthreads();
+    if (t == 0 && *status != 0) atomicOr(call_status, *status);
     if (PAIR) cluster_sync_all();
     if (warp == 1) {
         tc_fence_after_sync();
@@ -556,7 +663,7 @@ int operand_map(CUtensorMap* map, const Q8Operand& o, int extent, int k, int com
     return make_tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, o.values, 3, dims, strides, box, nullptr, CU_TENSOR_MAP_SWIZZLE_128B, what);
 }
 
-template <int BN, bool SWAP, bool PAIR>
+template <int BN, bool SWAP, bool PAIR, bool RAW = false>
 int launch(const Geom& g, const Q8Product& q, int splits, cudaStream_t stream) {
     using C = D8Config<BN, SWAP, PAIR>;
     D8Params p = {};
@@ -573,9 +680,10 @@ int launch(const Geom& g, const Q8Product& q, int splits, cudaStream_t stream) {
     p.dtype = q.dtype; p.out = q.out; p.bias = q.bias;
     p.out_ld = SWAP ? q.m : q.n;
     p.out_comp = (long long)q.m * q.n;
-    CUtensorMap ma, mb, mo = {};
+    CUtensorMap ma, mb = {}, mo = {};
     int rc = operand_map(&ma, q.a, q.m, q.k, g.nc, D8_BM, "8-bit operand A");
-    if (rc == PCB_OK) rc = operand_map(&mb, q.b, q.n, q.k, g.nc, PAIR ? C::B_ROWS : BN, "8-bit operand B");
+    p.tokens = q.tokens; p.clear = RAW ? q.status : nullptr;
+    if (rc == PCB_OK && !RAW) rc = operand_map(&mb, q.b, q.n, q.k, g.nc, PAIR ? C::B_ROWS : BN, "8-bit operand B");
     const size_t size = dtype_size(q.dtype);
     p.out_map = !SWAP && splits == 1 && q.n * size % 16 == 0 && reinterpret_cast<uintptr_t>(q.out) % 16 == 0;
     if (rc == PCB_OK && p.out_map) {
@@ -587,15 +695,16 @@ int launch(const Geom& g, const Q8Product& q, int splits, cudaStream_t stream) {
     if (rc != PCB_OK) return rc;
     const size_t smem = C::SMEM > ONE_CTA_SMEM ? C::SMEM : ONE_CTA_SMEM;
     static_assert(C::SMEM <= MAX_CTA_SMEM, "shared memory of a CTA");
-    PCB_CUDA_TRY((allow_cta_smem<dense8_kernel<BN, SWAP, PAIR>>()));
+    PCB_CUDA_TRY((allow_cta_smem<dense8_kernel<BN, SWAP, PAIR, RAW>>()));
     const int grid = PAIR ? 2 * (p.tiles < sm_pairs() ? p.tiles : sm_pairs()) : (splits > 1 ? p.tiles * splits : (p.tiles < sm_count() ? p.tiles : sm_count()));
-    PCB_CUDA_TRY(launch_clusters(PAIR ? 2 : splits, true, dense8_kernel<BN, SWAP, PAIR>, grid, D8_THREADS, smem, stream, ma, mb, mo, p, q.status));
+    PCB_CUDA_TRY(launch_clusters(PAIR ? 2 : splits, true, dense8_kernel<BN, SWAP, PAIR, RAW>, grid, D8_THREADS, smem, stream, ma, mb, mo, p, q.status));
     return PCB_OK;
 }
 
 }  // namespace
 
 bool q8_swapped(int tokens) { return tokens <= 128; }
+bool q8_raw_tokens(int tokens) { return tokens <= 16; }
 
 int q8_product(const Geom& g, const Q8Product& q, cudaStream_t stream) {
     const int m_tiles = q8_blocks(q.m), groups = g.nc * q8_groups(q.k);
@@ -606,6 +715,7 @@ int q8_product(const Geom& g, const Q8Product& q, cudaStream_t stream) {
         while (s < 8 && tiles * s * 2 <= sm_count() && s * 2 <= groups) s *= 2;
         return s;
     };
+    if (q.tokens) return launch<16, true, false, true>(g, q, splits_for(16), stream);
     if (q.swapped) {
         if (q.n <= 16) return launch<16, true, false>(g, q, splits_for(16), stream);
         if (q.n <= 64) return launch<64, true, false>(g, q, splits_for(64), stream);

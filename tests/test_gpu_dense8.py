@@ -119,3 +119,21 @@ def test_special_values():
     bad[7] = bad[200] = True
     assert torch.equal(torch.isnan(dw).all(dim=1).cpu(), bad) and torch.equal(torch.isnan(dw).any(dim=1).cpu(), bad)
     assert torch.isfinite(dx).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n,i,o", [(2, 1100, 300), (9, 2052, 130), (16, 3000, 64), (5, 513, 20000), (7, 1026, 19100)])
+def test_few_tokens(n, i, o, dtype):
+    """Tokens that the product quantises itself: long reductions cut over CTAs, features of every alignment, more tiles than SMs."""
+    verify("real", "oi" if o % 4 else "io", dtype, n, i, o)
+
+
+def test_few_tokens_special_values():
+    n, i, o = 3, 300, 70
+    dim, x, w, bias, dy = make("complex", "oi", "bf16", n, i, o)
+    x[1, 200] = float("inf")
+    x[0] = 0.0
+    x[dim * n - 1, 3] = float("nan")
+    f8, y, _, _ = run("complex", "oi", x, w, None, dy)
+    y = y.reshape(dim, n, o)
+    assert torch.isnan(y[:, 1]).all() and torch.isnan(y[:, 2]).all() and torch.isfinite(y[:, 0]).all()
