@@ -46,6 +46,7 @@ template <int BN, bool SWAP, bool PAIR> struct D8Config {
     static constexpr int CTAS = PAIR ? 2 : 1;
     static constexpr int M = D8_BM * CTAS;                       // rows of a tile
     static constexpr uint32_t OUT_BYTES = SWAP ? 0 : 4096;       // per epilogue warp: 32 rows of 128 bytes on their way out
+    static constexpr int PART_PITCH = SWAP ? D8_BM : BN + 4;     // words between rows of partial sums (16-byte accesses of eight rows meet no bank twice)
     static constexpr uint32_t BARS = 512;
     static constexpr size_t SMEM = 1024 + STAGES * STAGE + D8_EPI_WARPS * OUT_BYTES + D8_SF_STAGES * D8_SF_BYTES + BARS;
 };
@@ -545,14 +546,19 @@ dense8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             const int row = quarter * 32 + lane, row0 = mt * C::M + (int)rank * D8_BM + quarter * 32, m = row0 + lane, n0 = nt * BN + col0;
             if (p.splits > 1) {
                 // partial sums to shared memory (the ring: every MMA has read it), the fast axis of the output contiguous
-                float* part = reinterpret_cast<float*>(base);
 #pragma unroll
-                for (int b = 0; b < BLOCKS; ++b)
+                for (int b = 0; b < BLOCKS; ++b) {
+                    if constexpr (SWAP) {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        const int n = col0 + 32 * b + e;
-                        if (n < BN) part[SWAP ? n * D8_BM + row : row * (BN + 1) + n] = __uint_as_float(v[b][e]);
+                        for (int e = 0; e < 32; ++e) {
+                            const int n = col0 + 32 * b + e;
+                            if (n < BN) asm volatile("st.shared.u32 [%0], %1;" ::"r"(base_addr + (uint32_t)(n * C::PART_PITCH + row) * 4u), "r"(v[b][e]) : "memory");
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) st_shared_v4(base_addr + (uint32_t)(row * C::PART_PITCH + col0 + 32 * b + e) * 4u, v[b][e], v[b][e + 1], v[b][e + 2], v[b][e + 3]);
                     }
+                }
                 continue;
             }
             const long long comp0 = (long long)c * p.out_comp;
@@ -620,26 +626,48 @@ dense8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         int c, mt, nt;
         d8_tile(p, first, c, mt, nt);
         const int ms = min(D8_BM, p.m - mt * D8_BM), ns = min(BN, p.n - nt * BN);
-        const int fast_n = SWAP ? ms : ns, slow_n = SWAP ? ns : ms, fast0 = SWAP ? mt * D8_BM : nt * BN, slow0 = SWAP ? nt * BN : mt * D8_BM;
-        const int pitch = SWAP ? D8_BM : BN + 1;
+        const int fast_n = SWAP ? ms : ns, slow_n = SWAP ? ns : ms, fast0 = SWAP ? mt * D8_BM : nt * BN, slow0 = SWAP ? nt * BN : mt * D8_BM, extent = SWAP ? p.m : p.n;
         bool good = true;                   // no wait ran out in any CTA of the tile
         for (int r = 0; r < p.splits; ++r) {
             uint32_t word;
             asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(word) : "r"(map_to_cta(smem_u32(status), r)) : "memory");
             good = good && word == 0u;
         }
+        const size_t size = p.dtype == PCB_F32 ? 4 : 2;
+        const bool quads = p.out_ld % 4 == 0 && p.out_comp % 4 == 0 && reinterpret_cast<uintptr_t>(p.out) % (4 * size) == 0;
+        constexpr int F4 = (SWAP ? D8_BM : BN) / 4;
         if (good) {
-            for (int e = split * D8_THREADS + t; e < slow_n * fast_n; e += p.splits * D8_THREADS) {
-                const int slow = e / fast_n, fast = e - slow * fast_n;
-                const uint32_t local = base_addr + (uint32_t)(slow * pitch + fast) * 4u;
-                float sum = 0.f;
-                for (int r = 0; r < p.splits; ++r) {
-                    float x;
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(map_to_cta(local, r)) : "memory");
-                    sum += x;
+            // four neighbours of the output at a time (one by one, a tile of 128 x 128 took ten microseconds to add up)
+            for (int e = split * D8_THREADS + t; e < slow_n * F4; e += p.splits * D8_THREADS) {
+                const int slow = e / F4, fast = e % F4 * 4;
+                if (fast >= fast_n) continue;
+                const uint32_t local = base_addr + (uint32_t)(slow * C::PART_PITCH + fast) * 4u;
+                float part[8][4];
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    if (r < p.splits)
+                        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(part[r][0]), "=f"(part[r][1]), "=f"(part[r][2]), "=f"(part[r][3]) : "r"(map_to_cta(local, r)) : "memory");
+                float out[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    if (r < p.splits) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) out[i] += part[r][i];
+                    }
+                if (p.bias) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (fast + i < fast_n) out[i] += ld_typed(p.bias, p.dtype, (size_t)c * extent + fast0 + fast + i);
                 }
-                if (p.bias) sum += ld_typed(p.bias, p.dtype, (size_t)c * (SWAP ? p.m : p.n) + fast0 + fast);
-                st_typed(p.out, p.dtype, (long long)c * p.out_comp + (long long)(slow0 + slow) * p.out_ld + fast0 + fast, sum);
+                const size_t at = (size_t)((long long)c * p.out_comp + (long long)(slow0 + slow) * p.out_ld + fast0 + fast);
+                if (quads && fast + 4 <= fast_n) {
+                    if (p.dtype == PCB_F32) *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = make_float4(out[0], out[1], out[2], out[3]);
+                    else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = make_uint2(pack_16(out[0], out[1], p.dtype), pack_16(out[2], out[3], p.dtype));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (fast + i < fast_n) st_typed(p.out, p.dtype, at + i, out[i]);
+                }
             }
         }
         cluster_sync_all();                 // nobody leaves while its partial sums are read
