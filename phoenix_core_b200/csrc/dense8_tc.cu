@@ -186,12 +186,12 @@ struct D8Walk {
 
 // Tile order: the tiles of eight rows of tiles together, so that the CTAs at work share both operands' tiles in L2.
 __device__ __forceinline__ void d8_tile(const D8Params& p, int tile, int& c, int& mt, int& nt) {
-    const int per = p.m_tiles * p.n_tiles;
-    c = tile / per;
-    const int r = tile - c * per, band = 8 * p.n_tiles, b = r / band, in = r - b * band;
-    const int height = min(8, p.m_tiles - b * 8);
-    mt = b * 8 + in % height;
-    nt = in / height;
+    const unsigned per = (unsigned)(p.m_tiles * p.n_tiles), t = (unsigned)tile;
+    const unsigned comp = per > t ? 0u : t / per, r = t - comp * per, band = 8u * (unsigned)p.n_tiles, b = band > r ? 0u : r / band, in = r - b * band;
+    const unsigned height = min(8u, (unsigned)p.m_tiles - b * 8u), col = in / height;
+    c = (int)comp;
+    mt = (int)(b * 8u + in - col * height);
+    nt = (int)col;
 }
 
 // RAW: warp 8 + j quantises block j of every group of the reduction for up to BN tokens. It leaves byte j of the tokens' words before it waits for the stage, as the
@@ -293,6 +293,11 @@ dense8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     const uint32_t acc_full = sf_empty + 8 * D8_SF_STAGES, acc_empty = acc_full + 8 * C::ACC, slot = acc_empty + 8 * C::ACC;
     int* status = reinterpret_cast<int*>(bars + 2 * C::STAGES + 2 * D8_SF_STAGES + 2 * C::ACC + 1);
 
+    // (the first copies would wait for their maps)
+    if (warp == 2 && lane < 3 && (lane == 0 || (lane == 1 && !RAW) || (lane == 2 && p.out_map))) {
+        const CUtensorMap* map = lane == 0 ? &map_a : (lane == 1 ? &map_b : &map_out);
+        asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+    }
     if (t == 0) {
         *status = 0;
         for (int s = 0; s < C::STAGES; ++s) { mbar_init(full + 8 * s, RAW ? 2 : 1); mbar_init(empty + 8 * s, 1); }
@@ -734,14 +739,22 @@ int launch(const Geom& g, const Q8Product& q, int splits, cudaStream_t stream) {
 bool q8_swapped(int tokens) { return tokens <= 128; }
 bool q8_raw_tokens(int tokens) { return tokens <= 16; }
 
+// Measured on cold inputs, us (fitted to 1 to 4 rounds of tiles and reductions of 5 to 128 blocks): a single tile of 128 x 128 takes 0.27 a block behind 7.5 for launch, first
+// copies and epilogue; a pair's of 256 x 256 0.34 a block behind 12; a reduction cut over a cluster 3.5 more. 2048 x 4096 -> 4096: pairs 35.3, single 44.5;
+// 1024 x 4096 -> 4096 22.8 / 25.4; 2048 x 1024 -> 4096 17.2 / 16.9; 512 x 4096 -> 4096 21.8 / 15.6. Cut in two and not, 300 x 4096 -> 2048 14.0 / 14.6; 512 x 1024 ->
+// 1024 10.6 / 8.6.
 int q8_product(const Geom& g, const Q8Product& q, cudaStream_t stream) {
-    const int m_tiles = q8_blocks(q.m), groups = g.nc * q8_groups(q.k);
-    // CTAs that share a tile: as many as the SMs and the groups of the reduction allow, up to a portable cluster
+    const int m_tiles = q8_blocks(q.m), groups = g.nc * q8_groups(q.k), blocks = g.nc * q8_blocks(q.k);
+    // CTAs that share a tile, up to a portable cluster and the SMs there are
     auto splits_for = [&](int bn) {
         const long long tiles = (long long)m_tiles * ((q.n + bn - 1) / bn) * g.nc;
-        int s = 1;
-        while (s < 8 && tiles * s * 2 <= sm_count() && s * 2 <= groups) s *= 2;
-        return s;
+        int best = 1;
+        double least = groups;                               // a group of four blocks takes about a microsecond
+        for (int s = 2; s <= 8 && s <= groups && tiles * s <= sm_count(); s *= 2) {
+            const double cost = 3.5 + (groups + s - 1) / s;
+            if (cost < least) { least = cost; best = s; }
+        }
+        return best;
     };
     if (q.tokens) return launch<16, true, false, true>(g, q, splits_for(16), stream);
     if (q.swapped) {
@@ -749,8 +762,9 @@ int q8_product(const Geom& g, const Q8Product& q, cudaStream_t stream) {
         if (q.n <= 64) return launch<64, true, false>(g, q, splits_for(64), stream);
         return launch<128, true, false>(g, q, splits_for(128), stream);
     }
-    const long long wide = (long long)((q.m + 255) / 256) * ((q.n + 255) / 256) * g.nc;
-    if (wide >= sm_pairs()) return launch<256, false, true>(g, q, 1, stream);
+    auto rounds = [](long long tiles, int at_once) { return (double)((tiles + at_once - 1) / at_once); };
+    const long long wide = (long long)((q.m + 255) / 256) * ((q.n + 255) / 256) * g.nc, small = (long long)m_tiles * ((q.n + 127) / 128) * g.nc;
+    if (sm_pairs() > 0 && 12.0 + rounds(wide, sm_pairs()) * blocks * 0.34 < 7.5 + rounds(small, sm_count()) * blocks * 0.27) return launch<256, false, true>(g, q, 1, stream);
     return launch<128, false, false>(g, q, splits_for(128), stream);
 }
 
