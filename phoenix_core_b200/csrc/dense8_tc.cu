@@ -16,7 +16,7 @@
 //   single    128 x 128 tiles; a tile's reduction is cut over the CTAs of a cluster where there are fewer tiles than SMs, whose partial sums are added in a
 //             fixed order through distributed shared memory.
 //   SWAP      few tokens: the filter is operand A, a tile is 128 features x 16, 64 or 128 tokens; bound by the filter's bytes.
-//   RAW       the same for up to 16 tokens, which are quantised here: four warps each take a block of 128 of the reduction at a time straight from the caller's tensor
+//   RAW       the same for up to four tokens, which are quantised here: four warps each take a block of 128 of the reduction at a time straight from the caller's tensor
 //             into the stage and the scales' words, so that the call is one launch.
 #include "dense8.cuh"
 #include "e4m3.cuh"
@@ -32,6 +32,7 @@ constexpr int D8_BM = 128, D8_BK = 128;
 constexpr int D8_THREADS = 384, D8_EPI_WARPS = 8;
 constexpr uint32_t D8_A_BYTES = D8_BM * D8_BK;
 constexpr int D8_SF_STAGES = 4;
+constexpr int D8_RAW = 4;                                       // tokens that a product quantises itself, at most
 constexpr uint32_t D8_SF_BYTES = 512 * 3;                       // one set of 128 rows for A, up to two for B
 constexpr int ST_D8_PRODUCER = 0x100, ST_D8_MMA = 0x200, ST_D8_SCALES = 0x400, ST_D8_EPILOGUE = 0x800;
 
@@ -194,9 +195,9 @@ __device__ __forceinline__ void d8_tile(const D8Params& p, int tile, int& c, int
     nt = (int)col;
 }
 
-// RAW: warp 8 + j quantises block j of every group of the reduction for up to BN tokens. It leaves byte j of the tokens' words before it waits for the stage, as the
+// RAW: warp 8 + j quantises block j of every group of the reduction for up to D8_RAW tokens. It leaves byte j of the tokens' words before it waits for the stage, as the
 // products of the group wait for the words of all four.
-template <int BN, int STAGES, uint32_t STAGE>
+template <int STAGES, uint32_t STAGE>
 __device__ __forceinline__ void d8_quantize_tokens(const D8Params& p, uint32_t base, uint32_t sf, uint32_t full, uint32_t empty, uint32_t sf_full, uint32_t sf_empty, int first, int stride,
                                                    int g_begin, int g_end, int j_begin, int* status) {
     const int lane = threadIdx.x & 31, j = (threadIdx.x >> 5) & 3;
@@ -209,44 +210,53 @@ __device__ __forceinline__ void d8_quantize_tokens(const D8Params& p, uint32_t b
         d8_tile(p, tile, c, mt, nt);
         for (w.start(p, c, g_begin, g_end, j_begin); w.left > 0; w.step(p, c)) {
             const int blocks = w.blocks(p), k = (w.group * 4 + j) * D8_BK + lane * 4;
-            float v[BN][4];
+            // (every load is on its way before the first value is looked at)
+            uint4 raw[D8_RAW];
             if (j < blocks) {
 #pragma unroll
-                for (int r = 0; r < BN; ++r) {
-                    if (r >= p.n) break;
+                for (int r = 0; r < D8_RAW; ++r) {
+                    const bool live = r < p.n && k < p.k;
                     const size_t at = ((size_t)w.first * p.n + r) * p.k + k;
-                    if (quads && p.dtype == PCB_F32) {
-                        const float4 x = ld_chained(static_cast<const float4*>(p.tokens) + at / 4, k < p.k);
-                        v[r][0] = x.x; v[r][1] = x.y; v[r][2] = x.z; v[r][3] = x.w;
-                    } else if (quads) {
-                        const uint2 x = ld_chained(static_cast<const uint2*>(p.tokens) + at / 4, k < p.k);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const uint32_t h = (e < 2 ? x.x : x.y) >> (16 * (e & 1)) & 0xffffu;
-                            v[r][e] = p.dtype == PCB_F16 ? __half2float(__ushort_as_half((uint16_t)h)) : __uint_as_float(h << 16);
-                        }
+                    if (quads && p.dtype == PCB_F32) raw[r] = ld_chained(static_cast<const uint4*>(p.tokens) + at / 4, live);
+                    else if (quads) {
+                        const uint2 x = ld_chained(static_cast<const uint2*>(p.tokens) + at / 4, live);
+                        raw[r].x = x.x; raw[r].y = x.y;
+                    } else if (p.dtype == PCB_F32) {
+                        const uint32_t* x = static_cast<const uint32_t*>(p.tokens) + at;
+                        raw[r] = make_uint4(ld_chained(x, live), ld_chained(x + 1, live && k + 1 < p.k), ld_chained(x + 2, live && k + 2 < p.k), ld_chained(x + 3, live && k + 3 < p.k));
                     } else {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) v[r][e] = k + e < p.k ? ld_typed(p.tokens, p.dtype, at + e) : 0.f;
+                        const uint16_t* x = static_cast<const uint16_t*>(p.tokens) + at;
+                        raw[r].x = (uint32_t)ld_chained(x, live) | (uint32_t)ld_chained(x + 1, live && k + 1 < p.k) << 16;
+                        raw[r].y = (uint32_t)ld_chained(x + 2, live && k + 2 < p.k) | (uint32_t)ld_chained(x + 3, live && k + 3 < p.k) << 16;
                     }
                 }
             }
             if (!warp_wait_bounded(sf_empty + 8 * q, par, status, ST_D8_SCALES)) return;
-            uint32_t data[BN];
+            uint32_t data[D8_RAW];
             if (j < blocks) {
 #pragma unroll
-                for (int r = 0; r < BN; ++r) {
+                for (int r = 0; r < D8_RAW; ++r) {
                     if (r >= p.n) break;
+                    float v[4];
+                    if (p.dtype == PCB_F32) {
+                        v[0] = __uint_as_float(raw[r].x); v[1] = __uint_as_float(raw[r].y); v[2] = __uint_as_float(raw[r].z); v[3] = __uint_as_float(raw[r].w);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t h = (e < 2 ? raw[r].x : raw[r].y) >> (16 * (e & 1)) & 0xffffu;
+                            v[e] = p.dtype == PCB_F16 ? __half2float(__ushort_as_half((uint16_t)h)) : __uint_as_float(h << 16);
+                        }
+                    }
                     uint32_t top = 0;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const uint32_t key = __float_as_uint(v[r][e]) & 0x7fffffffu;
+                        const uint32_t key = __float_as_uint(v[e]) & 0x7fffffffu;
                         if (key < 0x7f800000u) top = max(top, key);
-                        else v[r][e] = __uint_as_float(0x7fffffffu);                // infinities too: the conversion would saturate them
+                        else v[e] = __uint_as_float(0x7fffffffu);                   // infinities too: the conversion would saturate them
                     }
                     const int byte = scale_byte(__reduce_max_sync(0xffffffffu, top));
                     const float f = inverse_scale(byte);
-                    data[r] = to_e4m3x2(v[r][0], v[r][1], make_float2(f, f)) | to_e4m3x2(v[r][2], v[r][3], make_float2(f, f)) << 16;
+                    data[r] = to_e4m3x2(v[0], v[1], make_float2(f, f)) | to_e4m3x2(v[2], v[3], make_float2(f, f)) << 16;
                     if (lane == 0) asm volatile("st.shared.u8 [%0], %1;" ::"r"(sf + q * D8_SF_BYTES + 512u + r * 16u + j), "r"(byte) : "memory");
                 }
                 fence_proxy_async_smem();
@@ -259,7 +269,7 @@ __device__ __forceinline__ void d8_quantize_tokens(const D8Params& p, uint32_t b
                 if (!warp_wait_bounded(empty + 8 * s, ((uint32_t)(block / STAGES) & 1u) ^ 1u, status, ST_D8_PRODUCER)) return;
                 const uint32_t b = base + s * STAGE + D8_A_BYTES + (uint32_t)(lane & 3) * 4u;
 #pragma unroll
-                for (int r = 0; r < BN; ++r) {
+                for (int r = 0; r < D8_RAW; ++r) {
                     if (r >= p.n) break;
                     asm volatile("st.shared.u32 [%0], %1;" ::"r"(b + r * 128u + (uint32_t)(((lane >> 2) ^ (r & 7)) << 4)), "r"(data[r]) : "memory");
                 }
@@ -431,7 +441,7 @@ dense8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             if (++acc == C::ACC) { acc = 0; acc_par ^= 1u; }
         }
     } else if (RAW && (warp == 3 || warp >= 8)) {
-        if (warp >= 8) d8_quantize_tokens<BN, C::STAGES, C::STAGE>(p, base_addr, sf_addr, full, empty, sf_full, sf_empty, first, stride, g_begin, g_end, j_begin, status);
+        if (warp >= 8) d8_quantize_tokens<C::STAGES, C::STAGE>(p, base_addr, sf_addr, full, empty, sf_full, sf_empty, first, stride, g_begin, g_end, j_begin, status);
     } else if (warp < 4) {
         // Warp 2 the scales of A, warp 3 those of B, a group of the reduction at a time. The words of the next group are loaded before those of this one are waited for: one
         // warp that loaded them when they were due took 2600 clocks a group, where the MMAs of a group take 2048.
@@ -737,7 +747,9 @@ int launch(const Geom& g, const Q8Product& q, int splits, cudaStream_t stream) {
 }  // namespace
 
 bool q8_swapped(int tokens) { return tokens <= 128; }
-bool q8_raw_tokens(int tokens) { return tokens <= 16; }
+// Each token adds its loads and a maximum over a warp to the way to the first product: 4096 -> 4096 by itself took 14.2 us for one token and 24 to 27 for 8 and 16
+// (in registers for 16), where quantising first takes 3.7 + 11 us and 3 us more of the host.
+bool q8_raw_tokens(int tokens) { return tokens <= D8_RAW; }
 
 // Measured on cold inputs, us (fitted to 1 to 4 rounds of tiles and reductions of 5 to 128 blocks): a single tile of 128 x 128 takes 0.27 a block behind 7.5 for launch, first
 // copies and epilogue; a pair's of 256 x 256 0.34 a block behind 12; a reduction cut over a cluster 3.5 more. 2048 x 4096 -> 4096: pairs 35.3, single 44.5;

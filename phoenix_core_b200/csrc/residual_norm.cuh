@@ -655,10 +655,10 @@ __global__ void __launch_bounds__(RN_WIDE_THREADS) residual_norm_bwd_wide_kernel
     }
 }
 
-// Adds the pieces. Weights: eight columns (a sector) per CTA, the slots and components over 32 threads of each column. Gates: a thread per value.
+// Adds the pieces. Weights: eight columns (a sector) per CTA, the slots and components over 64 threads of each column. Gates: 1, 8 or 64 threads per value.
 constexpr int RN_SUM_THREADS = 512;
 template <typename T>
-__global__ void __launch_bounds__(RN_SUM_THREADS) residual_norm_sum_kernel(const RNParams p, int slots, int weight_blocks) {
+__global__ void __launch_bounds__(RN_SUM_THREADS) residual_norm_sum_kernel(const RNParams p, int slots, int weight_blocks, int slices) {
     const int width = p.comps * p.features;
     chain_wait();
     chain_next();
@@ -687,14 +687,24 @@ __global__ void __launch_bounds__(RN_SUM_THREADS) residual_norm_sum_kernel(const
             if (out) out[f] = v;
         }
     } else {
-        const long long i = (long long)(blockIdx.x - weight_blocks) * RN_SUM_THREADS + threadIdx.x;
-        if (i >= (long long)p.groups * width) return;
-        const int group = (int)(i / width), e = (int)(i - (long long)group * width);
+        // `slices` threads of a value each add up their share of the parts
+        __shared__ float parts[RN_SUM_THREADS];
+        const int values = RN_SUM_THREADS / slices, col = threadIdx.x % values, slice = threadIdx.x / values;
+        const long long i = (long long)(blockIdx.x - weight_blocks) * values + col;
+        const bool live = i < (long long)p.groups * width;
+        const int group = live ? (int)(i / width) : 0, e = live ? (int)(i - (long long)group * width) : 0;
         float v = 0.f;
+        if (live) {
 #pragma unroll 4
-        for (int s = 0; s < p.parts; ++s) v += p.part_gate[((size_t)group * p.parts + s) * width + e];
-        const int c = e / p.features;
-        put<T>(p.dgate, (size_t)group * p.features + (size_t)c * (p.groups - 1) * p.features + e, v);
+            for (int s = slice; s < p.parts; s += slices) v += p.part_gate[((size_t)group * p.parts + s) * width + e];
+        }
+        parts[threadIdx.x] = v;
+        __syncthreads();
+        if (slice == 0 && live) {
+            for (int s = 1; s < slices; ++s) v += parts[s * values + col];
+            const int c = e / p.features;
+            put<T>(p.dgate, (size_t)group * p.features + (size_t)c * (p.groups - 1) * p.features + e, v);
+        }
     }
 }
 
@@ -767,9 +777,10 @@ int bwd_typed(RNParams p, RNPlan q, cudaStream_t s) {
     else if (p.period == 1) PCB_CUDA_TRY((bwd_any<T, VEC, true>(p, q, s)));
     else PCB_CUDA_TRY((bwd_any<T, VEC, false>(p, q, s)));
     const long long weight_blocks = p.part_w ? (p.features + 7) / 8 : 0;
-    const long long gate_blocks = p.part_gate ? ((long long)p.groups * p.comps * p.features + RN_SUM_THREADS - 1) / RN_SUM_THREADS : 0;
+    const int slices = q.parts > 32 ? 64 : (q.parts > 4 ? 8 : 1), values = RN_SUM_THREADS / slices;
+    const long long gate_blocks = p.part_gate ? ((long long)p.groups * p.comps * p.features + values - 1) / values : 0;
     if (weight_blocks + gate_blocks > 0)
-        PCB_CUDA_TRY(launch_chained(residual_norm_sum_kernel<T>, (unsigned)(weight_blocks + gate_blocks), RN_SUM_THREADS, 0, s, p, q.grid, (int)weight_blocks));
+        PCB_CUDA_TRY(launch_chained(residual_norm_sum_kernel<T>, (unsigned)(weight_blocks + gate_blocks), RN_SUM_THREADS, 0, s, p, q.grid, (int)weight_blocks, slices));
     return PCB_OK;
 }
 
