@@ -720,7 +720,7 @@ int pcb_qdense8_fwd(const pcb_dense_desc* desc, const void* x, const void* w8, c
     int* status = reinterpret_cast<int*>(ws);
     const Q8Target rows = {ws + at.x_rows, reinterpret_cast<uint32_t*>(ws + at.x_words)};
     const bool raw = q8_raw_tokens(g.Nb);
-    if (!raw && (rc = q8_quantize(desc->dtype, g.nc, g.Nb, g.Ci, x, rows, Q8Target{}, status, (cudaStream_t)stream)) != PCB_OK) return rc;
+    if (!raw && (rc = q8_quantize_rows(desc->dtype, g.nc, g.Nb, g.Ci, x, rows, status, (cudaStream_t)stream)) != PCB_OK) return rc;
     const Q8Operand tokens = {rows.values, rows.words, q8_pitch(g.Ci), 0, 0, 0, 0}, filter = dense8_filter(g, w8, w8_scales, true);
     Q8Product q = {PASS_FWD, q8_swapped(g.Nb) ? 1 : 0, g.Nb, g.Co, g.Ci, tokens, filter, y, desc->dtype, g.has_bias ? bias : nullptr, status};
     if (q.swapped) { q.m = g.Co; q.n = g.Nb; q.a = filter; q.b = tokens; }
@@ -748,9 +748,7 @@ int pcb_qdense8_bwd(const pcb_dense_desc* desc, const void* x, const void* w8, c
     const Q8Target dy_rows = {need_dx ? ws + at.dy_rows : nullptr, reinterpret_cast<uint32_t*>(ws + at.dy_row_words)};
     const Q8Target dy_cols = {ws + at.dy_cols, reinterpret_cast<uint32_t*>(ws + at.dy_col_words)};
     const Q8Target x_cols = {ws + at.x_cols, reinterpret_cast<uint32_t*>(ws + at.x_col_words)};
-    rc = q8_quantize(desc->dtype, g.nc, g.Nb, g.Co, dy, dy_rows, dy_cols, status, st);
-    if (rc == PCB_OK) rc = q8_quantize(desc->dtype, g.nc, g.Nb, g.Ci, x, Q8Target{}, x_cols, nullptr, st);
-    if (rc != PCB_OK) return rc;
+    if ((rc = q8_quantize_backward(desc->dtype, g.nc, g.Nb, g.Ci, g.Co, x, dy, x_cols, dy_rows, dy_cols, status, st)) != PCB_OK) return rc;
     const Q8Operand a = {x_cols.values, x_cols.words, q8_pitch(g.Ci), 0, 0, 0, 1}, b = {dy_cols.values, dy_cols.words, q8_pitch(g.Co), 0, 0, 0, 1};
     rc = q8_product(g, Q8Product{PASS_BWD_FILTER, 0, g.Ci, g.Co, g.Nb, a, b, dw, desc->dtype, nullptr, status}, st);
     if (rc != PCB_OK || !need_dx) return rc;

@@ -40,9 +40,12 @@ struct Q8Product {
     const void* tokens = nullptr;       // the tokens as the caller has them: quantised by the product itself (then operand b is not read)
 };
 
-// Quantises x ([components][rows][cols], dense): `by_rows` with blocks of 1 x 128, `by_cols` with blocks of 128 x 1 (either may be null values).
+// Quantises x ([components][rows][cols], dense) with blocks of 1 x 128; of the backward pass's tensors x with blocks of 128 x 1 and dy with those and, unless its values
+// are null, with blocks of 1 x 128, in one launch; a filter with blocks of 128 x 128. The status word is cleared by the first two.
 struct Q8Target { uint8_t* values; uint32_t* words; };
-int q8_quantize(int dtype, int comps, int rows, int cols, const void* x, Q8Target by_rows, Q8Target by_cols, int* status_to_clear, cudaStream_t stream);
+int q8_quantize_rows(int dtype, int comps, int rows, int cols, const void* x, Q8Target by_rows, int* status_to_clear, cudaStream_t stream);
+int q8_quantize_backward(int dtype, int comps, int rows, int x_cols, int dy_cols, const void* x, const void* dy, Q8Target x_by_cols, Q8Target dy_by_rows, Q8Target dy_by_cols,
+                         int* status_to_clear, cudaStream_t stream);
 int q8_quantize_blocks(int dtype, int comps, int rows, int cols, const void* x, uint8_t* values, uint8_t* scales, cudaStream_t stream);
 int q8_product(const Geom& g, const Q8Product& p, cudaStream_t stream);
 // Whether a forward or backward-data product of that many tokens takes the filter as operand A.

@@ -62,6 +62,11 @@ template <typename T> struct Eight16 {
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[i] = (uint32_t)ld_chained(h + 2 * i, 2 * i < valid) | ((uint32_t)ld_chained(h + 2 * i + 1, 2 * i + 1 < valid) << 16);
     }
+    // eight values `odd` (0 or 1) values behind the word x[0]
+    __device__ __forceinline__ void from(const uint32_t (&x)[5], uint32_t odd) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(x[i], x[i + 1], odd * 16u);
+    }
 };
 template <> struct Eight<__half> : Eight16<__half> {
     static constexpr uint32_t INF_KEY = 0x7c00u;
@@ -87,38 +92,65 @@ template <> struct Eight<__nv_bfloat16> : Eight16<__nv_bfloat16> {
 enum { QT_ROWS = 1, QT_COLS = 2, QT_BLOCKS = 4 };
 
 struct QTParams {
+    const void* x;
     int rows, cols, pitch;
-    uint8_t *row_values, *col_values;            // QT_BLOCKS: row_values
+    int row_blocks, col_blocks, tiles;           // tiles: of all components
+    uint8_t *row_values, *col_values;            // QT_BLOCKS: row_values; with QT_ROWS and QT_COLS either may be null
     uint32_t *row_words, *col_words;             // QT_BLOCKS: row_words is the byte array
     int row_groups, col_groups;                  // groups of four blocks along the columns (row scales) and along the rows (column scales)
-    int* status;                                 // cleared by the first CTA, or null
 };
 
 // Thread t holds columns 8 * (t % 16) .. + 7 of rows (t / 16) + 32 * i: the lanes of half a warp hold one row.
-// VEC: rows start on 16 bytes and are whole vectors.
+// VEC: rows start on 16 bytes and are whole vectors. A launch takes the tiles of one tensor or of two, one behind the other; status: cleared by the first CTA, or null.
 template <typename T, int MODE, bool VEC>
-__global__ void __launch_bounds__(QT_THREADS, sizeof(T) == 4 ? 1 : 2) quantize_tile_kernel(const T* x, QTParams p) {
+__global__ void __launch_bounds__(QT_THREADS, sizeof(T) == 4 ? 1 : 2) quantize_tile_kernel(const __grid_constant__ QTParams p0, const __grid_constant__ QTParams p1, int* status) {
     typedef Eight<T> E;
     __shared__ uint32_t col_max[QT_WARPS][16 * E::WORDS];
     __shared__ uint32_t warp_max[QT_WARPS];
     __shared__ __align__(16) float col_scale[Q8_BLOCK];
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31, c8 = (t & 15) * 8, r0 = t >> 4;
-    const int comp = blockIdx.z, row_block = blockIdx.y, col_block = blockIdx.x;
+    const QTParams& p = (int)blockIdx.x < p0.tiles ? p0 : p1;
+    const unsigned tile = blockIdx.x - ((int)blockIdx.x < p0.tiles ? 0u : (unsigned)p0.tiles), line = tile / (unsigned)p.col_blocks;
+    const int col_block = (int)(tile - line * (unsigned)p.col_blocks), comp = (int)(line / (unsigned)p.row_blocks), row_block = (int)line - comp * p.row_blocks;
     const int col = col_block * Q8_BLOCK + c8, first_row = row_block * Q8_BLOCK + r0;
     chain_wait();
     chain_next();
-    if (p.status && t == 0 && comp == 0 && row_block == 0 && col_block == 0) *p.status = 0;
+    if (status && t == 0 && blockIdx.x == 0) *status = 0;
     const int valid = min(8, p.cols - col);
     E v[QT_PER];
     {
+        const T* x = static_cast<const T*>(p.x);
         const T* src = x + ((size_t)comp * p.rows + first_row) * p.cols + col;
+        if constexpr (VEC) {
 #pragma unroll
-        for (int i = 0; i < QT_PER; ++i) {
-            const bool live = first_row + QT_STEP * i < p.rows && valid > 0;
-            if (VEC) {
-                if (live) v[i].load(src + (size_t)QT_STEP * i * p.cols);
+            for (int i = 0; i < QT_PER; ++i) {
+                if (first_row + QT_STEP * i < p.rows && valid > 0) v[i].load(src + (size_t)QT_STEP * i * p.cols);
                 else v[i].zero();
-            } else v[i].load(src + (size_t)QT_STEP * i * p.cols, live ? valid : 0);
+            }
+        } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < QT_PER; ++i) v[i].load(src + (size_t)QT_STEP * i * p.cols, first_row + QT_STEP * i < p.rows ? valid : 0);
+        } else {
+            // Rows that start on two bytes: as the words around them, five for eight values, but for the ends of rows (and of the tensor). Every load is on its way before the
+            // first value is looked at.
+            uint32_t word[QT_PER][5], odd_start[QT_PER];
+            const bool inside = valid == 8 && col > 0 && col + 8 < p.cols;
+#pragma unroll
+            for (int i = 0; i < QT_PER; ++i) {
+                const T* at = src + (size_t)QT_STEP * i * p.cols;
+                odd_start[i] = (uint32_t)(reinterpret_cast<uintptr_t>(at) >> 1) & 1u;
+                const uint32_t* u = reinterpret_cast<const uint32_t*>(at - odd_start[i]);
+                const bool live = inside && first_row + QT_STEP * i < p.rows;
+#pragma unroll
+                for (int k = 0; k < 5; ++k) word[i][k] = ld_chained(u + k, live && (k < 4 || odd_start[i]));
+            }
+#pragma unroll
+            for (int i = 0; i < QT_PER; ++i) v[i].from(word[i], odd_start[i]);
+            if (__any_sync(0xffffffffu, !inside)) {
+#pragma unroll
+                for (int i = 0; i < QT_PER; ++i)
+                    if (!inside && first_row + QT_STEP * i < p.rows && valid > 0) v[i].load(src + (size_t)QT_STEP * i * p.cols, valid);
+            }
         }
     }
     uint32_t row_keys[QT_PER], most = 0;
@@ -170,7 +202,7 @@ __global__ void __launch_bounds__(QT_THREADS, sizeof(T) == 4 ? 1 : 2) quantize_t
             *reinterpret_cast<uint2*>(dst + (size_t)QT_STEP * i * p.pitch) = make_uint2(lo, hi);
         }
     };
-    if constexpr ((MODE & QT_ROWS) != 0) {
+    if ((MODE & QT_ROWS) && p.row_values) {
         float f[QT_PER];
 #pragma unroll
         for (int i = 0; i < QT_PER; ++i) {
@@ -193,7 +225,7 @@ __global__ void __launch_bounds__(QT_THREADS, sizeof(T) == 4 ? 1 : 2) quantize_t
         const int byte = scale_byte(E::bits(most));
         const float f = inverse_scale(byte);
         store(p.row_values, [&](int, int) { return make_float2(f, f); });
-        if (t == 0) reinterpret_cast<uint8_t*>(p.row_words)[((size_t)comp * gridDim.y + row_block) * gridDim.x + col_block] = (uint8_t)byte;
+        if (t == 0) reinterpret_cast<uint8_t*>(p.row_words)[((size_t)comp * p.row_blocks + row_block) * p.col_blocks + col_block] = (uint8_t)byte;
     }
     if constexpr ((MODE & QT_COLS) != 0) {
         uint32_t m[E::WORDS];
@@ -233,38 +265,38 @@ __global__ void __launch_bounds__(QT_THREADS, sizeof(T) == 4 ? 1 : 2) quantize_t
 }
 
 template <typename T, int MODE>
-cudaError_t launch_tile(const void* x, const QTParams& p, int comps, cudaStream_t stream) {
-    const dim3 grid(q8_blocks(p.cols), q8_blocks(p.rows), comps);
-    const bool vec = p.cols % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid; cfg.blockDim = dim3(QT_THREADS); cfg.stream = stream;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr; cfg.numAttrs = 1;
-    const T* xt = static_cast<const T*>(x);
-    return vec ? cudaLaunchKernelEx(&cfg, quantize_tile_kernel<T, MODE, true>, xt, p) : cudaLaunchKernelEx(&cfg, quantize_tile_kernel<T, MODE, false>, xt, p);
+cudaError_t launch_tile(const QTParams& p0, const QTParams& p1, int* status, cudaStream_t stream) {
+    auto vectors = [](const QTParams& p) { return p.tiles == 0 || (p.cols % 8 == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0); };
+    const unsigned grid = (unsigned)p0.tiles + (unsigned)p1.tiles;
+    return vectors(p0) && vectors(p1) ? launch_chained(quantize_tile_kernel<T, MODE, true>, grid, QT_THREADS, 0, stream, p0, p1, status)
+                                      : launch_chained(quantize_tile_kernel<T, MODE, false>, grid, QT_THREADS, 0, stream, p0, p1, status);
 }
 template <int MODE>
-int launch_typed(int dtype, const void* x, const QTParams& p, int comps, cudaStream_t stream) {
-    if (q8_blocks(p.rows) > 65535) { set_error("more than 65535 blocks of 128 rows"); return PCB_ERR_TOO_LARGE; }
-    if (dtype == PCB_F32) PCB_CUDA_TRY((launch_tile<float, MODE>(x, p, comps, stream)));
-    else if (dtype == PCB_F16) PCB_CUDA_TRY((launch_tile<__half, MODE>(x, p, comps, stream)));
-    else PCB_CUDA_TRY((launch_tile<__nv_bfloat16, MODE>(x, p, comps, stream)));
+int launch_typed(int dtype, const QTParams& p0, const QTParams& p1, int* status, cudaStream_t stream) {
+    if (dtype == PCB_F32) PCB_CUDA_TRY((launch_tile<float, MODE>(p0, p1, status, stream)));
+    else if (dtype == PCB_F16) PCB_CUDA_TRY((launch_tile<__half, MODE>(p0, p1, status, stream)));
+    else PCB_CUDA_TRY((launch_tile<__nv_bfloat16, MODE>(p0, p1, status, stream)));
     return PCB_OK;
+}
+QTParams tile_params(int comps, int rows, int cols, const void* x, Q8Target by_rows, Q8Target by_cols) {
+    const int row_blocks = q8_blocks(rows), col_blocks = q8_blocks(cols);
+    return {x, rows, cols, q8_pitch(cols), row_blocks, col_blocks, comps * row_blocks * col_blocks, by_rows.values, by_cols.values, by_rows.words, by_cols.words,
+            q8_groups(cols), q8_groups(rows)};
 }
 
 }  // namespace
 
-int q8_quantize(int dtype, int comps, int rows, int cols, const void* x, Q8Target by_rows, Q8Target by_cols, int* status, cudaStream_t stream) {
-    const QTParams p = {rows, cols, q8_pitch(cols), by_rows.values, by_cols.values, by_rows.words, by_cols.words, q8_groups(cols), q8_groups(rows), status};
-    if (by_rows.values && by_cols.values) return launch_typed<QT_ROWS | QT_COLS>(dtype, x, p, comps, stream);
-    return by_rows.values ? launch_typed<QT_ROWS>(dtype, x, p, comps, stream) : launch_typed<QT_COLS>(dtype, x, p, comps, stream);
+int q8_quantize_rows(int dtype, int comps, int rows, int cols, const void* x, Q8Target by_rows, int* status, cudaStream_t stream) {
+    return launch_typed<QT_ROWS>(dtype, tile_params(comps, rows, cols, x, by_rows, Q8Target{}), QTParams{}, status, stream);
+}
+
+int q8_quantize_backward(int dtype, int comps, int rows, int x_cols, int dy_cols, const void* x, const void* dy, Q8Target x_by_cols, Q8Target dy_by_rows, Q8Target dy_by_cols, int* status,
+                         cudaStream_t stream) {
+    return launch_typed<QT_ROWS | QT_COLS>(dtype, tile_params(comps, rows, dy_cols, dy, dy_by_rows, dy_by_cols), tile_params(comps, rows, x_cols, x, Q8Target{}, x_by_cols), status, stream);
 }
 
 int q8_quantize_blocks(int dtype, int comps, int rows, int cols, const void* x, uint8_t* values, uint8_t* scales, cudaStream_t stream) {
-    const QTParams p = {rows, cols, q8_pitch(cols), values, nullptr, reinterpret_cast<uint32_t*>(scales), nullptr, 0, 0, nullptr};
-    return launch_typed<QT_BLOCKS>(dtype, x, p, comps, stream);
+    return launch_typed<QT_BLOCKS>(dtype, tile_params(comps, rows, cols, x, Q8Target{values, reinterpret_cast<uint32_t*>(scales)}, Q8Target{}), QTParams{}, nullptr, stream);
 }
 
 }  // namespace pcb

@@ -15,7 +15,7 @@
 //             0.53 us where the MMAs alone take 0.27; a pair moves a third less.
 //   single    128 x 128 tiles; a tile's reduction is cut over the CTAs of a cluster where there are fewer tiles than SMs, whose partial sums are added in a
 //             fixed order through distributed shared memory.
-//   SWAP      few tokens: the filter is operand A, a tile is 128 features x 16, 64 or 128 tokens; bound by the filter's bytes.
+//   SWAP      few tokens: the filter is operand A, a tile is 128 features x 16 or 64 tokens; bound by the filter's bytes.
 //   RAW       the same for up to four tokens, which are quantised here: four warps each take a block of 128 of the reduction at a time straight from the caller's tensor
 //             into the stage and the scales' words, so that the call is one launch.
 #include "dense8.cuh"
@@ -145,23 +145,52 @@ __device__ __forceinline__ uint32_t pack_16(float a, float b, int dtype) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// A warp's 32 rows (one per lane) x 32 columns of floats whose rows start anywhere: through shared memory, sixteen columns at a time, so that the
-// lanes of an instruction write neighbours. rows, cols: how many exist.
-__device__ __forceinline__ void store_floats(uint32_t buf, const uint32_t (&v)[32], float* out, int rows, int cols, int ld, int lane) {
+// A warp's 32 rows (one per lane) whose lines start anywhere, through 4 KB of shared memory so that the lanes of an instruction write neighbours: words w of row r lie at
+// r * 32 + (w ^ r), which meets no bank twice in either direction. rows, cols: how many exist; ld: elements between rows.
+__device__ __forceinline__ void park_words(uint32_t buf, int first, const uint32_t* v, int n, int lane) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        __syncwarp();
+    for (int e = 0; e < 32; ++e)
+        if (e < n) asm volatile("st.shared.u32 [%0], %1;" ::"r"(buf + (uint32_t)(lane * 32 + ((first + e) ^ lane)) * 4u), "r"(v[e]) : "memory");
+}
+// 32 columns of floats per row (eight reads in flight before the first of their stores, here and below)
+__device__ __forceinline__ void store_parked_floats(uint32_t buf, float* out, int rows, int cols, int ld, int lane) {
+    __syncwarp();
+    out += lane;
+#pragma unroll 1
+    for (int r0 = 0; r0 < 32; r0 += 8) {
+        float x[8];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) asm volatile("st.shared.u32 [%0], %1;" ::"r"(buf + (uint32_t)(lane * EPI_ROWS_PITCH + e) * 4u), "r"(v[16 * h + e]) : "memory");
-        __syncwarp();
-        const int col = lane & 15;
-#pragma unroll 4
-        for (int r = lane >> 4; r < 32; r += 2) {
-            float x;
-            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(buf + (uint32_t)(r * EPI_ROWS_PITCH + col) * 4u) : "memory");
-            if (r < rows && 16 * h + col < cols) out[(long long)r * ld + 16 * h + col] = x;
+        for (int i = 0; i < 8; ++i) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x[i]) : "r"(buf + (uint32_t)((r0 + i) * 32 + (lane ^ (r0 + i))) * 4u));
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (r0 + i < rows && lane < cols) out[(long long)(r0 + i) * ld] = x[i];
+    }
+    __syncwarp();
+}
+// 64 columns of 16-bit values per row, in words of two: stored as words where the row starts on four bytes, else as the words between (whose halves come from two
+// parked ones) and a value at either end
+__device__ __forceinline__ void store_parked_halves(uint32_t buf, uint16_t* out, int rows, int cols, int ld, int lane) {
+    __syncwarp();
+    cols = min(cols, 64);
+#pragma unroll 1
+    for (int r0 = 0; r0 < 32; r0 += 8) {
+        uint32_t w[8], next[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[i]) : "r"(buf + (uint32_t)((r0 + i) * 32 + (lane ^ (r0 + i))) * 4u));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) next[i] = __shfl_down_sync(0xffffffffu, w[i], 1);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            uint16_t* line = out + (long long)(r0 + i) * ld;
+            const uint32_t odd = (uint32_t)(reinterpret_cast<uintptr_t>(line) >> 1) & 1u, word = __funnelshift_r(w[i], next[i], odd * 16u);
+            const int col = 2 * lane + (int)odd;
+            const bool live = r0 + i < rows;
+            if (live && col + 1 < cols) *reinterpret_cast<uint32_t*>(line + col) = word;
+            if (live && col + 1 == cols) line[col] = (uint16_t)word;             // the last column of the tensor, or of the block
+            if (live && odd && lane == 0) line[0] = (uint16_t)w[i];
         }
     }
+    __syncwarp();
 }
 
 // Where a warp is in its CTA's part of a reduction: group `group` of component j, with the operands' components and the sign. Stepped, not computed anew: the
@@ -625,9 +654,12 @@ dense8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                             }
                         }
                     } else if (p.dtype == PCB_F32) {
-                        store_floats(buf, v[b], static_cast<float*>(p.out) + comp0 + (long long)row0 * p.out_ld + n, p.m - row0, p.n - n, p.out_ld, lane);
+                        park_words(buf, 0, v[b], 32, lane);
+                        store_parked_floats(buf, static_cast<float*>(p.out) + comp0 + (long long)row0 * p.out_ld + n, p.m - row0, p.n - n, p.out_ld, lane);
                     } else {
-                        store_rows<1>(buf, packed, static_cast<uint16_t*>(p.out) + comp0 + (long long)row0 * p.out_ld, m < p.m ? lane * p.out_ld : -1, n + lane < p.n ? n + lane : -1, lane);
+                        park_words(buf, 16 * (b & 1), packed, 16, lane);
+                        if ((b & 1) || n + 32 >= p.n)
+                            store_parked_halves(buf, static_cast<uint16_t*>(p.out) + comp0 + (long long)row0 * p.out_ld + n - 32 * (b & 1), p.m - row0, p.n - n + 32 * (b & 1), p.out_ld, lane);
                     }
                 }
             }
@@ -746,7 +778,7 @@ int launch(const Geom& g, const Q8Product& q, int splits, cudaStream_t stream) {
 
 }  // namespace
 
-bool q8_swapped(int tokens) { return tokens <= 128; }
+bool q8_swapped(int tokens) { return tokens <= 64; }
 // Each token adds its loads and a maximum over a warp to the way to the first product: 4096 -> 4096 by itself took 14.2 us for one token and 24 to 27 for 8 and 16
 // (in registers for 16), where quantising first takes 3.7 + 11 us and 3 us more of the host.
 bool q8_raw_tokens(int tokens) { return tokens <= D8_RAW; }
@@ -771,8 +803,7 @@ int q8_product(const Geom& g, const Q8Product& q, cudaStream_t stream) {
     if (q.tokens) return launch<16, true, false, true>(g, q, splits_for(16), stream);
     if (q.swapped) {
         if (q.n <= 16) return launch<16, true, false>(g, q, splits_for(16), stream);
-        if (q.n <= 64) return launch<64, true, false>(g, q, splits_for(64), stream);
-        return launch<128, true, false>(g, q, splits_for(128), stream);
+        return launch<64, true, false>(g, q, splits_for(64), stream);
     }
     auto rounds = [](long long tiles, int at_once) { return (double)((tiles + at_once - 1) / at_once); };
     const long long wide = (long long)((q.m + 255) / 256) * ((q.n + 255) / 256) * g.nc, small = (long long)m_tiles * ((q.n + 127) / 128) * g.nc;
