@@ -26,9 +26,10 @@ class Filter8:
     real-valued layers. Filled by ``quantizeFilter8``; one object serves ``dense8Fwd`` and ``dense8Bwd``.
 
     ``values`` is a view of the e4m3 numbers (its rows start on 16 bytes), ``scales`` the bytes e + 127 of the blocks,
-    ``[D, blocks of rows, blocks of columns]``. Numbers of another origin can be copied into both."""
+    ``[D, blocks of rows, blocks of columns]``. Numbers of another origin can be copied into both. ``fill=False`` leaves them unset, for a filter that is
+    rounded into the object next (a zero filter otherwise)."""
 
-    def __init__(self, filterShape, algebra=Algebra.QUATERNION, filterLayout=FilterLayout.IO, device="cuda"):
+    def __init__(self, filterShape, algebra=Algebra.QUATERNION, filterLayout=FilterLayout.IO, device="cuda", fill=True):
         self.shape = tuple(int(s) for s in filterShape)
         self.algebra, self.filterLayout = algebra, filterLayout
         dim = MULTIVECTOR_DIM[algebra]
@@ -40,12 +41,13 @@ class Filter8:
         if rows <= 0 or cols <= 0:
             raise ValueError("invalid filter shape %s" % (self.shape,))
         pitch = (cols + 15) // 16 * 16
-        self._storage = torch.zeros((dim, rows, pitch), dtype=torch.uint8, device=device)
+        self._storage = (torch.zeros if fill else torch.empty)((dim, rows, pitch), dtype=torch.uint8, device=device)
         self.values = self._storage.view(torch.float8_e4m3fn)[:, :, :cols].reshape(self.shape) if pitch == cols else \
             self._storage.view(torch.float8_e4m3fn)[:, :, :cols]
         if self.values.dim() != len(self.shape):
             self.values = self.values[0]
-        self.scales = torch.full((dim, (rows + BLOCK - 1) // BLOCK, (cols + BLOCK - 1) // BLOCK), 127, dtype=torch.uint8, device=device)
+        blocks = (dim, (rows + BLOCK - 1) // BLOCK, (cols + BLOCK - 1) // BLOCK)
+        self.scales = torch.full(blocks, 127, dtype=torch.uint8, device=device) if fill else torch.empty(blocks, dtype=torch.uint8, device=device)
 
         self._descs = {}
 

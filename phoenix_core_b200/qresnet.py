@@ -1,6 +1,6 @@
 """Quaternion ResNet-18 training step on the quaternion operators of this package, data-parallel with NCCL.
 
-    python -m phoenix_core_b200.qresnet [--batch 128] [--steps 10] [--warmup 3]          (torchrun for N > 1)
+    python -m phoenix_core_b200.qresnet [--batch 128] [--steps 10] [--warmup 3] [--distill 16]          (torchrun for N > 1)
 
 Standard ResNet-18 topology with every real channel count divided by 4 (quaternion channels 16/32/64/128,
 1000 classes = 250 quaternion outputs), every convolution and the classifier replaced by their quaternion
@@ -10,7 +10,8 @@ drop-in path. Batch-norm normalises each quaternion channel with one mean / vari
 components (statistics over the stacked `[4N, C, H, W]` tensor); it runs on helper kernels of the library
 (`pcb_aux_bn_*`: plain, with the residual add of a block's tail, and with the stem's max-pool fused in), because the
 framework's own batch-norm kernels idle the GPU at 16 channels. On one GPU the whole step is captured once and
-replayed as a CUDA graph (`QResNet18.capture` / `step`).
+replayed as a CUDA graph (`QResNet18.capture` / `step`). With a teacher (`Teacher`: its largest logits for each image) the loss is the
+library's distillation mixed with the labels' cross-entropy, on the classifier's stacked output as it lies.
 
 Precision: fp16 activations and filters (the reference's fp16 tensors; every kernel accumulates in fp32),
 fp32 master weights, static loss scale. All filter gradients are written by the kernels straight into ONE
@@ -23,6 +24,7 @@ import math
 import os
 import sys
 import time
+from collections import namedtuple
 
 import torch
 import torch.distributed as dist
@@ -35,9 +37,12 @@ if ROOT not in sys.path:
 import phoenix_core_b200 as pcb  # noqa: E402
 from phoenix_core_b200 import _lib  # noqa: E402
 from phoenix_core_b200.ops import _raw_stream  # noqa: E402
+from phoenix_core_b200.autograd import DistillFunction  # noqa: E402
 from phoenix_core_b200.context import Context  # noqa: E402
 
 LOSS_SCALE = 256.0
+# A teacher's largest logits for a batch: logits (fp16) and classes (int64), [N, k]; its weight against the labels and the temperature.
+Teacher = namedtuple("Teacher", ("logits", "indices", "alpha", "temperature"), defaults=(0.5, 2.0))
 _DT = {torch.float16: _lib.PCB_F16, torch.bfloat16: _lib.PCB_BF16}
 
 
@@ -468,6 +473,11 @@ class QResNet18:
     def forward(self, images):
         """images: [N, 3, H, W] real RGB (the quaternion with zero imaginary parts) -> logits [N, classes]."""
         n = images.shape[0]
+        y = self.forward_stacked(images)
+        return y.view(4, n, -1).permute(1, 0, 2).reshape(n, -1)  # class index = component * 250 + unit
+
+    def forward_stacked(self, images):
+        """The logits as the classifier writes them, [4N, classes / 4]."""
         x = self.bn1.relu_pool(self.conv1(images.contiguous()))
         for blocks in self.stages:
             for blk in blocks:
@@ -477,10 +487,9 @@ class QResNet18:
                     idt = blk["ds"][1](blk["ds"][0](x), relu=False)
                 x = blk["b2"].add_relu(blk["c2"](out), idt)
         x = x.mean(dim=(2, 3))                                   # [4N, 128]
-        y = self.fc(x.contiguous())                              # [4N, 250]
-        return y.view(4, n, -1).permute(1, 0, 2).reshape(n, -1)  # class index = component * 250 + unit
+        return self.fc(x.contiguous())                           # [4N, 250]
 
-    def capture(self, images, labels, lr=0.1, momentum=0.9):
+    def capture(self, images, labels, lr=0.1, momentum=0.9, teacher=None):
         """Captures one single-GPU training step (forward, loss, backward, update) as a CUDA graph over static copies of
         the batch; `step` then replays it. The step is ~400 launches behind ~4.7 ms of Python per step against ~6.5 ms
         of kernels, so an eager loop turns host-bound as soon as the host is slower than usual; the replay is one launch.
@@ -490,10 +499,11 @@ class QResNet18:
             # the caller has run a few eager steps (workspaces grown, kernels loaded); every parameter gradient is written by
             # the kernels into flat buffers, so autograd holds no accumulation node tied to another stream
             self.static_images, self.static_labels = images.clone(), labels.clone()
+            self.static_teacher = None if teacher is None else teacher._replace(logits=teacher.logits.clone(), indices=teacher.indices.clone())
             torch.cuda.synchronize()
             graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(graph):
-                self.static_loss = self.train_step(self.static_images, self.static_labels, 1, lr, momentum)
+                self.static_loss = self.train_step(self.static_images, self.static_labels, 1, lr, momentum, self.static_teacher)
             self.graph = graph
         except Exception as err:                                # noqa: BLE001 -- any capture problem: run eagerly
             sys.stderr.write("qresnet: CUDA graph capture failed (%s); running eagerly\n" % (err,))
@@ -501,21 +511,32 @@ class QResNet18:
             torch.cuda.synchronize()
         return self.graph is not None
 
-    def step(self, images, labels, world=1, lr=0.1, momentum=0.9):
+    def step(self, images, labels, world=1, lr=0.1, momentum=0.9, teacher=None):
         """One training step: the captured graph if there is one (single GPU), the eager step otherwise."""
         if world == 1 and getattr(self, "graph", None) is not None:
+            if (teacher is None) != (self.static_teacher is None):
+                raise ValueError("the step was captured %s a teacher" % ("without" if self.static_teacher is None else "with"))
+            if teacher is not None:
+                if teacher[2:] != self.static_teacher[2:]:
+                    raise ValueError("the step was captured with another weight or temperature of the teacher")
+                self.static_teacher.logits.copy_(teacher.logits, non_blocking=True)
+                self.static_teacher.indices.copy_(teacher.indices, non_blocking=True)
             if images.data_ptr() != self.static_images.data_ptr():
                 self.static_images.copy_(images, non_blocking=True)
                 self.static_labels.copy_(labels, non_blocking=True)
             self.graph.replay()
             return self.static_loss
-        return self.train_step(images, labels, world, lr, momentum)
+        return self.train_step(images, labels, world, lr, momentum, teacher)
 
-    def train_step(self, images, labels, world=1, lr=0.1, momentum=0.9):
+    def train_step(self, images, labels, world=1, lr=0.1, momentum=0.9, teacher=None):
+        """`teacher`: a `Teacher` for these images, or None (cross-entropy alone)."""
         self.flat_w16.copy_(self.flat_w32)
         self.world, self.pending = world, None
-        logits = self.forward(images)
-        loss = F.cross_entropy(logits.float(), labels)
+        if teacher is None:
+            loss = F.cross_entropy(self.forward(images).float(), labels)
+        else:
+            loss = DistillFunction.apply(self.forward_stacked(images), labels, teacher.logits, teacher.indices, teacher.alpha, teacher.temperature,
+                                         pcb.Algebra.QUATERNION).mean()
         (loss * LOSS_SCALE).backward()
         reduce_and_apply(self.flat_w32, self.flat_mom, self.flat_g16, world, lr, momentum, LOSS_SCALE, self.split, self.pending)
         self.pending = None
@@ -583,7 +604,7 @@ def layer_table(batch=128, reps=10, peak_tflops=None):
     return {"batch": batch, "rows": rows, "conv_ms_per_step": round(per_step, 3)}
 
 
-def run(batch, steps, warmup, image=224, quiet=False):
+def run(batch, steps, warmup, image=224, quiet=False, distill=0):
     world = int(os.environ.get("WORLD_SIZE", "1"))
     rank = int(os.environ.get("RANK", "0"))
     local_rank = int(os.environ.get("LOCAL_RANK", "0"))
@@ -601,6 +622,12 @@ def run(batch, steps, warmup, image=224, quiet=False):
     host_images = torch.randn((batch, 3, image, image), generator=g).to(torch.float16).pin_memory()
     host_labels = torch.randint(0, 1000, (batch,), generator=g).pin_memory()
     images, labels = host_images.to(device), host_labels.to(device)
+    teacher = None
+    if distill:                                                  # synthetic logits of distinct classes, the label's the largest
+        classes = torch.stack([torch.randperm(1000, generator=g)[:distill] for _ in range(batch)])
+        classes[:, 0] = torch.where((classes[:, 1:] == host_labels[:, None]).any(1), classes[:, 0], host_labels)
+        values = torch.randn((batch, distill), generator=g).sort(1, descending=True).values * 2.0 + 8.0
+        teacher = Teacher(values.to(torch.float16).to(device), classes.to(device))
 
     def sync():
         if world > 1:
@@ -608,18 +635,18 @@ def run(batch, steps, warmup, image=224, quiet=False):
         torch.cuda.synchronize()
 
     for _ in range(max(5, warmup)):                              # the first steps grow the device workspace
-        loss = model.train_step(images, labels, world)
+        loss = model.train_step(images, labels, world, teacher=teacher)
     sync()
     graphed = False
     if world == 1 and os.environ.get("PCB_QRESNET_GRAPH", "1") not in ("", "0"):
-        graphed = model.capture(images, labels)
+        graphed = model.capture(images, labels, teacher=teacher)
         for _ in range(2):
-            loss = model.step(images, labels, world)
+            loss = model.step(images, labels, world, teacher=teacher)
         sync()
     e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
     e0.record()
     for _ in range(steps):
-        loss = model.step(images, labels, world)
+        loss = model.step(images, labels, world, teacher=teacher)
     e1.record()
     sync()
     ms = e0.elapsed_time(e1)
@@ -648,7 +675,7 @@ def run(batch, steps, warmup, image=224, quiet=False):
         torch.cuda.current_stream().wait_event(ready[i & 1])
         if i + 1 < e2e_steps:
             prefetch(i + 1)
-        loss = model.step(bufs[i & 1][0], bufs[i & 1][1], world)
+        loss = model.step(bufs[i & 1][0], bufs[i & 1][1], world, teacher=teacher)
         used[i & 1].record()
         losses_host[i].copy_(loss.detach(), non_blocking=True)
     b.record()
@@ -683,8 +710,9 @@ def main():
     ap.add_argument("--steps", type=int, default=10)
     ap.add_argument("--warmup", type=int, default=3)
     ap.add_argument("--image", type=int, default=224)
+    ap.add_argument("--distill", type=int, default=0, help="logits of a (synthetic) teacher per image; 0: labels alone")
     a = ap.parse_args()
-    run(a.batch, a.steps, a.warmup, a.image)
+    run(a.batch, a.steps, a.warmup, a.image, distill=a.distill)
 
 
 if __name__ == "__main__":
