@@ -126,6 +126,25 @@ def lib():
     return _lib
 
 
+_binding = None
+
+
+def binding():
+    """The extension module of the block operators (csrc/binding.cpp); raises if it has not been built."""
+    global _binding
+    if _binding is None:
+        import torch  # noqa: F401  (its libraries first)
+        path = os.path.join(_HERE, "_binding.so")
+        if not os.path.exists(path):
+            raise ImportError("%s is missing. Run `python -m phoenix_core_b200.csrc.build`." % path)
+        import importlib.util
+        spec = importlib.util.spec_from_file_location("phoenix_core_b200._binding", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _binding = module
+    return _binding
+
+
 def check(status):
     """Maps a C-ABI status to the exception classes of the reference (std::invalid_argument ->
     ValueError, std::runtime_error -> RuntimeError)."""

@@ -3,6 +3,8 @@
 Every source is compiled to an object file of its own (in parallel, and only when it or a header is newer than
 the object), then the objects are linked into one shared library next to the sources.
 
+The extension module through which Python calls the block operators (binding.cpp, against torch's headers) is built next to the package's modules.
+
 Usage: python -m phoenix_core_b200.csrc.build [--force] [--verbose]
 """
 import os
@@ -23,6 +25,31 @@ NVCC_FLAGS = [
 ]
 
 
+BINDING_SOURCE = os.path.join(HERE, "binding.cpp")
+BINDING = os.path.join(os.path.dirname(HERE), "_binding.so")
+
+
+def build_binding(force=False):
+    """Compiles binding.cpp into phoenix_core_b200/_binding.so (host code: g++, torch's headers and libraries)."""
+    if not force and _mtime(BINDING) >= max(_mtime(BINDING_SOURCE), _mtime(os.path.join(HERE, "build.py"))):
+        return BINDING
+    import sysconfig
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    includes = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"), os.path.join(cuda, "include"),
+                sysconfig.get_paths()["include"]]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI]
+    for i in includes:
+        cmd += ["-isystem", i]
+    cmd += ["-o", BINDING, BINDING_SOURCE, "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        sys.stderr.write(res.stdout + res.stderr)
+        raise RuntimeError("building %s failed" % BINDING)
+    return BINDING
+
+
 def _mtime(path):
     return os.path.getmtime(path) if os.path.exists(path) else 0.0
 
@@ -40,6 +67,7 @@ def build(force=False, verbose=False):
     """Compiles every CUDA source of the backend into one shared library next to the sources."""
     nvcc = os.environ.get("NVCC", "nvcc")
     os.makedirs(OBJ_DIR, exist_ok=True)
+    build_binding(force)
     newest_header = max([_mtime(os.path.join(HERE, h)) for h in HEADERS] + [_mtime(os.path.join(HERE, "build.py"))])
     todo = []
     objs = []

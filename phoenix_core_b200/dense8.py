@@ -16,7 +16,7 @@ import torch
 from . import _lib
 from .context import Context
 from .descriptors import MULTIVECTOR_DIM, Algebra, FilterLayout
-from .ops import _ALGEBRAS, _DTYPES, Device, _build_dense_desc, _launch, _need, _need_input
+from .ops import _ALGEBRAS, _DTYPES, Device, _build_dense_desc, _Entry, _input_device
 
 BLOCK = 128
 
@@ -40,16 +40,23 @@ class Filter8:
         rows, cols = self.shape[-2:]
         if rows <= 0 or cols <= 0:
             raise ValueError("invalid filter shape %s" % (self.shape,))
-        pitch = (cols + 15) // 16 * 16
-        self._storage = (torch.zeros if fill else torch.empty)((dim, rows, pitch), dtype=torch.uint8, device=device)
+        storage, blocks = Filter8.shapes(self.shape, algebra)
+        pitch = storage[2]
+        self._storage = (torch.zeros if fill else torch.empty)(storage, dtype=torch.uint8, device=device)
         self.values = self._storage.view(torch.float8_e4m3fn)[:, :, :cols].reshape(self.shape) if pitch == cols else \
             self._storage.view(torch.float8_e4m3fn)[:, :, :cols]
         if self.values.dim() != len(self.shape):
             self.values = self.values[0]
-        blocks = (dim, (rows + BLOCK - 1) // BLOCK, (cols + BLOCK - 1) // BLOCK)
         self.scales = torch.full(blocks, 127, dtype=torch.uint8, device=device) if fill else torch.empty(blocks, dtype=torch.uint8, device=device)
 
-        self._descs = {}
+        self._entries = {}
+
+    @staticmethod
+    def shapes(filterShape, algebra):
+        """Shapes of the bytes that hold a filter's numbers and its scales."""
+        rows, cols = filterShape[-2:]
+        dim = MULTIVECTOR_DIM[algebra]
+        return (dim, rows, (cols + 15) // 16 * 16), (dim, (rows + BLOCK - 1) // BLOCK, (cols + BLOCK - 1) // BLOCK)
 
     @property
     def device(self):
@@ -64,18 +71,23 @@ class Filter8:
 
 
 class _Call:
-    """What a call with a descriptor needs and does not change: the C descriptor, its sizes and shapes."""
+    """What a call with a descriptor needs and does not change."""
 
     def __init__(self, descriptor, dtype, engine, flag, forward):
         context = Context({})                                # (the formulation that a context chooses has no meaning here)
-        self.desc = _build_dense_desc(descriptor, dtype, context, engine, has_bias=forward and flag, require_input_grad=not forward and flag)
-        self.ref = ctypes.byref(self.desc)
+        desc = _build_dense_desc(descriptor, dtype, context, engine, has_bias=forward and flag, require_input_grad=not forward and flag)
         L = _lib.lib()
-        self.workspace = (L.pcb_qdense8_fwd_workspace_size if forward else L.pcb_qdense8_bwd_workspace_size)(self.ref)
-        self.input, self.output, self.bias = descriptor.getInputShape(), descriptor.getOutputShape(), descriptor.getBiasShape()
-        self.filter = tuple(descriptor.getFilterShape())
-        self.filter_grad = self.filter[:-2] + (descriptor.getInputChannels(), descriptor.getOutputChannels())
-        self.algebra, self.layout = descriptor.getAlgebra(), descriptor.getFilterLayout()
+        self.workspace = (L.pcb_qdense8_fwd_workspace_size if forward else L.pcb_qdense8_bwd_workspace_size)(ctypes.byref(desc))
+        shape, out, self.filter = descriptor.getInputShape(), descriptor.getOutputShape(), tuple(descriptor.getFilterShape())
+        self.algebra, self.layout, self.empty = descriptor.getAlgebra(), descriptor.getFilterLayout(), shape[0] == 0
+        held = Filter8.shapes(self.filter, self.algebra)
+        operands = [("input", dtype, shape), ("filter", torch.uint8, held[0]), ("filter scales", torch.uint8, held[1])]
+        if forward:
+            operands += [("bias", dtype, descriptor.getBiasShape()), ("output", dtype, out)]
+        else:
+            grad = self.filter[:-2] + (descriptor.getInputChannels(), descriptor.getOutputChannels())
+            operands += [("grad", dtype, out), ("filterGrad", dtype, grad), ("inputGrad", dtype, shape)]
+        self.entry = _Entry("pcb_qdense8_fwd" if forward else "pcb_qdense8_bwd", desc, operands)
 
     @staticmethod
     def of(descriptor, dtype, engine, flag, forward):
@@ -86,68 +98,63 @@ class _Call:
             call = cache[key] = _Call(descriptor, dtype, engine, flag, forward)
         return call
 
-    def check_filter(self, filter8, index):
+    def check_filter(self, filter8):
         if not isinstance(filter8, Filter8):
             raise ValueError("filter must be a Filter8 (see quantizeFilter8)")
         if filter8.shape != self.filter or filter8.algebra != self.algebra or filter8.filterLayout != self.layout:
             raise ValueError("filter mismatch: %s vs expected %s" % (filter8.shape, self.filter))
-        if filter8._storage.get_device() != index:
-            raise ValueError("filter is on %s, other tensors of the call on cuda:%d" % (filter8.device, index))
 
 
 def quantizeFilter8(filterTensor, filter8):
     """Rounds a filter of 16- or 32-bit numbers into ``filter8``."""
-    index = _need_input(filterTensor, "filter", filter8.shape)
-    if filter8._storage.get_device() != index:
-        raise ValueError("the Filter8 is on %s, the filter on %s" % (filter8.device, filterTensor.device))
-    ref = filter8._descs.get(filterTensor.dtype)
-    if ref is None:
+    _input_device(filterTensor, "filter")
+    entry = filter8._entries.get(filterTensor.dtype)
+    if entry is None:
         d = _lib.DenseDesc()
         oi = filter8.filterLayout == FilterLayout.OI
         d.dtype, d.algebra, d.filter_oi = _DTYPES[filterTensor.dtype], _ALGEBRAS[filter8.algebra], int(oi)
         d.in_features, d.out_features = filter8.shape[-1 if oi else -2], filter8.shape[-2 if oi else -1]
-        ref = filter8._descs[filterTensor.dtype] = ctypes.byref(d)
-    _launch(index, _lib.lib().pcb_quantize_filter8, ref, filterTensor.data_ptr(), filter8._storage.data_ptr(), filter8.scales.data_ptr())
+        held = Filter8.shapes(filter8.shape, filter8.algebra)
+        entry = filter8._entries[filterTensor.dtype] = _Entry("pcb_quantize_filter8", d, [
+            ("filter", filterTensor.dtype, filter8.shape), ("8-bit filter", torch.uint8, held[0]), ("8-bit filter's scales", torch.uint8, held[1])])
+    entry.call(None, 0, filterTensor, filter8._storage, filter8.scales)
 
 
 def dense8Fwd(inputTensor, filter8, biasTensor, outputTensor, descriptor, context=None, engine=_lib.ENGINE_AUTO):
     """``denseFwd`` with a filter held in 8 bits and the input quantised along its features. Input, bias and output share a type."""
-    dtype, bias = inputTensor.dtype, biasTensor is not None
-    index = _need_input(inputTensor, "input", descriptor.inputShape)
-    call = _Call.of(descriptor, dtype, engine, bias, True)
-    call.check_filter(filter8, index)
-    _need(outputTensor, "output", dtype, call.output, index)
-    if bias:
-        if not descriptor.isBiasUsed():
-            raise ValueError("Bias application is not configured for this scalar Dense operation")
-        _need(biasTensor, "bias", dtype, call.bias, index)
-    if call.input[0] == 0:
-        return
+    index, bias = _input_device(inputTensor, "input"), biasTensor is not None
+    call = _Call.of(descriptor, inputTensor.dtype, engine, bias, True)
+    call.check_filter(filter8)
+    if bias and not descriptor.isBiasUsed():
+        raise ValueError("Bias application is not configured for this scalar Dense operation")
+    if outputTensor is None:
+        raise ValueError("output expected")
+    if call.empty:
+        return call.entry.check(inputTensor, filter8._storage, filter8.scales, biasTensor, outputTensor)
     dev = Device.at(index)
     with dev.accessControl:
         ws = dev.requestWorkspace(call.workspace)
-        _launch(index, _lib.lib().pcb_qdense8_fwd, call.ref, inputTensor.data_ptr(), filter8._storage.data_ptr(), filter8.scales.data_ptr(),
-                biasTensor.data_ptr() if bias else None, outputTensor.data_ptr(), ws.data_ptr(), ws.numel())
-        dev._after_op()
+        call.entry.call(ws, 0, inputTensor, filter8._storage, filter8.scales, biasTensor, outputTensor)
+        if dev.check_after_each_op:
+            dev.checkStatus()
 
 
 def dense8Bwd(inputTensor, filter8, gradTensor, filterGradTensor, inputGradTensor, descriptor, context=None, engine=_lib.ENGINE_AUTO):
     """``denseBwd`` in 8 bits: the filter gradient (input-major, ``[D, I, O]``, whatever the filter layout) from the input and the output
     gradient quantised along the samples, the input gradient from the filter and the output gradient quantised along the features."""
-    dtype, need_dx = inputTensor.dtype, descriptor.isInputGradientRequired()
-    index = _need_input(inputTensor, "input", descriptor.inputShape)
-    call = _Call.of(descriptor, dtype, engine, need_dx, False)
-    call.check_filter(filter8, index)
-    _need(gradTensor, "grad", dtype, call.output, index)
-    _need(filterGradTensor, "filterGrad", dtype, call.filter_grad, index)
-    if need_dx:
-        _need(inputGradTensor, "inputGrad", dtype, call.input, index)
-    if call.input[0] == 0:
+    index, need_dx = _input_device(inputTensor, "input"), descriptor.isInputGradientRequired()
+    call = _Call.of(descriptor, inputTensor.dtype, engine, need_dx, False)
+    call.check_filter(filter8)
+    if gradTensor is None or filterGradTensor is None or (need_dx and inputGradTensor is None):
+        raise ValueError("grad, filterGrad and, where the descriptor asks for it, inputGrad expected")
+    operands = (inputTensor, filter8._storage, filter8.scales, gradTensor, filterGradTensor, inputGradTensor if need_dx else None)
+    if call.empty:
+        call.entry.check(*operands)
         filterGradTensor.zero_()
         return
     dev = Device.at(index)
     with dev.accessControl:
         ws = dev.requestWorkspace(call.workspace)
-        _launch(index, _lib.lib().pcb_qdense8_bwd, call.ref, inputTensor.data_ptr(), filter8._storage.data_ptr(), filter8.scales.data_ptr(),
-                gradTensor.data_ptr(), filterGradTensor.data_ptr(), inputGradTensor.data_ptr() if need_dx else None, ws.data_ptr(), ws.numel())
-        dev._after_op()
+        call.entry.call(ws, 0, *operands)
+        if dev.check_after_each_op:
+            dev.checkStatus()

@@ -14,7 +14,7 @@ import torch
 
 from . import _lib
 from .descriptors import MULTIVECTOR_DIM, Algebra
-from .ops import _ALGEBRAS, _DTYPES, _launch, _need, _need_input
+from .ops import _ALGEBRAS, _DTYPES, _Entry, _input_device
 
 
 class DistillDescriptor:
@@ -42,49 +42,50 @@ class DistillDescriptor:
     def getAlgebra(self): return self.algebra
 
     def _call(self, dtype):
-        ref = self._calls.get(dtype)
-        if ref is None:
+        call = self._calls.get(dtype)
+        if call is None:
             d = _lib.DistillDesc()
             d.dtype, d.algebra, d.batch, d.units = _DTYPES[dtype], _ALGEBRAS[self.algebra], self.samples, self.logitsShape[1]
             d.entries, d.alpha, d.temperature = self.teacherEntries, self.alpha, self.temperature
-            ref = self._calls[dtype] = ctypes.byref(d)
-        return ref
+            sample, stats = (torch.float32, self.lossShape), (torch.float32, self.statsShape)
+            operands = [("logits", dtype, self.logitsShape), ("labels", torch.int64, self.lossShape), ("teacherLogits", dtype, self.teacherShape),
+                        ("teacherIndices", torch.int64, self.teacherShape)]
+            call = self._calls[dtype] = (_Entry("pcb_distill_fwd", d, operands + [("loss",) + sample, ("stats",) + stats]),
+                                         _Entry("pcb_distill_bwd", d, operands + [("stats",) + stats, ("gradLoss",) + sample, ("gradLogits", dtype, self.logitsShape)]))
+        return call
 
 
-def _check_operands(logits, labels, teacher, index, descriptor):
-    """The device's index, and the pointers of labels, teacher and index."""
-    device = _need_input(logits, "logits", descriptor.logitsShape)
-    if labels is not None:
-        _need(labels, "labels", torch.int64, descriptor.lossShape, device)
-        labels = labels.data_ptr()
+def _teacher(descriptor, teacher, index):
     if descriptor.teacherEntries == 0:
-        return device, labels, None, None
+        return None, None
     if teacher is None or index is None:
         raise ValueError("the descriptor has %d entries of a teacher" % descriptor.teacherEntries)
-    _need(teacher, "teacherLogits", logits.dtype, descriptor.teacherShape, device)
-    _need(index, "teacherIndices", torch.int64, descriptor.teacherShape, device)
-    return device, labels, teacher.data_ptr(), index.data_ptr()
+    return teacher, index
 
 
 def distillFwd(logitsTensor, labels, teacherLogits, teacherIndices, lossTensor, statsTensor, descriptor):
     """Losses (fp32, one per sample) of logits against ``labels`` (int64, None: no such term; a value outside the classes leaves a sample's out) and
     the teacher's logits at ``teacherIndices`` (int64; an index outside the classes leaves an entry out). ``statsTensor`` (fp32,
     ``getStatsShape()``) is kept for ``distillBwd`` and may be None."""
-    device, *operands = _check_operands(logitsTensor, labels, teacherLogits, teacherIndices, descriptor)
-    _need(lossTensor, "loss", torch.float32, descriptor.lossShape, device)
-    if statsTensor is not None:
-        _need(statsTensor, "stats", torch.float32, descriptor.statsShape, device)
+    _input_device(logitsTensor, "logits")
+    teacher, index = _teacher(descriptor, teacherLogits, teacherIndices)
+    if lossTensor is None:
+        raise ValueError("loss expected")
+    fwd, operands = descriptor._call(logitsTensor.dtype)[0], (logitsTensor, labels, teacher, index, lossTensor, statsTensor)
     if descriptor.samples:
-        _launch(device, _lib.lib().pcb_distill_fwd, descriptor._call(logitsTensor.dtype), logitsTensor.data_ptr(), *operands, lossTensor.data_ptr(),
-                None if statsTensor is None else statsTensor.data_ptr())
+        fwd.call(None, 0, *operands)
+    else:
+        fwd.check(*operands)
 
 
 def distillBwd(logitsTensor, labels, teacherLogits, teacherIndices, statsTensor, gradLoss, gradLogits, descriptor):
     """The gradient of the logits, ``gradLoss`` (fp32) being that of each sample's loss. ``gradLogits`` must not be the logits themselves."""
-    device, *operands = _check_operands(logitsTensor, labels, teacherLogits, teacherIndices, descriptor)
-    _need(statsTensor, "stats", torch.float32, descriptor.statsShape, device)
-    _need(gradLoss, "gradLoss", torch.float32, descriptor.lossShape, device)
-    _need(gradLogits, "gradLogits", logitsTensor.dtype, descriptor.logitsShape, device)
+    _input_device(logitsTensor, "logits")
+    teacher, index = _teacher(descriptor, teacherLogits, teacherIndices)
+    if statsTensor is None or gradLoss is None or gradLogits is None:
+        raise ValueError("stats, gradLoss and gradLogits expected")
+    bwd, operands = descriptor._call(logitsTensor.dtype)[1], (logitsTensor, labels, teacher, index, statsTensor, gradLoss, gradLogits)
     if descriptor.samples:
-        _launch(device, _lib.lib().pcb_distill_bwd, descriptor._call(logitsTensor.dtype), logitsTensor.data_ptr(), *operands, statsTensor.data_ptr(),
-                gradLoss.data_ptr(), gradLogits.data_ptr())
+        bwd.call(None, 0, *operands)
+    else:
+        bwd.check(*operands)

@@ -161,34 +161,49 @@ class _OnDevice:
         return False
 
 
-_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+class _Entry:
+    """An entry point with its descriptor and what its operands have to be: ``call`` checks them, takes the device's current stream and calls it."""
+
+    __slots__ = ("names", "expected", "specs", "entry", "desc", "address", "_call")
+
+    def __init__(self, entry, desc, operands):
+        """operands: (name, dtype, shape) of each, in the entry point's order."""
+        self.names, self.expected = [n for n, _, _ in operands], [(t, tuple(s)) for _, t, s in operands]
+        binding = _lib.binding()
+        self.specs, self._call = binding.make_specs(tuple(self.expected)), binding.call
+        self.entry, self.desc = ctypes.cast(getattr(_lib.lib(), entry), ctypes.c_void_p).value, desc
+        self.address = ctypes.addressof(desc)
+
+    def call(self, workspace, offset, *operands):
+        status = self._call(self.entry, self.address, self.specs, workspace, offset, *operands)
+        if status:
+            self._raise(status, operands)
+
+    def check(self, *operands):
+        status = self._call(0, 0, self.specs, None, 0, *operands)
+        if status:
+            self._raise(status, operands)
+
+    def _raise(self, status, operands):
+        if status < 0:
+            _lib.check(status)
+        name, t = self.names[status - 1], operands[status - 1]
+        if not isinstance(t, torch.Tensor):
+            raise ValueError("%s: a tensor expected" % name)
+        _check_tensor(t, name, *self.expected[status - 1])
+        raise ValueError("%s is on %s, other tensors of the call on another device" % (name, t.device))
 
 
-def _need(t, name, dtype, shape, index):
-    """Raises unless a tensor is what ``_check_tensor`` asks for, on the device `index`: one look for the call that is in order (a microsecond less per
-    tensor than the checks that can say what is wrong, which then follow)."""
-    if t.dtype is not dtype or t.shape != shape or t.get_device() != index or not t.is_contiguous():
-        _check_tensor(t, name, dtype, shape)
-        raise ValueError("%s is on %s, other tensors of the call on cuda:%d" % (name, t.device, index))
-
-
-def _need_input(t, name, shape):
-    """Checks the tensor that settles the type and the device of a call; returns the device's index."""
+def _input_device(t, name):
+    """The device's index of the tensor that settles the type and the device of a call."""
+    if not isinstance(t, torch.Tensor):
+        raise ValueError("%s: a tensor expected" % name)
     if t.dtype not in _DTYPES:
         raise ValueError("%s dtype %s: float32, float16 or bfloat16 expected" % (name, t.dtype))
     index = t.get_device()
-    if index < 0 or t.shape != shape or not t.is_contiguous():
-        _check_tensor(t, name, shape=shape)
+    if index < 0:
+        _check_tensor(t, name)
     return index
-
-
-def _launch(index, entry, *args):
-    """Calls an entry point of the library on a device's current stream (its last argument)."""
-    if _current_device() == index:
-        _lib.check(entry(*args, _raw_stream(index)))
-    else:
-        with torch.cuda.device(index):
-            _lib.check(entry(*args, _raw_stream(index)))
 
 
 # upstride::Algebra -> pcb_algebra (the C ABI keeps quaternion at zero)

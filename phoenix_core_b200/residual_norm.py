@@ -17,7 +17,7 @@ import torch
 
 from . import _lib
 from .descriptors import MULTIVECTOR_DIM, Algebra
-from .ops import _ALGEBRAS, _DTYPES, Device, _launch, _need, _need_input
+from .ops import _ALGEBRAS, _DTYPES, Device, _Entry, _input_device
 
 
 class ResidualNormDescriptor:
@@ -49,52 +49,40 @@ class ResidualNormDescriptor:
             d = _lib.NormDesc()
             d.dtype, d.algebra, d.batch, d.features = _DTYPES[dtype], _ALGEBRAS[self.algebra], self.samples, self.inputShape[1]
             d.gate_rows, d.residual_scale, d.epsilon = self.gateRows, self.residualScale, self.epsilon
-            ref = ctypes.byref(d)
-            call = self._calls[dtype] = (ref, _lib.lib().pcb_residual_norm_bwd_workspace_size(ref))
+            row, gate = (dtype, self.inputShape), (dtype, self.gateShape)
+            weight, stats = (torch.float32, self.weightShape), (torch.float32, self.statsShape)
+            block = [("branch",) + row, ("gate",) + gate, ("postWeight",) + weight, ("preWeight",) + weight]
+            fwd = _Entry("pcb_residual_norm_fwd", d, [("residual",) + row] + block + [("output",) + row, ("norm",) + row, ("stats",) + stats])
+            bwd = _Entry("pcb_residual_norm_bwd", d, [("output",) + row] + block + [
+                ("stats",) + stats, ("gradOutput",) + row, ("gradNorm",) + row, ("gradResidual",) + row, ("gradBranch",) + row, ("gradGate",) + gate,
+                ("gradPostWeight",) + weight, ("gradPreWeight",) + weight])
+            call = self._calls[dtype] = (fwd, bwd, _lib.lib().pcb_residual_norm_bwd_workspace_size(ctypes.byref(d)))
         return call
 
 
-def _check_parts(descriptor, dtype, index, branch, gate, post, pre):
-    if branch is not None:
-        _need(branch, "branch", dtype, descriptor.inputShape, index)
-    elif gate is not None or post is not None:
-        raise ValueError("a gate or postWeight without a branch")
+def _check_parts(descriptor, branch, gate, post):
     if (gate is None) != (descriptor.gateRows == 0):
         raise ValueError("the descriptor has %d rows of a gate" % descriptor.gateRows)
-    if gate is not None:
-        _need(gate, "gate", dtype, descriptor.gateShape, index)
-    if post is not None:
-        _need(post, "postWeight", torch.float32, descriptor.weightShape, index)
-    if pre is not None:
-        _need(pre, "preWeight", torch.float32, descriptor.weightShape, index)
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
+    if branch is None and (gate is not None or post is not None):
+        raise ValueError("a gate or postWeight without a branch")
 
 
 def residualNormFwd(residualTensor, branchTensor, gateTensor, postWeight, preWeight, outputTensor, normTensor, statsTensor, descriptor):
     """y into ``outputTensor`` and h into ``normTensor``; ``statsTensor`` (fp32, ``getStatsShape()``) keeps the factors of both norms for the
     backward call and may be None. Without a branch (None, with gate and postWeight) h is the norm of the residual itself and
     ``outputTensor`` may be None; without ``normTensor`` (None, with preWeight) there is no norm behind the block. Weights may be None (ones)."""
-    x, dtype = residualTensor, residualTensor.dtype
-    shape = descriptor.inputShape
-    index = _need_input(x, "residual", shape)
-    _check_parts(descriptor, dtype, index, branchTensor, gateTensor, postWeight, preWeight)
+    _input_device(residualTensor, "residual")
+    _check_parts(descriptor, branchTensor, gateTensor, postWeight)
     if (branchTensor is not None or normTensor is None) and outputTensor is None:
         raise ValueError("output expected")
-    if outputTensor is not None:
-        _need(outputTensor, "output", dtype, shape, index)
-    if normTensor is not None:
-        _need(normTensor, "norm", dtype, shape, index)
-    elif preWeight is not None:
+    if normTensor is None and preWeight is not None:
         raise ValueError("preWeight without normTensor")
-    if statsTensor is not None:
-        _need(statsTensor, "stats", torch.float32, descriptor.statsShape, index)
-    if shape[0] == 0:
-        return
-    _launch(index, _lib.lib().pcb_residual_norm_fwd, descriptor._call(dtype)[0], x.data_ptr(), _ptr(branchTensor), _ptr(gateTensor), _ptr(postWeight),
-            _ptr(preWeight), _ptr(outputTensor), _ptr(normTensor), _ptr(statsTensor))
+    fwd = descriptor._call(residualTensor.dtype)[0]
+    operands = (residualTensor, branchTensor, gateTensor, postWeight, preWeight, outputTensor, normTensor, statsTensor)
+    if descriptor.samples:
+        fwd.call(None, 0, *operands)
+    else:
+        fwd.check(*operands)
 
 
 def residualNormBwd(outputTensor, branchTensor, gateTensor, postWeight, preWeight, statsTensor, gradOutput, gradNorm, gradResidual, gradBranch,
@@ -102,47 +90,34 @@ def residualNormBwd(outputTensor, branchTensor, gateTensor, postWeight, preWeigh
     """From ``gradOutput`` (of y, from the residual path; None: none) and ``gradNorm`` (of h; None: there was no norm behind the block) the
     gradients of the residual, the branch, the gate and the weights; those of the gate and the weights may be None. ``outputTensor`` is the forward
     call's y (the residual itself where there was no branch), needed where there is a ``gradNorm``."""
-    dtype, shape, weights = gradResidual.dtype, descriptor.inputShape, descriptor.weightShape
-    index = _need_input(gradResidual, "gradResidual", shape)
-    _check_parts(descriptor, dtype, index, branchTensor, gateTensor, postWeight, preWeight)
+    index = _input_device(gradResidual, "gradResidual")
+    _check_parts(descriptor, branchTensor, gateTensor, postWeight)
     if gradOutput is None and gradNorm is None:
         raise ValueError("gradOutput or gradNorm expected")
     if gradNorm is None:
         if preWeight is not None or gradPreWeight is not None:
             raise ValueError("preWeight without gradNorm")
-    else:
-        if outputTensor is None:
-            raise ValueError("output expected: the gradient of its norm needs it")
-        _need(gradNorm, "gradNorm", dtype, shape, index)
-        _need(outputTensor, "output", dtype, shape, index)
-    if gradOutput is not None:
-        _need(gradOutput, "gradOutput", dtype, shape, index)
-    if branchTensor is not None:
-        if gradBranch is None:
-            raise ValueError("gradBranch expected")
-        _need(gradBranch, "gradBranch", dtype, shape, index)
-    elif gradPostWeight is not None:
-        raise ValueError("gradPostWeight without a branch")
-    if gradGate is not None:
-        if gateTensor is None:
-            raise ValueError("gradGate without a gate")
-        _need(gradGate, "gradGate", dtype, descriptor.gateShape, index)
-    if gradPostWeight is not None:
-        _need(gradPostWeight, "gradPostWeight", torch.float32, weights, index)
-    if gradPreWeight is not None:
-        _need(gradPreWeight, "gradPreWeight", torch.float32, weights, index)
+    elif outputTensor is None:
+        raise ValueError("output expected: the gradient of its norm needs it")
+    if branchTensor is None:
+        if gradPostWeight is not None:
+            raise ValueError("gradPostWeight without a branch")
+    elif gradBranch is None:
+        raise ValueError("gradBranch expected")
+    if gradGate is not None and gateTensor is None:
+        raise ValueError("gradGate without a gate")
     if statsTensor is None:
         raise ValueError("stats expected")
-    _need(statsTensor, "stats", torch.float32, descriptor.statsShape, index)
-    if shape[0] == 0:
+    _, bwd, need = descriptor._call(gradResidual.dtype)
+    operands = (outputTensor, branchTensor, gateTensor, postWeight, preWeight, statsTensor, gradOutput, gradNorm, gradResidual, gradBranch, gradGate, gradPostWeight,
+                gradPreWeight)
+    if descriptor.samples == 0:
+        bwd.check(*operands)
         for t in (gradPostWeight, gradPreWeight, gradGate):
             if t is not None:
                 t.zero_()
         return
-    ref, need = descriptor._call(dtype)
     dev = Device.at(index)
     with dev.accessControl:
         ws = dev.requestWorkspace(need + 256)                          # behind the workspace's status block
-        _launch(index, _lib.lib().pcb_residual_norm_bwd, ref, _ptr(outputTensor), _ptr(branchTensor), _ptr(gateTensor), _ptr(postWeight), _ptr(preWeight),
-                statsTensor.data_ptr(), _ptr(gradOutput), _ptr(gradNorm), gradResidual.data_ptr(), _ptr(gradBranch), _ptr(gradGate), _ptr(gradPostWeight),
-                _ptr(gradPreWeight), ws.data_ptr() + 256, ws.numel() - 256)
+        bwd.call(ws, 256, *operands)
