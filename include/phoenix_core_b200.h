@@ -204,7 +204,8 @@ int pcb_qdense_bwd(const pcb_dense_desc* desc, const void* x, const void* w, con
  *   x and dy come in desc->dtype and are quantised inside the call, in the workspace, with one scale for each 128 values along the axis that
  *   the product sums over: features for y and dx, samples for dw.
  * Products are exact, sums are held in fp32, results are rounded once to desc->dtype. Every algebra; engine AUTO or TENSOR; `variant` has no
- * meaning here. The workspace must be 16-byte aligned. dw is written in [D, I, O] orientation whatever filter_oi says. In backward w8 may be
+ * meaning here. The workspace must be 16-byte aligned. dw is written in [D, I, O] orientation whatever filter_oi says. y must
+ * not share memory with x. In backward w8 may be
  * null when require_input_grad is 0. pcb_quantize_filter8 does not read desc->batch. */
 size_t pcb_filter8_values_size(const pcb_dense_desc* desc);
 size_t pcb_filter8_scales_size(const pcb_dense_desc* desc);

@@ -112,6 +112,7 @@ class QDense8Function(torch.autograd.Function):
         return y
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         (x,) = ctx.saved_tensors
         dy, f = dy.contiguous(), ctx.filter8
@@ -150,6 +151,7 @@ class ResidualNormFunction(torch.autograd.Function):
         return (residual if y is None else y), h
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dh):
         y, branch, gate, post, pre, stats = ctx.saved_tensors
         if dy is None and dh is None:
@@ -185,6 +187,7 @@ class DistillFunction(torch.autograd.Function):
         return losses
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         logits, labels, teacher_logits, teacher_indices, stats = ctx.saved_tensors
         dlogits = torch.empty_like(logits)

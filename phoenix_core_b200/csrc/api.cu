@@ -715,6 +715,8 @@ int pcb_qdense8_fwd(const pcb_dense_desc* desc, const void* x, const void* w8, c
     if (!x || !w8 || !w8_scales || !y || (g.has_bias && !bias)) { set_error("null tensor pointer"); return PCB_ERR_INVALID_ARGUMENT; }
     const Dense8Space at = dense8_space(g, false, false);
     if ((rc = dense8_workspace(workspace, workspace_bytes_, at.total)) != PCB_OK || (rc = dense8_check_filter(w8)) != PCB_OK) return rc;
+    const size_t size = dtype_size(desc->dtype);
+    if (overlaps(y, (size_t)g.nc * g.Nb * g.Co * size, x, (size_t)g.nc * g.Nb * g.Ci * size)) { set_error("y must not share memory with x"); return PCB_ERR_INVALID_ARGUMENT; }
     forget_kept(workspace);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     int* status = reinterpret_cast<int*>(ws);

@@ -18,6 +18,18 @@ int check_norm(const pcb_norm_desc* d) {
     if ((long long)g.nc * d->batch * d->features > 2147483647LL || (long long)g.nc * d->features > 2147483647LL) { set_error("tensor too large for 32-bit element offsets"); return PCB_ERR_TOO_LARGE; }
     return PCB_OK;
 }
+// No result may lie where an operand or another result does: rows are read ahead of those that are written.
+struct Span { const void* at; size_t bytes; };
+int check_apart(const Span* results, int n, const Span* operands, int m) {
+    for (int i = 0; i < n; ++i) {
+        if (!results[i].at) continue;
+        for (int k = 0; k < m + i; ++k) {
+            const Span& o = k < m ? operands[k] : results[k - m];
+            if (o.at && overlaps(results[i].at, results[i].bytes, o.at, o.bytes)) { set_error("a result shares memory with another tensor of the call"); return PCB_ERR_INVALID_ARGUMENT; }
+        }
+    }
+    return PCB_OK;
+}
 int norm_comps(const pcb_norm_desc* d) { Geom g = {}; algebra_setup(d->algebra, g); return g.nc; }
 
 RNParams norm_params(const pcb_norm_desc* d) {
@@ -46,6 +58,9 @@ int pcb_residual_norm_fwd(const pcb_norm_desc* d, const void* x, const void* bra
     if (!x || (branch && !y) || (!y && !h)) { set_error("null tensor pointer"); return PCB_ERR_INVALID_ARGUMENT; }
     if ((gate != nullptr) != (d->gate_rows > 0) || (!branch && (gate || post)) || (!h && pre)) { set_error("gate or weights without what they apply to"); return PCB_ERR_INVALID_ARGUMENT; }
     RNParams p = norm_params(d);
+    const size_t size = dtype_size(d->dtype), row = (size_t)p.comps * d->batch * d->features * size, gates = (size_t)p.comps * d->gate_rows * d->features * size, weight = (size_t)d->features * 4;
+    const Span results[] = {{y, row}, {h, row}, {stats, (size_t)d->batch * 8}}, operands[] = {{x, row}, {branch, row}, {gate, gates}, {post, weight}, {pre, weight}};
+    if (const int apart = check_apart(results, 3, operands, 5)) return apart;
     p.x = x; p.branch = branch; p.gate = gate; p.post = post; p.pre = pre; p.y = y; p.h = h; p.stats = stats;
     const cudaStream_t s = (cudaStream_t)stream;
     if (d->dtype == PCB_F32) return norm_fwd_f32(p, s);
@@ -74,6 +89,10 @@ int pcb_residual_norm_bwd(const pcb_norm_desc* d, const void* y, const void* bra
     if (!workspace || workspace_bytes < q.total) { set_error("workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : (size_t)0, q.total); return PCB_ERR_WORKSPACE; }
     if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) { set_error("the workspace must be 16-byte aligned"); return PCB_ERR_INVALID_ARGUMENT; }
     RNParams p = norm_params(d);
+    const size_t size = dtype_size(d->dtype), row = (size_t)comps * d->batch * d->features * size, gates = (size_t)comps * d->gate_rows * d->features * size, weight = (size_t)d->features * 4;
+    const Span results[] = {{dx, row}, {dbranch, branch ? row : 0}, {dgate, gates}, {dpost, weight}, {dpre, weight}, {workspace, q.total}};
+    const Span operands[] = {{dh ? y : nullptr, row}, {branch, row}, {gate, gates}, {post, weight}, {pre, weight}, {stats, (size_t)d->batch * 8}, {dy, row}, {dh, row}};
+    if (const int apart = check_apart(results, 6, operands, 8)) return apart;
     p.branch = branch; p.gate = gate; p.post = post; p.pre = pre; p.y = const_cast<void*>(y); p.stats = const_cast<float*>(stats);
     p.dy = dy; p.dh = dh; p.dx = dx; p.dbranch = dbranch; p.dgate = dgate; p.dpost = dpost; p.dpre = dpre;
     p.workspace = static_cast<uint8_t*>(workspace);

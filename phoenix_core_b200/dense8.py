@@ -41,14 +41,8 @@ class Filter8:
         if rows <= 0 or cols <= 0:
             raise ValueError("invalid filter shape %s" % (self.shape,))
         storage, blocks = Filter8.shapes(self.shape, algebra)
-        pitch = storage[2]
         self._storage = (torch.zeros if fill else torch.empty)(storage, dtype=torch.uint8, device=device)
-        self.values = self._storage.view(torch.float8_e4m3fn)[:, :, :cols].reshape(self.shape) if pitch == cols else \
-            self._storage.view(torch.float8_e4m3fn)[:, :, :cols]
-        if self.values.dim() != len(self.shape):
-            self.values = self.values[0]
         self.scales = torch.full(blocks, 127, dtype=torch.uint8, device=device) if fill else torch.empty(blocks, dtype=torch.uint8, device=device)
-
         self._entries = {}
 
     @staticmethod
@@ -57,6 +51,11 @@ class Filter8:
         rows, cols = filterShape[-2:]
         dim = MULTIVECTOR_DIM[algebra]
         return (dim, rows, (cols + 15) // 16 * 16), (dim, (rows + BLOCK - 1) // BLOCK, (cols + BLOCK - 1) // BLOCK)
+
+    @property
+    def values(self):
+        v = self._storage.view(torch.float8_e4m3fn)[:, :, :self.shape[-1]]
+        return v if len(self.shape) == 3 else v[0]
 
     @property
     def device(self):

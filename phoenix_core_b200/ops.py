@@ -164,15 +164,18 @@ class _OnDevice:
 class _Entry:
     """An entry point with its descriptor and what its operands have to be: ``call`` checks them, takes the device's current stream and calls it."""
 
-    __slots__ = ("names", "expected", "specs", "entry", "desc", "address", "_call")
+    __slots__ = ("name", "operands", "specs", "entry", "desc", "address", "_call")
 
     def __init__(self, entry, desc, operands):
         """operands: (name, dtype, shape) of each, in the entry point's order."""
-        self.names, self.expected = [n for n, _, _ in operands], [(t, tuple(s)) for _, t, s in operands]
+        self.name, self.operands = entry, operands
         binding = _lib.binding()
-        self.specs, self._call = binding.make_specs(tuple(self.expected)), binding.call
+        self.specs, self._call = binding.make_specs(tuple((t, tuple(s)) for _, t, s in operands)), binding.call
         self.entry, self.desc = ctypes.cast(getattr(_lib.lib(), entry), ctypes.c_void_p).value, desc
         self.address = ctypes.addressof(desc)
+
+    def __reduce__(self):                                  # (descriptors and filters are copied and pickled with what they keep)
+        return _Entry, (self.name, self.desc, self.operands)
 
     def call(self, workspace, offset, *operands):
         status = self._call(self.entry, self.address, self.specs, workspace, offset, *operands)
@@ -187,10 +190,10 @@ class _Entry:
     def _raise(self, status, operands):
         if status < 0:
             _lib.check(status)
-        name, t = self.names[status - 1], operands[status - 1]
+        (name, dtype, shape), t = self.operands[status - 1], operands[status - 1]
         if not isinstance(t, torch.Tensor):
             raise ValueError("%s: a tensor expected" % name)
-        _check_tensor(t, name, *self.expected[status - 1])
+        _check_tensor(t, name, dtype, tuple(shape))
         raise ValueError("%s is on %s, other tensors of the call on another device" % (name, t.device))
 
 

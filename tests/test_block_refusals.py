@@ -97,3 +97,24 @@ def test_distill_python():
     assert d.getClasses() == 1000 and d.getTeacherShape() == (2, 3) and d.getStatsShape() == (3, 2)
     with pytest.raises(ValueError, match="CUDA"):
         pcb.distillFwd(torch.zeros(8, 250), None, None, None, torch.zeros(2), None, d)
+
+
+def test_results_apart(library):
+    """A result on an operand, on another result, or across the end of one is refused (addresses are only compared: nothing is launched)."""
+    bad, step = _lib.PCB_ERR_INVALID_ARGUMENT, 1 << 20
+    at = [step * (i + 1) for i in range(16)]
+    x, b, g, post, pre, y, h, stats = at[:8]
+    row = 4 * 12 * 64 * 2                                            # bytes of the descriptor's rows
+    for y_, h_, stats_ in ((x, h, stats), (y, b, stats), (y, y, stats), (x + row - 2, h, stats), (y, h, y), (g, h, stats), (y, pre, stats), (y, h, post)):
+        assert library.pcb_residual_norm_fwd(ctypes.byref(norm()), x, b, g, post, pre, y_, h_, stats_, None) == bad
+        assert b"shares memory" in library.pcb_last_error_message()
+    need = library.pcb_residual_norm_bwd_workspace_size(ctypes.byref(norm()))
+    dy, dh, dx, db, dg, dpost, dpre, ws = at[8:]
+    for results in ((dy, db, dg, dpost, dpre), (dh, db, dg, dpost, dpre), (dx, dx, dg, dpost, dpre), (dx, b, dg, dpost, dpre), (dx, db, g, dpost, dpre), (dx, db, dg, post, dpre),
+                    (dx, db, dg, dpost, dpost), (y, db, dg, dpost, dpre), (dx, db, dg, dpost, ws)):
+        assert library.pcb_residual_norm_bwd(ctypes.byref(norm()), y, b, g, post, pre, stats, dy, dh, *results, ws, need, None) == bad
+        assert b"shares memory" in library.pcb_last_error_message()
+    d = _lib.DenseDesc()
+    d.dtype, d.algebra, d.batch, d.in_features, d.out_features = _lib.PCB_F16, 0, 2, 128, 128
+    need = library.pcb_qdense8_fwd_workspace_size(ctypes.byref(d))
+    assert library.pcb_qdense8_fwd(ctypes.byref(d), x, b, g, None, x + 16, ws, need, None) == bad and b"share memory" in library.pcb_last_error_message()
