@@ -655,7 +655,7 @@ __global__ void __launch_bounds__(RN_WIDE_THREADS) residual_norm_bwd_wide_kernel
     }
 }
 
-// Adds the pieces. Weights: eight columns (a sector) per CTA, the slots and components over 64 threads of each column. Gates: 1, 8 or 64 threads per value.
+// Adds the pieces. Weights: eight columns (a sector) per CTA, the slots and components over 64 threads of each column. Gates: 1 to 64 threads per value.
 constexpr int RN_SUM_THREADS = 512;
 template <typename T>
 __global__ void __launch_bounds__(RN_SUM_THREADS) residual_norm_sum_kernel(const RNParams p, int slots, int weight_blocks, int slices) {
@@ -777,7 +777,11 @@ int bwd_typed(RNParams p, RNPlan q, cudaStream_t s) {
     else if (p.period == 1) PCB_CUDA_TRY((bwd_any<T, VEC, true>(p, q, s)));
     else PCB_CUDA_TRY((bwd_any<T, VEC, false>(p, q, s)));
     const long long weight_blocks = p.part_w ? (p.features + 7) / 8 : 0;
-    const int slices = q.parts > 32 ? 64 : (q.parts > 4 ? 8 : 1), values = RN_SUM_THREADS / slices;
+    // threads per value of a gate: up to two values' worth for every SM's 2048, while each has two parts at least (5358 x 174, one gate: 17 us, 177 by one thread each; 16384 x 4096,
+    // 16 gates of 111 parts: 13 us, 47 with 64 each)
+    int slices = 1;
+    while (slices < 64 && slices * 4 <= q.parts && (long long)p.groups * p.comps * p.features * slices < 2048LL * device_sms()) slices *= 2;
+    const int values = RN_SUM_THREADS / slices;
     const long long gate_blocks = p.part_gate ? ((long long)p.groups * p.comps * p.features + values - 1) / values : 0;
     if (weight_blocks + gate_blocks > 0)
         PCB_CUDA_TRY(launch_chained(residual_norm_sum_kernel<T>, (unsigned)(weight_blocks + gate_blocks), RN_SUM_THREADS, 0, s, p, q.grid, (int)weight_blocks, slices));
