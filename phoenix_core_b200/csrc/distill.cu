@@ -6,7 +6,8 @@
 //   dz_j = g * ((1 - a) * (softmax(z)_j - [j = c]) + a * T * (q_j - p_j))
 // Both sums over the vocabulary are taken in one pass with a running maximum; the gradient reads the logits once more and writes
 // them once. With T = 2 the exponentials of T = 1 are the squares of the others: one exponential per logit, which keeps the pass bound by memory
-// (16 exponentials per clock and SM are two thirds of what a pass over 16-bit logits takes at full bandwidth).
+// (16 exponentials per clock and SM are two thirds of what a pass over 16-bit logits takes at full bandwidth). 4096 x 131072 bf16: 190 us forward (5.6 TB/s), 342
+// backward (6.3 TB/s both ways); bound by memory.
 // Few rows are cut over the CTAs of a cluster, whose maxima and sums are joined through distributed shared memory.
 #include "common.cuh"
 #include "packed.cuh"
@@ -35,7 +36,8 @@ struct DIParams {
 template <typename T> struct Bits;       // one value, and 16 bytes of them
 template <> struct Bits<float> {
     static constexpr int VEC = 4;
-    static __device__ __forceinline__ float one(const float* p) { return ld_chained(p); }
+    static constexpr uint32_t NOTHING = 0xff800000u;              // minus infinity throughout a word
+    static __device__ __forceinline__ float one(const float* p, bool ok) { return __uint_as_float(ld_chained(reinterpret_cast<const uint32_t*>(p), ok)); }
     static __device__ __forceinline__ void unpack(const uint4& r, float* v) { v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y); v[2] = __uint_as_float(r.z); v[3] = __uint_as_float(r.w); }
     static __device__ __forceinline__ uint4 pack(const float* v) { return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])); }
     static __device__ __forceinline__ void put(float* p, float v) { *p = v; }
@@ -48,7 +50,8 @@ template <> struct Bits<float> {
 };
 template <> struct Bits<__half> {
     static constexpr int VEC = 8;
-    static __device__ __forceinline__ float one(const __half* p) { return __half2float(__ushort_as_half(ld_chained(reinterpret_cast<const uint16_t*>(p)))); }
+    static constexpr uint32_t NOTHING = 0xfc00fc00u;
+    static __device__ __forceinline__ float one(const __half* p, bool ok) { return __half2float(__ushort_as_half(ld_chained(reinterpret_cast<const uint16_t*>(p), ok))); }
     static __device__ __forceinline__ void unpack(const uint4& r, float* v) {
         const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
@@ -75,7 +78,8 @@ template <> struct Bits<__half> {
 };
 template <> struct Bits<__nv_bfloat16> {
     static constexpr int VEC = 8;
-    static __device__ __forceinline__ float one(const __nv_bfloat16* p) { return __uint_as_float((uint32_t)ld_chained(reinterpret_cast<const uint16_t*>(p)) << 16); }
+    static constexpr uint32_t NOTHING = 0xff80ff80u;
+    static __device__ __forceinline__ float one(const __nv_bfloat16* p, bool ok) { return __uint_as_float((uint32_t)ld_chained(reinterpret_cast<const uint16_t*>(p), ok) << 16); }
     static __device__ __forceinline__ void unpack(const uint4& r, float* v) {
         const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
@@ -202,33 +206,55 @@ __device__ __forceinline__ Sums sums_of(const Running& a) {
     return r;
 }
 
-// Over classes [lo, hi) of a sample, `threads` threads together: vec(UNROLL times 16 bytes, UNROLL, where the first of them lies, bytes between them),
-// vec1 for single ones behind those, one(pointer) for what is not whole 16 bytes of the row.
-template <typename T, bool VECTORS, int UNROLL, typename VecFn, typename Vec1Fn, typename OneFn>
-__device__ __forceinline__ void over_classes(const T* logits, const DIParams& p, int row, int lo, int hi, int tid, int threads, VecFn vec, Vec1Fn vec1, OneFn one) {
-    constexpr int VEC = Bits<T>::VEC;
-    for (int c = lo / p.units; c * p.units < hi; ++c) {
+// Over classes [lo, hi) of a sample, all THREADS threads of a CTA together: vec(1 or 4 times 16 bytes, where the first of them lies, vectors between them, vectors
+// from the first one to the end) and one(value, where it lies) for what is not whole 16 bytes of the row. Past the end there is minus infinity. BESIDE: a whole row's components are
+// read side by side, each by its share of the threads (1000 rows of 8 x 10654 bf16: 58 us, 80 one behind another). In short rows what a thread reads is on its way before it looks at
+// the first of it; in long ones that would only cost registers (4096 x 131072 bf16: 227 us, 190 without).
+template <typename T, bool VECTORS, int THREADS, bool BESIDE, typename VecFn, typename OneFn>
+__device__ __forceinline__ void over_classes(const T* logits, const DIParams& p, int row, int lo, int hi, VecFn vec, OneFn one) {
+    constexpr int VEC = Bits<T>::VEC, UNROLL = 4;
+    constexpr bool LONG = THREADS == 512;
+    const int threads = BESIDE ? THREADS / p.comps : THREADS, tid = BESIDE ? threadIdx.x % threads : threadIdx.x;
+    for (int c = BESIDE ? threadIdx.x / threads : lo / p.units, end = BESIDE ? c + 1 : (hi + p.units - 1) / p.units; c < end; ++c) {
         const int a = max(lo, c * p.units), b = min(hi, (c + 1) * p.units);
         const T* first = logits + ((size_t)c * p.n + row) * p.units + (a - c * p.units);
         if (!VECTORS) {
-            for (int i = tid; i < b - a; i += threads) one(first + i);
+            for (int i = tid; i < b - a; i += threads) one(Bits<T>::one(first + i, true), first + i);
             continue;
         }
         const int head = min(b - a, (int)((16 - (reinterpret_cast<uintptr_t>(first) & 15)) & 15) / (int)sizeof(T)), body = (b - a - head) / VEC;
-        if (tid < head) one(first + tid);
         const T* start = first + head;
         int v = tid;
-        for (; v + (UNROLL - 1) * threads < body; v += UNROLL * threads) {
-            uint4 raw[UNROLL];
+        if constexpr (LONG) {
+            if (tid < head) one(Bits<T>::one(first + tid, true), first + tid);
+            for (; v + (UNROLL - 1) * threads < body; v += UNROLL * threads) {
+                uint4 raw[UNROLL];
 #pragma unroll
-            for (int u = 0; u < UNROLL; ++u) raw[u] = ld_chained(reinterpret_cast<const uint4*>(start) + v + u * threads);
-            vec(raw, start + (size_t)v * VEC);
+                for (int u = 0; u < UNROLL; ++u) raw[u] = ld_chained(reinterpret_cast<const uint4*>(start) + v + u * threads);
+                vec(raw, start + (size_t)v * VEC, threads, UNROLL * threads);
+            }
+            for (; v < body; v += threads) {
+                const uint4 raw[1] = {ld_chained(reinterpret_cast<const uint4*>(start) + v)};
+                vec(raw, start + (size_t)v * VEC, threads, threads);
+            }
+            for (int i = head + body * VEC + tid; i < b - a; i += threads) one(Bits<T>::one(first + i, true), first + i);
+        } else {
+            const int tail = b - a - head - body * VEC;        // (at most seven values at either end: fewer than the threads)
+            const T* rest = start + body * VEC + tid;
+            const float early = Bits<T>::one(first + tid, tid < head), late = Bits<T>::one(rest, tid < tail);
+            for (; v < body; v += UNROLL * threads) {
+                uint4 raw[UNROLL];
+#pragma unroll
+                for (int u = 0; u < UNROLL; ++u) {
+                    const bool ok = v + u * threads < body;
+                    raw[u] = ld_chained(reinterpret_cast<const uint4*>(start) + v + u * threads, ok);
+                    if (!ok) raw[u] = make_uint4(Bits<T>::NOTHING, Bits<T>::NOTHING, Bits<T>::NOTHING, Bits<T>::NOTHING);
+                }
+                vec(raw, start + (size_t)v * VEC, threads, body - v);
+            }
+            if (tid < head) one(early, first + tid);
+            if (tid < tail) one(late, rest);
         }
-        for (; v < body; v += threads) {
-            const uint4 raw[1] = {ld_chained(reinterpret_cast<const uint4*>(start) + v)};
-            vec1(raw, start + (size_t)v * VEC);
-        }
-        for (int i = head + body * VEC + tid; i < b - a; i += threads) one(first + i);
     }
 }
 
@@ -245,7 +271,7 @@ __device__ __forceinline__ float warp_max(float v) {
 template <typename T>
 __device__ __forceinline__ float logit(const DIParams& p, int row, int cls) {
     const int c = cls / p.units;
-    return Bits<T>::one(static_cast<const T*>(p.logits) + ((size_t)c * p.n + row) * p.units + (cls - c * p.units));
+    return Bits<T>::one(static_cast<const T*>(p.logits) + ((size_t)c * p.n + row) * p.units + (cls - c * p.units), true);
 }
 // The class of the teacher's entry i of a row, or -1 where it names none, and its logit over T.
 template <typename T>
@@ -254,8 +280,25 @@ __device__ __forceinline__ int entry(const DIParams& p, int row, int i, float& t
     const uint2 w = ld_chained(reinterpret_cast<const uint2*>(p.index + at));
     const long long cls = (long long)(((unsigned long long)w.y << 32) | w.x);
     if (cls < 0 || cls >= (long long)p.comps * p.units) { t = -INFINITY; return -1; }
-    t = Bits<T>::one(static_cast<const T*>(p.teacher) + at) * p.inv_temp;
+    t = Bits<T>::one(static_cast<const T*>(p.teacher) + at, true) * p.inv_temp;
     return (int)cls;
+}
+// Has a row's entries (up to four for each lane of a warp) brought near before they are due, and the logits that they name: a short row's time is a chain of such loads.
+template <typename T>
+__device__ __forceinline__ void fetch_entries(const DIParams& p, int row, int lane) {
+    for (int i = lane; i < min(p.entries, 128); i += 32) {
+        const long long at = (long long)row * p.entries + i;
+        ld_chained(reinterpret_cast<const uint2*>(p.index + at));
+        Bits<T>::one(static_cast<const T*>(p.teacher) + at, true);
+    }
+}
+template <typename T>
+__device__ __forceinline__ void fetch_their_logits(const DIParams& p, int row, int lane) {
+    for (int i = lane; i < min(p.entries, 128); i += 32) {
+        float x;
+        const int cls = entry<T>(p, row, i, x);
+        if (cls >= 0) logit<T>(p, row, cls);
+    }
 }
 __device__ __forceinline__ int label_of(const DIParams& p, int row) {
     if (!p.labels) return -1;
@@ -264,8 +307,11 @@ __device__ __forceinline__ int label_of(const DIParams& p, int row) {
     return cls < 0 || cls >= (long long)p.comps * p.units ? -1 : (int)cls;
 }
 
-template <typename T, bool VECTORS, int KIND, int THREADS>
-__global__ void __launch_bounds__(THREADS) distill_fwd_kernel(const DIParams p) {
+// CTAs of a size that an SM is to hold: long rows (512 threads each) need 1536 threads with four vectors on their way, short ones are latency after latency
+constexpr int di_ctas(int threads) { return threads == 512 ? 3 : (threads == 128 ? 8 : (threads == 64 ? 20 : 32)); }
+
+template <typename T, bool VECTORS, int KIND, int THREADS, bool BESIDE>
+__global__ void __launch_bounds__(THREADS, di_ctas(THREADS)) distill_fwd_kernel(const DIParams p) {
     constexpr int WARPS = THREADS / 32;
     __shared__ Sums words[WARPS];
     __shared__ Sums whole;
@@ -277,10 +323,17 @@ __global__ void __launch_bounds__(THREADS) distill_fwd_kernel(const DIParams p) 
     chain_wait();
     chain_next();
     Running run = {-INFINITY, pair(0.f, 0.f), pair(0.f, 0.f)};
-    over_classes<T, VECTORS, 4>(static_cast<const T*>(p.logits), p, row, lo, hi, t, THREADS,
-        [&](const uint4 (&raw)[4], const T*) { add<KIND, T, 4>(run, raw, c_temp); },
-        [&](const uint4 (&raw)[1], const T*) { add<KIND, T, 1>(run, raw, c_temp); },
-        [&](const T* at) { add<KIND>(run, Bits<T>::one(at), c_temp); });
+    const bool last = split == 0 && warp == 0;                 // the warp that writes the row's loss
+    constexpr bool LONG = THREADS == 512;
+    int label = -1;
+    float labelled = 0.f;
+    if (!LONG && KIND != DI_SOFT && last) label = label_of(p, row);
+    if (!LONG && KIND != DI_HARD && last) fetch_entries<T>(p, row, lane);
+    over_classes<T, VECTORS, THREADS, BESIDE>(static_cast<const T*>(p.logits), p, row, lo, hi,
+        [&](const auto& raw, const T*, int, int) { add<KIND, T>(run, raw, c_temp); },
+        [&](float v, const T*) { add<KIND>(run, v, c_temp); });
+    if (!LONG && label >= 0) labelled = logit<T>(p, row, label);
+    if (!LONG && KIND != DI_HARD && last) fetch_their_logits<T>(p, row, lane);
     Sums a = sums_of<KIND>(run);
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
@@ -320,14 +373,15 @@ __global__ void __launch_bounds__(THREADS) distill_fwd_kernel(const DIParams p) 
         }
         cluster_sync_all();                       // nobody leaves while its sums are read
     }
-    if (split != 0 || warp != 0) return;
+    if (!last) return;
     a.m = __shfl_sync(0xffffffffu, a.m, 0); a.s1 = __shfl_sync(0xffffffffu, a.s1, 0); a.st = __shfl_sync(0xffffffffu, a.st, 0);
     const bool none = a.m == -INFINITY && a.s1 == 0.f && a.st == 0.f;    // no class left: the row counts for nothing
     float loss = 0.f;
-    if (KIND != DI_SOFT && !none) {
-        const int cls = label_of(p, row);
-        if (cls >= 0) loss = (1.f - p.alpha) * (logf(a.s1) - (logit<T>(p, row, cls) - a.m));
+    if (LONG && KIND != DI_SOFT && !none) {
+        label = label_of(p, row);
+        if (label >= 0) labelled = logit<T>(p, row, label);
     }
+    if (label >= 0 && !none) loss = (1.f - p.alpha) * (logf(a.s1) - (labelled - a.m));
     bool any = false;
     if (KIND != DI_HARD && !none) {
         float peak = -INFINITY;
@@ -358,11 +412,12 @@ __global__ void __launch_bounds__(THREADS) distill_fwd_kernel(const DIParams p) 
     }
 }
 
-template <typename T, bool VECTORS, int KIND, int THREADS>
-__global__ void __launch_bounds__(THREADS) distill_bwd_kernel(const DIParams p) {
-    extern __shared__ float shared[];                          // [entries] classes of the teacher's entries, [entries] probabilities
+template <typename T, bool VECTORS, int KIND, int THREADS, bool BESIDE>
+__global__ void __launch_bounds__(THREADS, di_ctas(THREADS)) distill_bwd_kernel(const DIParams p) {
+    extern __shared__ __align__(16) float shared[];            // [places] classes of the teacher's entries, [places] probabilities; places: entries in whole fours
+    const int places = (p.entries + 3) & ~3;
     int* classes_of = reinterpret_cast<int*>(shared);
-    float* probs = shared + p.entries;
+    float* probs = shared + places;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     // from the last row on: the forward pass has left the last rows in L2
     const int back = blockIdx.x / p.splits, row = p.n - 1 - back, split = blockIdx.x - back * p.splits;
@@ -373,6 +428,7 @@ __global__ void __launch_bounds__(THREADS) distill_bwd_kernel(const DIParams p) 
     chain_next();
     const float g = ld_chained(p.grad + row), m = ld_chained(p.stats + row), s1 = ld_chained(p.stats + p.n + row), st = ld_chained(p.stats + 2 * p.n + row);
     const int label = KIND == DI_SOFT ? -1 : label_of(p, row);
+    if (THREADS < 512 && KIND != DI_HARD && warp == 0) fetch_entries<T>(p, row, lane);
     const bool none = m == -INFINITY, soft = KIND != DI_HARD && st != INFINITY;
     const float c1 = label >= 0 && !none ? g * (1.f - p.alpha) / s1 : 0.f, ct = soft && !none ? g * p.alpha * p.temp / st : 0.f;
     const float base = none ? 0.f : m;
@@ -407,13 +463,14 @@ __global__ void __launch_bounds__(THREADS) distill_bwd_kernel(const DIParams p) 
         }
         *reinterpret_cast<uint4*>(at) = Bits<T>::pack(v);
     };
-    over_classes<T, VECTORS, 4>(in, p, row, lo, hi, t, THREADS,
-        [&](const uint4 (&raw)[4], const T* at) {
+    over_classes<T, VECTORS, THREADS, BESIDE>(in, p, row, lo, hi,
+        [&](const auto& raw, const T* at, int step, int left) {
+            constexpr int VECTORS_AT_ONCE = sizeof(raw) / sizeof(uint4);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) values(raw[u], out + (at - in) + (size_t)u * THREADS * Bits<T>::VEC);
+            for (int u = 0; u < VECTORS_AT_ONCE; ++u)
+                if (u * step < left) values(raw[u], out + (at - in) + (size_t)u * step * Bits<T>::VEC);
         },
-        [&](const uint4 (&raw)[1], const T* at) { values(raw[0], out + (at - in)); },
-        [&](const T* at) { Bits<T>::put(out + (at - in), value(Bits<T>::one(at))); });
+        [&](float v, const T* at) { Bits<T>::put(out + (at - in), value(v)); });
     // the classes of the label and of the teacher's entries once more, with their own terms
     if (soft && !none && warp == 0) {
         float peak = -INFINITY;
@@ -428,6 +485,7 @@ __global__ void __launch_bounds__(THREADS) distill_bwd_kernel(const DIParams p) 
         for (int i = lane; i < p.entries; i += 32) { const float e = classes_of[i] >= 0 ? ex2((probs[i] - peak) * LOG2E) : 0.f; probs[i] = e; total += e; }
         total = warp_sum(total);
         for (int i = lane; i < p.entries; i += 32) probs[i] /= total;
+        if (lane < places - p.entries) { classes_of[p.entries + lane] = -1; probs[p.entries + lane] = 0.f; }
     }
     __syncthreads();
     if (none) return;
@@ -435,9 +493,17 @@ __global__ void __launch_bounds__(THREADS) distill_bwd_kernel(const DIParams p) 
     for (int i = t; i <= entries; i += THREADS) {
         const int cls = i < entries ? classes_of[i] : label;
         if (cls < lo || cls >= hi) continue;
+        const float z = logit<T>(p, row, cls);
         float prob = 0.f;
-        for (int j = 0; j < entries; ++j) prob += classes_of[j] == cls ? probs[j] : 0.f;      // (a class may be named twice; all who write it write the same)
-        float v = value(logit<T>(p, row, cls)) - g * p.alpha * p.temp * prob;
+        for (int j = 0; j < entries; j += 4) {                    // (a class may be named twice; all who write it write the same)
+            const int4 c4 = *reinterpret_cast<const int4*>(classes_of + j);
+            const float4 p4 = *reinterpret_cast<const float4*>(probs + j);
+            prob += c4.x == cls ? p4.x : 0.f;
+            prob += c4.y == cls ? p4.y : 0.f;
+            prob += c4.z == cls ? p4.z : 0.f;
+            prob += c4.w == cls ? p4.w : 0.f;
+        }
+        float v = value(z) - g * p.alpha * p.temp * prob;
         if (cls == label) v -= g * (1.f - p.alpha);
         const int c = cls / p.units;
         Bits<T>::put(out + ((size_t)c * p.n + row) * p.units + (cls - c * p.units), v);
@@ -484,13 +550,21 @@ template <typename T, bool VECTORS, int KIND>
 cudaError_t launch_kind(bool forward, const DIParams& p, cudaStream_t s) {
     const long long per = (long long)p.comps * p.units / p.splits;
     const unsigned grid = (unsigned)p.n * (unsigned)p.splits;
-    if (forward) {
-        if (per <= 4096) return launch_clusters(p.splits, true, distill_fwd_kernel<T, VECTORS, KIND, 128>, grid, 128, 0, s, p);
-        return launch_clusters(p.splits, true, distill_fwd_kernel<T, VECTORS, KIND, 512>, grid, 512, 0, s, p);
-    }
-    const size_t smem = (size_t)p.entries * 8;
-    if (per <= 4096) return launch_chained(distill_bwd_kernel<T, VECTORS, KIND, 128>, grid, 128, smem, s, p);
-    return launch_chained(distill_bwd_kernel<T, VECTORS, KIND, 512>, grid, 512, smem, s, p);
+    const size_t smem = forward ? 0 : (size_t)((p.entries + 3) & ~3) * 8;
+    auto launch = [&](auto threads, auto beside) {
+        constexpr int THREADS = decltype(threads)::value;
+        constexpr bool BESIDE = decltype(beside)::value;
+        auto kernel = forward ? distill_fwd_kernel<T, VECTORS, KIND, THREADS, BESIDE> : distill_bwd_kernel<T, VECTORS, KIND, THREADS, BESIDE>;
+        return launch_clusters(forward ? p.splits : 1, true, kernel, grid, THREADS, smem, s, p);
+    };
+    const std::true_type beside;
+    // A short row is a chain of latencies, and its threads count for nothing but the rows that an SM can hold: forward 4030 x 103 f32 8.5 us with a warp each, 17 with 128
+    // threads; 2637 x (8 x 189) bf16 11.8 us with 64, 16 with 128. (A component's share is eight threads at least.)
+    if (per <= 512 && p.comps <= 4) return launch(std::integral_constant<int, 32>(), beside);
+    if (per <= 2048) return launch(std::integral_constant<int, 64>(), beside);
+    if (per <= 4096 && p.splits == 1) return launch(std::integral_constant<int, 128>(), beside);
+    if (p.comps > 1 && p.splits == 1) return launch(std::integral_constant<int, 512>(), beside);
+    return launch(std::integral_constant<int, 512>(), std::false_type());
 }
 template <typename T, bool VECTORS>
 cudaError_t launch_any(bool forward, int kind, const DIParams& p, cudaStream_t s) {
