@@ -2,7 +2,8 @@
 
 The package holds the CUDA backend (``csrc/``: hand-written sm_100a kernels behind a C ABI declared in
 ``include/phoenix_core_b200.h``), the C++ operator layer mirroring ``upstride::conv2DFwd`` & co.
-(``cpp/``), and this Python host layer used by the tests, the benchmark and the data-parallel harness.
+(``cpp/``), and this Python host layer used by the tests, the benchmark and the data-parallel harness. Beside the
+reference's operators it has those of a dense residual block: the dense layer in 8 bits, its norms, a distillation loss.
 """
 from . import _lib
 from .descriptors import (Algebra, Conv2DBwdDescriptor, Conv2DFwdDescriptor, DataFormat, DenseBwdDescriptor,

@@ -752,12 +752,12 @@ int pcb_qdense8_bwd(const pcb_dense_desc* desc, const void* x, const void* w8, c
     const Q8Target x_cols = {ws + at.x_cols, reinterpret_cast<uint32_t*>(ws + at.x_col_words)};
     if ((rc = q8_quantize_backward(desc->dtype, g.nc, g.Nb, g.Ci, g.Co, x, dy, x_cols, dy_rows, dy_cols, status, st)) != PCB_OK) return rc;
     const Q8Operand a = {x_cols.values, x_cols.words, q8_pitch(g.Ci), 0, 0, 0, 1}, b = {dy_cols.values, dy_cols.words, q8_pitch(g.Co), 0, 0, 0, 1};
-    rc = q8_product(g, Q8Product{PASS_BWD_FILTER, 0, g.Ci, g.Co, g.Nb, a, b, dw, desc->dtype, nullptr, status}, st);
-    if (rc != PCB_OK || !need_dx) return rc;
+    const Q8Product of_filter = {PASS_BWD_FILTER, 0, g.Ci, g.Co, g.Nb, a, b, dw, desc->dtype, nullptr, status};
+    if (!need_dx) return q8_product(g, of_filter, st);
     const Q8Operand tokens = {dy_rows.values, dy_rows.words, q8_pitch(g.Co), 0, 0, 0, 0}, filter = dense8_filter(g, w8, w8_scales, false);
     Q8Product q = {PASS_BWD_DATA, q8_swapped(g.Nb) ? 1 : 0, g.Nb, g.Ci, g.Co, tokens, filter, dx, desc->dtype, nullptr, status};
     if (q.swapped) { q.m = g.Ci; q.n = g.Nb; q.a = filter; q.b = tokens; }
-    return q8_product(g, q, st);
+    return q8_two_products(g, of_filter, q, st);
 }
 
 }  // extern "C"

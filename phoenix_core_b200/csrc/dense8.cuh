@@ -48,6 +48,8 @@ int q8_quantize_backward(int dtype, int comps, int rows, int x_cols, int dy_cols
                          int* status_to_clear, cudaStream_t stream);
 int q8_quantize_blocks(int dtype, int comps, int rows, int cols, const void* x, uint8_t* values, uint8_t* scales, cudaStream_t stream);
 int q8_product(const Geom& g, const Q8Product& p, cudaStream_t stream);
+// The two gradients of a backward call, in one launch or two.
+int q8_two_products(const Geom& g, const Q8Product& first, const Q8Product& second, cudaStream_t stream);
 // Whether a forward or backward-data product of that many tokens takes the filter as operand A.
 bool q8_swapped(int tokens);
 // Whether the product quantises that many tokens itself.

@@ -9,6 +9,7 @@ import torch
 import dense8_reference as ref
 import phoenix_core_b200 as pcb
 from phoenix_core_b200.autograd import DistillFunction, QDense8, QDense8Function, ResidualNormFunction
+from test_gpu_dense8 import check as check_dense
 from test_gpu_dense8 import make as make_dense
 from test_gpu_dense8 import run as run_dense
 from test_gpu_distill import check as check_distill
@@ -86,6 +87,18 @@ def test_dense8_tensors_start_anywhere(dtype, n, i, o):
         torch.cuda.synchronize()
         for k, want in dict(y=y, dw=dw, dx=dx).items():
             assert torch.equal(out[k][1], want) and guarded(out[k][0], places, want.numel()), k
+
+
+@pytest.mark.parametrize("n,i,o", [(40, 128, 136), (200, 130, 257), (600, 512, 40)])
+@pytest.mark.parametrize("algebra", ["quaternion", "real"])
+def test_dense8_filter_gradient_alone(algebra, n, i, o):
+    """The filter's gradient without the input's is the same sum, in this call's own cut."""
+    dim, x, w, _, dy = make_dense(algebra, "io", "f32", n, i, o)
+    _, _, dw, dx = run_dense(algebra, "io", x, w, None, dy, need_dx=False)
+    assert dx is None
+    w8 = ref.quantized(w.double().reshape(dim, *w.shape[-2:]), 128, 128)
+    _, _, want, size = ref.backward(dim, x.double().reshape(dim, n, i), w8, dy.double().reshape(dim, n, o))
+    check_dense(dw, want, size, dim * n, torch.float32, "dw")
 
 
 def test_no_samples():
