@@ -119,7 +119,8 @@ __device__ __forceinline__ void copy_scales(uint32_t tmem, uint32_t smem_addr) {
     if constexpr (PAIR) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
     else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
 }
-// The scales of the odd CTA are written by its own threads: the arrival that announces them in the even CTA releases at cluster scope, the wait acquires there.
+// The scales of the odd CTA are written by its own threads: the arrival that announces them in the even CTA releases at cluster scope (what its thread has waited for included), the
+// wait acquires there.
 __device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
@@ -349,7 +350,7 @@ __global__ void __launch_bounds__(D8_THREADS, 1) dense8_kernel(const __grid_cons
     if (t == 0) {
         *status = 0;
         for (int s = 0; s < C::STAGES; ++s) { mbar_init(full + 8 * s, RAW ? 2 : 1); mbar_init(empty + 8 * s, 1); }
-        for (int s = 0; s < D8_SF_STAGES; ++s) { mbar_init(sf_full + 8 * s, RAW ? 5 : 2 * C::CTAS); mbar_init(sf_empty + 8 * s, 1); }
+        for (int s = 0; s < D8_SF_STAGES; ++s) { mbar_init(sf_full + 8 * s, RAW ? 5 : (PAIR && rank == 0 ? 3 : 2)); mbar_init(sf_empty + 8 * s, 1); }
         for (int s = 0; s < C::ACC; ++s) { mbar_init(acc_full + 8 * s, 1); mbar_init(acc_empty + 8 * s, RAW ? 4 : D8_EPI_WARPS * C::CTAS); }
         fence_barrier_init();
     }
@@ -420,6 +421,16 @@ __global__ void __launch_bounds__(D8_THREADS, 1) dense8_kernel(const __grid_cons
             }
         }
     } else if (warp == 1 && rank != 0) {
+        // The odd CTA's word to the even one that its scales are laid out. (The release at cluster scope waits for every load that its thread has under way: in the warps
+        // that load the scales it took 1000 to 1800 clocks a group.)
+        int q = 0, left = 0;
+        uint32_t par = 0;
+        for (int i = first; i < tiles; i += stride) left += end_of(args.p[args.product(i)]) - g_begin;
+        for (; left > 0 && warp_wait_bounded(sf_full + 8 * q, par, status, ST_D8_SCALES); --left) {
+            if (elect_one()) mbar_arrive_release_cluster(map_to_cta(sf_full + 8 * q, 0));
+            __syncwarp();
+            if (++q == D8_SF_STAGES) { q = 0; par ^= 1u; }
+        }
     } else if (warp == 1) {
         const bool elected = elect_one();              // one lane issues and commits throughout
         int s = 0, q = 0, acc = 0;
@@ -572,10 +583,7 @@ __global__ void __launch_bounds__(D8_THREADS, 1) dense8_kernel(const __grid_cons
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (elect_one()) {
-                    if constexpr (PAIR) mbar_arrive_release_cluster(map_to_cta(sf_full + 8 * q, 0));
-                    else mbar_arrive(sf_full + 8 * q);
-                }
+                if (elect_one()) mbar_arrive(sf_full + 8 * q);
                 __syncwarp();
                 if (++q == D8_SF_STAGES) { q = 0; par ^= 1u; }
             }
