@@ -504,24 +504,26 @@ __global__ void __launch_bounds__(D8_THREADS, 1) dense8_kernel(const __grid_cons
         const bool b_side = warp == 3;
         bool blocks = false;
         const uint8_t* scales = nullptr;
-        int bk = 0, bm = 0, bc = 0, extent = 0, product = 0;
+        int bk = 0, bm = 0, extent = 0, product = 0;
+        uint32_t per_group = 0, per_comp = 0;                    // bytes (fewer than 2^31: a word for 128 values, and those have fewer)
         auto operand = [&]() {
             const D8Params& p = args.p[product];
             blocks = b_side ? p.b_blocks : p.a_blocks;
             scales = b_side ? p.b_scales : p.a_scales;
-            bk = b_side ? p.b_bk : p.a_bk; bm = b_side ? p.b_bm : p.a_bm; bc = b_side ? p.b_bc : p.a_bc; extent = b_side ? p.n : p.m;
+            bk = b_side ? p.b_bk : p.a_bk; bm = b_side ? p.b_bm : p.a_bm; extent = b_side ? p.n : p.m;
+            per_group = blocks ? 4u * bk : 4u * extent;
+            per_comp = blocks ? (uint32_t)(b_side ? p.b_bc : p.a_bc) : per_group * p.groups;
         };
         operand();
         constexpr int SETS = BN > 128 ? 2 : 1;                   // sets of 128 rows of B
         struct Words { uint32_t w[SETS][4]; bool blocks; };
         int tile = first, c = 0, row0[SETS];
         const uint8_t* at[SETS];                                 // where this lane's words (blocks: byte) of the walk's group lie
+        const uint8_t* origin[SETS];                             // the same of component 0 and group 0
         auto aim = [&]() {
-            const int comp = SWAP == b_side ? w.first : w.second;
+            const uint32_t comp = SWAP == b_side ? w.first : w.second;
 #pragma unroll
-            for (int h = 0; h < SETS; ++h)
-                at[h] = blocks ? scales + (size_t)comp * bc + (size_t)(row0[h] / 128) * bm + (size_t)(w.group * 4 + (lane & 3)) * bk
-                               : scales + (((size_t)comp * args.p[product].groups + w.group) * extent + row0[h] + lane) * 4;
+            for (int h = 0; h < SETS; ++h) at[h] = origin[h] + (size_t)(comp * per_comp + (uint32_t)w.group * per_group);
         };
         auto begin = [&]() {
             if (tile >= tiles) return;
@@ -531,6 +533,8 @@ __global__ void __launch_bounds__(D8_THREADS, 1) dense8_kernel(const __grid_cons
             d8_tile(p, args.local(tile), c, mt, nt);
 #pragma unroll
             for (int h = 0; h < SETS; ++h) row0[h] = b_side ? nt * BN + h * 128 : mt * C::M + (int)rank * D8_BM;
+#pragma unroll
+            for (int h = 0; h < SETS; ++h) origin[h] = scales + (blocks ? (row0[h] / 128) * bm + (lane & 3) * bk : (row0[h] + lane) * 4);
             w.start(p, c, g_begin, end_of(p), j_begin);
             aim();
         };
@@ -546,17 +550,14 @@ __global__ void __launch_bounds__(D8_THREADS, 1) dense8_kernel(const __grid_cons
                 if (blocks) {
                     // (a set of 128 rows that starts on a multiple of 128 lies in one block: lane e loads the byte of block e of the reduction)
                     out.w[h][0] = row0[h] < extent && w.group * 4 + (lane & 3) < p.chunks ? *reinterpret_cast<const volatile uint8_t*>(at[h]) : 127u;
-                    at[h] += 4 * (size_t)bk;
                 } else {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) out.w[h][i] = ld_chained(reinterpret_cast<const uint32_t*>(at[h]) + 32 * i, row0[h] + lane + 32 * i < extent);
-                    at[h] += 4 * (size_t)extent;
                 }
             }
-            const int j = w.j;
             w.step(p, c);
             if (w.left == 0) { tile += stride; begin(); }
-            else if (w.j != j) aim();
+            else aim();
         };
         int q = 0;
         uint32_t par = 1;
