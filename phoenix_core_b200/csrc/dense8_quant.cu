@@ -98,10 +98,11 @@ struct QTParams {
     uint8_t *row_values, *col_values;            // QT_BLOCKS: row_values; with QT_ROWS and QT_COLS either may be null
     uint32_t *row_words, *col_words;             // QT_BLOCKS: row_words is the byte array
     int row_groups, col_groups;                  // groups of four blocks along the columns (row scales) and along the rows (column scales)
+    int vectors;                                 // rows start on 16 bytes and end on them
 };
 
 // Thread t holds columns 8 * (t % 16) .. + 7 of rows (t / 16) + 32 * i: the lanes of half a warp hold one row.
-// VEC: rows start on 16 bytes and are whole vectors. A launch takes the tiles of one tensor or of two, one behind the other; status: cleared by the first CTA, or null.
+// VEC: every tensor's rows are whole eights and start on 16 bytes. A launch takes the tiles of one tensor or of two, one behind the other; status: cleared by the first CTA, or null.
 template <typename T, int MODE, bool VEC>
 __global__ void __launch_bounds__(QT_THREADS, sizeof(T) == 4 ? 1 : 2) quantize_tile_kernel(const __grid_constant__ QTParams p0, const __grid_constant__ QTParams p1, int* status) {
     typedef Eight<T> E;
@@ -126,6 +127,19 @@ __global__ void __launch_bounds__(QT_THREADS, sizeof(T) == 4 ? 1 : 2) quantize_t
             for (int i = 0; i < QT_PER; ++i) {
                 if (first_row + QT_STEP * i < p.rows && valid > 0) v[i].load(src + (size_t)QT_STEP * i * p.cols);
                 else v[i].zero();
+            }
+        } else if (p.vectors) {
+            // (one tensor of the launch may be so without the other; an fp32 row may end in the middle of an eight)
+#pragma unroll
+            for (int i = 0; i < QT_PER; ++i) {
+                const uint4* at = reinterpret_cast<const uint4*>(src + (size_t)QT_STEP * i * p.cols);
+                const bool live = first_row + QT_STEP * i < p.rows;
+                const uint4 a = ld_chained(at, live && valid > 0);
+                v[i].w[0] = a.x; v[i].w[1] = a.y; v[i].w[2] = a.z; v[i].w[3] = a.w;
+                if constexpr (sizeof(T) == 4) {
+                    const uint4 b = ld_chained(at + 1, live && valid > 4);
+                    v[i].w[4] = b.x; v[i].w[5] = b.y; v[i].w[6] = b.z; v[i].w[7] = b.w;
+                }
             }
         } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -266,7 +280,7 @@ __global__ void __launch_bounds__(QT_THREADS, sizeof(T) == 4 ? 1 : 2) quantize_t
 
 template <typename T, int MODE>
 cudaError_t launch_tile(const QTParams& p0, const QTParams& p1, int* status, cudaStream_t stream) {
-    auto vectors = [](const QTParams& p) { return p.tiles == 0 || (p.cols % 8 == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0); };
+    auto vectors = [](const QTParams& p) { return p.tiles == 0 || (p.vectors && p.cols % 8 == 0); };
     const unsigned grid = (unsigned)p0.tiles + (unsigned)p1.tiles;
     return vectors(p0) && vectors(p1) ? launch_chained(quantize_tile_kernel<T, MODE, true>, grid, QT_THREADS, 0, stream, p0, p1, status)
                                       : launch_chained(quantize_tile_kernel<T, MODE, false>, grid, QT_THREADS, 0, stream, p0, p1, status);
@@ -278,25 +292,25 @@ int launch_typed(int dtype, const QTParams& p0, const QTParams& p1, int* status,
     else PCB_CUDA_TRY((launch_tile<__nv_bfloat16, MODE>(p0, p1, status, stream)));
     return PCB_OK;
 }
-QTParams tile_params(int comps, int rows, int cols, const void* x, Q8Target by_rows, Q8Target by_cols) {
+QTParams tile_params(int dtype, int comps, int rows, int cols, const void* x, Q8Target by_rows, Q8Target by_cols) {
     const int row_blocks = q8_blocks(rows), col_blocks = q8_blocks(cols);
     return {x, rows, cols, q8_pitch(cols), row_blocks, col_blocks, comps * row_blocks * col_blocks, by_rows.values, by_cols.values, by_rows.words, by_cols.words,
-            q8_groups(cols), q8_groups(rows)};
+            q8_groups(cols), q8_groups(rows), cols * dtype_size(dtype) % 16 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0};
 }
 
 }  // namespace
 
 int q8_quantize_rows(int dtype, int comps, int rows, int cols, const void* x, Q8Target by_rows, int* status, cudaStream_t stream) {
-    return launch_typed<QT_ROWS>(dtype, tile_params(comps, rows, cols, x, by_rows, Q8Target{}), QTParams{}, status, stream);
+    return launch_typed<QT_ROWS>(dtype, tile_params(dtype, comps, rows, cols, x, by_rows, Q8Target{}), QTParams{}, status, stream);
 }
 
 int q8_quantize_backward(int dtype, int comps, int rows, int x_cols, int dy_cols, const void* x, const void* dy, Q8Target x_by_cols, Q8Target dy_by_rows, Q8Target dy_by_cols, int* status,
                          cudaStream_t stream) {
-    return launch_typed<QT_ROWS | QT_COLS>(dtype, tile_params(comps, rows, dy_cols, dy, dy_by_rows, dy_by_cols), tile_params(comps, rows, x_cols, x, Q8Target{}, x_by_cols), status, stream);
+    return launch_typed<QT_ROWS | QT_COLS>(dtype, tile_params(dtype, comps, rows, dy_cols, dy, dy_by_rows, dy_by_cols), tile_params(dtype, comps, rows, x_cols, x, Q8Target{}, x_by_cols), status, stream);
 }
 
 int q8_quantize_blocks(int dtype, int comps, int rows, int cols, const void* x, uint8_t* values, uint8_t* scales, cudaStream_t stream) {
-    return launch_typed<QT_BLOCKS>(dtype, tile_params(comps, rows, cols, x, Q8Target{values, reinterpret_cast<uint32_t*>(scales)}, Q8Target{}), QTParams{}, nullptr, stream);
+    return launch_typed<QT_BLOCKS>(dtype, tile_params(dtype, comps, rows, cols, x, Q8Target{values, reinterpret_cast<uint32_t*>(scales)}, Q8Target{}), QTParams{}, nullptr, stream);
 }
 
 }  // namespace pcb
