@@ -8,8 +8,9 @@
 //
 // A CTA takes a tile of 128 x 128 values in registers, 4 x 8 per thread: the blocks of 1 x 128, of 128 x 1 and of 128 x 128 all lie within it, so the
 // backward pass reads dy once for both of its products. The tile stays as it was loaded (as fp32 it took 176 registers, and one CTA per SM moved 2.2 TB/s);
-// maxima are taken over the bits of the magnitudes, two 16-bit values at a time. Two CTAs of 512 threads on an SM, whose loads and stores then lie beside each other (fp32 too, though
-// some words spill: 2420 x 8096 22 us, 27 with one). 8192 x 4096 bf16: by rows 24 us (4.2 TB/s read and written), in both orientations with x beside it 54; issue slots and memory.
+// maxima are taken over the bits of the magnitudes, two 16-bit values at a time. Three CTAs of 512 threads on an SM (fp32, and rows that start anywhere, whose words take registers: two), whose loads and stores lie beside each other, though
+// some words spill for it. 8192 x 4096 bf16: by rows 23.5 us (4.3 TB/s read and written), both orientations of one and the columns of another 46 (54 with two CTAs); 2420 x 8096 fp32 by rows
+// 21.5 (26.5 with one). What is left is latency: a CTA's loads are over before its stores begin.
 #include "dense8.cuh"
 #include "e4m3.cuh"
 #include "tc_common.cuh"
@@ -105,7 +106,7 @@ struct QTParams {
 // Thread t holds columns 8 * (t % 16) .. + 7 of rows (t / 16) + 32 * i: the lanes of half a warp hold one row.
 // VEC: every tensor's rows are whole eights and start on 16 bytes. A launch takes the tiles of one tensor or of two, one behind the other; status: cleared by the first CTA, or null.
 template <typename T, int MODE, bool VEC>
-__global__ void __launch_bounds__(QT_THREADS, 2) quantize_tile_kernel(const __grid_constant__ QTParams p0, const __grid_constant__ QTParams p1, int* status) {
+__global__ void __launch_bounds__(QT_THREADS, sizeof(T) == 2 && VEC ? 3 : 2) quantize_tile_kernel(const __grid_constant__ QTParams p0, const __grid_constant__ QTParams p1, int* status) {
     typedef Eight<T> E;
     __shared__ uint32_t col_max[QT_WARPS][16 * E::WORDS];
     __shared__ uint32_t warp_max[QT_WARPS];
