@@ -59,6 +59,10 @@ class Device:
             return dev
 
     def requestWorkspace(self, nbytes):
+        """The current stream's workspace. A call that is being captured gets one of its own from the graph's memory, in the order of the captured
+        stream as any other tensor of the capture: graphs share none with each other, nor with what the stream runs later."""
+        if _capturing():
+            return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=torch.device("cuda", self.index))
         key = _raw_stream(self.index)
         ws = self.workspaces.get(key)
         if ws is None or ws.numel() < nbytes:
@@ -123,6 +127,7 @@ def _check_tensor(t, name, dtype=None, shape=None):
         raise ValueError("%s shape mismatch: %s vs expected %s" % (name, tuple(t.shape), tuple(shape)))
 
 
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None) or (lambda: False)       # (absent from a torch without CUDA, which captures nothing)
 _get_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 

@@ -188,6 +188,49 @@ def test_captured_and_replayed():
         assert all(torch.equal(a, b) for a, b in zip(eager, want[0]))
 
 
+def capture(p, stream):
+    with torch.cuda.stream(stream):
+        for _ in range(2):
+            autograd_step(p)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        out = autograd_step(p)
+    return graph, out
+
+
+def test_two_graphs_of_one_stream_at_once():
+    """Two steps captured one after the other on the same stream and replayed beside each other on two others."""
+    problems = [Problem(11, n=300), Problem(12, n=300)]
+    want = [autograd_step(p) for p in problems]
+    stream = torch.cuda.Stream()
+    graphs = [capture(p, stream) for p in problems]
+    streams = [torch.cuda.Stream() for _ in problems]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for (graph, _), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    for (_, out), w in zip(graphs, want):
+        assert all(torch.equal(a, b) for a, b in zip(out, w))
+
+
+def test_a_graph_outlives_the_workspace_of_its_stream():
+    """A larger eager call on the capture's stream replaces the stream's workspace; what takes its memory is left alone by a replay."""
+    p, larger = Problem(13, n=42), Problem(14, n=2001)
+    want = autograd_step(p)
+    stream = torch.cuda.Stream()
+    graph, out = capture(p, stream)
+    with torch.cuda.stream(stream):
+        autograd_step(larger)
+        others = [torch.full((1 << 20,), 7, dtype=torch.uint8, device="cuda") for _ in range(8)]
+    torch.cuda.synchronize()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all((t == 7).all() for t in others) and all(torch.equal(a, b) for a, b in zip(out, want))
+
+
 def test_two_streams_at_once():
     problems = [Problem(7, n=300), Problem(8, n=90)]
     want = [autograd_step(p) for p in problems]
