@@ -70,9 +70,11 @@ __device__ __forceinline__ float row_sum(float v, float* words, int& turn) {
     const int warp = (threadIdx.x >> 5) % WPR, lane = threadIdx.x & 31;
     if (lane == 0) words[turn * WPR + warp] = v;
     row_sync<WPR>();
-    v = words[turn * WPR + (lane & (WPR - 1))];
+    constexpr int SPREAD = WPR <= 2 ? 2 : (WPR <= 4 ? 4 : (WPR <= 8 ? 8 : 16));      // lanes that the words are spread over, in a power of two
+    const int word = lane & (SPREAD - 1);
+    v = SPREAD == WPR || word < WPR ? words[turn * WPR + word] : 0.f;
 #pragma unroll
-    for (int o = WPR / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    for (int o = SPREAD / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     turn ^= 1;
     return v;
 }
@@ -735,6 +737,7 @@ template <typename T, int VEC, bool ALIGNED>
 cudaError_t fwd_any(const RNParams& p, const RNShape& k, cudaStream_t s) {
     if (k.warps == 1) return k.values == 8 ? fwd_launch<T, VEC, ALIGNED, 8, 1, 16>(p, s) : fwd_launch<T, VEC, ALIGNED, 32, 1, 12>(p, s);
     if (k.warps == 4) return k.values == 16 ? fwd_launch<T, VEC, ALIGNED, 16, 4, 4>(p, s) : fwd_launch<T, VEC, ALIGNED, 32, 4, 3>(p, s);
+    if (k.warps == 5) return fwd_launch<T, VEC, ALIGNED, 16, 5, 3>(p, s);
     return k.warps == 8 ? fwd_launch<T, VEC, ALIGNED, 32, 8, 1>(p, s) : fwd_launch<T, VEC, ALIGNED, 32, 16, 1>(p, s);
 }
 template <typename T, int VEC, bool ALIGNED, int EPT, int WPR, int ROWS, int GATE>
@@ -751,7 +754,10 @@ template <typename T, int VEC, bool ALIGNED>
 cudaError_t bwd_any(const RNParams& p, const RNPlan& q, cudaStream_t s) {
     switch (q.shape.warps) {
         case 1: return q.shape.values == 8 ? bwd_launch<T, VEC, ALIGNED, 8, 1, 16>(p, q, s) : bwd_launch<T, VEC, ALIGNED, 16, 1, 12>(p, q, s);
+        case 2: return bwd_launch<T, VEC, ALIGNED, 16, 2, 6>(p, q, s);
+        case 3: return bwd_launch<T, VEC, ALIGNED, 16, 3, 4>(p, q, s);
         case 4: return bwd_launch<T, VEC, ALIGNED, 16, 4, 3>(p, q, s);
+        case 5: return bwd_launch<T, VEC, ALIGNED, 16, 5, 3>(p, q, s);
         case 8: return bwd_launch<T, VEC, ALIGNED, 16, 8, 2>(p, q, s);
         default: return bwd_launch<T, VEC, ALIGNED, 16, 16, 1>(p, q, s);
     }

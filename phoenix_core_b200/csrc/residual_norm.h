@@ -24,12 +24,15 @@ struct RNParams {
     int parts, pieces, items;                      // per group: sums that make its gate's gradient, pieces of each class's rows; pieces in all
 };
 
-// Warps per row, values per thread and rows of a CTA (one per SM) for a width; warps 0: wider than the registers.
+// Warps per row, values per thread and rows of a CTA (one per SM) for a width; warps 0: wider than the registers. A thread's values are few enough that the backward pass keeps a row
+// of four tensors in registers, and idle lanes cost rows in flight: backward, 3001 x (4 x 509) f16 30 us with five warps a row, 41 with eight; 16384 x 1024 bf16 40 with two, 57 with
+// four; 16384 x 1536 bf16 55 with three, 61 with four; forward 3001 x (4 x 509) 20 with five of 16 values, 26 with four of 32.
 struct RNShape { int warps, values, rows; };
 inline RNShape fwd_shape(long long width) {
     if (width <= 32 * 8) return {1, 8, 16};
     if (width <= 32 * 32) return {1, 32, 12};
     if (width <= 128 * 16) return {4, 16, 4};
+    if (width <= 160 * 16) return {5, 16, 3};
     if (width <= 128 * 32) return {4, 32, 3};
     if (width <= 256 * 32) return {8, 32, 1};
     if (width <= 512 * 32) return {16, 32, 1};
@@ -38,7 +41,10 @@ inline RNShape fwd_shape(long long width) {
 inline RNShape bwd_shape(long long width) {
     if (width <= 32 * 8) return {1, 8, 16};
     if (width <= 32 * 16) return {1, 16, 12};
+    if (width <= 64 * 16) return {2, 16, 6};
+    if (width <= 96 * 16) return {3, 16, 4};
     if (width <= 128 * 16) return {4, 16, 3};
+    if (width <= 160 * 16) return {5, 16, 3};
     if (width <= 256 * 16) return {8, 16, 2};
     if (width <= 512 * 16) return {16, 16, 1};
     return {0, 0, 1};

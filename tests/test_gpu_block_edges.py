@@ -42,6 +42,13 @@ def test_gates_of_few_rows(gates, algebra, f, dtype):
     Case(algebra, dtype, 600, f, gates).check()
 
 
+@pytest.mark.parametrize("algebra,f", [("real", 700), ("real", 1030), ("quaternion", 375), ("real", 1537), ("complex", 1150), ("real", 2560), ("real", 2561), ("ga300", 300)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_widths_of_every_number_of_warps(algebra, f, dtype):
+    for gates in (0, 4, 60):
+        Case(algebra, dtype, 60, f, gates).check()
+
+
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("n,f,gates", [(9, 512, 3), (70, 130, 1), (3, 8200, 3)])
 def test_norm_tensors_start_anywhere(dtype, n, f, gates):
