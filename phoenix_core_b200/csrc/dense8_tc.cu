@@ -12,7 +12,9 @@
 // Three forms:
 //   PAIR      256 x 256 tiles on pairs of SMs, half of either operand in each one's shared memory. An 8-bit MMA of 128 x 256 x 32 takes 128 clocks and reads 12 KB of
 //             shared memory, into which TMA writes as much again: more than the 128 bytes a clock that shared memory moves. On one SM a block of 128 took
-//             0.53 us where the MMAs alone take 0.27; a pair moves a third less.
+//             0.53 us where the MMAs alone take 0.27; a pair moves a third less. 8192 x 4096 -> 4096: 98 us, 2.8 PFLOP/s (86 % of twice the bf16 burst rate); with the clocks that
+//             this load leaves, a block takes 589 clocks of which the MMAs take 512: one accumulator of 256 columns is all that tensor memory holds beside the scales, so the epilogue
+//             is not covered.
 //   single    128 x 128 tiles; a tile's reduction is cut over the CTAs of a cluster where there are fewer tiles than SMs, whose partial sums are added in a
 //             fixed order through distributed shared memory.
 //   SWAP      few tokens: the filter is operand A, a tile is 128 features x 16 or 64 tokens; bound by the filter's bytes.
@@ -860,8 +862,8 @@ bool q8_swapped(int tokens) { return tokens <= 64; }
 bool q8_raw_tokens(int tokens) { return tokens <= D8_RAW; }
 
 // Measured on cold inputs, us (fitted to 1 to 4 rounds of tiles and reductions of 5 to 128 blocks): a single tile of 128 x 128 takes 0.27 a block behind 7.5 for launch, first
-// copies and epilogue; a pair's of 256 x 256 0.34 a block behind 12; a reduction cut over a cluster 3.5 more. 2048 x 4096 -> 4096: pairs 35.3, single 44.5;
-// 1024 x 4096 -> 4096 22.8 / 25.4; 2048 x 1024 -> 4096 17.2 / 16.9; 512 x 4096 -> 4096 21.8 / 15.6. Cut in two and not, 300 x 4096 -> 2048 14.0 / 14.6; 512 x 1024 ->
+// copies and epilogue; a pair's of 256 x 256 0.34 a block behind 12; a reduction cut over a cluster 3.5 more. 2048 x 4096 -> 4096: pairs 33.9, single 44.4;
+// 1024 x 4096 -> 4096 24.4 / 25.5; 2048 x 1024 -> 4096 18.0 / 17.4; 512 x 4096 -> 4096 23.0 / 16.1; GA(3,0,0) 4608 x 512 -> 768 85.5 / 129.8. Cut in two and not, 300 x 4096 -> 2048 14.0 / 14.6; 512 x 1024 ->
 // 1024 10.6 / 8.6.
 int q8_product(const Geom& g, const Q8Product& q, cudaStream_t stream) {
     if (q.tokens) return launch<16, true, false, true>(g, q, splits_for(g, q, 16), stream);
