@@ -108,6 +108,25 @@ def test_dense8_filter_gradient_alone(algebra, n, i, o):
     check_dense(dw, want, size, dim * n, torch.float32, "dw")
 
 
+@pytest.mark.parametrize("margin", [2, 61, 64])
+def test_dense8_beside_other_kernels(margin):
+    """With SMs left free the tiles are dealt to fewer CTAs, and cut otherwise: results within the bounds of the sums."""
+    dim, n, i, o = 4, 300, 200, 520
+    _, x, w, bias, dy = make_dense("quaternion", "io", "f32", n, i, o)
+    w8 = ref.quantized(w.double(), 128, 128)
+    want, size = ref.forward(dim, x.double().reshape(dim, n, i), w8, bias.double().reshape(dim, o))
+    wdx, sdx, wdw, sdw = ref.backward(dim, x.double().reshape(dim, n, i), w8, dy.double().reshape(dim, n, o))
+    before = pcb.getSmMargin()
+    pcb.setSmMargin(margin)
+    try:
+        _, y, dw, dx = run_dense("quaternion", "io", x, w, bias, dy)
+    finally:
+        pcb.setSmMargin(before)
+    check_dense(y, want, size + bias.double().reshape(dim, 1, o).abs(), dim * i, torch.float32, "y")
+    check_dense(dx, wdx, sdx, dim * o, torch.float32, "dx")
+    check_dense(dw, wdw, sdw, dim * n, torch.float32, "dw")
+
+
 def test_no_samples():
     """Calls without samples write no values but the zeros of the sums over samples; what does not fit is refused all the same."""
     e = lambda *s, t=torch.float16: torch.empty(s, dtype=t, device="cuda")                       # noqa: E731
