@@ -18,7 +18,7 @@ OBJ_DIR = os.path.join(HERE, "build")
 SOURCES = ["api.cu", "simt_qgemm.cu", "tensor_path.cu", "pointwise_tc.cu", "pointwise2_tc.cu", "pointwise8_tc.cu", "conv_tc.cu", "narrow_tc.cu",
            "conv_tf32.cu", "qgemm_tc.cu", "aux_bn.cu", "probe.cu", "dense8_quant.cu", "dense8_tc.cu", 
            "residual_norm.cu", "residual_norm_f32.cu", "residual_norm_f16.cu", "residual_norm_bf16.cu", "distill.cu"]
-HEADERS = ["common.cuh", "tensor_path.cuh", "dense8.cuh", "residual_norm.h", "residual_norm.cuh", "packed.cuh", "e4m3.cuh", "umma.cuh", "tc_common.cuh", "unaligned_chunk.h", "column_halves.h", "sm_share.h", os.path.join("..", "..", "include", "phoenix_core_b200.h")]
+HEADERS = ["common.cuh", "tensor_path.cuh", "dense8.cuh", "residual_norm.h", "residual_norm.cuh", "packed.cuh", "e4m3.cuh", "umma.cuh", "tc_common.cuh", "unaligned_chunk.h", "column_halves.h", "sm_share.h", "class_shares.h", os.path.join("..", "..", "include", "phoenix_core_b200.h")]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall",

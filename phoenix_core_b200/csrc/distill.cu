@@ -9,6 +9,7 @@
 // (16 exponentials per clock and SM are two thirds of what a pass over 16-bit logits takes at full bandwidth). 4096 x 131072 bf16: 190 us forward (5.6 TB/s), 342
 // backward (6.3 TB/s both ways); bound by memory.
 // Few rows are cut over the CTAs of a cluster, whose maxima and sums are joined through distributed shared memory.
+#include "class_shares.h"
 #include "common.cuh"
 #include "packed.cuh"
 #include "tc_common.cuh"
@@ -215,7 +216,7 @@ __device__ __forceinline__ void over_classes(const T* logits, const DIParams& p,
     constexpr int VEC = Bits<T>::VEC, UNROLL = 4;
     constexpr bool LONG = THREADS == 512;
     const int threads = BESIDE ? THREADS / p.comps : THREADS, tid = BESIDE ? threadIdx.x % threads : threadIdx.x;
-    for (int c = BESIDE ? threadIdx.x / threads : lo / p.units, end = BESIDE ? c + 1 : (hi + p.units - 1) / p.units; c < end; ++c) {
+    for (int c = BESIDE ? threadIdx.x / threads : lo / p.units, end = BESIDE ? c + 1 : components_below(hi, p.units); c < end; ++c) {
         const int a = max(lo, c * p.units), b = min(hi, (c + 1) * p.units);
         const T* first = logits + ((size_t)c * p.n + row) * p.units + (a - c * p.units);
         if (!VECTORS) {
@@ -318,7 +319,7 @@ __global__ void __launch_bounds__(THREADS, di_ctas(THREADS)) distill_fwd_kernel(
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int row = blockIdx.x / p.splits, split = blockIdx.x - row * p.splits;
     const int classes = p.comps * p.units;
-    const int lo = (int)((long long)classes * split / p.splits), hi = (int)((long long)classes * (split + 1) / p.splits);
+    const int lo = share_start(classes, split, p.splits), hi = share_start(classes, split + 1, p.splits);
     const float c_temp = LOG2E * p.inv_temp;
     chain_wait();
     chain_next();
@@ -422,7 +423,7 @@ __global__ void __launch_bounds__(THREADS, di_ctas(THREADS)) distill_bwd_kernel(
     // from the last row on: the forward pass has left the last rows in L2
     const int back = blockIdx.x / p.splits, row = p.n - 1 - back, split = blockIdx.x - back * p.splits;
     const int classes = p.comps * p.units;
-    const int lo = (int)((long long)classes * split / p.splits), hi = (int)((long long)classes * (split + 1) / p.splits);
+    const int lo = share_start(classes, split, p.splits), hi = share_start(classes, split + 1, p.splits);
     const float c_temp = LOG2E * p.inv_temp;
     chain_wait();
     chain_next();
