@@ -11,11 +11,14 @@
 // only.
 #include <Python.h>
 
+#include <cuda_runtime_api.h>
+
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <atomic>
 #include <vector>
 
 namespace {
@@ -139,7 +142,75 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     }
 }
 
+// The capture that a stream is part of, as a number of its own (0: none). A capture holds on to what its kernels use until the graph and everything
+// instantiated from it are gone: watch_capture gives the graph an object that the runtime releases then, ended(watch) says whether it has.
+unsigned long long capture_of(W stream, cudaGraph_t* graph = nullptr) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (cudaStreamGetCaptureInfo(reinterpret_cast<cudaStream_t>(stream), &status, &id, graph) != cudaSuccess) {
+        cudaGetLastError();                                        // (the legacy stream beside a capture: it is part of none)
+        return 0;
+    }
+    return status == cudaStreamCaptureStatusActive ? id + 1 : 0;
+}
+PyObject* capture_id(PyObject*, PyObject* stream) {
+    const W s = PyLong_AsUnsignedLongLong(stream);
+    return PyErr_Occurred() ? nullptr : PyLong_FromUnsignedLongLong(capture_of(s));
+}
+
+constexpr const char* WATCH = "phoenix_core_b200.watch";
+struct Watch {
+    std::atomic<int> holders{2};                                   // the graph and Python
+    std::atomic<bool> ended{false};
+    void drop() {
+        if (holders.fetch_sub(1) == 1) delete this;
+    }
+};
+void CUDART_CB watch_released(void* w) {                            // (on a thread of the runtime's: no call into it or into Python)
+    static_cast<Watch*>(w)->ended = true;
+    static_cast<Watch*>(w)->drop();
+}
+void free_watch(PyObject* capsule) { static_cast<Watch*>(PyCapsule_GetPointer(capsule, WATCH))->drop(); }
+
+PyObject* watch_capture(PyObject*, PyObject* stream) {
+    const W s = PyLong_AsUnsignedLongLong(stream);
+    if (PyErr_Occurred()) return nullptr;
+    cudaGraph_t graph = nullptr;
+    if (capture_of(s, &graph) == 0) {
+        PyErr_SetString(PyExc_RuntimeError, "the stream is not being captured");
+        return nullptr;
+    }
+    Watch* watch = new Watch;
+    PyObject* capsule = PyCapsule_New(watch, WATCH, free_watch);
+    if (!capsule) {
+        delete watch;
+        return nullptr;
+    }
+    cudaUserObject_t object = nullptr;
+    cudaError_t e = cudaUserObjectCreate(&object, watch, watch_released, 1, cudaUserObjectNoDestructorSync);
+    if (e == cudaSuccess) {
+        e = cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove);
+        if (e != cudaSuccess) cudaUserObjectRelease(object, 1);
+    } else {
+        watch->drop();
+    }
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        Py_DECREF(capsule);
+        PyErr_Format(PyExc_RuntimeError, "the captured graph takes no object: %s", cudaGetErrorString(e));
+        return nullptr;
+    }
+    return capsule;
+}
+PyObject* ended(PyObject*, PyObject* capsule) {
+    const Watch* watch = static_cast<const Watch*>(PyCapsule_GetPointer(capsule, WATCH));
+    return watch ? PyBool_FromLong(watch->ended) : nullptr;
+}
+
 PyMethodDef methods[] = {{"make_specs", make_specs, METH_O, "What a call's operands have to be."},
+                         {"capture_id", capture_id, METH_O, "A number for the capture that a stream is part of, 0 for none."},
+                         {"watch_capture", watch_capture, METH_O, "What tells when the graph that a stream is captured into is gone."},
+                         {"ended", ended, METH_O, "Whether a watched graph and all that was instantiated from it are gone."},
                          {"call", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(call)), METH_FASTCALL, "Checks the operands and calls an entry point."},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

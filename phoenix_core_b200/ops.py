@@ -37,6 +37,8 @@ class Device:
         self.index = index
         self.accessControl = threading.Lock()
         self.workspaces = {}
+        self.captures = {}                     # by the capture's number: what graphs hold that still live
+        self._captureLock = threading.Lock()
         self.context = Context()
         self.check_after_each_op = os.environ.get("PCB_CHECK_DEVICE_STATUS", "0") not in ("", "0")
 
@@ -59,17 +61,47 @@ class Device:
             return dev
 
     def requestWorkspace(self, nbytes):
-        """The current stream's workspace. A call that is being captured gets one of its own from the graph's memory, in the order of the captured
-        stream as any other tensor of the capture: graphs share none with each other, nor with what the stream runs later."""
-        if _capturing():
-            return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=torch.device("cuda", self.index))
+        """The current stream's workspace. Calls that are being captured share one of their own, for each captured stream of each capture, which stays
+        theirs until the graph and everything instantiated from it are gone, whoever began the capture: graphs share none with each other, nor
+        with what a stream runs later."""
         key = _raw_stream(self.index)
+        capture = _capture_id(key)
+        if capture:
+            return self._capturedWorkspace(capture, key, nbytes)
         ws = self.workspaces.get(key)
         if ws is None or ws.numel() < nbytes:
             with torch.cuda.device(self.index):
                 ws = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=torch.device("cuda", self.index))
             self.workspaces[key] = ws      # allocated and used on this stream only, so torch's stream-ordered reuse holds
         return ws
+
+    def _capture(self, number, stream):
+        """What the calls of a capture hold (under ``_captureLock``); what belongs to graphs that are gone is let go."""
+        for ended in [k for k, c in self.captures.items() if _lib.binding().ended(c.watch)]:
+            del self.captures[ended]
+        c = self.captures.get(number)
+        if c is None:
+            c = self.captures[number] = _Capture(_lib.binding().watch_capture(stream))
+        return c
+
+    def _capturedWorkspace(self, capture, stream, nbytes):
+        with self._captureLock:
+            c = self._capture(capture, stream)
+            ws = c.workspaces.get(stream)
+            if ws is None or ws.numel() < nbytes:
+                if ws is not None:         # (the graph's earlier calls use it; doubled, so that all of them together are twice the last at most)
+                    c.others.append(ws)
+                    nbytes = max(nbytes, 2 * ws.numel())
+                ws = c.workspaces[stream] = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=torch.device("cuda", self.index))
+            return ws
+
+    def holdForCapture(self, tensor):
+        """Keeps a tensor that a call uses beside its operands for as long as a graph may, if the call is being captured."""
+        stream = _raw_stream(self.index)
+        capture = _capture_id(stream)
+        if capture:
+            with self._captureLock:
+                self._capture(capture, stream).others.append(tensor)
 
     @property
     def workspace(self):
@@ -89,6 +121,20 @@ class Device:
 
     def getContext(self):
         return self.context
+
+
+class _Capture:
+    """What the calls of one capture use for as long as a graph may run them."""
+
+    def __init__(self, watch):
+        self.watch, self.workspaces, self.others = watch, {}, []
+
+
+def _capture_id(stream):
+    """A number for the capture that a stream (a handle) is part of, 0 for none."""
+    global _capture_id
+    _capture_id = _lib.binding().capture_id
+    return _capture_id(stream)
 
 
 class KeptInput:
@@ -127,7 +173,6 @@ def _check_tensor(t, name, dtype=None, shape=None):
         raise ValueError("%s shape mismatch: %s vs expected %s" % (name, tuple(t.shape), tuple(shape)))
 
 
-_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None) or (lambda: False)       # (absent from a torch without CUDA, which captures nothing)
 _get_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
@@ -296,6 +341,7 @@ def conv2DFwd(inputTensor, filterTensor, biasTensor, outputTensor, descriptor, c
             if keep.workspace is None or keep.workspace.numel() < need or keep.workspace.device != inputTensor.device:
                 keep.workspace = torch.empty(need, dtype=torch.uint8, device=inputTensor.device)
             ws = keep.workspace
+            dev.holdForCapture(ws)
         else:
             ws = dev.requestWorkspace(need)
         _lib.check(L.pcb_qconv2d_fwd(ctypes.byref(d), _ptr(inputTensor), _ptr(filterTensor), _ptr(biasTensor),
