@@ -225,13 +225,19 @@ int pcb_qconv2d_engine_for(const pcb_conv2d_desc* desc, int pass);
 int pcb_qdense_engine_for(const pcb_dense_desc* desc, int pass);
 
 /* Device-side wait budget. The tensor-core kernels bound every barrier wait; when a wait expires the
- * kernel records it in a status word inside the workspace and returns. Every entry point above clears the
+ * kernel records it in a status word at the head of the workspace and returns. Every entry point above clears the
  * word once, before or in its first launch, and kernels only OR into it, so after a call the word covers all the
  * launches of that call (a later launch of the same call gives up at its first slow wait once the word is
  * set). This reads the word back (synchronises the stream). Returns PCB_OK or PCB_ERR_DEVICE_TIMEOUT.
  * (Stands where the reference checks cudnnStatus_t / cudaError_t after each library call,
  * src/backend/cudnn/context.hpp:68-110.) */
 int pcb_check_device_status(const void* workspace, size_t workspace_bytes, void* stream);
+
+/* Has the calls that are given `workspace` from now on report into `word` (4 bytes of device memory, 0 before its first use) instead of the workspace's
+ * head; null: into the head again. For calls that a graph replays: each can have a word of its own, which the calls behind it in the graph do not
+ * reset. The address is kept until it is taken back; the memory has to live as long as the calls may run. pcb_check_device_status looks where the
+ * workspace's next call would report. (No counterpart in the reference.) */
+int pcb_set_status_word(const void* workspace, void* word);
 
 /* Self-test of that mechanism (no counterpart in the reference). Clears the status word, then launches a
  * one-thread kernel that waits at most `limit_clocks` SM clocks (1 .. 2^24) on a barrier nothing signals, so

@@ -1,5 +1,6 @@
 // C ABI of the backend: argument validation, geometry, kernel-family selection and dispatch.
 // Nothing here allocates device memory; scratch comes from the caller's workspace.
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -123,17 +124,30 @@ int tensor_variant(int variant, int engine) { return engine == PCB_ENGINE_AUTO ?
 // Layout of the caller's workspace: [0, 256) status block (first word: device wait status), then scratch.
 constexpr size_t WS_HEADER = 256;
 
+// Status words that lie elsewhere than at the head of their workspace (pcb_set_status_word), by workspace address.
+std::mutex g_word_mutex;
+std::unordered_map<const void*, int*> g_words;
+std::atomic<int> g_word_count{0};            // (looked at first: a program without such words takes no lock)
+int* status_of(const void* workspace) {
+    if (workspace && g_word_count.load(std::memory_order_acquire) > 0) {
+        std::lock_guard<std::mutex> lock(g_word_mutex);
+        const auto it = g_words.find(workspace);
+        if (it != g_words.end()) return it->second;
+    }
+    return static_cast<int*>(const_cast<void*>(workspace));
+}
+
 // Clears the device wait status at the start of an API call. Every kernel launched by the call only ORs into the
 // word, so pcb_check_device_status afterwards reports an expiry in ANY launch of the call, not just the last one.
 // A call that hands the reset to its first launch (StatusClear) settles it with finish_status: a call that launched nothing
 // resets the word all the same.
 int reset_status(void* workspace, size_t ws_bytes, cudaStream_t stream) {
-    return workspace && ws_bytes >= sizeof(int) ? clear_status_word(static_cast<int*>(workspace), stream) : (int)PCB_OK;
+    return workspace && ws_bytes >= sizeof(int) ? clear_status_word(status_of(workspace), stream) : (int)PCB_OK;
 }
 
 StatusClear owe_status(void* workspace, size_t ws_bytes) {
     StatusClear sc;
-    sc.word = static_cast<int*>(workspace);
+    sc.word = status_of(workspace);
     sc.pending = workspace && ws_bytes >= sizeof(int);
     return sc;
 }
@@ -198,7 +212,7 @@ int run_pass(Pass pass, int dtype, int variant, int engine, const Geom& full, co
         return PCB_ERR_WORKSPACE;
     }
     float* scratch = workspace ? reinterpret_cast<float*>(static_cast<char*>(workspace) + WS_HEADER + offset) : nullptr;
-    int* status = static_cast<int*>(workspace);
+    int* status = status_of(workspace);
     // the tensor-core kernels move 16-byte chunks of NCHW / OIHW tensors: every tensor (and the workspace) must be 16-byte
     // aligned. Tensors of other layouts and the channel slices of grouped layers are addressed element by element (staged
     // operands, strided stores), so there only the workspace has to be.
@@ -599,7 +613,7 @@ int pcb_qdense_fwd(const pcb_dense_desc* desc, const void* x, const void* w, con
     const bool apart = !overlaps(y, n.y, x, n.x) && !overlaps(y, n.y, w, n.w);
     if (dense_route(desc, g, all, apart, false, workspace, workspace_bytes_) == DENSE_DIRECT) {
         forget_kept(workspace);
-        rc = dense_tc_fwd(desc->dtype, g, x, w, bias, y, static_cast<int*>(workspace), (cudaStream_t)stream, sc);
+        rc = dense_tc_fwd(desc->dtype, g, x, w, bias, y, status_of(workspace), (cudaStream_t)stream, sc);
     } else {
         rc = run_pass(PASS_FWD, desc->dtype, variant_for(g, desc->variant), desc->engine, g, w, x, bias, y, workspace, workspace_bytes_, (cudaStream_t)stream, nullptr, &sc);
     }
@@ -627,7 +641,7 @@ int pcb_qdense_bwd(const pcb_dense_desc* desc, const void* x, const void* w, con
     const DenseRoute route = dense_route(desc, g, all, apart, true, workspace, workspace_bytes_);
     if (route != DENSE_STAGED) {
         forget_kept(workspace);
-        rc = dense_tc_bwd(desc->dtype, g, x, w, dy, dw, route == DENSE_DIRECT ? gx : nullptr, static_cast<int*>(workspace), (cudaStream_t)stream, sc);
+        rc = dense_tc_bwd(desc->dtype, g, x, w, dy, dw, route == DENSE_DIRECT ? gx : nullptr, status_of(workspace), (cudaStream_t)stream, sc);
     } else {
         rc = run_pass(PASS_BWD_FILTER, desc->dtype, variant_for(g, desc->variant), desc->engine, g, dy, x, nullptr, dw, workspace, workspace_bytes_, (cudaStream_t)stream, nullptr, &sc);
     }
@@ -660,17 +674,27 @@ int pcb_selftest_wait_expiry(const pcb_conv2d_desc* desc, const void* x, const v
     if (limit_clocks < 1 || limit_clocks > (1ll << 24)) { set_error("limit_clocks must be in [1, 2^24]"); return PCB_ERR_INVALID_ARGUMENT; }
     int rc = reset_status(workspace, workspace_bytes_, (cudaStream_t)stream);
     if (rc != PCB_OK) return rc;
-    wait_expiry_kernel<<<1, 32, 0, (cudaStream_t)stream>>>(static_cast<int*>(workspace), limit_clocks);
+    wait_expiry_kernel<<<1, 32, 0, (cudaStream_t)stream>>>(status_of(workspace), limit_clocks);
     PCB_CUDA_TRY(cudaGetLastError());
     // a further launch of the same call: it must leave the recorded expiry in place
     if (desc) rc = conv_fwd(desc, x, w, nullptr, y, workspace, workspace_bytes_, (cudaStream_t)stream);
     return rc;
 }
 
+int pcb_set_status_word(const void* workspace, void* word) {
+    if (!workspace) { set_error("null workspace"); return PCB_ERR_INVALID_ARGUMENT; }
+    if (reinterpret_cast<uintptr_t>(word) % sizeof(int) != 0) { set_error("a status word must be 4-byte aligned"); return PCB_ERR_INVALID_ARGUMENT; }
+    std::lock_guard<std::mutex> lock(g_word_mutex);
+    if (word) g_words[workspace] = static_cast<int*>(word);
+    else g_words.erase(workspace);
+    g_word_count.store((int)g_words.size(), std::memory_order_release);
+    return PCB_OK;
+}
+
 int pcb_check_device_status(const void* workspace, size_t workspace_bytes_, void* stream) {
     if (!workspace || workspace_bytes_ < sizeof(int)) return PCB_OK;
     int word = 0;
-    PCB_CUDA_TRY(cudaMemcpyAsync(&word, workspace, sizeof(int), cudaMemcpyDeviceToHost, (cudaStream_t)stream));
+    PCB_CUDA_TRY(cudaMemcpyAsync(&word, status_of(workspace), sizeof(int), cudaMemcpyDeviceToHost, (cudaStream_t)stream));
     PCB_CUDA_TRY(cudaStreamSynchronize((cudaStream_t)stream));
     if (word != 0) {
         set_error("device-side wait expired (status word 0x%08x)", word);
@@ -719,7 +743,7 @@ int pcb_qdense8_fwd(const pcb_dense_desc* desc, const void* x, const void* w8, c
     if (overlaps(y, (size_t)g.nc * g.Nb * g.Co * size, x, (size_t)g.nc * g.Nb * g.Ci * size)) { set_error("y must not share memory with x"); return PCB_ERR_INVALID_ARGUMENT; }
     forget_kept(workspace);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
-    int* status = reinterpret_cast<int*>(ws);
+    int* status = status_of(workspace);
     const Q8Target rows = {ws + at.x_rows, reinterpret_cast<uint32_t*>(ws + at.x_words)};
     const bool raw = q8_raw_tokens(g.Nb);
     if (!raw && (rc = q8_quantize_rows(desc->dtype, g.nc, g.Nb, g.Ci, x, rows, status, (cudaStream_t)stream)) != PCB_OK) return rc;
@@ -745,7 +769,7 @@ int pcb_qdense8_bwd(const pcb_dense_desc* desc, const void* x, const void* w8, c
     if ((rc = dense8_workspace(workspace, workspace_bytes_, at.total)) != PCB_OK || (need_dx && (rc = dense8_check_filter(w8)) != PCB_OK)) return rc;
     forget_kept(workspace);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
-    int* status = reinterpret_cast<int*>(ws);
+    int* status = status_of(workspace);
     const cudaStream_t st = (cudaStream_t)stream;
     const Q8Target dy_rows = {need_dx ? ws + at.dy_rows : nullptr, reinterpret_cast<uint32_t*>(ws + at.dy_row_words)};
     const Q8Target dy_cols = {ws + at.dy_cols, reinterpret_cast<uint32_t*>(ws + at.dy_col_words)};

@@ -159,6 +159,7 @@ PyObject* capture_id(PyObject*, PyObject* stream) {
 }
 
 constexpr const char* WATCH = "phoenix_core_b200.watch";
+std::atomic<long long> g_ended{0};                                  // graphs that are gone
 struct Watch {
     std::atomic<int> holders{2};                                   // the graph and Python
     std::atomic<bool> ended{false};
@@ -168,6 +169,7 @@ struct Watch {
 };
 void CUDART_CB watch_released(void* w) {                            // (on a thread of the runtime's: no call into it or into Python)
     static_cast<Watch*>(w)->ended = true;
+    ++g_ended;
     static_cast<Watch*>(w)->drop();
 }
 void free_watch(PyObject* capsule) { static_cast<Watch*>(PyCapsule_GetPointer(capsule, WATCH))->drop(); }
@@ -202,16 +204,89 @@ PyObject* watch_capture(PyObject*, PyObject* stream) {
     }
     return capsule;
 }
+PyObject* ended_count(PyObject*, PyObject*) { return PyLong_FromLongLong(g_ended); }
 PyObject* ended(PyObject*, PyObject* capsule) {
     const Watch* watch = static_cast<const Watch*>(PyCapsule_GetPointer(capsule, WATCH));
     return watch ? PyBool_FromLong(watch->ended) : nullptr;
 }
 
+// Status words of captured calls: memory that no graph's and no stream's allocations are given, zero from the start, never given back.
+// new_words(device, count) -> address; take_words(device, stream, address, count) -> what they held, as a tuple; what was not zero is from then on. Both wait for the stream.
+struct RelaxedCapture {                                            // (an allocation beside somebody's capture is no part of it)
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+    ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+PyObject* cuda_failed(const char* what, cudaError_t e) {
+    cudaGetLastError();
+    PyErr_Format(PyExc_RuntimeError, "%s: %s", what, cudaGetErrorString(e));
+    return nullptr;
+}
+PyObject* new_words(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    const long device = nargs == 2 ? PyLong_AsLong(args[0]) : -1, count = nargs == 2 ? PyLong_AsLong(args[1]) : 0;
+    if (PyErr_Occurred()) return nullptr;
+    if (device < 0 || count <= 0) {
+        PyErr_SetString(PyExc_ValueError, "new_words(device, count)");
+        return nullptr;
+    }
+    int before = 0;
+    cudaGetDevice(&before);
+    cudaError_t e = cudaSetDevice((int)device);
+    void* words = nullptr;
+    cudaStream_t stream = nullptr;
+    {
+        const RelaxedCapture relaxed;
+        if (e == cudaSuccess) e = cudaMalloc(&words, (size_t)count * 4);
+        if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&stream, cudaStreamNonBlocking);
+        if (e == cudaSuccess) e = cudaMemsetAsync(words, 0, (size_t)count * 4, stream);
+        if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
+        if (stream) cudaStreamDestroy(stream);
+        if (e != cudaSuccess && words) cudaFree(words);
+    }
+    cudaSetDevice(before);
+    return e == cudaSuccess ? PyLong_FromUnsignedLongLong(reinterpret_cast<W>(words)) : cuda_failed("status words", e);
+}
+PyObject* take_words(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    if (nargs != 4) {
+        PyErr_SetString(PyExc_TypeError, "take_words(device, stream, address, count)");
+        return nullptr;
+    }
+    const long device = PyLong_AsLong(args[0]), count = PyLong_AsLong(args[3]);
+    const W stream = PyLong_AsUnsignedLongLong(args[1]), words = PyLong_AsUnsignedLongLong(args[2]);
+    if (PyErr_Occurred()) return nullptr;
+    const size_t n = count > 0 ? (size_t)count : 0;
+    std::vector<int> held(n);
+    bool any = false;
+    int before = 0;
+    cudaGetDevice(&before);
+    cudaError_t e = cudaSetDevice((int)device);
+    Py_BEGIN_ALLOW_THREADS
+    if (e == cudaSuccess) e = cudaMemcpyAsync(held.data(), reinterpret_cast<const void*>(words), n * 4, cudaMemcpyDeviceToHost, reinterpret_cast<cudaStream_t>(stream));
+    if (e == cudaSuccess) e = cudaStreamSynchronize(reinterpret_cast<cudaStream_t>(stream));
+    // (only those: another one may be written meanwhile)
+    for (size_t i = 0; e == cudaSuccess && i < n; ++i)
+        if (held[i] != 0) {
+            e = cudaMemsetAsync(reinterpret_cast<int*>(words) + i, 0, 4, reinterpret_cast<cudaStream_t>(stream));
+            any = true;
+        }
+    if (e == cudaSuccess && any) e = cudaStreamSynchronize(reinterpret_cast<cudaStream_t>(stream));
+    Py_END_ALLOW_THREADS
+    cudaSetDevice(before);
+    if (e != cudaSuccess) return cuda_failed("status words", e);
+    PyObject* tuple = PyTuple_New((Py_ssize_t)n);
+    for (size_t i = 0; tuple && i < n; ++i) PyTuple_SET_ITEM(tuple, (Py_ssize_t)i, PyLong_FromLong(held[i]));
+    return tuple;
+}
+template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)> PyCFunction fast() { return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(F)); }
+
 PyMethodDef methods[] = {{"make_specs", make_specs, METH_O, "What a call's operands have to be."},
                          {"capture_id", capture_id, METH_O, "A number for the capture that a stream is part of, 0 for none."},
                          {"watch_capture", watch_capture, METH_O, "What tells when the graph that a stream is captured into is gone."},
+                         {"new_words", fast<new_words>(), METH_FASTCALL, "Status words of captured calls."},
+                         {"take_words", fast<take_words>(), METH_FASTCALL, "What status words hold; zero from then on."},
+                         {"ended_count", ended_count, METH_NOARGS, "Watched graphs that are gone."},
                          {"ended", ended, METH_O, "Whether a watched graph and all that was instantiated from it are gone."},
-                         {"call", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(call)), METH_FASTCALL, "Checks the operands and calls an entry point."},
+                         {"call", fast<call>(), METH_FASTCALL, "Checks the operands and calls an entry point."},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

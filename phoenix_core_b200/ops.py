@@ -28,7 +28,7 @@ class Device:
     (``src/backend/cudnn/cudnn.cc:5-14``). Here the workspace is keyed by the torch stream that is current at the
     call, for the same reason: it holds the split-K / staging scratch and the device status word, so operations
     issued on different streams must not share it. ``checkStatus`` reads the status word of the current stream's
-    workspace back (it synchronises that stream); with ``PCB_CHECK_DEVICE_STATUS=1`` in the environment every
+    workspace back, and those of captured operations, each of which has one of its own (it synchronises that stream); with ``PCB_CHECK_DEVICE_STATUS=1`` in the environment every
     operation does so before it returns."""
     _devices = {}
     _registry_lock = threading.Lock()
@@ -38,6 +38,8 @@ class Device:
         self.accessControl = threading.Lock()
         self.workspaces = {}
         self.captures = {}                     # by the capture's number: what graphs hold that still live
+        self._freeWords, self._endedWords = [], []     # status words, in blocks of _WORDS, of no capture and of captures whose graphs are gone
+        self._endedGraphs = 0                          # graphs of the process that were gone at the last look
         self._captureLock = threading.Lock()
         self.context = Context()
         self.check_after_each_op = os.environ.get("PCB_CHECK_DEVICE_STATUS", "0") not in ("", "0")
@@ -68,6 +70,9 @@ class Device:
         capture = _capture_id(key)
         if capture:
             return self._capturedWorkspace(capture, key, nbytes)
+        if self.captures and _lib.binding().ended_count() != self._endedGraphs:
+            with self._captureLock:
+                self._letGo()
         ws = self.workspaces.get(key)
         if ws is None or ws.numel() < nbytes:
             with torch.cuda.device(self.index):
@@ -76,13 +81,32 @@ class Device:
         return ws
 
     def _capture(self, number, stream):
-        """What the calls of a capture hold (under ``_captureLock``); what belongs to graphs that are gone is let go."""
-        for ended in [k for k, c in self.captures.items() if _lib.binding().ended(c.watch)]:
-            del self.captures[ended]
+        """What the calls of a capture hold (under ``_captureLock``)."""
+        self._letGo()
         c = self.captures.get(number)
         if c is None:
             c = self.captures[number] = _Capture(_lib.binding().watch_capture(stream))
         return c
+
+    def _letGo(self):
+        """Gives back what belongs to graphs that are gone (under ``_captureLock``)."""
+        self._endedGraphs = _lib.binding().ended_count()
+        for number in [k for k, c in self.captures.items() if _lib.binding().ended(c.watch)]:
+            c = self.captures.pop(number)
+            for ws in [*c.workspaces.values(), *c.others]:
+                _lib.check(_lib.lib().pcb_set_status_word(ws.data_ptr(), None))
+            self._endedWords += c.words
+
+    def _giveWord(self, c, ws):
+        """Has the next call of a capture that uses the workspace report into a word of its own."""
+        if c.wordsLeft == 0:
+            if not self._freeWords:
+                base = _lib.binding().new_words(self.index, 64 * _WORDS)
+                self._freeWords = [base + 4 * _WORDS * i for i in range(64)]
+            c.words.append(self._freeWords.pop())
+            c.wordsLeft = _WORDS
+        c.wordsLeft -= 1
+        _lib.check(_lib.lib().pcb_set_status_word(ws.data_ptr(), c.words[-1] + 4 * c.wordsLeft))
 
     def _capturedWorkspace(self, capture, stream, nbytes):
         with self._captureLock:
@@ -93,27 +117,47 @@ class Device:
                     c.others.append(ws)
                     nbytes = max(nbytes, 2 * ws.numel())
                 ws = c.workspaces[stream] = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=torch.device("cuda", self.index))
+            self._giveWord(c, ws)
             return ws
 
-    def holdForCapture(self, tensor):
-        """Keeps a tensor that a call uses beside its operands for as long as a graph may, if the call is being captured."""
+    def holdForCapture(self, ws):
+        """Keeps a workspace that a call brings itself for as long as a graph may use it, if the call is being captured."""
         stream = _raw_stream(self.index)
         capture = _capture_id(stream)
         if capture:
             with self._captureLock:
-                self._capture(capture, stream).others.append(tensor)
+                c = self._capture(capture, stream)
+                c.others.append(ws)
+                self._giveWord(c, ws)
 
     @property
     def workspace(self):
         return self.workspaces.get(_raw_stream(self.index))
 
     def checkStatus(self):
-        """Raises BackendError(PCB_ERR_DEVICE_TIMEOUT) if a bounded device-side wait expired in the last operation
-        issued on the current stream; synchronises that stream."""
-        ws = self.workspace
-        if ws is not None:
-            with torch.cuda.device(self.index):
-                _lib.check(_lib.lib().pcb_check_device_status(_ptr(ws), ws.numel(), _stream()))
+        """Raises BackendError(PCB_ERR_DEVICE_TIMEOUT) if a bounded device-side wait expired in the last operation issued on the current stream, or in
+        the last replay of any captured operation of the device: replays on the current stream are waited for, of others what they have reported
+        so far is seen. An expiry in a replay is reported once. Synchronises the current stream."""
+        ws, status = self.workspace, _lib.PCB_OK
+        with torch.cuda.device(self.index):
+            if ws is not None:
+                status = _lib.lib().pcb_check_device_status(_ptr(ws), ws.numel(), _stream())
+            replayed = self._takeWords()
+        if replayed:
+            raise _lib.BackendError(_lib.PCB_ERR_DEVICE_TIMEOUT, "device-side wait expired in a replayed operation (status word 0x%08x)" % replayed)
+        _lib.check(status)
+
+    def _takeWords(self):
+        """What captured operations have reported, all of them together."""
+        with self._captureLock:
+            self._letGo()
+            ended, self._endedWords = self._endedWords, []
+            replayed = 0
+            for words in [*ended, *(w for c in self.captures.values() for w in c.words)]:
+                for word in _lib.binding().take_words(self.index, _raw_stream(self.index), words, _WORDS):
+                    replayed |= word & 0xffffffff
+            self._freeWords += ended                   # (zero again, for captures to come)
+            return replayed
 
     def _after_op(self):
         if self.check_after_each_op:
@@ -123,11 +167,15 @@ class Device:
         return self.context
 
 
+_WORDS = 64      # status words that a capture takes at a time
+
+
 class _Capture:
     """What the calls of one capture use for as long as a graph may run them."""
 
     def __init__(self, watch):
         self.watch, self.workspaces, self.others = watch, {}, []
+        self.words, self.wordsLeft = [], 0
 
 
 def _capture_id(stream):

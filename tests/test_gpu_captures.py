@@ -121,7 +121,8 @@ def test_what_a_graph_holds_goes_with_it():
     first = capture()
     number = max(dev.captures)
     second = capture()
-    assert number in dev.captures and max(dev.captures) > number               # (the first lives)
+    later = max(dev.captures)
+    assert number in dev.captures and later > number                            # (the first lives)
     first.replay()
     assert layer.same(layer.results(), want)
     first.reset()
@@ -134,6 +135,14 @@ def test_what_a_graph_holds_goes_with_it():
         if number not in dev.captures:
             break
     assert number not in dev.captures
+    second.reset()
+    for _ in range(50):
+        time.sleep(0.02)
+        layer.run()                                                             # eager calls look too
+        if later not in dev.captures:
+            break
+    assert later not in dev.captures
+    second = capture()
     for graph in (second, third):
         graph.replay()
         assert layer.same(layer.results(), want)
