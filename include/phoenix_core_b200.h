@@ -259,7 +259,8 @@ int pcb_selftest_wait_expiry(const pcb_conv2d_desc* desc, const void* x, const v
  * follows. y and h are rounded once; h is computed from y before its rounding.
  * Backward: dy is the gradient of y from elsewhere (null: none), dh the gradient of h (null: no norm behind the block; one of them is given).
  * dx, the gradient of x, is written always, dbranch where there is a branch, dgate, dpost and dpre where not null. Tensors of fewer than 2^31
- * elements; results must not share memory with operands. Sums over samples are fp32, in an order that depends on the sizes alone. */
+ * elements; results must not share memory with operands. The workspace is laid out as every call's (status word at its head) and 16-byte aligned. Sums
+ * over samples are fp32, in an order that depends on the sizes alone. */
 typedef struct pcb_norm_desc {
     int32_t dtype;            /* pcb_dtype of x, branch, gate, y, h and their gradients */
     int32_t algebra;          /* pcb_algebra */

@@ -37,6 +37,32 @@ void set_error(const char* fmt, ...) {
     va_end(ap);
 }
 
+// Status words that lie elsewhere than at the head of their workspace (pcb_set_status_word), by workspace address.
+static std::mutex g_word_mutex;
+static std::unordered_map<const void*, int*> g_words;
+static std::atomic<int> g_word_count{0};            // (looked at first: a program without such words takes no lock)
+int* status_of(const void* workspace) {
+    if (workspace && g_word_count.load(std::memory_order_acquire) > 0) {
+        std::lock_guard<std::mutex> lock(g_word_mutex);
+        const auto it = g_words.find(workspace);
+        if (it != g_words.end()) return it->second;
+    }
+    return static_cast<int*>(const_cast<void*>(workspace));
+}
+
+// Staged inputs kept by forward calls, by workspace address (host-side bookkeeping; the data itself lives in that workspace).
+// A forward call that stages x in the layout its filter gradient reads records (x, problem signature) under its workspace;
+// every later call that is given the same workspace erases the record before it writes there. pcb_qconv2d_bwd_kept reads the
+// staged copy only when the record still matches its own x and problem, and stages x itself otherwise.
+struct KeptInput { const void* x; unsigned long long signature; };
+static std::mutex g_kept_mutex;
+static std::unordered_map<const void*, KeptInput> g_kept;
+void forget_kept(const void* workspace) {
+    if (!workspace) return;
+    std::lock_guard<std::mutex> lock(g_kept_mutex);
+    g_kept.erase(workspace);
+}
+
 namespace {
 
 constexpr long long MAX_NUMEL = 2147483647LL;   // tensor offsets are 32-bit element indices inside kernels
@@ -121,22 +147,6 @@ int variant_for(const Geom& g, int variant) { return g.nc == 4 ? variant : (int)
 // kernels keep the problems the tensor cores do not take. PCB_ENGINE_TENSOR and PCB_ENGINE_SIMT take the variant literally.
 int tensor_variant(int variant, int engine) { return engine == PCB_ENGINE_AUTO ? (int)PCB_VARIANT_16_PRODUCT : variant; }
 
-// Layout of the caller's workspace: [0, 256) status block (first word: device wait status), then scratch.
-constexpr size_t WS_HEADER = 256;
-
-// Status words that lie elsewhere than at the head of their workspace (pcb_set_status_word), by workspace address.
-std::mutex g_word_mutex;
-std::unordered_map<const void*, int*> g_words;
-std::atomic<int> g_word_count{0};            // (looked at first: a program without such words takes no lock)
-int* status_of(const void* workspace) {
-    if (workspace && g_word_count.load(std::memory_order_acquire) > 0) {
-        std::lock_guard<std::mutex> lock(g_word_mutex);
-        const auto it = g_words.find(workspace);
-        if (it != g_words.end()) return it->second;
-    }
-    return static_cast<int*>(const_cast<void*>(workspace));
-}
-
 // Clears the device wait status at the start of an API call. Every kernel launched by the call only ORs into the
 // word, so pcb_check_device_status afterwards reports an expiry in ANY launch of the call, not just the last one.
 // A call that hands the reset to its first launch (StatusClear) settles it with finish_status: a call that launched nothing
@@ -156,24 +166,11 @@ int finish_status(StatusClear& sc, int rc, cudaStream_t stream) {
     return rc != PCB_OK ? rc : rs;
 }
 
-// Staged inputs kept by forward calls, by workspace address (host-side bookkeeping; the data itself lives in that workspace).
-// A forward call that stages x in the layout its filter gradient reads records (x, problem signature) under its workspace;
-// every later call that is given the same workspace erases the record before it writes there. pcb_qconv2d_bwd_kept reads the
-// staged copy only when the record still matches its own x and problem, and stages x itself otherwise.
-struct KeptInput { const void* x; unsigned long long signature; };
-std::mutex g_kept_mutex;
-std::unordered_map<const void*, KeptInput> g_kept;
-
 unsigned long long problem_signature(int dtype, const Geom& g) {
     const int v[] = {dtype, g.nc, g.ga, g.real_in, g.Nb, g.Ci, g.Co, g.H, g.W, g.KH, g.KW, g.SH, g.SW, g.DH, g.DW, g.PT, g.PL, g.HO, g.WO};
     unsigned long long h = 1469598103934665603ull;                   // FNV-1a over the geometry
     for (int x : v) { h ^= (unsigned long long)(unsigned)x; h *= 1099511628211ull; }
     return h;
-}
-void forget_kept(const void* workspace) {
-    if (!workspace) return;
-    std::lock_guard<std::mutex> lock(g_kept_mutex);
-    g_kept.erase(workspace);
 }
 void remember_kept(const void* workspace, const void* x, unsigned long long signature) {
     std::lock_guard<std::mutex> lock(g_kept_mutex);

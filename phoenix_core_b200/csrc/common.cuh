@@ -152,6 +152,12 @@ void set_error(const char* fmt, ...);
         }                                                                                       \
     } while (0)
 
+// Layout of the caller's workspace: [0, 256) status block (first word: device wait status), then scratch.
+constexpr size_t WS_HEADER = 256;
+// The word that calls given this workspace report expired waits into, and the end of any record of a staged input in it (api.cu): for every call that takes a workspace.
+int* status_of(const void* workspace);
+void forget_kept(const void* workspace);
+
 // Launchers implemented by the kernel translation units. Operand roles per pass:
 //   forward:         a = filters, b = input,          out = output
 //   backward-data:   a = filters, b = output gradient, out = input gradient

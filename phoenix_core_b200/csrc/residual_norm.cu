@@ -48,7 +48,7 @@ extern "C" {
 
 size_t pcb_residual_norm_bwd_workspace_size(const pcb_norm_desc* d) {
     if (check_norm(d) != PCB_OK || d->batch == 0) return 0;
-    return bwd_plan(norm_comps(d), d->batch, d->features, d->gate_rows, (int)dtype_size(d->dtype)).total;
+    return WS_HEADER + bwd_plan(norm_comps(d), d->batch, d->features, d->gate_rows, (int)dtype_size(d->dtype)).total;
 }
 
 int pcb_residual_norm_fwd(const pcb_norm_desc* d, const void* x, const void* branch, const void* gate, const float* post, const float* pre, void* y, void* h,
@@ -86,16 +86,19 @@ int pcb_residual_norm_bwd(const pcb_norm_desc* d, const void* y, const void* bra
         return PCB_ERR_INVALID_ARGUMENT;
     }
     const RNPlan q = bwd_plan(comps, d->batch, d->features, d->gate_rows, (int)dtype_size(d->dtype));
-    if (!workspace || workspace_bytes < q.total) { set_error("workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : (size_t)0, q.total); return PCB_ERR_WORKSPACE; }
+    const size_t need = WS_HEADER + q.total;
+    if (!workspace || workspace_bytes < need) { set_error("workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : (size_t)0, need); return PCB_ERR_WORKSPACE; }
     if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) { set_error("the workspace must be 16-byte aligned"); return PCB_ERR_INVALID_ARGUMENT; }
     RNParams p = norm_params(d);
     const size_t size = dtype_size(d->dtype), row = (size_t)comps * d->batch * d->features * size, gates = (size_t)comps * d->gate_rows * d->features * size, weight = (size_t)d->features * 4;
-    const Span results[] = {{dx, row}, {dbranch, branch ? row : 0}, {dgate, gates}, {dpost, weight}, {dpre, weight}, {workspace, q.total}};
+    const Span results[] = {{dx, row}, {dbranch, branch ? row : 0}, {dgate, gates}, {dpost, weight}, {dpre, weight}, {workspace, need}};
     const Span operands[] = {{dh ? y : nullptr, row}, {branch, row}, {gate, gates}, {post, weight}, {pre, weight}, {stats, (size_t)d->batch * 8}, {dy, row}, {dh, row}};
     if (const int apart = check_apart(results, 6, operands, 8)) return apart;
     p.branch = branch; p.gate = gate; p.post = post; p.pre = pre; p.y = const_cast<void*>(y); p.stats = const_cast<float*>(stats);
     p.dy = dy; p.dh = dh; p.dx = dx; p.dbranch = dbranch; p.dgate = dgate; p.dpost = dpost; p.dpre = dpre;
-    p.workspace = static_cast<uint8_t*>(workspace);
+    forget_kept(workspace);
+    p.workspace = static_cast<uint8_t*>(workspace) + WS_HEADER;
+    p.status = status_of(workspace);
     if (!gate) p.per_group = d->batch;
     if (d->dtype == PCB_F32) return norm_bwd_f32(p, q, s);
     return d->dtype == PCB_F16 ? norm_bwd_f16(p, q, s) : norm_bwd_bf16(p, q, s);

@@ -381,6 +381,7 @@ __global__ void __launch_bounds__(32 * WPR * ROWS, 1) residual_norm_bwd_kernel(c
     const R r(smem_u32(ring_smem), p, cls);
     chain_wait();
     chain_next();
+    if (blockIdx.x == 0 && threadIdx.x == 0) *p.status = 0;
     r.hold_weights(p);
     const float inv_width = 1.f / (float)r.width;
     const int slots = of * R::ROWS, slot = rank * R::ROWS + threadIdx.x / R::TPR;
@@ -599,6 +600,7 @@ __global__ void __launch_bounds__(RN_WIDE_THREADS) residual_norm_bwd_wide_kernel
     int turn = 0;
     chain_wait();
     chain_next();
+    if (blockIdx.x == 0 && threadIdx.x == 0) *p.status = 0;
     const size_t F = p.features, N = p.n, width = (size_t)p.comps * F;
     const float inv_width = 1.f / (float)width;
     float* mine = p.part_w ? p.part_w + (size_t)blockIdx.x * 2 * width : nullptr;     // this CTA's sums, each element one thread's

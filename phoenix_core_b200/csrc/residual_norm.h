@@ -18,7 +18,8 @@ struct RNParams {
     const void *dy, *dh;
     void *dx, *dbranch, *dgate;
     float *dpost, *dpre;
-    uint8_t* workspace;
+    uint8_t* workspace;                            // where the sums lie
+    int* status;                                   // the call's status word, which the first CTA resets (the call has no waits to report)
     float *part_w;                                 // [CTAs][2][comps * features]: dpre, dpost
     float *part_gate;                              // [groups * parts][comps * features]
     int parts, pieces, items;                      // per group: sums that make its gate's gradient, pieces of each class's rows; pieces in all

@@ -119,5 +119,7 @@ def residualNormBwd(outputTensor, branchTensor, gateTensor, postWeight, preWeigh
         return
     dev = Device.at(index)
     with dev.accessControl:
-        ws = dev.requestWorkspace(need + 256)                          # behind the workspace's status block
-        bwd.call(ws, 256, *operands)
+        ws = dev.requestWorkspace(need)
+        bwd.call(ws, 0, *operands)
+        if dev.check_after_each_op:
+            dev.checkStatus()
