@@ -260,7 +260,7 @@ int pcb_selftest_wait_expiry(const pcb_conv2d_desc* desc, const void* x, const v
  * Backward: dy is the gradient of y from elsewhere (null: none), dh the gradient of h (null: no norm behind the block; one of them is given).
  * dx, the gradient of x, is written always, dbranch where there is a branch, dgate, dpost and dpre where not null. Tensors of fewer than 2^31
  * elements; results must not share memory with operands. The workspace is laid out as every call's (status word at its head) and 16-byte aligned. Sums
- * over samples are fp32, in an order that depends on the sizes alone. */
+ * over samples are fp32, in an order that depends on the sizes and the SM margin alone. */
 typedef struct pcb_norm_desc {
     int32_t dtype;            /* pcb_dtype of x, branch, gate, y, h and their gradients */
     int32_t algebra;          /* pcb_algebra */
@@ -333,7 +333,7 @@ int pcb_aux_bn_relu_maxpool_bwd(int dtype, const void* x, const void* dy, const 
 int pcb_aux_maxpool3x3s2_fwd(int dtype, const void* x, void* y, void* argmax, int rows, int h, int w, void* stream);
 int pcb_aux_maxpool3x3s2_bwd(int dtype, const void* dy, const void* argmax, void* dx, int rows, int h, int w, void* stream);
 
-/* Deployment knob (no reference counterpart): the persistent tensor-core kernels occupy every SM with one CTA each; with a margin
+/* Deployment knob (no reference counterpart): the persistent kernels (tensor cores, block norms) occupy every SM with one CTA each; with a margin
  * of `sms` (0 .. 64, process-wide, default 0) they size their grids for that many SMs fewer, so that a kernel enqueued on another
  * stream -- a data-parallel all-reduce of the filter gradient beside backward-data -- finds SMs to run on instead of waiting
  * for a CTA to retire. Takes effect from the next call. */

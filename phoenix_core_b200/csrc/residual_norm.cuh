@@ -743,25 +743,25 @@ cudaError_t fwd_any(const RNParams& p, const RNShape& k, cudaStream_t s) {
     return k.warps == 8 ? fwd_launch<T, VEC, ALIGNED, 32, 8, 1>(p, s) : fwd_launch<T, VEC, ALIGNED, 32, 16, 1>(p, s);
 }
 template <typename T, int VEC, bool ALIGNED, int EPT, int WPR, int ROWS, int GATE>
-cudaError_t bwd_gate(const RNParams& p, const RNPlan& q, cudaStream_t s) {
+cudaError_t bwd_gate(const RNParams& p, int grid, cudaStream_t s) {
     typedef BwdRow<T, VEC, ALIGNED, EPT, WPR, ROWS, GATE> R;
-    return norm_launch<residual_norm_bwd_kernel<T, VEC, ALIGNED, EPT, WPR, ROWS, GATE>>(q.grid, R::THREADS, R::SMEM, s, p);
+    return norm_launch<residual_norm_bwd_kernel<T, VEC, ALIGNED, EPT, WPR, ROWS, GATE>>(grid, R::THREADS, R::SMEM, s, p);
 }
 template <typename T, int VEC, bool ALIGNED, int EPT, int WPR, int ROWS>
-cudaError_t bwd_launch(const RNParams& p, const RNPlan& q, cudaStream_t s) {
-    if (!p.gate) return bwd_gate<T, VEC, ALIGNED, EPT, WPR, ROWS, 0>(p, q, s);
-    return p.groups == p.n ? bwd_gate<T, VEC, ALIGNED, EPT, WPR, ROWS, 1>(p, q, s) : bwd_gate<T, VEC, ALIGNED, EPT, WPR, ROWS, 2>(p, q, s);
+cudaError_t bwd_launch(const RNParams& p, int grid, cudaStream_t s) {
+    if (!p.gate) return bwd_gate<T, VEC, ALIGNED, EPT, WPR, ROWS, 0>(p, grid, s);
+    return p.groups == p.n ? bwd_gate<T, VEC, ALIGNED, EPT, WPR, ROWS, 1>(p, grid, s) : bwd_gate<T, VEC, ALIGNED, EPT, WPR, ROWS, 2>(p, grid, s);
 }
 template <typename T, int VEC, bool ALIGNED>
-cudaError_t bwd_any(const RNParams& p, const RNPlan& q, cudaStream_t s) {
-    switch (q.shape.warps) {
-        case 1: return q.shape.values == 8 ? bwd_launch<T, VEC, ALIGNED, 8, 1, 16>(p, q, s) : bwd_launch<T, VEC, ALIGNED, 16, 1, 12>(p, q, s);
-        case 2: return bwd_launch<T, VEC, ALIGNED, 16, 2, 6>(p, q, s);
-        case 3: return bwd_launch<T, VEC, ALIGNED, 16, 3, 4>(p, q, s);
-        case 4: return bwd_launch<T, VEC, ALIGNED, 16, 4, 3>(p, q, s);
-        case 5: return bwd_launch<T, VEC, ALIGNED, 16, 5, 3>(p, q, s);
-        case 8: return bwd_launch<T, VEC, ALIGNED, 16, 8, 2>(p, q, s);
-        default: return bwd_launch<T, VEC, ALIGNED, 16, 16, 1>(p, q, s);
+cudaError_t bwd_any(const RNParams& p, const RNShape& k, int grid, cudaStream_t s) {
+    switch (k.warps) {
+        case 1: return k.values == 8 ? bwd_launch<T, VEC, ALIGNED, 8, 1, 16>(p, grid, s) : bwd_launch<T, VEC, ALIGNED, 16, 1, 12>(p, grid, s);
+        case 2: return bwd_launch<T, VEC, ALIGNED, 16, 2, 6>(p, grid, s);
+        case 3: return bwd_launch<T, VEC, ALIGNED, 16, 3, 4>(p, grid, s);
+        case 4: return bwd_launch<T, VEC, ALIGNED, 16, 4, 3>(p, grid, s);
+        case 5: return bwd_launch<T, VEC, ALIGNED, 16, 5, 3>(p, grid, s);
+        case 8: return bwd_launch<T, VEC, ALIGNED, 16, 8, 2>(p, grid, s);
+        default: return bwd_launch<T, VEC, ALIGNED, 16, 16, 1>(p, grid, s);
     }
 }
 template <typename T, int VEC>
@@ -779,11 +779,13 @@ int bwd_typed(RNParams p, RNPlan q, cudaStream_t s) {
     const bool wide = q.shape.warps == 0 || !aligned_bases(p);
     if (wide) q = q.shape.warps == 0 ? q : wide_plan(p.comps, p.n, p.features, p.gate ? p.groups : 0);
     p.parts = q.parts; p.pieces = q.pieces; p.items = q.items;
+    // (beside an SM margin fewer CTAs take the same pieces: the plan, and with it the workspace, is that of the whole device)
+    const int grid = wide ? (q.grid < 4 * sm_count() ? q.grid : 4 * sm_count()) : ctas_beside(q.grid, p.period, sm_count());
     p.part_w = p.dpost || p.dpre ? reinterpret_cast<float*>(p.workspace) : nullptr;
     p.part_gate = p.dgate && q.part_gate ? reinterpret_cast<float*>(p.workspace + q.part_w) : nullptr;
-    if (wide) PCB_CUDA_TRY(launch_chained(residual_norm_bwd_wide_kernel<T>, q.grid, RN_WIDE_THREADS, 0, s, p));
-    else if (p.period == 1) PCB_CUDA_TRY((bwd_any<T, VEC, true>(p, q, s)));
-    else PCB_CUDA_TRY((bwd_any<T, VEC, false>(p, q, s)));
+    if (wide) PCB_CUDA_TRY(launch_chained(residual_norm_bwd_wide_kernel<T>, grid, RN_WIDE_THREADS, 0, s, p));
+    else if (p.period == 1) PCB_CUDA_TRY((bwd_any<T, VEC, true>(p, q.shape, grid, s)));
+    else PCB_CUDA_TRY((bwd_any<T, VEC, false>(p, q.shape, grid, s)));
     const long long weight_blocks = p.part_w ? (p.features + 7) / 8 : 0;
     // threads per value of a gate: up to two values' worth for every SM's 2048, while each has two parts at least (5358 x 174, one gate: 17 us, 177 by one thread each; 16384 x 4096,
     // 16 gates of 111 parts: 13 us, 47 with 64 each)
@@ -792,7 +794,7 @@ int bwd_typed(RNParams p, RNPlan q, cudaStream_t s) {
     const int values = RN_SUM_THREADS / slices;
     const long long gate_blocks = p.part_gate ? ((long long)p.groups * p.comps * p.features + values - 1) / values : 0;
     if (weight_blocks + gate_blocks > 0)
-        PCB_CUDA_TRY(launch_chained(residual_norm_sum_kernel<T>, (unsigned)(weight_blocks + gate_blocks), RN_SUM_THREADS, 0, s, p, q.grid, (int)weight_blocks, slices));
+        PCB_CUDA_TRY(launch_chained(residual_norm_sum_kernel<T>, (unsigned)(weight_blocks + gate_blocks), RN_SUM_THREADS, 0, s, p, grid, (int)weight_blocks, slices));
     return PCB_OK;
 }
 
