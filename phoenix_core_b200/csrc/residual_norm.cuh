@@ -641,6 +641,7 @@ __global__ void __launch_bounds__(RN_WIDE_THREADS) residual_norm_bwd_wide_kernel
                         const float dn = p.gate ? sdx * at<T>(p.gate, (c * (size_t)p.groups + group) * F + f) : sdx, dg = sdx * u * w;
                         if (mine) mine[width + c * F + f] = fmaf(dn, u, mine[width + c * F + f]);
                         if (gates) gates[c * F + f] = row == begin ? dg : gates[c * F + f] + dg;
+                        else if (p.dgate) put<T>(p.dgate, (c * (size_t)p.groups + group) * F + f, dg);       // (a gate for each value)
                         sum = fmaf(dn * w, u, sum);
                     }
                 fb = row_sum<WPR>(sum, words, turn) * inv_width * rb;

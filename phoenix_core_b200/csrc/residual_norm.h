@@ -75,9 +75,10 @@ inline int pieces_of(int groups, int per, long long most) {
     }
     return pieces;
 }
+// (A gate for each value has no sums over samples: its gradient is written where it is made.)
 inline void sums_of(RNPlan& q, long long width, int gates, int n) {
     q.part_w = (size_t)q.grid * 2 * width * 4;
-    q.part_gate = gates > 0 && (q.shape.warps == 0 || (gates < n && q.parts > 1)) ? (size_t)gates * q.parts * width * 4 : 0;
+    q.part_gate = gates > 0 && gates < n && (q.shape.warps == 0 || q.parts > 1) ? (size_t)gates * q.parts * width * 4 : 0;
     q.total = q.part_w + q.part_gate;
 }
 // Rows wider than the registers, tensors that start anywhere, and groups of fewer rows than there are places for them to start at: four CTAs on an SM, a row each.

@@ -69,3 +69,34 @@ def test_a_staged_input_is_forgotten(gpu, shape):
     # the same kernel on the same staged values; only the order of the atomic additions may differ (as where kept and plain backward passes are compared)
     got = gpu.host(t["dw"])
     assert np.abs(got - want).max() <= 1e-3 * np.abs(want).max()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("algebra,n,f", [("real", 40, 8200), ("real", 1300, 8193), ("quaternion", 9, 2100), ("complex", 7, 5001)])
+def test_gates_of_wide_rows(algebra, n, f, dtype):
+    """A gate for each value, and shared ones, of rows wider than the registers."""
+    from test_gpu_residual_norm import Case
+    for gates in (n, 1):
+        Case(algebra, dtype, n, f, gates).check()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_gates_that_start_anywhere(dtype):
+    """The same of tensors that do not start on 16 bytes, which take the same kernel whatever their width."""
+    import phoenix_core_b200 as pcb
+    from test_gpu_block_edges import guarded, shifted
+    from test_gpu_residual_norm import Case
+    case = Case("real", dtype, 300, 130, 300)
+    y, _, stats, want = case.run()
+    b, g, post, pre, dy, dh = (t.cuda() for t in (case.branch, case.gate, case.post, case.pre, case.dy, case.dh))
+    out = {k: shifted(want[k], 1, float("nan")) for k in ("dx", "db", "dgate", "dpost", "dpre")}
+    pcb.residualNormBwd(y, b, g, post, pre, stats, dy, dh, *(out[k][1] for k in ("dx", "db", "dgate", "dpost", "dpre")), case.desc)
+    torch.cuda.synchronize()
+    width = case.f
+    for k, (whole, got) in out.items():
+        assert guarded(whole, 1, got.numel()), k
+        # each side is within its own bound of the definition (Case.check): chains of 64 + width / 32 steps of 2^-24, three of them, of terms that are no larger than
+        # eight times the largest result here, and one rounding each
+        step = torch.finfo(got.dtype).eps
+        count = case.n if k in ("dpost", "dpre") else 0
+        assert ((got.double() - want[k].double()).abs() <= step * want[k].double().abs() + 2 * (3 * (64 + width / 32) + count) * 2.0 ** -24 * 8 * want[k].double().abs().max()).all(), k
