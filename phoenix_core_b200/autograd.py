@@ -157,15 +157,18 @@ class ResidualNormFunction(torch.autograd.Function):
         if dy is None and dh is None:
             return (None,) * 8
         dy, dh = (None if t is None else t.contiguous() for t in (dy, dh))
-        if dh is None:                                     # nothing came back through the norm behind the block
-            dh = torch.zeros_like(y)
         need = ctx.needs_input_grad
         dx = torch.empty_like(y)
         db = None if branch is None else torch.empty_like(branch)
         dgate = torch.empty_like(gate) if gate is not None and need[2] else None
         dpost = torch.empty_like(post) if post is not None and need[3] else None
         dpre = torch.empty_like(pre) if pre is not None and need[4] else None
-        residualNormBwd(y, branch, gate, post, pre, stats, dy, dh, dx, db, dgate, dpost, dpre, ctx.descriptor)
+        if dh is None:                                     # nothing came back through the norm behind the block
+            residualNormBwd(y, branch, gate, post, None, stats, dy, None, dx, db, dgate, dpost, None, ctx.descriptor)
+            if dpre is not None:
+                dpre.zero_()
+        else:
+            residualNormBwd(y, branch, gate, post, pre, stats, dy, dh, dx, db, dgate, dpost, dpre, ctx.descriptor)
         return dx, db, dgate, dpost, dpre, None, None, None
 
 
