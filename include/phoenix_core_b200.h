@@ -281,8 +281,9 @@ int pcb_residual_norm_bwd(const pcb_norm_desc* desc, const void* y, const void* 
  *   loss = (1 - alpha) * cross_entropy(logits, label) + alpha * T^2 * sum_i p_i (log p_i - log q_i)
  * `teacher` and `index` are [batch, entries]: logits (of the type of `logits`) and their classes, in any order; an entry whose class is outside
  * [0, D * units) is left out, a class named twice counts twice. `labels` is [batch]; one outside the classes leaves the first term out. A sample without an entry
- * has no second term, one whose logits are all -infinity counts for nothing. labels may be null, and so may teacher and index with entries 0; their term is then
- * left out. `loss` is fp32 [batch]. `stats` (fp32 [3][batch], may be null) is kept for the backward call: maximum, sum of
+ * (or of entries of -infinity alone) has no second term, one whose logits are all -infinity counts for nothing; a NaN in a sample's entries or logits
+ * reaches the terms that it has. labels may be null, and so may teacher and index with entries 0; their term is then left out. `loss` is fp32 [batch].
+ * `stats` (fp32 [3][batch], may be null) is kept for the backward call: maximum, sum of
  * exp(z - max), sum of exp((z - max) / T), infinity in place of a sum that the gradient has no term of.
  * Backward: dlogits = grad_loss[sample] * d loss / d logits; must not share memory with the logits. Up to 4096 entries, D * units < 2^31. */
 typedef struct pcb_distill_desc {

@@ -386,9 +386,10 @@ __global__ void __launch_bounds__(THREADS, di_ctas(THREADS)) distill_fwd_kernel(
     bool any = false;
     if (KIND != DI_HARD && !none) {
         float peak = -INFINITY;
-        for (int i = lane; i < p.entries; i += 32) { float x; if (entry<T>(p, row, i, x) >= 0) { any = true; peak = fmaxf(peak, x); } }
+        // (entries with weight: minus infinity has none, and a NaN, which is no maximum, is to be seen)
+        for (int i = lane; i < p.entries; i += 32) { float x; if (entry<T>(p, row, i, x) >= 0) { any = any || x != -INFINITY; peak = fmaxf(peak, x); } }
         peak = warp_max(peak);
-        any = __any_sync(0xffffffffu, any) && peak != -INFINITY;
+        any = __any_sync(0xffffffffu, any);
         float total = 0.f;
         for (int i = lane; i < p.entries; i += 32) { float x; if (entry<T>(p, row, i, x) >= 0 && any) total += ex2((x - peak) * LOG2E); }
         total = warp_sum(total);
