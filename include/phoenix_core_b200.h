@@ -285,7 +285,8 @@ int pcb_residual_norm_bwd(const pcb_norm_desc* desc, const void* y, const void* 
  * reaches the terms that it has. labels may be null, and so may teacher and index with entries 0; their term is then left out. `loss` is fp32 [batch].
  * `stats` (fp32 [3][batch], may be null) is kept for the backward call: maximum, sum of
  * exp(z - max), sum of exp((z - max) / T), infinity in place of a sum that the gradient has no term of.
- * Backward: dlogits = grad_loss[sample] * d loss / d logits; must not share memory with the logits. Up to 4096 entries, D * units < 2^31. */
+ * Backward: dlogits = grad_loss[sample] * d loss / d logits; must not share memory with the logits. Up to 4096 entries, D * units < 2^31;
+ * 1 / T and T^2 are to be fp32 numbers. */
 typedef struct pcb_distill_desc {
     int32_t dtype;            /* pcb_dtype of logits, teacher, dlogits */
     int32_t algebra;          /* pcb_algebra: components of the layer that made the logits */
