@@ -216,6 +216,15 @@ int pcb_qdense8_fwd(const pcb_dense_desc* desc, const void* x, const void* w8, c
                     void* workspace, size_t workspace_bytes, void* stream);
 int pcb_qdense8_bwd(const pcb_dense_desc* desc, const void* x, const void* w8, const void* w8_scales, const void* dy, void* dw, void* dx,
                     void* workspace, size_t workspace_bytes, void* stream);
+/* The form of the kernel that a call takes for a product (pass: 0 forward, 1 backward-data, 2 backward-filter), by its sizes and the SM margin. Negative = status. */
+typedef enum {
+    PCB_DENSE8_TOKENS = 1,          /* up to four tokens, quantised by the product itself */
+    PCB_DENSE8_FILTER_FIRST = 2,    /* up to 64 tokens: tiles of 128 features x 16 or 64 tokens */
+    PCB_DENSE8_TILES = 3,           /* tiles of 128 x 128, the reduction cut over a cluster where there are few */
+    PCB_DENSE8_PAIRS = 4,           /* tiles of 256 x 256 on pairs of SMs */
+    PCB_DENSE8_BOTH_GRADIENTS = 5   /* both gradients in one launch of tiles of 128 x 128 */
+} pcb_dense8_form;
+int pcb_qdense8_form_for(const pcb_dense_desc* desc, int pass);
 
 /* Which kernel family a forward / backward call with this descriptor will run: 1 = CUDA-core fp32,
  * 2 = tcgen05 tensor-core. pass: 0 forward, 1 backward-data, 2 backward-filter. Negative = status.

@@ -78,6 +78,7 @@ SYMBOLS = {
     "pcb_qdense8_bwd_workspace_size": (_sz, [_dd]),
     "pcb_qdense8_fwd": (_i, [_dd, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "pcb_qdense8_bwd": (_i, [_dd, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "pcb_qdense8_form_for": (_i, [_dd, _i]),
     "pcb_residual_norm_fwd": (_i, [_nd] + [_vp] * 9),
     "pcb_residual_norm_bwd_workspace_size": (_sz, [_nd]),
     "pcb_residual_norm_bwd": (_i, [_nd] + [_vp] * 14 + [_sz, _vp]),

@@ -459,6 +459,13 @@ Q8Operand dense8_filter(const Geom& g, const void* values, const void* scales, b
     o.bytes_mn = o.mn_major ? 1 : row_stride;
     return o;
 }
+// A product of the layer: tokens by the filter, or for the filter gradient x by dy (both as they lie).
+Q8Product dense8_product(const Geom& g, Pass pass, const Q8Operand& first, const Q8Operand& second, void* out, int dtype, int* status) {
+    if (pass == PASS_BWD_FILTER) return {pass, 0, g.Ci, g.Co, g.Nb, first, second, out, dtype, nullptr, status};
+    const int features = pass == PASS_FWD ? g.Co : g.Ci, summed = pass == PASS_FWD ? g.Ci : g.Co;
+    if (q8_swapped(g.Nb)) return {pass, 1, features, g.Nb, summed, second, first, out, dtype, nullptr, status};
+    return {pass, 0, g.Nb, features, summed, first, second, out, dtype, nullptr, status};
+}
 int dense8_check_filter(const void* values) {
     if (reinterpret_cast<uintptr_t>(values) % 16 != 0) { set_error("8-bit filter values must be 16-byte aligned"); return PCB_ERR_INVALID_ARGUMENT; }
     return PCB_OK;
@@ -727,6 +734,17 @@ size_t pcb_qdense8_bwd_workspace_size(const pcb_dense_desc* desc) {
     Geom g;
     return dense8_geom(desc, g) == PCB_OK ? dense8_space(g, true, desc->require_input_grad != 0).total : 0;
 }
+int pcb_qdense8_form_for(const pcb_dense_desc* desc, int pass) {
+    Geom g;
+    const int rc = dense8_geom(desc, g);
+    if (rc != PCB_OK) return rc;
+    if (pass < 0 || pass > 2 || (pass == 1 && !desc->require_input_grad)) { set_error("pass must be 0, 2 or, with an input gradient, 1"); return PCB_ERR_INVALID_ARGUMENT; }
+    if (g.Nb == 0) { set_error("no samples: nothing is launched"); return PCB_ERR_INVALID_ARGUMENT; }
+    auto sizes = [&](Pass p) { return dense8_product(g, p, Q8Operand{}, Q8Operand{}, nullptr, desc->dtype, nullptr); };
+    if (pass != 0 && desc->require_input_grad && q8_together(g, sizes(PASS_BWD_FILTER), sizes(PASS_BWD_DATA))) return PCB_DENSE8_BOTH_GRADIENTS;
+    int splits;
+    return q8_form(g, sizes(pass == 0 ? PASS_FWD : (pass == 1 ? PASS_BWD_DATA : PASS_BWD_FILTER)), &splits);
+}
 int pcb_qdense8_fwd(const pcb_dense_desc* desc, const void* x, const void* w8, const void* w8_scales, const void* bias, void* y, void* workspace,
                     size_t workspace_bytes_, void* stream) {
     Geom g;
@@ -745,8 +763,8 @@ int pcb_qdense8_fwd(const pcb_dense_desc* desc, const void* x, const void* w8, c
     const bool raw = q8_raw_tokens(g.Nb);
     if (!raw && (rc = q8_quantize_rows(desc->dtype, g.nc, g.Nb, g.Ci, x, rows, status, (cudaStream_t)stream)) != PCB_OK) return rc;
     const Q8Operand tokens = {rows.values, rows.words, q8_pitch(g.Ci), 0, 0, 0, 0}, filter = dense8_filter(g, w8, w8_scales, true);
-    Q8Product q = {PASS_FWD, q8_swapped(g.Nb) ? 1 : 0, g.Nb, g.Co, g.Ci, tokens, filter, y, desc->dtype, g.has_bias ? bias : nullptr, status};
-    if (q.swapped) { q.m = g.Co; q.n = g.Nb; q.a = filter; q.b = tokens; }
+    Q8Product q = dense8_product(g, PASS_FWD, tokens, filter, y, desc->dtype, status);
+    if (g.has_bias) q.bias = bias;
     if (raw) q.tokens = x;
     return q8_product(g, q, (cudaStream_t)stream);
 }
@@ -773,11 +791,10 @@ int pcb_qdense8_bwd(const pcb_dense_desc* desc, const void* x, const void* w8, c
     const Q8Target x_cols = {ws + at.x_cols, reinterpret_cast<uint32_t*>(ws + at.x_col_words)};
     if ((rc = q8_quantize_backward(desc->dtype, g.nc, g.Nb, g.Ci, g.Co, x, dy, x_cols, dy_rows, dy_cols, status, st)) != PCB_OK) return rc;
     const Q8Operand a = {x_cols.values, x_cols.words, q8_pitch(g.Ci), 0, 0, 0, 1}, b = {dy_cols.values, dy_cols.words, q8_pitch(g.Co), 0, 0, 0, 1};
-    const Q8Product of_filter = {PASS_BWD_FILTER, 0, g.Ci, g.Co, g.Nb, a, b, dw, desc->dtype, nullptr, status};
+    const Q8Product of_filter = dense8_product(g, PASS_BWD_FILTER, a, b, dw, desc->dtype, status);
     if (!need_dx) return q8_product(g, of_filter, st);
     const Q8Operand tokens = {dy_rows.values, dy_rows.words, q8_pitch(g.Co), 0, 0, 0, 0}, filter = dense8_filter(g, w8, w8_scales, false);
-    Q8Product q = {PASS_BWD_DATA, q8_swapped(g.Nb) ? 1 : 0, g.Nb, g.Ci, g.Co, tokens, filter, dx, desc->dtype, nullptr, status};
-    if (q.swapped) { q.m = g.Ci; q.n = g.Nb; q.a = filter; q.b = tokens; }
+    const Q8Product q = dense8_product(g, PASS_BWD_DATA, tokens, filter, dx, desc->dtype, status);
     return q8_two_products(g, of_filter, q, st);
 }
 

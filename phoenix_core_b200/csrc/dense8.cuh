@@ -48,8 +48,11 @@ int q8_quantize_backward(int dtype, int comps, int rows, int x_cols, int dy_cols
                          int* status_to_clear, cudaStream_t stream);
 int q8_quantize_blocks(int dtype, int comps, int rows, int cols, const void* x, uint8_t* values, uint8_t* scales, cudaStream_t stream);
 int q8_product(const Geom& g, const Q8Product& p, cudaStream_t stream);
+// The form (pcb_dense8_form) that q8_product takes, and the CTAs that share a tile: of the product's sizes alone.
+int q8_form(const Geom& g, const Q8Product& p, int* splits);
 // The two gradients of a backward call, in one launch or two.
 int q8_two_products(const Geom& g, const Q8Product& first, const Q8Product& second, cudaStream_t stream);
+bool q8_together(const Geom& g, const Q8Product& first, const Q8Product& second);
 // Whether a forward or backward-data product of that many tokens takes the filter as operand A.
 bool q8_swapped(int tokens);
 // Whether the product quantises that many tokens itself.

@@ -329,7 +329,7 @@ __device__ __forceinline__ void d8_quantize_tokens(const D8Params& p, uint32_t b
 // The waits look at a status word of the CTA's own; the call's gets it at the end.
 template <int BN, bool SWAP, bool PAIR, bool RAW, int N>
 __global__ void __launch_bounds__(D8_THREADS, 1) dense8_kernel(const __grid_constant__ D8Args<N> args, int* call_status) {
-    static_assert(!RAW || (SWAP && BN == 16), "raw tokens: up to 16");
+    static_assert(!RAW || (SWAP && BN == 16 && D8_RAW <= BN), "raw tokens lie in one narrow tile");
     using C = D8Config<BN, SWAP, PAIR>;
     extern __shared__ uint8_t smem_raw[];
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
@@ -865,36 +865,48 @@ bool q8_raw_tokens(int tokens) { return tokens <= D8_RAW; }
 // copies and epilogue; a pair's of 256 x 256 0.34 a block behind 12; a reduction cut over a cluster 3.5 more. 2048 x 4096 -> 4096: pairs 33.9, single 44.4;
 // 1024 x 4096 -> 4096 24.4 / 25.5; 2048 x 1024 -> 4096 18.0 / 17.4; 512 x 4096 -> 4096 23.0 / 16.1; GA(3,0,0) 4608 x 512 -> 768 85.5 / 129.8. Cut in two and not, 300 x 4096 -> 2048 14.0 / 14.6; 512 x 1024 ->
 // 1024 10.6 / 8.6.
-int q8_product(const Geom& g, const Q8Product& q, cudaStream_t stream) {
-    if (q.tokens) return launch<16, true, false, true>(g, q, splits_for(g, q, 16), stream);
+int q8_form(const Geom& g, const Q8Product& q, int* splits) {
+    *splits = 1;
     if (q.swapped) {
-        if (q.n <= 16) return launch<16, true, false>(g, q, splits_for(g, q, 16), stream);
-        return launch<64, true, false>(g, q, splits_for(g, q, 64), stream);
+        *splits = splits_for(g, q, q.n <= 16 ? 16 : 64);
+        return q8_raw_tokens(q.n) && q.pass == PASS_FWD ? PCB_DENSE8_TOKENS : PCB_DENSE8_FILTER_FIRST;
     }
     double single = 0.0;
-    const int splits = splits_for(g, q, 128, &single);
-    if (pair_cost(g, q) < single) return launch<256, false, true>(g, q, 1, stream);
-    return launch<128, false, false>(g, q, splits, stream);
+    const int cut = splits_for(g, q, 128, &single);
+    if (pair_cost(g, q) < single) return PCB_DENSE8_PAIRS;
+    *splits = cut;
+    return PCB_DENSE8_TILES;
+}
+int q8_product(const Geom& g, const Q8Product& q, cudaStream_t stream) {
+    int splits;
+    switch (q8_form(g, q, &splits)) {
+        case PCB_DENSE8_TOKENS: return launch<16, true, false, true>(g, q, splits, stream);
+        case PCB_DENSE8_FILTER_FIRST: return q.n <= 16 ? launch<16, true, false>(g, q, splits, stream) : launch<64, true, false>(g, q, splits, stream);
+        case PCB_DENSE8_PAIRS: return launch<256, false, true>(g, q, 1, stream);
+        default: return launch<128, false, false>(g, q, splits, stream);
+    }
 }
 
 // Both gradients in one launch where that is the cheaper by the costs above: tiles of 128 x 128, dealt to the CTAs in turn. A second launch costs its 7.5 us less some 2 that lie
 // beside the end of the first. Measured, f16, with the quantisation in front: quaternion 777 x 500 -> 1001 36.6 us, 42.7 in two launches; 256 x 512 -> 512 13.2 / 19.7; real 4096 x 1024 -> 1024
 // 25.7 / 29.9; complex 6096 x 389 -> 3136, which the costs call equal, 156.8 / 146.8: hence the margin.
-int q8_two_products(const Geom& g, const Q8Product& first, const Q8Product& second, cudaStream_t stream) {
-    if (!first.swapped && !second.swapped) {
-        double a = 0.0, b = 0.0;
-        splits_for(g, first, 128, &a);
-        splits_for(g, second, 128, &b);
-        const double apart = fmin(a, pair_cost(g, first)) + fmin(b, pair_cost(g, second)) - 2.0;
-        const long long sms = sm_count(), t0 = (long long)q8_blocks(first.m) * q8_blocks(first.n) * g.nc, all = t0 + (long long)q8_blocks(second.m) * q8_blocks(second.n) * g.nc;
-        // the CTA with the most to do is the first, or the first that has one tile fewer of either
-        double most = 0.0;
-        for (long long i : {0LL, t0 % sms, all % sms}) {
-            const long long ours = (t0 - i + sms - 1) / sms, both = (all - i + sms - 1) / sms;
-            most = fmax(most, (double)(ours * q8_blocks(first.k) + (both - ours) * q8_blocks(second.k)) * g.nc);
-        }
-        if (7.5 + most * 0.27 < 0.85 * apart) return launch_two<128>(g, first, second, stream);
+bool q8_together(const Geom& g, const Q8Product& first, const Q8Product& second) {
+    if (first.swapped || second.swapped) return false;
+    double a = 0.0, b = 0.0;
+    splits_for(g, first, 128, &a);
+    splits_for(g, second, 128, &b);
+    const double apart = fmin(a, pair_cost(g, first)) + fmin(b, pair_cost(g, second)) - 2.0;
+    const long long sms = sm_count(), t0 = (long long)q8_blocks(first.m) * q8_blocks(first.n) * g.nc, all = t0 + (long long)q8_blocks(second.m) * q8_blocks(second.n) * g.nc;
+    // the CTA with the most to do is the first, or the first that has one tile fewer of either
+    double most = 0.0;
+    for (long long i : {0LL, t0 % sms, all % sms}) {
+        const long long ours = (t0 - i + sms - 1) / sms, both = (all - i + sms - 1) / sms;
+        most = fmax(most, (double)(ours * q8_blocks(first.k) + (both - ours) * q8_blocks(second.k)) * g.nc);
     }
+    return 7.5 + most * 0.27 < 0.85 * apart;
+}
+int q8_two_products(const Geom& g, const Q8Product& first, const Q8Product& second, cudaStream_t stream) {
+    if (q8_together(g, first, second)) return launch_two<128>(g, first, second, stream);
     const int rc = q8_product(g, first, stream);
     return rc != PCB_OK ? rc : q8_product(g, second, stream);
 }
