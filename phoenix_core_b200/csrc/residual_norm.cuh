@@ -593,7 +593,7 @@ __global__ void __launch_bounds__(RN_WIDE_THREADS) residual_norm_fwd_wide_kernel
     }
 }
 
-template <typename T>
+template <typename T, bool OWN>
 __global__ void __launch_bounds__(RN_WIDE_THREADS) residual_norm_bwd_wide_kernel(const RNParams p) {
     constexpr int WPR = RN_WIDE_THREADS / 32;
     __shared__ float words[2 * WPR];
@@ -640,8 +640,9 @@ __global__ void __launch_bounds__(RN_WIDE_THREADS) residual_norm_bwd_wide_kernel
                         const float u = at<T>(p.branch, i) * rb, sdx = p.scale * grad(i, f), w = weight(p.post, f);
                         const float dn = p.gate ? sdx * at<T>(p.gate, (c * (size_t)p.groups + group) * F + f) : sdx, dg = sdx * u * w;
                         if (mine) mine[width + c * F + f] = fmaf(dn, u, mine[width + c * F + f]);
-                        if (gates) gates[c * F + f] = row == begin ? dg : gates[c * F + f] + dg;
-                        else if (p.dgate) put<T>(p.dgate, (c * (size_t)p.groups + group) * F + f, dg);       // (a gate for each value)
+                        if constexpr (OWN) {
+                            if (p.dgate) put<T>(p.dgate, (c * (size_t)p.groups + group) * F + f, dg);
+                        } else if (gates) gates[c * F + f] = row == begin ? dg : gates[c * F + f] + dg;
                         sum = fmaf(dn * w, u, sum);
                     }
                 fb = row_sum<WPR>(sum, words, turn) * inv_width * rb;
@@ -784,7 +785,8 @@ int bwd_typed(RNParams p, RNPlan q, cudaStream_t s) {
     const int grid = wide ? (q.grid < 4 * sm_count() ? q.grid : 4 * sm_count()) : ctas_beside(q.grid, p.period, sm_count());
     p.part_w = p.dpost || p.dpre ? reinterpret_cast<float*>(p.workspace) : nullptr;
     p.part_gate = p.dgate && q.part_gate ? reinterpret_cast<float*>(p.workspace + q.part_w) : nullptr;
-    if (wide) PCB_CUDA_TRY(launch_chained(residual_norm_bwd_wide_kernel<T>, grid, RN_WIDE_THREADS, 0, s, p));
+    if (wide && p.gate && p.groups == p.n) PCB_CUDA_TRY((launch_chained(residual_norm_bwd_wide_kernel<T, true>, grid, RN_WIDE_THREADS, 0, s, p)));
+    else if (wide) PCB_CUDA_TRY((launch_chained(residual_norm_bwd_wide_kernel<T, false>, grid, RN_WIDE_THREADS, 0, s, p)));
     else if (p.period == 1) PCB_CUDA_TRY((bwd_any<T, VEC, true>(p, q.shape, grid, s)));
     else PCB_CUDA_TRY((bwd_any<T, VEC, false>(p, q.shape, grid, s)));
     const long long weight_blocks = p.part_w ? (p.features + 7) / 8 : 0;
