@@ -162,7 +162,7 @@ constexpr const char* WATCH = "phoenix_core_b200.watch";
 std::atomic<long long> g_ended{0};                                  // graphs that are gone
 struct Watch {
     std::atomic<int> holders{2};                                   // the graph and Python
-    std::atomic<bool> ended{false};
+    std::atomic<bool> told{false}, ended{false};                   // told: the graph took the object (where it took none, it never ends for us)
     void drop() {
         if (holders.fetch_sub(1) == 1) delete this;
     }
@@ -189,25 +189,22 @@ PyObject* watch_capture(PyObject*, PyObject* stream) {
         return nullptr;
     }
     cudaUserObject_t object = nullptr;
-    cudaError_t e = cudaUserObjectCreate(&object, watch, watch_released, 1, cudaUserObjectNoDestructorSync);
-    if (e == cudaSuccess) {
-        e = cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove);
-        if (e != cudaSuccess) cudaUserObjectRelease(object, 1);
+    if (cudaUserObjectCreate(&object, watch, watch_released, 1, cudaUserObjectNoDestructorSync) != cudaSuccess) {
+        watch->drop();                                             // (the graph's share: nothing will say when it ends)
     } else {
-        watch->drop();
+        watch->told = true;
+        if (cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove) != cudaSuccess) {
+            watch->told = false;
+            cudaUserObjectRelease(object, 1);
+        }
     }
-    if (e != cudaSuccess) {
-        cudaGetLastError();
-        Py_DECREF(capsule);
-        PyErr_Format(PyExc_RuntimeError, "the captured graph takes no object: %s", cudaGetErrorString(e));
-        return nullptr;
-    }
+    cudaGetLastError();
     return capsule;
 }
 PyObject* ended_count(PyObject*, PyObject*) { return PyLong_FromLongLong(g_ended); }
 PyObject* ended(PyObject*, PyObject* capsule) {
     const Watch* watch = static_cast<const Watch*>(PyCapsule_GetPointer(capsule, WATCH));
-    return watch ? PyBool_FromLong(watch->ended) : nullptr;
+    return watch ? PyBool_FromLong(watch->told && watch->ended) : nullptr;
 }
 
 // Status words of captured calls: memory that no graph's and no stream's allocations are given, zero from the start, never given back.
