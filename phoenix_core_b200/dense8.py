@@ -134,8 +134,7 @@ def dense8Fwd(inputTensor, filter8, biasTensor, outputTensor, descriptor, contex
     with dev.accessControl:
         ws = dev.requestWorkspace(call.workspace)
         call.entry.call(ws, 0, inputTensor, filter8._storage, filter8.scales, biasTensor, outputTensor)
-        if dev.check_after_each_op:
-            dev.checkStatus()
+        dev._after_op()
 
 
 def dense8Bwd(inputTensor, filter8, gradTensor, filterGradTensor, inputGradTensor, descriptor, context=None, engine=_lib.ENGINE_AUTO):
@@ -155,5 +154,4 @@ def dense8Bwd(inputTensor, filter8, gradTensor, filterGradTensor, inputGradTenso
     with dev.accessControl:
         ws = dev.requestWorkspace(call.workspace)
         call.entry.call(ws, 0, *operands)
-        if dev.check_after_each_op:
-            dev.checkStatus()
+        dev._after_op()

@@ -160,7 +160,7 @@ class Device:
             return replayed
 
     def _after_op(self):
-        if self.check_after_each_op:
+        if self.check_after_each_op and not _capture_id(_raw_stream(self.index)):      # (what is being captured has not run)
             self.checkStatus()
 
     def getContext(self):

@@ -121,5 +121,4 @@ def residualNormBwd(outputTensor, branchTensor, gateTensor, postWeight, preWeigh
     with dev.accessControl:
         ws = dev.requestWorkspace(need)
         bwd.call(ws, 0, *operands)
-        if dev.check_after_each_op:
-            dev.checkStatus()
+        dev._after_op()

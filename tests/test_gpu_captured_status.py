@@ -130,3 +130,23 @@ def test_eager_calls_still_report(dev):
     assert reported(dev) and reported(dev)                         # until the stream's next call
     Layer(40).run()
     assert not reported(dev)
+
+
+def test_checks_after_each_operation(dev):
+    """With them on (PCB_CHECK_DEVICE_STATUS=1) a capture goes through as without, and what its replays report is seen by the next eager operation."""
+    layer, stream = Layer(40), torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        layer.run()
+    want = layer.results()
+    dev.check_after_each_op = True
+    try:
+        clean, bad = capture(layer.run, stream), capture(lambda: (layer.run(), expire(dev)), stream)
+        clean.replay()
+        assert layer.same(layer.results(), want)
+        layer.run()
+        bad.replay()
+        with pytest.raises(_lib.BackendError, match="wait expired"):
+            layer.run()
+        layer.run()
+    finally:
+        dev.check_after_each_op = False
