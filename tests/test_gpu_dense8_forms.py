@@ -86,3 +86,18 @@ def test_the_same_bits_again(case):
     first = run(algebra, layout, x, w, bias, dy)[1:]
     for _ in range(3):
         assert all(torch.equal(a, b) for a, b in zip(run(algebra, layout, x, w, bias, dy)[1:], first))
+
+
+@pytest.mark.parametrize("case", [PAIRS[7], PAIRS[2], BOTH[0], ("quaternion", "oi", "f32", 130, 200, 200), ("real", "io", "bf16", 40, 260, 260), ("complex", "io", "f16", 3, 130, 130)])
+def test_the_input_gradient_in_place(case):
+    """dx may replace x or, where it has its shape, dy: both are read before anything is written."""
+    algebra, layout, dtype, n, i, o = case
+    _, x, w, _, dy = make(algebra, layout, dtype, n, i, o)
+    f8, _, dw, dx = run(algebra, layout, x, w, None, dy)
+    bwd = pcb.DenseBwdDescriptor(tuple(x.shape), tuple(w.shape), f8.algebra, f8.filterLayout, True)
+    places = ["x", "dy"] if i == o else ["x"]
+    for place in places:
+        xd, dyd, again = x.cuda(), dy.cuda(), torch.full_like(dw, float("nan"))
+        target = xd if place == "x" else dyd
+        pcb.dense8Bwd(xd, f8, dyd, again, target, bwd)
+        assert torch.equal(again, dw) and torch.equal(target, dx), place
