@@ -9,7 +9,7 @@
 // A CTA takes a tile of 128 x 128 values in registers, 4 x 8 per thread: the blocks of 1 x 128, of 128 x 1 and of 128 x 128 all lie within it, so the
 // backward pass reads dy once for both of its products. The tile stays as it was loaded (as fp32 it took 176 registers, and one CTA per SM moved 2.2 TB/s);
 // maxima are taken over the bits of the magnitudes, two 16-bit values at a time. Three CTAs of 512 threads on an SM (fp32, and rows that start anywhere, whose words take registers: two), whose loads and stores lie beside each other, though
-// some words spill for it. 8192 x 4096 bf16: by rows 23.5 us (4.3 TB/s read and written), both orientations of one and the columns of another 46 (54 with two CTAs); 2420 x 8096 fp32 by rows
+// some words spill for it. 8192 x 4096 bf16: by rows 23.5 to 27.4 us by the machine (3.7 to 4.3 TB/s read and written), both orientations of one and the columns of another 46 to 48 (54 with two CTAs); 2420 x 8096 fp32 by rows
 // 21.5 (26.5 with one). What is left is latency: a CTA's loads are over before its stores begin.
 #include "dense8.cuh"
 #include "e4m3.cuh"

@@ -9,10 +9,10 @@
 //
 // Roles: warp 0 copies the operand tiles (TMA; both majornesses are read where they lie), warp 1 issues, warps 2 and 3 lay the scales out (a word per
 // row holds the bytes of four blocks; 32 x 4 words are 512 bytes in the order that tcgen05.cp takes to tensor memory), warps 4-11 drain the accumulators.
-// Three forms:
+// Four forms:
 //   PAIR      256 x 256 tiles on pairs of SMs, half of either operand in each one's shared memory. An 8-bit MMA of 128 x 256 x 32 takes 128 clocks and reads 12 KB of
 //             shared memory, into which TMA writes as much again: more than the 128 bytes a clock that shared memory moves. On one SM a block of 128 took
-//             0.53 us where the MMAs alone take 0.27; a pair moves a third less. 8192 x 4096 -> 4096: 98 us, 2.8 PFLOP/s (86 % of twice the bf16 burst rate); with the clocks that
+//             0.53 us where the MMAs alone take 0.27; a pair moves a third less. 8192 x 4096 -> 4096: 100 us, 2.75 PFLOP/s (84 % of twice the bf16 burst rate); with the clocks that
 //             this load leaves, a block takes 589 clocks of which the MMAs take 512: one accumulator of 256 columns is all that tensor memory holds beside the scales, so the epilogue
 //             is not covered.
 //   single    128 x 128 tiles; a tile's reduction is cut over the CTAs of a cluster where there are fewer tiles than SMs, whose partial sums are added in a

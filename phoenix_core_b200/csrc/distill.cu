@@ -6,8 +6,8 @@
 //   dz_j = g * ((1 - a) * (softmax(z)_j - [j = c]) + a * T * (q_j - p_j))
 // Both sums over the vocabulary are taken in one pass with a running maximum; the gradient reads the logits once more and writes
 // them once. With T = 2 the exponentials of T = 1 are the squares of the others: one exponential per logit, which keeps the pass bound by memory
-// (16 exponentials per clock and SM are two thirds of what a pass over 16-bit logits takes at full bandwidth). 4096 x 131072 bf16: 190 us forward (5.6 TB/s), 342
-// backward (6.3 TB/s both ways); bound by memory.
+// (16 exponentials per clock and SM are two thirds of what a pass over 16-bit logits takes at full bandwidth). 4096 x 131072 bf16: 192 us forward (5.6 TB/s), 346
+// backward (6.2 TB/s both ways) from cold caches, 178 and 337 behind themselves; bound by memory.
 // Few rows are cut over the CTAs of a cluster, whose maxima and sums are joined through distributed shared memory.
 #include "class_shares.h"
 #include "common.cuh"
