@@ -19,6 +19,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <atomic>
+#include <new>
 #include <vector>
 
 namespace {
@@ -182,7 +183,8 @@ PyObject* watch_capture(PyObject*, PyObject* stream) {
         PyErr_SetString(PyExc_RuntimeError, "the stream is not being captured");
         return nullptr;
     }
-    Watch* watch = new Watch;
+    Watch* watch = new (std::nothrow) Watch;
+    if (!watch) return PyErr_NoMemory();
     PyObject* capsule = PyCapsule_New(watch, WATCH, free_watch);
     if (!capsule) {
         delete watch;
@@ -251,14 +253,18 @@ PyObject* take_words(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     const long device = PyLong_AsLong(args[0]), count = PyLong_AsLong(args[3]);
     const W stream = PyLong_AsUnsignedLongLong(args[1]), words = PyLong_AsUnsignedLongLong(args[2]);
     if (PyErr_Occurred()) return nullptr;
+    int held[1024];
     const size_t n = count > 0 ? (size_t)count : 0;
-    std::vector<int> held(n);
+    if (n > sizeof(held) / 4) {
+        PyErr_SetString(PyExc_ValueError, "up to 1024 words at a time");
+        return nullptr;
+    }
     bool any = false;
     int before = 0;
     cudaGetDevice(&before);
     cudaError_t e = cudaSetDevice((int)device);
     Py_BEGIN_ALLOW_THREADS
-    if (e == cudaSuccess) e = cudaMemcpyAsync(held.data(), reinterpret_cast<const void*>(words), n * 4, cudaMemcpyDeviceToHost, reinterpret_cast<cudaStream_t>(stream));
+    if (e == cudaSuccess) e = cudaMemcpyAsync(held, reinterpret_cast<const void*>(words), n * 4, cudaMemcpyDeviceToHost, reinterpret_cast<cudaStream_t>(stream));
     if (e == cudaSuccess) e = cudaStreamSynchronize(reinterpret_cast<cudaStream_t>(stream));
     // (only those: another one may be written meanwhile)
     for (size_t i = 0; e == cudaSuccess && i < n; ++i)
