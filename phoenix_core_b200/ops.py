@@ -120,15 +120,16 @@ class Device:
             self._giveWord(c, ws)
             return ws
 
-    def holdForCapture(self, ws):
-        """Keeps a workspace that a call brings itself for as long as a graph may use it, if the call is being captured."""
+    def holdForCapture(self, ws, reports=True):
+        """Keeps a workspace that a call brings itself for as long as a graph may use it, if the call is being captured. ``reports``: the call has its status word in it."""
         stream = _raw_stream(self.index)
         capture = _capture_id(stream)
         if capture:
             with self._captureLock:
                 c = self._capture(capture, stream)
                 c.others.append(ws)
-                self._giveWord(c, ws)
+                if reports:
+                    self._giveWord(c, ws)
 
     @property
     def workspace(self):
@@ -427,6 +428,7 @@ def conv2DBwd(inputTensor, filterTensor, gradTensor, filterGradTensor, inputGrad
             need = d._bwd_need = L.pcb_qconv2d_bwd_workspace_size(ctypes.byref(d))
         ws = dev.requestWorkspace(need)
         if kept is not None and kept.workspace is not None and on_filter_grad is None:
+            dev.holdForCapture(kept.workspace, reports=False)
             _lib.check(L.pcb_qconv2d_bwd_kept(ctypes.byref(d), _ptr(inputTensor), _ptr(filterTensor), _ptr(gradTensor),
                                               _ptr(filterGradTensor), _ptr(inputGradTensor) if need_dx else None,
                                               _ptr(kept.workspace), kept.workspace.numel(), _ptr(ws), ws.numel(), _stream()))

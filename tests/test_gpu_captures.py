@@ -60,14 +60,17 @@ class Layer:
         return out
 
 
-    def same(self, got, want):
-        """Bit for bit but for the convolution's filter gradient, whose partial sums are added by atomics: up to three rounds of one for each SM, in fp32 and any order, so
-        two runs lie within 2 * 444 * 2^-24 of the sum of the absolute products (by Cauchy and Schwarz no larger than the product of the channels' norms) and,
-        rounded to fp16 each, a step (2^-10) of the value."""
+    def order(self):
+        """How far two runs of the convolution's filter gradient may lie apart before they are rounded: its partial sums are added by atomics, up to three rounds of one for
+        each SM, in fp32 and any order, so within 2 * 444 * 2^-24 of the sum of the absolute products (by Cauchy and Schwarz no larger than the product of the
+        channels' norms)."""
         image, dimage = (t.double().transpose(0, 1).flatten(1).norm(dim=1) for t in (self.image, self.dimage))
-        order = 2 * 444 * 2.0 ** -24 * (dimage[:, None] * image[None, :])[None, :, :, None, None]
+        return 2 * 444 * 2.0 ** -24 * (dimage[:, None] * image[None, :])[None, :, :, None, None]
+
+    def same(self, got, want):
+        """Bit for bit but for the convolution's filter gradient, of which two runs lie within `order` and, rounded to fp16 each, a step (2^-10) of the value."""
         a, b = got[6].double(), want[6].double()
-        return all(torch.equal(a, b) for a, b in zip(got[:6] + got[7:], want[:6] + want[7:])) and bool(((a - b).abs() <= order + 2.0 ** -10 * b.abs()).all())
+        return all(torch.equal(a, b) for a, b in zip(got[:6] + got[7:], want[:6] + want[7:])) and bool(((a - b).abs() <= self.order() + 2.0 ** -10 * b.abs()).all())
 
 
 def take_what_is_free():
@@ -169,3 +172,27 @@ def test_streams_of_one_capture_share_nothing():
         graph.replay()
         for layer, want in zip(layers, wants):
             assert layer.same(layer.results(), want)
+
+
+def test_a_kept_input_outlives_its_owner():
+    """A backward call captured by itself reads what an eager forward call kept, and goes on doing so when the owner of that is gone."""
+    layer, dev, stream = Layer(40), device(), torch.cuda.Stream()
+    image, dkernel, dimage = layer.out[5:]
+    keep = pcb.KeptInput()
+    pcb.conv2DFwd(layer.image, layer.kernel, None, image, layer.conv, keep=keep)
+    pcb.conv2DBwd(layer.image, layer.kernel, layer.dimage, dkernel, dimage, layer.conv_bwd, kept=keep)
+    want = layer.results()
+    size, order = keep.workspace.numel(), layer.order()
+    pcb.conv2DFwd(layer.image, layer.kernel, None, image, layer.conv, keep=keep)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        pcb.conv2DBwd(layer.image, layer.kernel, layer.dimage, dkernel, dimage, layer.conv_bwd, kept=keep)
+    assert any(t is keep.workspace for t in dev.captures[max(dev.captures)].others)
+    del keep
+    gc.collect()
+    mine = [torch.full((size,), 7, dtype=torch.uint8, device="cuda") for _ in range(8)]
+    layer.image.zero_()                                                         # (the filter gradient is of what was kept)
+    graph.replay()
+    got = layer.results()
+    assert all((t == 7).all() for t in mine) and torch.equal(got[7], want[7])
+    assert ((got[6].double() - want[6].double()).abs() <= order + 2.0 ** -10 * want[6].double().abs()).all()
