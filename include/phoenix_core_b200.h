@@ -295,7 +295,7 @@ int pcb_residual_norm_bwd(const pcb_norm_desc* desc, const void* y, const void* 
  * `stats` (fp32 [3][batch], may be null) is kept for the backward call: maximum, sum of
  * exp(z - max), sum of exp((z - max) / T), infinity in place of a sum that the gradient has no term of.
  * Backward: dlogits = grad_loss[sample] * d loss / d logits; must not share memory with the logits. Up to 4096 entries, D * units < 2^31;
- * 1 / T and T^2 are to be fp32 numbers. Sums are fp32; exponentials are right to a few units in the last place (ex2.approx, and the square of one where T = 2), which an
+ * 1.45 / T and T^2 are to be in fp32's range. Sums are fp32; exponentials are right to a few units in the last place (ex2.approx, and the square of one where T = 2), which an
  * fp32 loss shows: some 2e-7 of its terms. */
 typedef struct pcb_distill_desc {
     int32_t dtype;            /* pcb_dtype of logits, teacher, dlogits */

@@ -519,9 +519,9 @@ int check_distill(const pcb_distill_desc* d, int& comps) {
     if (!algebra_setup(d->algebra, g)) { set_error("unknown algebra %d", d->algebra); return PCB_ERR_INVALID_ARGUMENT; }
     comps = g.nc;
     if (d->batch < 0 || d->units <= 0 || d->entries < 0) { set_error("invalid distillation geometry"); return PCB_ERR_INVALID_ARGUMENT; }
-    // (1 / T divides the logits and T^2 multiplies the second term, both in fp32)
-    if (!(d->alpha >= 0.f && d->alpha <= 1.f) || !(d->temperature > 0.f) || 1.f / d->temperature == INFINITY || d->temperature * d->temperature == INFINITY) {
-        set_error("alpha in [0, 1] and a positive temperature whose reciprocal and square are fp32 numbers expected");
+    // (log2(e) / T multiplies the logits and T^2 the second term, both in fp32)
+    if (!(d->alpha >= 0.f && d->alpha <= 1.f) || !(d->temperature > 0.f) || LOG2E * (1.f / d->temperature) == INFINITY || d->temperature * d->temperature == INFINITY) {
+        set_error("alpha in [0, 1] and a positive temperature with 1.45 / T and T^2 in fp32's range expected");
         return PCB_ERR_INVALID_ARGUMENT;
     }
     if (d->entries > DI_MAX_ENTRIES) { set_error("%d entries of the teacher's, %d at most", d->entries, DI_MAX_ENTRIES); return PCB_ERR_UNSUPPORTED; }

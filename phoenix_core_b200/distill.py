@@ -28,9 +28,9 @@ class DistillDescriptor:
             raise ValueError("logits shape %s: (components * samples, units) expected, with %d components" % (self.logitsShape, dim))
         if self.teacherEntries < 0:
             raise ValueError("negative number of entries")
-        most = torch.finfo(torch.float32).max                    # (1 / T and T^2 are taken in fp32)
-        if not 0.0 <= self.alpha <= 1.0 or not 1.0 / most < self.temperature < most ** 0.5:
-            raise ValueError("alpha in [0, 1] and a positive temperature whose reciprocal and square are fp32 numbers expected")
+        most = torch.finfo(torch.float32).max                    # (log2(e) / T and T^2 are taken in fp32)
+        if not 0.0 <= self.alpha <= 1.0 or not 1.45 / most < self.temperature < most ** 0.5:
+            raise ValueError("alpha in [0, 1] and a positive temperature with 1.45 / T and T^2 in fp32's range expected")
         self.samples = self.logitsShape[0] // dim
         self.teacherShape, self.lossShape, self.statsShape = (self.samples, self.teacherEntries), (self.samples,), (3, self.samples)
         self._calls = {}

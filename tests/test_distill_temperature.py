@@ -14,9 +14,9 @@ def library():
     return _lib.lib()
 
 
-@pytest.mark.parametrize("temperature,taken", [(1e-45, False), (1e-39, False), (2.9e-39, False), (1e-30, True), (0.1, True), (1e9, True), (1.8e19, True), (1.9e19, False), (3e38, False)])
+@pytest.mark.parametrize("temperature,taken", [(1e-45, False), (1e-39, False), (2.9e-39, False), (3.5e-39, False), (4.2e-39, False), (4.3e-39, True), (1e-30, True), (0.1, True), (1e9, True), (1.8e19, True), (1.9e19, False), (3e38, False)])
 def test_reciprocal_and_square(library, temperature, taken):
-    """Both are taken in fp32: 1 / T divides the logits, T^2 multiplies the second term. (A call without samples is checked and does nothing.)"""
+    """Both are taken in fp32: log2(e) / T multiplies the logits, T^2 the second term. (A call without samples is checked and does nothing.)"""
     d = _lib.DistillDesc()
     d.dtype, d.algebra, d.batch, d.units, d.entries, d.alpha, d.temperature = _lib.PCB_F16, 0, 0, 250, 4, 0.5, temperature
     status = library.pcb_distill_fwd(ctypes.byref(d), None, None, None, None, None, None, None)
